@@ -561,6 +561,91 @@ int lkv_lse_merge(const float* outs, const float* lses, int n_parts, int64_t row
 int lkv_lse_merge_packed(const float* parts, int n_parts, int64_t rows, int d, void* out, int out_dtype,
                          float* lse_out, void* stream);
 
+/*
+ * The paged cache of a batch of sequences (no reference counterpart: the reference is batch-1 and its
+ * int8 tier quantises whole sealed blocks, lazykv/quant.py:73-87). pages [n_pages, h, 2, bs, d], keys
+ * then values, in the model dtype (LKV_CACHE_MODEL) or as int8 codes (LKV_CACHE_INT8) with one float32
+ * scale per row, scales [n_pages, h, 2, bs]; d 64 or 128, bs 16, 32, 64 or 128. Token pos of sequence
+ * b is row pos % bs of page table[b * table_ld + pos / bs]; a page id outside [0, n_pages) and a
+ * position outside the table's table_cols columns have no page. Two tokens of one call must not name
+ * one row.
+ */
+typedef enum { LKV_CACHE_MODEL = 0, LKV_CACHE_INT8 = 1 } lkv_cache_kind;
+
+/*
+ * Writes tokens [batch, tokens] with keys and values [batch, tokens, h, d] (element strides, channels
+ * contiguous, dtype float32 or bfloat16) to positions starts[b] .. starts[b] + tokens - 1 of their
+ * sequences; a token without a page is not written. int8: the row's scale is s = max(max |x| / 127,
+ * FLT_MIN), at most what keeps 127 s finite, and its codes the whole numbers nearest to x / s (halfway: even); a row that holds an
+ * infinity or a NaN gets the scale NaN. Model dtype: copied. batch * tokens * h < 2^31.
+ */
+int lkv_paged_write(const void* keys, int64_t k_sb, int64_t k_st, int64_t k_sh, const void* values, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                    int dtype, int batch, int tokens, int h, int d, void* pages, int kind, float* scales, int64_t n_pages, int bs,
+                    const int32_t* table, int64_t table_ld, int table_cols, const int32_t* starts, void* stream);
+
+/*
+ * Reads tokens starts[b] .. starts[b] + tokens - 1 of every sequence back as out_k, out_v [batch,
+ * tokens, h, d] in dtype (model-dtype pages: that dtype): code * scale, rounded once. Tokens at or past
+ * lens[b] (where lens is given) and tokens without a page are zeros.
+ */
+int lkv_paged_read(const void* pages, int kind, const float* scales, int64_t n_pages, int bs, int batch, int tokens, int h, int d,
+                   const int32_t* table, int64_t table_ld, int table_cols, const int32_t* starts, const int32_t* lens, void* out_k, void* out_v,
+                   int dtype, void* stream);
+
+/*
+ * Attention of a batch whose sequences share a prefix (no reference counterpart). Query t of sequence b
+ * (q [batch, tokens, hq, d] bfloat16, element strides, 16-byte aligned rows) attends the prefix's
+ * prefix_len tokens, whose pages prefix_table lists, and the first lens[b] - tokens + t + 1 of its
+ * sequence's own lens[b] tokens (the step's tokens are its last; none where that is not positive). A
+ * token without a page is not attended. out [batch, tokens, hq, d] contiguous in out_dtype and lse
+ * [batch, tokens, hq] float32; a row that attends nothing gets out = 0, lse = -inf. lens and the tables
+ * are read on the device, so a captured graph follows them; prefix_len and the shapes are the call's.
+ * The prefix is read once for the batch: partials in the workspace (any contents,
+ * lkv_prefix_attention_workspace bytes, 16-byte aligned), folded in by the launch over the sequences'
+ * own tokens. Calls that may overlap on the GPU need a workspace each.
+ */
+typedef struct {
+  const void* q;
+  int dtype; /* of q and of model-dtype pages: LKV_BF16 */
+  int64_t q_sb, q_st, q_sh;
+  const void* pages;
+  int kind;
+  const float* scales;
+  int64_t n_pages;
+  int bs;
+  int batch, tokens, hq, h, d;
+  const int32_t* table;
+  int64_t table_ld;
+  int table_cols;
+  const int32_t* lens;
+  const int32_t* prefix_table;
+  int prefix_cols;
+  int64_t prefix_len;
+  float scale;
+  void* out;
+  int out_dtype;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+} lkv_prefix_args;
+size_t lkv_prefix_attention_workspace(int batch, int tokens, int hq, int h, int d, int64_t prefix_len);
+int lkv_prefix_attention(const lkv_prefix_args* args, void* stream);
+
+/*
+ * Verification of k drafted tokens per sequence (no reference counterpart; the reference decodes one
+ * token at a time, lazykv/generate.py:134-154). target [batch, k + 1, vocab] and draft [batch, k,
+ * vocab] float32 probabilities (element strides, rows contiguous; draft null: the drafted token was
+ * certain), tokens [batch, k] int64, uniforms [batch, k + 1] float32 in [0, 1). kept[b] is the number n
+ * of leading tokens with u_i draft_i(x_i) < target_i(x_i), computed exactly; token[b] the least v whose
+ * cumulative weight passes u_k times the total, weights max(target_n - draft_n, 0) after a rejection
+ * (target_n itself where those are all 0) and target_k where all were kept, in float64. A token outside
+ * [0, vocab) ends its sequence's drafts (as if all before it had been all). token[b] = -1 where the
+ * weights are all 0 or have no finite sum. vocab <= 4,194,304.
+ */
+int lkv_verify_drafts(const float* target, int64_t p_sb, int64_t p_st, const float* draft, int64_t q_sb, int64_t q_st, const int64_t* tokens,
+                      int64_t t_sb, const float* uniforms, int64_t u_sb, int batch, int k, int vocab, int32_t* kept, int64_t* token,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,7 @@ LIB_PATH = Path(__file__).resolve().parent / "liblkv_sm100.so"
 LKV_F32, LKV_BF16 = 0, 1
 LKV_COLD_INT8, LKV_COLD_PAIRS = 0, 1
 LKV_ORDER_BOUND, LKV_ORDER_BLOCK = 0, 1
+LKV_CACHE_MODEL, LKV_CACHE_INT8 = 0, 1
 LKV_DEBUG_SELECT_WAIT_ITERS, LKV_DEBUG_SELECT_STALL_NEXT, LKV_DEBUG_EXCHANGE_WAIT_ITERS = 1, 2, 3
 LKV_DEV_WAIT_TIMEOUT, LKV_DEV_LIST_OVERFLOW = 1, 2
 
@@ -80,6 +81,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lkv_split_join": (c_int, [c_void_p, c_void_p]),
     "lkv_split_wait": (c_int, [c_void_p]),
     "lkv_append_tokens": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p]),
+    "lkv_paged_write": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int,
+                                c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p]),
+    "lkv_paged_read": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p,
+                               c_void_p, c_void_p, c_int, c_void_p]),
+    "lkv_prefix_attention_workspace": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int64]),
+    "lkv_prefix_attention": (c_int, [c_void_p, c_void_p]),
+    "lkv_verify_drafts": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int,
+                                  c_void_p, c_void_p, c_void_p]),
     "lkv_ragged_stage_records": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p,
                                          c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
 }
@@ -111,6 +120,16 @@ class SplitStepArgs(ctypes.Structure):
                 ("last_used", c_void_p), ("n_slots", c_int), ("evicted_at", c_void_p), ("step", c_int64), ("store", c_void_p),
                 ("store_kind", c_int), ("pool", c_void_p), ("pool_dtype", c_int), ("miss_blk", c_void_p), ("miss_slot", c_void_p),
                 ("n_miss", c_void_p), ("miss_total", c_void_p), ("selected", c_int)]
+
+
+class PrefixArgs(ctypes.Structure):
+    """lkv_prefix_args of include/lkv.h (same fields, same order)."""
+
+    _fields_ = [("q", c_void_p), ("dtype", c_int), ("q_sb", c_int64), ("q_st", c_int64), ("q_sh", c_int64), ("pages", c_void_p), ("kind", c_int),
+                ("scales", c_void_p), ("n_pages", c_int64), ("bs", c_int), ("batch", c_int), ("tokens", c_int), ("hq", c_int), ("h", c_int),
+                ("d", c_int), ("table", c_void_p), ("table_ld", c_int64), ("table_cols", c_int), ("lens", c_void_p), ("prefix_table", c_void_p),
+                ("prefix_cols", c_int), ("prefix_len", c_int64), ("scale", c_float), ("out", c_void_p), ("out_dtype", c_int), ("lse", c_void_p),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
 class LkvError(RuntimeError):

@@ -1,0 +1,321 @@
+// The paged cache: tokens written into pages (quantised on the way in) and read back.
+//
+// One page holds bs tokens of every KV head, keys then values, as the pairs of the tiered store do:
+// pages [n_pages, h, 2, bs, d]. The elements are the model's type, or int8 codes with one float32
+// scale per (token, head, key or value) row, scales [n_pages, h, 2, bs]. A sequence's token `pos` is
+// row pos % bs of page table[b][pos / bs]. Unlike the sealed blocks' records (codec.cu), whose keys
+// are quantised per channel over a whole block, a row's scale needs that row only, so a token is
+// final as soon as it is written.
+//
+// The row's code: s = max(max_c |x_c| / 127, FLT_MIN) (at most what keeps 127 s finite), code_c = the whole number nearest to x_c / s
+// (halfway: the even one), value code_c * s. The quotient is never rounded before the rounding to a
+// whole number: k = rint(x * (1 / s)) is within one of it, the remainder x - k s is exact in one fused
+// multiply-add, and k moves by one where the remainder passes s / 2. A row that holds an infinity or a
+// NaN has no scale: it gets s = NaN and codes 0 and reads back as NaN throughout.
+//
+// What bounds both kernels is memory: every byte moves once. A thread carries 16 channels of one
+// token's key row and of its value row (64 bytes in flight per thread for bf16), d / 16 threads a row.
+#include <float.h>
+
+#include "common.cuh"
+
+namespace lkv {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kCh = 16;  // channels per thread
+constexpr float kMaxScale = 0x1.020406p+121f;  // the largest whose 127-fold is finite
+
+struct PagedParams {
+  const void* keys;    // write: [b, t, h, d] with these element strides (channels contiguous)
+  const void* values;
+  int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  void* pages;
+  float* scales;
+  int64_t n_pages;
+  const int32_t* table;
+  int64_t table_ld;
+  int table_cols;
+  const int32_t* starts;
+  const int32_t* lens;  // read: tokens a sequence has (null: as many as its table)
+  uint32_t rows;        // batch * tokens * h
+  uint32_t tokens, h;
+  int page_shift;
+  void* out_k;  // read: contiguous [b, n, h, d]
+  void* out_v;
+};
+
+// 16 consecutive elements as float; VEC: 16-byte aligned. Plain loads: the read-only path may serve a
+// line that the kernel before this one, still running when this one started, has written since.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load16(const T* p, float* x) {
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int i = 0; i < kCh; ++i) x[i] = to_f32<T>(p[i]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 a = reinterpret_cast<const float4*>(p)[i];
+      x[4 * i] = a.x, x[4 * i + 1] = a.y, x[4 * i + 2] = a.z, x[4 * i + 3] = a.w;
+    }
+  } else {
+    const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const float* x) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+  } else {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
+// The page of token `pos` of sequence b, or -1 where it has none (outside the table, a hole, a bad id).
+__device__ __forceinline__ int64_t page_of(const PagedParams& p, uint32_t b, int64_t pos) {
+  if (pos < 0) return -1;
+  const int64_t blk = pos >> p.page_shift;
+  if (blk >= p.table_cols) return -1;
+  const int64_t id = p.table[(int64_t)b * p.table_ld + blk];
+  return id < p.n_pages ? id : -1;
+}
+
+// One quantised row, 16 channels per lane of a group of L lanes: the codes and the row's scale.
+template <int L>
+__device__ __forceinline__ uint4 quantise_row(const float* x, float& scale) {
+  uint32_t top = 0;  // magnitudes compare as their bits; infinities and NaN come out above FLT_MAX
+#pragma unroll
+  for (int i = 0; i < kCh; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (top >= 0x7f800000u) {
+    scale = __uint_as_float(0x7fc00000u);
+    return make_uint4(0, 0, 0, 0);
+  }
+  const float s = fminf(fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), FLT_MIN), kMaxScale), inv = 1.0f / s, half = 0.5f * s;
+  scale = s;
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < kCh; ++i) {
+    float k = rintf(x[i] * inv);
+    const float r = fmaf(-k, s, x[i]);
+    // A remainder of exactly half a step belongs to the even neighbour.
+    const bool odd = (static_cast<int>(k) & 1) != 0;
+    if (r > half || (r == half && odd)) k += 1.0f;
+    if (r < -half || (r == -half && odd)) k -= 1.0f;
+    w[i / 4] |= (static_cast<uint32_t>(static_cast<int>(k)) & 0xffu) << (8 * (i % 4));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Grid: rows of (sequence, token, head), D / 16 threads each.
+template <typename T, int D, bool INT8, bool VEC>
+__global__ void __launch_bounds__(kThreads) paged_write_kernel(const PagedParams p) {
+  constexpr int L = D / kCh;
+  pdl_wait();
+  pdl_release();
+  const uint32_t row = blockIdx.x * (kThreads / L) + threadIdx.x / L;
+  const int c = (threadIdx.x % L) * kCh;
+  const bool live = row < p.rows;
+  const uint32_t j = row % p.h, bt = row / p.h, t = bt % p.tokens, b = bt / p.tokens;
+  int64_t page = -1, pos = 0;
+  float k[kCh], v[kCh];
+  if (live) {
+    load16<T, VEC>(static_cast<const T*>(p.keys) + b * p.k_sb + t * p.k_st + j * p.k_sh + c, k);
+    load16<T, VEC>(static_cast<const T*>(p.values) + b * p.v_sb + t * p.v_st + j * p.v_sh + c, v);
+    pos = (int64_t)p.starts[b] + t;
+    page = page_of(p, b, pos);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kCh; ++i) k[i] = v[i] = 0.0f;
+  }
+  const int bs = 1 << p.page_shift, at = (int)(pos & (bs - 1));
+  const int64_t kr = ((page * p.h + j) * 2) * bs + at, vr = kr + bs;  // rows of the page's keys and values
+  if constexpr (INT8) {
+    float ks, vs;
+    const uint4 kq = quantise_row<L>(k, ks), vq = quantise_row<L>(v, vs);
+    if (page < 0) return;
+    *reinterpret_cast<uint4*>(static_cast<int8_t*>(p.pages) + kr * D + c) = kq;
+    *reinterpret_cast<uint4*>(static_cast<int8_t*>(p.pages) + vr * D + c) = vq;
+    if (c == 0) {
+      p.scales[kr] = ks;
+      p.scales[vr] = vs;
+    }
+  } else {
+    if (page < 0) return;
+    store16<T>(static_cast<T*>(p.pages) + kr * D + c, k);
+    store16<T>(static_cast<T*>(p.pages) + vr * D + c, v);
+  }
+}
+
+// 16 codes and their scale as values.
+__device__ __forceinline__ void dequantise16(const int8_t* p, float s, float* x) {
+  const uint4 w = *reinterpret_cast<const uint4*>(p);
+  const int8_t* q = reinterpret_cast<const int8_t*>(&w);
+#pragma unroll
+  for (int i = 0; i < kCh; ++i) x[i] = (float)q[i] * s;
+}
+
+template <typename T, int D, bool INT8>
+__global__ void __launch_bounds__(kThreads) paged_read_kernel(const PagedParams p) {
+  constexpr int L = D / kCh;
+  pdl_wait();
+  pdl_release();
+  const uint32_t row = blockIdx.x * (kThreads / L) + threadIdx.x / L;
+  if (row >= p.rows) return;
+  const int c = (threadIdx.x % L) * kCh;
+  const uint32_t j = row % p.h, bt = row / p.h, t = bt % p.tokens, b = bt / p.tokens;
+  const int64_t pos = (int64_t)p.starts[b] + t;
+  int64_t page = -1;
+  if (p.lens == nullptr || pos < p.lens[b]) page = page_of(p, b, pos);
+  float k[kCh], v[kCh];
+  if (page < 0) {
+#pragma unroll
+    for (int i = 0; i < kCh; ++i) k[i] = v[i] = 0.0f;
+  } else {
+    const int bs = 1 << p.page_shift, at = (int)(pos & (bs - 1));
+    const int64_t kr = ((page * p.h + j) * 2) * bs + at, vr = kr + bs;
+    if constexpr (INT8) {
+      const int8_t* pages = static_cast<const int8_t*>(p.pages);
+      dequantise16(pages + kr * D + c, p.scales[kr], k);
+      dequantise16(pages + vr * D + c, p.scales[vr], v);
+    } else {
+      load16<T, true>(static_cast<const T*>(p.pages) + kr * D + c, k);
+      load16<T, true>(static_cast<const T*>(p.pages) + vr * D + c, v);
+    }
+  }
+  store16<T>(static_cast<T*>(p.out_k) + (int64_t)row * D + c, k);
+  store16<T>(static_cast<T*>(p.out_v) + (int64_t)row * D + c, v);
+}
+
+int check_cache(const char* who, int kind, int dtype, int h, int bs, int d, int64_t n_pages, const void* pages, const void* scales) {
+  if (!dtype_ok(dtype)) return fail(LKV_ERR_ARG, "%s: bad dtype %d", who, dtype);
+  if (kind != LKV_CACHE_MODEL && kind != LKV_CACHE_INT8) return fail(LKV_ERR_ARG, "%s: bad cache kind %d", who, kind);
+  if (d != 64 && d != 128) return fail(LKV_ERR_ARG, "%s: head_dim %d (64 or 128)", who, d);
+  if (bs != 16 && bs != 32 && bs != 64 && bs != 128) return fail(LKV_ERR_ARG, "%s: pages of %d tokens (16, 32, 64 or 128)", who, bs);
+  if (h < 1 || n_pages < 0 || n_pages > INT32_MAX) return fail(LKV_ERR_ARG, "%s: bad shape (h %d, pages %lld)", who, h, (long long)n_pages);
+  if (pages == nullptr || (kind == LKV_CACHE_INT8 && scales == nullptr)) return fail(LKV_ERR_PTR, "%s: null pointer", who);
+  if (!aligned(pages, 16) || !aligned(scales, 4)) return fail(LKV_ERR_PTR, "%s: pages must be 16-byte aligned", who);
+  return LKV_OK;
+}
+
+int shift_of(int bs) { return bs == 16 ? 4 : bs == 32 ? 5 : bs == 64 ? 6 : 7; }
+
+template <typename T, int D>
+cudaError_t launch_write(const PagedParams& p, bool int8, bool vec, unsigned grid, cudaStream_t st) {
+  if (int8) return vec ? launch_pdl(paged_write_kernel<T, D, true, true>, dim3(grid), dim3(kThreads), 0, st, 0, p)
+                       : launch_pdl(paged_write_kernel<T, D, true, false>, dim3(grid), dim3(kThreads), 0, st, 0, p);
+  return vec ? launch_pdl(paged_write_kernel<T, D, false, true>, dim3(grid), dim3(kThreads), 0, st, 0, p)
+             : launch_pdl(paged_write_kernel<T, D, false, false>, dim3(grid), dim3(kThreads), 0, st, 0, p);
+}
+
+template <typename T, int D>
+cudaError_t launch_read(const PagedParams& p, bool int8, unsigned grid, cudaStream_t st) {
+  return int8 ? launch_pdl(paged_read_kernel<T, D, true>, dim3(grid), dim3(kThreads), 0, st, 0, p)
+              : launch_pdl(paged_read_kernel<T, D, false>, dim3(grid), dim3(kThreads), 0, st, 0, p);
+}
+
+}  // namespace
+}  // namespace lkv
+
+using namespace lkv;
+
+extern "C" {
+
+int lkv_paged_write(const void* keys, int64_t k_sb, int64_t k_st, int64_t k_sh, const void* values, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                    int dtype, int batch, int tokens, int h, int d, void* pages, int kind, float* scales, int64_t n_pages, int bs,
+                    const int32_t* table, int64_t table_ld, int table_cols, const int32_t* starts, void* stream) {
+  if (int rc = check_cache("lkv_paged_write", kind, dtype, h, bs, d, n_pages, pages, scales)) return rc;
+  if (batch < 0 || tokens < 0 || table_cols < 0 || (batch > 1 && table_ld < table_cols))
+    return fail(LKV_ERR_ARG, "lkv_paged_write: bad shape (batch %d, tokens %d, table of %d columns)", batch, tokens, table_cols);
+  const int64_t rows = (int64_t)batch * tokens * h;
+  if (rows > INT32_MAX) return fail(LKV_ERR_ARG, "lkv_paged_write: %lld rows of one call", (long long)rows);
+  if (rows == 0 || n_pages == 0 || table_cols == 0) return LKV_OK;
+  if (keys == nullptr || values == nullptr || table == nullptr || starts == nullptr) return fail(LKV_ERR_PTR, "lkv_paged_write: null pointer");
+  const int size = (int)dtype_size(dtype), per = 16 / size;
+  if (!aligned(keys, size) || !aligned(values, size)) return fail(LKV_ERR_PTR, "lkv_paged_write: misaligned keys or values");
+  const bool vec = aligned(keys, 16) && aligned(values, 16) && k_sb % per == 0 && k_st % per == 0 && k_sh % per == 0 && v_sb % per == 0 &&
+                   v_st % per == 0 && v_sh % per == 0;
+  PagedParams p = {};
+  p.keys = keys;
+  p.values = values;
+  p.k_sb = k_sb, p.k_st = k_st, p.k_sh = k_sh;
+  p.v_sb = v_sb, p.v_st = v_st, p.v_sh = v_sh;
+  p.pages = pages;
+  p.scales = scales;
+  p.n_pages = n_pages;
+  p.table = table;
+  p.table_ld = table_ld;
+  p.table_cols = table_cols;
+  p.starts = starts;
+  p.rows = (uint32_t)rows;
+  p.tokens = tokens;
+  p.h = h;
+  p.page_shift = shift_of(bs);
+  const unsigned per_cta = kThreads / (d / kCh), grid = (unsigned)((rows + per_cta - 1) / per_cta);
+  const bool int8 = kind == LKV_CACHE_INT8;
+  cudaStream_t st = as_stream(stream);
+  cudaError_t e;
+  if (dtype == LKV_BF16)
+    e = d == 64 ? launch_write<__nv_bfloat16, 64>(p, int8, vec, grid, st) : launch_write<__nv_bfloat16, 128>(p, int8, vec, grid, st);
+  else
+    e = d == 64 ? launch_write<float, 64>(p, int8, vec, grid, st) : launch_write<float, 128>(p, int8, vec, grid, st);
+  if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "lkv_paged_write: %s", cudaGetErrorString(e));
+  return LKV_OK;
+}
+
+int lkv_paged_read(const void* pages, int kind, const float* scales, int64_t n_pages, int bs, int batch, int tokens, int h, int d,
+                   const int32_t* table, int64_t table_ld, int table_cols, const int32_t* starts, const int32_t* lens, void* out_k, void* out_v,
+                   int dtype, void* stream) {
+  if (int rc = check_cache("lkv_paged_read", kind, dtype, h, bs, d, n_pages, pages, scales)) return rc;
+  if (batch < 0 || tokens < 0 || table_cols < 0 || (batch > 1 && table_ld < table_cols))
+    return fail(LKV_ERR_ARG, "lkv_paged_read: bad shape (batch %d, tokens %d, table of %d columns)", batch, tokens, table_cols);
+  const int64_t rows = (int64_t)batch * tokens * h;
+  if (rows > INT32_MAX) return fail(LKV_ERR_ARG, "lkv_paged_read: %lld rows of one call", (long long)rows);
+  if (rows == 0) return LKV_OK;
+  if ((table == nullptr && table_cols > 0) || starts == nullptr || out_k == nullptr || out_v == nullptr)
+    return fail(LKV_ERR_PTR, "lkv_paged_read: null pointer");
+  if (!aligned(out_k, 16) || !aligned(out_v, 16)) return fail(LKV_ERR_PTR, "lkv_paged_read: outputs must be 16-byte aligned");
+  PagedParams p = {};
+  p.pages = const_cast<void*>(pages);
+  p.scales = const_cast<float*>(scales);
+  p.n_pages = n_pages;
+  p.table = table;
+  p.table_ld = table_ld;
+  p.table_cols = table_cols;
+  p.starts = starts;
+  p.lens = lens;
+  p.rows = (uint32_t)rows;
+  p.tokens = tokens;
+  p.h = h;
+  p.page_shift = shift_of(bs);
+  p.out_k = out_k;
+  p.out_v = out_v;
+  const unsigned per_cta = kThreads / (d / kCh), grid = (unsigned)((rows + per_cta - 1) / per_cta);
+  const bool int8 = kind == LKV_CACHE_INT8;
+  cudaStream_t st = as_stream(stream);
+  cudaError_t e;
+  if (dtype == LKV_BF16)
+    e = d == 64 ? launch_read<__nv_bfloat16, 64>(p, int8, grid, st) : launch_read<__nv_bfloat16, 128>(p, int8, grid, st);
+  else
+    e = d == 64 ? launch_read<float, 64>(p, int8, grid, st) : launch_read<float, 128>(p, int8, grid, st);
+  if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "lkv_paged_read: %s", cudaGetErrorString(e));
+  return LKV_OK;
+}
+
+}  // extern "C"

@@ -435,3 +435,179 @@ def quest_topk_admit(query: torch.Tensor, kmin: torch.Tensor, kmax: torch.Tensor
          pool.shape[-2], dtype_code(pool.dtype), ptr(miss_blk), ptr(miss_slot), ptr(n_miss), ptr(slots_out),
          0 if slots_out is None else slots_out.stride(0), ptr(miss_total), stream_handle(dev))
     return chosen
+
+
+# -- the paged cache of a batch, the attention over a shared prefix, and draft verification --------------
+
+
+def _on(dev: torch.device, name: str, *args: object) -> None:
+    """call(name, *args, the current stream of `dev`) with `dev` current."""
+    if dev.index == torch.cuda.current_device():
+        call(name, *args, stream_handle(dev))
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, stream_handle(dev))
+
+
+def _one_device(who: str, *tensors: torch.Tensor | None) -> torch.device:
+    dev = require_cuda(*tensors)
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{who}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def _cache_geometry(who: str, pages: torch.Tensor, scales: torch.Tensor | None, table: torch.Tensor) -> tuple[int, int, int, int, int]:
+    """(n_pages, h, bs, d, cache kind) of pages [n_pages, h, 2, bs, d] and their page table."""
+    if pages.dim() != 5 or pages.shape[2] != 2 or not pages.is_contiguous():
+        raise ValueError(f"{who}: pages must be a contiguous [n_pages, h, 2, block_size, head_dim], got {tuple(pages.shape)}")
+    n, h, _, bs, d = pages.shape
+    int8 = pages.dtype == torch.int8
+    if int8 and (scales is None or scales.dtype != torch.float32 or scales.shape != (n, h, 2, bs) or not scales.is_contiguous()):
+        raise ValueError(f"{who}: int8 pages need contiguous float32 scales [{n}, {h}, 2, {bs}]")
+    if not int8 and scales is not None:
+        raise ValueError(f"{who}: scales belong to int8 pages, these are {pages.dtype}")
+    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"{who}: the page table must be int32 [batch, columns] with unit column stride")
+    return n, h, bs, d, L.LKV_CACHE_INT8 if int8 else L.LKV_CACHE_MODEL
+
+
+def _per_sequence(who: str, name: str, t: torch.Tensor, batch: int) -> None:
+    if t.dtype != torch.int32 or t.shape != (batch,) or (batch > 1 and t.stride(0) != 1):
+        raise ValueError(f"{who}: {name} must be a contiguous int32 [{batch}]")
+
+
+def paged_write(keys: torch.Tensor, values: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
+                scales: torch.Tensor | None = None) -> None:
+    """Tokens keys / values [batch, T, h, d] (any strides with contiguous channels) into positions
+    starts[b] .. starts[b] + T - 1 of their sequences' pages, one launch (lkv_paged_write).
+
+    pages [n_pages, h, 2, bs, d] hold the keys' dtype, or int8 codes with scales [n_pages, h, 2, bs]: one
+    scale per token, head and key or value, the row's largest magnitude / 127. table [batch, columns]
+    int32 lists each sequence's pages; a token whose page is missing (past the table, an id outside
+    [0, n_pages)) is not written, so a batch may be padded. Two tokens must not share a row.
+    """
+    dev = _one_device("paged_write", keys, values, pages, table, starts, scales)
+    if keys.dim() != 4 or values.shape != keys.shape or values.dtype != keys.dtype:
+        raise ValueError(f"paged_write: keys and values must be alike, [batch, T, h, d]; got {tuple(keys.shape)} and {tuple(values.shape)}")
+    batch, t, h, d = keys.shape
+    n, ph, bs, pd, kind = _cache_geometry("paged_write", pages, scales, table)
+    if (ph, pd) != (h, d) or (kind == L.LKV_CACHE_MODEL and pages.dtype != keys.dtype):
+        raise ValueError(f"paged_write: {tuple(keys.shape)} {keys.dtype} tokens do not fit pages {tuple(pages.shape)} {pages.dtype}")
+    if table.shape[0] != batch or keys.stride(3) != 1 or values.stride(3) != 1:
+        raise ValueError("paged_write: one table row per sequence, and contiguous channels")
+    _per_sequence("paged_write", "starts", starts, batch)
+    _on(dev, "lkv_paged_write", keys.data_ptr(), keys.stride(0), keys.stride(1), keys.stride(2), values.data_ptr(), values.stride(0), values.stride(1),
+        values.stride(2), dtype_code(keys.dtype), batch, t, h, d, pages.data_ptr(), kind, ptr(scales), n, bs, table.data_ptr(), table.stride(0),
+        table.shape[1], starts.data_ptr())
+
+
+def paged_read(pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, n_tokens: int, lens: torch.Tensor | None = None,
+               scales: torch.Tensor | None = None, dtype: torch.dtype | None = None,
+               out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Tokens starts[b] .. starts[b] + n_tokens - 1 of every sequence, read back as (keys, values)
+    [batch, n_tokens, h, d], one launch (lkv_paged_read): code * scale rounded once to `dtype` (bfloat16
+    by default; model-dtype pages are copied). Tokens at or past lens[b] (int32 [batch], optional) and
+    tokens without a page are zeros.
+    """
+    dev = _one_device("paged_read", pages, table, starts, lens, scales)
+    n, h, bs, d, kind = _cache_geometry("paged_read", pages, scales, table)
+    batch = table.shape[0]
+    if dtype is None:
+        dtype = pages.dtype if kind == L.LKV_CACHE_MODEL else torch.bfloat16
+    if kind == L.LKV_CACHE_MODEL and dtype != pages.dtype:
+        raise ValueError(f"paged_read: {pages.dtype} pages are read back as {pages.dtype}, not {dtype}")
+    if n_tokens < 0:
+        raise ValueError(f"paged_read: {n_tokens} tokens")
+    _per_sequence("paged_read", "starts", starts, batch)
+    if lens is not None:
+        _per_sequence("paged_read", "lens", lens, batch)
+    shape = (batch, n_tokens, h, d)
+    if out is None:
+        out = (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
+    for o in out:
+        if o.shape != shape or o.dtype != dtype or o.device != dev or not o.is_contiguous():
+            raise ValueError(f"paged_read: out must be two contiguous {dtype} {shape} on {dev}")
+    _on(dev, "lkv_paged_read", pages.data_ptr(), kind, ptr(scales), n, bs, batch, n_tokens, h, d, table.data_ptr(), table.stride(0), table.shape[1],
+        starts.data_ptr(), ptr(lens), out[0].data_ptr(), out[1].data_ptr(), dtype_code(dtype))
+    return out
+
+
+def prefix_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, prefix_table: torch.Tensor, prefix_len: int,
+                     scale: float, scales: torch.Tensor | None = None, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+                     lse: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention of query [batch, T, hq, d] (bfloat16) for a batch that shares a prefix, whose pages are
+    read once for all (lkv_prefix_attention, two launches). Query t of sequence b attends the prefix_len
+    tokens of the pages that prefix_table [columns] lists, and the first lens[b] - T + t + 1 of its own
+    lens[b] tokens in the pages of table[b]: the step's T tokens (drafted ones included) are written
+    before the call and are the last of lens[b].
+
+    pages are bfloat16 or int8 with scales (paged_write). Returns (out [batch, T, hq, d] in `out_dtype`,
+    bfloat16 by default, lse [batch, T, hq] float32); a row that attends nothing (no prefix, no own token,
+    all pages missing) gets out = 0 and lse = -inf. lens and both tables are read on the device, so a
+    captured graph follows them as they change; prefix_len and the shapes are fixed at capture.
+    The partials' workspace comes from torch's allocator call by call, so calls on several streams and
+    several captured graphs do not share it.
+    """
+    dev = _one_device("prefix_attention", query, pages, table, lens, prefix_table, scales, out, lse)
+    if query.dim() != 4 or query.dtype != torch.bfloat16:
+        raise ValueError(f"prefix_attention: query must be bfloat16 [batch, T, hq, d], got {query.dtype} {tuple(query.shape)}")
+    batch, t, hq, d = query.shape
+    n, h, bs, pd, kind = _cache_geometry("prefix_attention", pages, scales, table)
+    if pd != d or hq % h or table.shape[0] != batch or (kind == L.LKV_CACHE_MODEL and pages.dtype != torch.bfloat16):
+        raise ValueError(f"prefix_attention: query {tuple(query.shape)} and table {tuple(table.shape)} do not fit {pages.dtype} pages {tuple(pages.shape)}")
+    _per_sequence("prefix_attention", "lens", lens, batch)
+    cols = prefix_table.numel()
+    if prefix_table.dtype != torch.int32 or prefix_table.dim() != 1 or (cols > 1 and prefix_table.stride(0) != 1) or not 0 <= prefix_len <= cols * bs:
+        raise ValueError(f"prefix_attention: prefix_table must be a contiguous int32 [columns] holding the {prefix_len} tokens of the prefix")
+    if query.stride(3) != 1 or query.stride(0) % 8 or query.stride(1) % 8 or query.stride(2) % 8 or query.data_ptr() % 16:
+        query = query.clone(memory_format=torch.contiguous_format)
+    if out is None:
+        out = torch.empty((batch, t, hq, d), dtype=out_dtype or torch.bfloat16, device=dev)
+    elif out.shape != query.shape or not out.is_contiguous() or out.dtype != (out_dtype or out.dtype):
+        raise ValueError(f"prefix_attention: out must be a contiguous {tuple(query.shape)}")
+    if lse is None:
+        lse = torch.empty((batch, t, hq), dtype=torch.float32, device=dev)
+    elif lse.shape != (batch, t, hq) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise ValueError(f"prefix_attention: lse must be a contiguous float32 {(batch, t, hq)}")
+    nbytes = L.lib().lkv_prefix_attention_workspace(batch, t, hq, h, d, prefix_len)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    args = L.PrefixArgs(query.data_ptr(), L.LKV_BF16, query.stride(0), query.stride(1), query.stride(2), pages.data_ptr(), kind, ptr(scales), n, bs,
+                        batch, t, hq, h, d, table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(), prefix_table.data_ptr(), cols,
+                        prefix_len, scale, out.data_ptr(), dtype_code(out.dtype), lse.data_ptr(), ptr(ws), nbytes)
+    _on(dev, "lkv_prefix_attention", ctypes.byref(args))
+    return out, lse
+
+
+def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torch.Tensor, uniforms: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Which of k drafted tokens per sequence are kept, and the token that follows them (one launch,
+    lkv_verify_drafts). target [batch, k + 1, vocab] and draft [batch, k, vocab] are float32
+    probabilities (draft None: a draft that proposed its token with certainty), tokens [batch, k] int64,
+    uniforms [batch, k + 1] float32 in [0, 1).
+
+    Token i is kept while uniforms_i * draft_i(x_i) < target_i(x_i). After a rejection at n the next token
+    is drawn from max(target_n - draft_n, 0), after k kept tokens from target_k, by inverting the
+    cumulative sum at uniforms_k: kept tokens and drawn token are distributed as the target's own samples.
+    A token outside [0, vocab) (say -1) ends its sequence's drafts, and the next one is drawn from the
+    target there. Returns (kept [batch] int32, token [batch] int64); token is -1 where the weights are all
+    zero or have no finite sum.
+    """
+    dev = _one_device("verify_drafts", target, draft, tokens, uniforms)
+    if target.dim() != 3 or tokens.dim() != 2:
+        raise ValueError("verify_drafts: target must be [batch, k + 1, vocab] and tokens [batch, k]")
+    batch, k = tokens.shape
+    vocab = target.shape[2]
+    if target.shape[:2] != (batch, k + 1) or uniforms.shape != (batch, k + 1) or (draft is not None and draft.shape != (batch, k, vocab)):
+        raise ValueError(f"verify_drafts: {k} tokens drafted for {batch} sequences do not fit target {tuple(target.shape)}, uniforms "
+                         f"{tuple(uniforms.shape)}, draft {None if draft is None else tuple(draft.shape)}")
+    if target.dtype != torch.float32 or uniforms.dtype != torch.float32 or tokens.dtype != torch.int64 or (draft is not None and draft.dtype != torch.float32):
+        raise ValueError("verify_drafts: probabilities and uniforms are float32, tokens int64")
+    for t in (target, draft, tokens, uniforms):
+        if t is not None and t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError("verify_drafts: rows must be contiguous")
+    kept = torch.empty((batch,), dtype=torch.int32, device=dev)
+    token = torch.empty((batch,), dtype=torch.int64, device=dev)
+    _on(dev, "lkv_verify_drafts", target.data_ptr(), target.stride(0), target.stride(1), ptr(draft), 0 if draft is None else draft.stride(0),
+        0 if draft is None else draft.stride(1), tokens.data_ptr(), tokens.stride(0), uniforms.data_ptr(), uniforms.stride(0), batch, k, vocab,
+        kept.data_ptr(), token.data_ptr())
+    return kept, token
