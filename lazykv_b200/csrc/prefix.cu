@@ -10,7 +10,8 @@
 // The second launch starts under the first (programmatic dependent launch) and waits for it only before
 // it folds.
 //
-// stream_kernel does the second launch, and the first where the batch has few rows: each warp takes a
+// prefix_tile.cu does the first launch. stream_kernel does the second, and the first where the batch has
+// few rows: each warp takes a
 // tile of 16 rows through its share of the tokens with mma.sync.m16n8k16 (bf16 operands, float32
 // accumulators). A lane copies by cp.async exactly the bytes that it will hold as mma fragments, into
 // slots of shared memory of its own, so the pipeline needs no barrier and no bank conflicts arise; the
@@ -517,9 +518,13 @@ cudaError_t launch_stream(const Params& p, dim3 grid, int cluster, int n_ctas, c
   return launch_pdl(k, grid, dim3(kThreads), kSmem, st, cluster, p, n_ctas);
 }
 
+// Batches of at most this many rows per KV head take the prefix through stream_kernel, one row tile.
+bool streams(int rows) { return rows <= kRows; }
+
 // Splits of the prefix: enough CTAs for two on each SM, no split shorter than two stages per warp.
 int prefix_splits(int rows, int h, int64_t prefix_len, int d) {
   if (prefix_len <= 0) return 0;
+  if (!streams(rows)) return tile_splits(rows, h, prefix_len);
   const int tok = stage_tokens(d);
   const int64_t tiles = (rows + kRows - 1) / kRows, most = (prefix_len + 2 * kWarps * tok - 1) / (2 * kWarps * tok);
   int64_t n = (2 * kNumSMs) / (tiles * h);
@@ -599,7 +604,9 @@ int lkv_prefix_attention(const lkv_prefix_args* a, void* stream) {
   cudaStream_t st = as_stream(stream);
   const bool int8 = a->kind == LKV_CACHE_INT8, wide = a->d == 128;
   cudaError_t e = cudaSuccess;
-  if (p.n_splits > 0) {
+  if (p.n_splits > 0 && !streams(p.rows)) {
+    if (int rc = run_tiles(p, a->d, int8, st)) return rc;
+  } else if (p.n_splits > 0) {
     const int tiles = (p.rows + kRows - 1) / kRows;
     if (p.n_splits > 65535) return fail(LKV_ERR_ARG, "%s: prefix too long", who);
     const dim3 grid(tiles, p.n_splits, a->h);

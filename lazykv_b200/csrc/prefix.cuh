@@ -62,5 +62,9 @@ __device__ __forceinline__ int page_at(const int32_t* table, int cols, int n_pag
   return id < n_pages ? id : -1;
 }
 
+// prefix_tile.cu: the prefix's partials for many rows, and how many splits of the prefix they take.
+int tile_splits(int rows, int h, int64_t prefix_len);
+int run_tiles(const Params& p, int d, bool int8, cudaStream_t st);
+
 }  // namespace prefix
 }  // namespace lkv

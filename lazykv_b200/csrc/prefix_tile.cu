@@ -1,0 +1,787 @@
+// The prefix's part of the shared-prefix attention for batches of many rows, on the 5th-generation
+// tensor cores.
+//
+// A CTA holds up to 256 query rows of one KV head as two tiles of 128 and takes a chunk of the prefix
+// through them, 128 tokens at a time. Per tile of rows: S = Q K^T (tcgen05.mma, both operands in shared
+// memory, S in tensor memory), one thread per row turns its 128 scores into weights (running maximum and
+// sum in registers, float32), writes them back as 16-bit P over S, and O += P V (P read from tensor
+// memory, V from shared memory) accumulates in tensor memory. The two tiles alternate, so that one
+// computes weights while the tensor core works for the other. With 128 rows or fewer both tiles are the
+// same queries and take the prefix's tiles in turn; their results are merged at the end. Each CTA writes
+// one partial (m, l, o) per row, which stream_kernel (prefix.cu) folds into the output.
+//
+// Warps 0-3 and 4-7 are the two tiles' rows, warp 8 issues the matrix products, warp 9 the copies; with
+// int8 pages warps 12-15 turn codes into f16 operands. All of it is joined by mbarriers, every wait
+// bounded (tma.cuh).
+//
+// bf16 pages: P and V are bf16; the pages come by tensor-map TMA straight into the swizzled operand
+// layout (a page that is missing as a row past the tensor's end, that is as zeros).
+// int8 pages: codes are exact in f16, and so is a query row after a power of two that brings its largest
+// element to [1, 2) (smaller ones lose bits below 2^-25 of it). A key's scale multiplies its column of
+// scores in float32. A value's scale multiplies the weight before the rounding to f16: with 2^E the
+// least power of two not below any scale of the tile, the reference that weights are taken from is
+// m + E - 7 instead of m, which keeps weight x scale within 2^15 (the reference may lag by 2^8 before
+// the accumulator is rescaled) and its last bit at 2^-24, 2^-31 of the largest weight: 11 bits for every
+// weight that counts, against the 8 of bf16.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "prefix.cuh"
+#include "tma.cuh"
+
+namespace lkv {
+namespace prefix {
+namespace {
+
+constexpr int kTile = 128;       // rows of a tile of queries, tokens of a tile of the prefix
+constexpr int kInfo = 8;         // tiles whose scales and page bits are kept (see the producer)
+constexpr int kLag = 8;          // powers of two that the reference may lag behind the maximum
+
+template <int D, bool INT8>
+struct Tiles {
+  static constexpr int kHalves = D / 64;                 // 64 channels (128 bytes) per swizzled column
+  static constexpr int kHalfBytes = kTile * 128;
+  static constexpr int kBytes = kHalves * kHalfBytes;    // one operand tile
+  static constexpr int kStages = INT8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8);
+  static constexpr int kRawBytes = INT8 ? kTile * D : 0; // one tile of codes
+  static constexpr int kRaw = INT8 ? 3 : 0;
+  static constexpr int kThreads = INT8 ? 512 : 384;      // four warpgroups, or three
+  // Registers per thread, of the launch's 65,536 / kThreads (128, or 168): the warpgroups that compute
+  // weights take what the others leave, 256 x kMany + (kThreads - 256) x kFew = kThreads x the launch's.
+  static constexpr int kMany = INT8 ? 168 : 208, kFew = 88;
+  static_assert(256 * kMany + (kThreads - 256) * kFew == kThreads * (INT8 ? 128 : 168), "the register split is the launch's own");
+  static constexpr int kScaleBytes = INT8 ? kInfo * 2 * kTile * 4 : 0;
+  static constexpr int kSmem = 2 * kBytes + kStages * kBytes + kRaw * kRawBytes + kScaleBytes + 1024;
+};
+
+struct Barriers {
+  uint64_t q_full, o_full[2], s_full[2], p_full[2], tail, drain;
+  uint64_t full[8], empty[8], raw_full[3], raw_empty[3], info[kInfo];
+  uint32_t have[kInfo][4];   // together, bit g: tokens 16 g .. 16 g + 15 of the tile have a page
+  int32_t top[kInfo][4];     // largest exponent of a finite value scale, per warp of converters
+  float back[2][kTile];      // int8: what a row's scores are multiplied with (stage_query)
+  uint32_t tmem;
+  int quit;
+};
+
+// Waits for the phase of `bar` with the given parity, two seconds at most, or until another role gave up.
+// Without a suspend-time hint: the waits here are short and many, and a hinted one was seen to resume late.
+constexpr uint64_t kMaxWaitNs = 2000000000ull;
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ bool try_once(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(done)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool wait_long(Barriers& s, uint64_t* bar, uint32_t parity) {
+  const uint64_t from = now_ns();
+  while (!try_once(bar, parity)) {
+    if (*static_cast<volatile int*>(&s.quit)) return false;
+    if (now_ns() - from > kMaxWaitNs) {
+      *static_cast<volatile int*>(&s.quit) = 1;
+      record_status(LKV_DEV_WAIT_TIMEOUT);
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ bool wait_for(Barriers& s, uint64_t* bar, uint32_t parity) { return try_once(bar, parity) || wait_long(s, bar, parity); }
+
+// One arrival for the warp, after what all of its lanes did before.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+
+// Packed float32 pairs.
+__device__ __forceinline__ uint64_t pair(float a, float b) { return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32); }
+__device__ __forceinline__ float first_of(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float second_of(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// Shared-memory operand descriptors, 128-byte swizzle: rows of 128 bytes, eight of them an atom of 1 KB.
+// K-major (Q, K): atoms of eight rows 1 KB apart. MN-major (V: rows are tokens, the product's K): atoms of
+// eight tokens 1 KB apart, the next 64 channels a half tile further.
+__device__ __forceinline__ uint64_t desc_of(uint32_t addr, uint32_t leading) {
+  return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// kind::f16 instruction descriptor: float32 accumulator, M = 128, both operands f16 or both bf16.
+template <bool F16>
+constexpr uint32_t instruction(int n, bool b_mn_major) {
+  return (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+
+// The whole warp comes here with the same operands, so that they are computed in uniform registers, and
+// the lane that elect() chose issues (issued by one thread of a diverged warp, each product took 80 to
+// 100 cycles of moves to uniform registers).
+__device__ __forceinline__ uint32_t elect() {
+  uint32_t mine;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(mine));
+  return mine;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t inst, bool add, uint32_t mine) {
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+               "l"(a), "l"(b), "r"(inst), "r"((uint32_t)add), "r"(mine)
+               : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t inst, bool add, uint32_t mine) {
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+               "r"(a), "l"(b), "r"(inst), "r"((uint32_t)add), "r"(mine)
+               : "memory");
+}
+// Arrives on `bar` when every product issued so far is done.
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t mine) {
+  asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(
+                   smem_u32(bar)),
+               "r"(mine)
+               : "memory");
+}
+
+#define LKV_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define LKV_S8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+
+// Tensor memory is read and written in the shape of mma fragments: lane (g, c) = (lane / 4, lane % 4) of
+// a warp holds rows g + 8 i of the warp's 32 (i = 0 .. 3) and columns 8 k + 2 c, 8 k + 2 c + 1. A thread
+// then needs the scales of a quarter of the columns, each for four rows; with a thread per row every
+// scale is a broadcast to every thread, and shared memory's return path was the bound (three
+// broadcasts of 128 floats per row and tile).
+//
+// 16 columns of the 32 rows: word 4 k + e of rows 16 h ..: column group k, rows g (e < 2) and g + 8.
+struct Frag {
+  uint32_t v[2][8];
+};
+// In flight until ld_wait.
+__device__ __forceinline__ void ld(Frag& f, uint32_t addr) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : LKV_R8(f.v[h], 0) : "r"(addr + (h << 20)));
+}
+// The registers pass through the wait, so that no use of them is scheduled before it.
+__device__ __forceinline__ void ld_wait(Frag& f) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(f.v[i / 8][i % 8]));
+}
+__device__ __forceinline__ void st(uint32_t addr, const Frag& f) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr + (h << 20)), LKV_S8(f.v[h], 0) : "memory");
+}
+// The 16 columns packed to 8 words of two: word 2 k + e: column group k, rows g and g + 8.
+__device__ __forceinline__ void st_packed(uint32_t addr, const uint32_t (&w)[2][4]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr + (h << 20)), "r"(w[h][0]), "r"(w[h][1]), "r"(w[h][2]),
+                 "r"(w[h][3])
+                 : "memory");
+}
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 b = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// Four int8 codes as f16, exactly: byte b with its sign bit turned is u = code + 128, and 0x6400 | u is
+// 1024 + u.
+__device__ __forceinline__ uint2 codes_to_f16(uint32_t w) {
+  const uint32_t u = w ^ 0x80808080u, a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+  const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+// This thread's query row into its place of the operand tile; returns what its scores have to be
+// multiplied with for int8 pages (a power of two). `flip`: negated (a negative softmax scale).
+template <int D, bool INT8>
+__device__ __forceinline__ float stage_query(const __nv_bfloat16* row, char* tile, int r, bool write, uint32_t flip) {
+  uint4 w[D / 8];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) {
+    w[i] = row != nullptr ? reinterpret_cast<const uint4*>(row)[i] : make_uint4(0, 0, 0, 0);
+    w[i].x ^= flip, w[i].y ^= flip, w[i].z ^= flip, w[i].w ^= flip;
+  }
+  float back = 1.0f;
+  if constexpr (INT8) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = max(top, max(x[k] & 0x7fffu, (x[k] >> 16) & 0x7fffu));
+    }
+    // The exponent e of the largest magnitude, kept where both 2^-e and 2^e are normal numbers. An
+    // infinity or NaN is what it is at any scale.
+    int e = (int)(top >> 7) - 127;
+    e = e > 126 ? 126 : e < -126 ? -126 : e;
+    const float down = __int_as_float((127 - e) << 23);
+    back = __int_as_float((127 + e) << 23);
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = pack_f16(__uint_as_float(x[k] << 16) * down, __uint_as_float(x[k] & 0xffff0000u) * down);
+      w[i] = make_uint4(x[0], x[1], x[2], x[3]);
+    }
+  }
+  if (write) {
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(tile + (i / 8) * (kTile * 128) + r * 128 + (((i % 8) ^ (r & 7)) << 4)) = w[i];
+  }
+  return back;
+}
+
+template <int D, bool INT8>
+__global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kernel(const Params p, const __grid_constant__ CUtensorMap pages_map, int chunk) {
+  using T = Tiles<D, INT8>;
+  extern __shared__ char raw_smem[];
+  __shared__ Barriers s;
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  char* q_tiles = smem;
+  char* stages = q_tiles + 2 * T::kBytes;
+  char* raws = stages + T::kStages * T::kBytes;
+  float* scale_ring = reinterpret_cast<float*>(raws + T::kRaw * T::kRawBytes);  // [kInfo][2][kTile]: keys', values'
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int split = blockIdx.x, j = blockIdx.y, row0 = blockIdx.z * 2 * kTile;
+  const int n_rows = min(2 * kTile, p.rows - row0);
+  const bool two = n_rows > kTile;
+  const int first = split * chunk;                                               // this CTA's tiles of the prefix
+  const int n_tiles = min(chunk, (p.prefix_len + kTile - 1) / kTile - first);
+  const int n_jobs = two ? 2 * n_tiles : n_tiles;                                // job i: rows i % 2, tile two ? i / 2 : i
+  const int end = p.prefix_len - first * kTile;                                  // tokens from the chunk's start on
+  if (tid == 0) {
+    mbar_init(&s.q_full, 8);
+    mbar_init(&s.tail, 1);
+    mbar_init(&s.drain, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.o_full[i], 1);
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], 4);
+    }
+    for (int i = 0; i < T::kStages; ++i) {
+      mbar_init(&s.full[i], INT8 ? 4 : 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < T::kRaw; ++i) {
+      mbar_init(&s.raw_full[i], 1);
+      mbar_init(&s.raw_empty[i], 4);
+    }
+    for (int i = 0; i < kInfo; ++i) mbar_init(&s.info[i], INT8 ? 4 : 1);
+    s.quit = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = s.tmem;  // columns: S or P of the two row tiles at 0 and 128, O at 256 and 256 + D
+  pdl_wait();
+  pdl_release();
+
+  if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kMany));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kFew));
+  if (warp < 8) {
+    // ---- weights: a warp has 32 rows, a thread four of them (Frag) -----------------------------------
+    const int u = warp / 4, g = lane / 4, c2 = 2 * (lane % 4);
+    const int base = (two ? u * kTile : 0) + (warp % 4) * 32 + g;  // this thread's rows: base + 8 i
+    const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
+    {
+      const int r = tid % kTile, row = two ? u * kTile + r : r;
+      const __nv_bfloat16* src = nullptr;
+      if (row < n_rows) {
+        const int x = row0 + row, gr = x % p.group, bt = x / p.group;
+        src = p.q + (int64_t)(bt / p.tokens) * p.q_sb + (int64_t)(bt % p.tokens) * p.q_st + (int64_t)(j * p.group + gr) * p.q_sh;
+      }
+      const float back = stage_query<D, INT8>(src, q_tiles + (two ? u * T::kBytes : 0), r, two || u == 0, sign < 0.0f ? 0x80008000u : 0u);
+      if (INT8) s.back[u][r] = back;
+      fence_async();
+      warp_arrive(&s.q_full, lane);
+    }
+    float scale[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) scale[i] = p.scale_log2 * sign * (INT8 ? s.back[u][(warp % 4) * 32 + g + 8 * i] : 1.0f);  // this warp's own rows
+    const uint32_t lanes = (uint32_t)(warp % 4) << 21;  // lane 32 (warp % 4) of tensor memory
+    const uint32_t ts = tmem + lanes + u * kTile, to = tmem + lanes + 2 * kTile + u * D;
+    const bool any_live = base - g < n_rows;  // does this warp hold a row at all
+    float from[4], l[4];                      // per row: the reference that weights are taken from (log2 domain), their sum
+#pragma unroll
+    for (int i = 0; i < 4; ++i) from[i] = -INFINITY, l[i] = 0.0f;
+    bool ok = true;
+    int n_done = 0;
+    for (int i = u; i < n_jobs; i += 2, ++n_done) {
+      const int t = two ? i >> 1 : i, slot = t % kInfo;
+      ok = wait_for(s, &s.info[slot], (t / kInfo) & 1) && wait_for(s, &s.s_full[u], n_done & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_after();
+      if (any_live) {
+        const uint32_t have = (s.have[slot][0] | s.have[slot][1]) | (s.have[slot][2] | s.have[slot][3]);
+        const int seen = end - t * kTile;  // tokens of this tile inside the prefix
+        [[maybe_unused]] const uint64_t* ks = reinterpret_cast<const uint64_t*>(scale_ring + slot * 2 * kTile + c2);  // pair 4 k: columns 8 k + c2, + 1
+        [[maybe_unused]] const uint64_t* vs = ks + kTile / 2;
+        auto weigh = [&](auto masked) {
+          constexpr bool kMasked = decltype(masked)::value;
+          constexpr int N = kTile / 16;
+          auto sees = [&](int x) { return !kMasked || (x < seen && ((have >> (x / 16)) & 1)); };
+          Frag f[2];
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          ld(f[0], ts);
+          ld_wait(f[0]);
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            if (n + 1 < N) ld(f[(n + 1) & 1], ts + 16 * (n + 1));
+            const Frag& a = f[n & 1];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              [[maybe_unused]] uint64_t kk = 0;
+              if constexpr (INT8) kk = ks[4 * (2 * n + k)];
+              const bool s0 = sees(16 * n + 8 * k + c2), s1 = sees(16 * n + 8 * k + c2 + 1);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                uint64_t z = pair(__uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1)]), __uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1) + 1]));
+                if constexpr (INT8) z = mul2(z, kk);
+                if constexpr (kMasked) {
+                  if (s0) top[r] = fmaxf(top[r], first_of(z));
+                  if (s1) top[r] = fmaxf(top[r], second_of(z));
+                } else {
+                  top[r] = fmaxf(fmaxf(top[r], first_of(z)), second_of(z));
+                }
+              }
+            }
+            if (n + 1 < N) ld_wait(f[(n + 1) & 1]);
+          }
+          ld(f[0], ts);  // the first columns again, while the reference is found
+          float e = 0.0f;
+          if constexpr (INT8) e = (float)(max(max(s.top[slot][0], s.top[slot][1]), max(s.top[slot][2], s.top[slot][3])) - 7);
+          float want[4];
+          bool move = false;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+            want[r] = top[r] == -INFINITY ? -INFINITY : fmaf(top[r], scale[r], e);
+            move = move || want[r] > from[r] + kLag || (from[r] == -INFINITY && want[r] > from[r]);
+          }
+          if (__any_sync(0xffffffffu, move)) {
+            float by[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float to_ref = fmaxf(from[r], want[r]);
+              by[r] = to_ref == -INFINITY ? 1.0f : ex2(from[r] - to_ref);
+              from[r] = to_ref;
+              l[r] *= by[r];
+            }
+            if (n_done > 0) {  // the products of this row tile's last job are done: its scores came after them
+#pragma unroll 1
+              for (int n = 0; n < D / 16; ++n) {
+                ld(f[1], to + 16 * n);
+                ld_wait(f[1]);
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                  uint32_t& w = f[1].v[x / 8][x % 8];
+                  w = __float_as_uint(__uint_as_float(w) * by[2 * (x / 8) + (x % 4) / 2]);
+                }
+                st(to + 16 * n, f[1]);
+              }
+            }
+          }
+          uint64_t ref[4], scale2[4], sum[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float x = from[r] == -INFINITY ? 0.0f : -from[r];
+            ref[r] = pair(x, x), scale2[r] = pair(scale[r], scale[r]);
+          }
+          ld_wait(f[0]);
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            if (n + 1 < N) ld(f[(n + 1) & 1], ts + 16 * (n + 1));
+            const Frag& a = f[n & 1];
+            uint32_t w[2][4];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              [[maybe_unused]] uint64_t kk = 0, vv = 0;
+              if constexpr (INT8) kk = ks[4 * (2 * n + k)], vv = vs[4 * (2 * n + k)];
+              const bool s0 = sees(16 * n + 8 * k + c2), s1 = sees(16 * n + 8 * k + c2 + 1);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                uint64_t z = pair(__uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1)]), __uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1) + 1]));
+                if constexpr (INT8) z = mul2(z, kk);
+                z = fma2(z, scale2[r], ref[r]);
+                z = pair(s0 ? ex2(first_of(z)) : 0.0f, s1 ? ex2(second_of(z)) : 0.0f);
+                sum[r] = add2(sum[r], z);
+                if constexpr (INT8) z = mul2(z, vv);
+                w[r / 2][2 * k + (r & 1)] = INT8 ? pack_f16(first_of(z), second_of(z)) : pack_bf16(first_of(z), second_of(z));
+              }
+            }
+            if (n + 1 < N) ld_wait(f[(n + 1) & 1]);
+            st_packed(ts + 8 * n, w);  // over scores that have been read
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) l[r] += first_of(sum[r]) + second_of(sum[r]);
+        };
+        if (have != 0xffu || seen < kTile) weigh(std::true_type{});
+        else weigh(std::false_type{});
+        st_wait();
+      }
+      tc_before();
+      warp_arrive(&s.p_full[u], lane);
+    }
+    // ---- the rows' partials -------------------------------------------------------------------------
+    const bool any_job = n_done > 0;
+    if (ok && any_job) ok = wait_for(s, &s.o_full[u], 0);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_after();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    }
+    const int64_t at = ((int64_t)split * p.h + j) * p.rows + row0 + base;  // row i: at + 8 i
+    constexpr int kLd = D + 8;  // a row of the hand-over
+    float* swap = reinterpret_cast<float*>(stages);
+    float2* swap_ml = reinterpret_cast<float2*>(swap + kTile * kLd);
+    float f0[4] = {1.f, 1.f, 1.f, 1.f}, f1[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!two) {
+      // Both row tiles hold the same rows: the second hands its part over in shared memory. The stages are
+      // free: every product that read them is done once both have passed o_full.
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (u == 1 && any_live) {
+#pragma unroll 1
+        for (int n = 0; n < D / 16; ++n) {
+          Frag f;
+          if (any_job) {
+            ld(f, to + 16 * n);
+            ld_wait(f);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) f.v[x / 8][x % 8] = 0;
+          }
+#pragma unroll
+          for (int x = 0; x < 8; ++x)  // x = 4 k + i: column group k, row i
+            *reinterpret_cast<uint2*>(swap + (base + 8 * (x % 4)) * kLd + 16 * n + 8 * (x / 4) + c2) =
+                make_uint2(f.v[(x % 4) / 2][4 * (x / 4) + 2 * (x & 1)], f.v[(x % 4) / 2][4 * (x / 4) + 2 * (x & 1) + 1]);
+        }
+        if (c2 == 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) swap_ml[base + 8 * i] = make_float2(from[i], l[i]);
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (u == 0 && any_live) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 other = swap_ml[base + 8 * i];
+          const float both = fmaxf(from[i], other.x), ref = both == -INFINITY ? 0.0f : both;
+          f0[i] = ex2(from[i] - ref), f1[i] = ex2(other.x - ref);
+          from[i] = both;
+          l[i] = l[i] * f0[i] + other.y * f1[i];
+        }
+      }
+    }
+    if ((two || u == 0) && any_live) {
+#pragma unroll 1
+      for (int n = 0; n < D / 16; ++n) {
+        Frag f;
+        ld(f, to + 16 * n);
+        ld_wait(f);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int i = x % 4, ch = 16 * n + 8 * (x / 4) + c2;
+          float2 o = make_float2(__uint_as_float(f.v[i / 2][4 * (x / 4) + 2 * (i & 1)]), __uint_as_float(f.v[i / 2][4 * (x / 4) + 2 * (i & 1) + 1]));
+          if (!two) {
+            const float2 other = *reinterpret_cast<const float2*>(swap + (base + 8 * i) * kLd + ch);
+            o.x = o.x * f0[i] + other.x * f1[i], o.y = o.y * f0[i] + other.y * f1[i];
+          }
+          if (base + 8 * i < n_rows) *reinterpret_cast<float2*>(p.part_o + (at + 8 * i) * D + ch) = o;
+        }
+      }
+      ok = ok && *static_cast<volatile int*>(&s.quit) == 0;
+      // Where a wait ran out the row is poisoned (its status word tells why).
+      if (c2 == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (base + 8 * i < n_rows) p.part_ml[at + 8 * i] = ok ? make_float2(from[i], l[i]) : make_float2(0.0f, __uint_as_float(0x7fc00000u));
+      }
+    }
+    tc_before();
+  } else if (warp == 8) {
+    // ---- matrix products: issued by one lane, in order -----------------------------------------------
+    constexpr uint32_t kQk = instruction<INT8>(kTile, false), kPv = instruction<INT8>(D, true);
+    const uint32_t q_u = smem_u32(q_tiles), st_u = smem_u32(stages), mine = elect(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_for(s, bar, parity)) != 0; };
+    auto qk = [&](int i) {
+      const int t = two ? i >> 1 : i, u = i & 1, n = 2 * t, slot = n % T::kStages;
+      if ((!two || u == 0) && !wait_all(&s.full[slot], (n / T::kStages) & 1)) return false;
+      tc_after();
+      const uint64_t a = desc_of(q_u + (two ? u * T::kBytes : 0), 16), b = desc_of(st_u + slot * T::kBytes, 16);
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {  // 16 channels further: 32 bytes, in units of 16
+        const uint64_t step = ((x / 4) * T::kHalfBytes + (x % 4) * 32) / 16;
+        mma_ss(tm + u * kTile, a + step, b + step, kQk, x > 0, mine);
+      }
+      commit(&s.s_full[u], mine);
+      if (!two || u == 1) commit(&s.empty[slot], mine);
+      return true;
+    };
+    auto pv = [&](int i) {
+      const int t = two ? i >> 1 : i, u = i & 1, n = 2 * t + 1, slot = n % T::kStages;
+      if (!wait_all(&s.p_full[u], (i >> 1) & 1)) return false;
+      if ((!two || u == 0) && !wait_all(&s.full[slot], (n / T::kStages) & 1)) return false;
+      if (!INT8 && end - t * kTile < kTile && (!two || u == 0) && !wait_all(&s.tail, 0)) return false;
+      tc_after();
+      const uint64_t b = desc_of(st_u + slot * T::kBytes, T::kHalfBytes);
+#pragma unroll
+      for (int x = 0; x < kTile / 16; ++x)  // 16 tokens further: 2 KB of V, 8 columns of P
+        mma_ts(tm + 2 * kTile + u * D, tm + u * kTile + 8 * x, b + x * (2048 / 16), kPv, x > 0 || i > 1, mine);
+      if (!two || u == 1) commit(&s.empty[slot], mine);
+      if (i + 2 >= n_jobs) commit(&s.o_full[u], mine);
+      return true;
+    };
+    bool ok = wait_all(&s.q_full, 0);
+    for (int i = 0; ok && i < 2 && i < n_jobs; ++i) ok = qk(i);
+    for (int i = 0; ok && i < n_jobs; ++i) {
+      ok = pv(i);
+      if (ok && i + 2 < n_jobs) ok = qk(i + 2);
+    }
+    if (!ok) {  // nothing is freed under a product in flight
+      commit(&s.drain, mine);
+      mbar_wait(&s.drain, 0);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // ---- copies: the pages of one operand tile at a time, keys then values ----------------------------
+    // An entry of the info ring is written again kInfo tiles later. The keys of that tile need a stage
+    // that the keys of a tile at most kStages / 2 + 1 earlier have left, and those products follow the
+    // weights of all but the two jobs before them: more than that many tiles lie between.
+    const int bs = 1 << p.page_shift, per = kTile >> p.page_shift;  // pages per tile
+    int filled = 0;
+    bool ok = true;
+    for (int n = 0; ok && n < 2 * n_tiles; ++n) {
+      const int t = n >> 1, kv = n & 1, pos = (first + t) * kTile;
+      if constexpr (!INT8) {
+        const int slot = n % T::kStages;
+        if (n >= T::kStages) ok = wait_for(s, &s.empty[slot], (n / T::kStages - 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int tok = pos + lane * bs;
+        int page = -1;
+        if (lane < per && tok < p.prefix_len) page = page_at(p.prefix_table, p.prefix_cols, p.n_pages, tok, p.page_shift);
+        const uint32_t granules = lane < per && page >= 0 ? ((1u << (bs / 16)) - 1) << (lane * (bs / 16)) : 0u;
+        const uint32_t have = __reduce_or_sync(0xffffffffu, granules);
+        if (lane == 0) mbar_arrive_expect_tx(&s.full[slot], T::kBytes);
+        __syncwarp();
+        if (lane < per) {
+          const int rows = p.n_pages * 2 * p.h * bs;  // one past the last: zeros
+          const int y = page >= 0 ? ((page * p.h + j) * 2 + kv) * bs : rows;
+          const uint32_t dst = smem_u32(stages) + slot * T::kBytes + lane * bs * 128;
+#pragma unroll
+          for (int h2 = 0; h2 < T::kHalves; ++h2) tma_2d(dst + h2 * T::kHalfBytes, &pages_map, 64 * h2, y, &s.full[slot]);
+        }
+        filled = n + 1;
+        if (lane == 0 && kv == 0) {
+          s.have[t % kInfo][0] = have;
+          s.have[t % kInfo][1] = s.have[t % kInfo][2] = s.have[t % kInfo][3] = 0;
+          mbar_arrive(&s.info[t % kInfo]);
+        }
+        const int seen = end - t * kTile;
+        if (kv == 1 && seen < kTile) {
+          // Rows of the last page past the prefix hold anything, a NaN too, and 0 x NaN is NaN.
+          ok = wait_for(s, &s.full[slot], (n / T::kStages) & 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          for (int h2 = 0; h2 < T::kHalves; ++h2)
+            for (int x = seen * 8 + lane; x < kTile * 8; x += 32)
+              reinterpret_cast<uint4*>(stages + slot * T::kBytes + h2 * T::kHalfBytes)[x] = make_uint4(0, 0, 0, 0);
+          fence_async();
+          warp_arrive(&s.tail, lane);
+        }
+      } else {
+        const int slot = n % T::kRaw;
+        if (n >= T::kRaw) ok = wait_for(s, &s.raw_empty[slot], (n / T::kRaw - 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int tok = pos + lane * bs;
+        int page = -1;
+        if (lane < per && tok < p.prefix_len) page = page_at(p.prefix_table, p.prefix_cols, p.n_pages, tok, p.page_shift);
+        const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[slot], n_copies * bs * D);
+        __syncwarp();
+        if (page >= 0)
+          tma_load_1d(raws + slot * T::kRawBytes + lane * bs * D,
+                      static_cast<const char*>(p.pages) + (((int64_t)page * p.h + j) * 2 + kv) * ((int64_t)bs * D), bs * D, &s.raw_full[slot]);
+        filled = n + 1;
+      }
+    }
+    if (!ok) {  // no copy may land after the CTA has gone
+      constexpr int kSlots = INT8 ? T::kRaw : T::kStages;
+      for (int n = max(0, filled - kSlots); n < filled; ++n) mbar_wait(INT8 ? &s.raw_full[n % kSlots] : &s.full[n % kSlots], (n / kSlots) & 1);
+    }
+    __syncwarp();
+  } else if (warp >= 12) {
+    if constexpr (INT8) {
+      // ---- codes to f16 operands: thread i also carries token i's scales --------------------------------
+      const int i = tid - 12 * 32;
+      bool ok = true;
+      float ks = 0.0f, vs = 0.0f;
+      bool there = false;
+      auto scales_of = [&](int t) {  // looked up a tile ahead
+        ks = vs = 0.0f;
+        there = false;
+        const int pos = (first + t) * kTile + i;
+        if (t < n_tiles && pos < p.prefix_len) {
+          const int page = page_at(p.prefix_table, p.prefix_cols, p.n_pages, pos, p.page_shift), bs = 1 << p.page_shift;
+          if (page >= 0) {
+            const float* src = p.scales + (((int64_t)page * p.h + j) * 2) * bs + (pos & (bs - 1));
+            ks = src[0], vs = src[bs];
+            there = true;
+          }
+        }
+      };
+      scales_of(0);
+      for (int n = 0; n < 2 * n_tiles; ++n) {
+        const int t = n >> 1, kv = n & 1, raw = n % T::kRaw, slot = n % T::kStages;
+        ok = wait_for(s, &s.raw_full[raw], (n / T::kRaw) & 1);
+        if (ok && n >= T::kStages) ok = wait_for(s, &s.empty[slot], (n / T::kStages - 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (kv == 0) {
+          float* ring = scale_ring + (t % kInfo) * 2 * kTile;
+          ring[i] = ks;
+          ring[kTile + i] = vs;
+          // vs < 2^e, e from its exponent; what is not finite stays what it is. At least -40, so that the
+          // sum of the weights stays far from float32's end where the values are all but zero.
+          const int bits = (int)((__float_as_uint(vs) >> 23) & 0xffu);
+          const int e = bits == 0xff ? -40 : max(bits - 126, -40);
+          const int top = __reduce_max_sync(0xffffffffu, e);
+          if (lane == 0) s.top[t % kInfo][warp - 12] = top;
+          const uint32_t mask = __ballot_sync(0xffffffffu, there);
+          if (lane == 0) s.have[t % kInfo][warp - 12] = ((mask & 0xffffu) != 0 ? 1u : 0u) << (2 * (warp - 12)) | (mask >> 16 != 0 ? 2u : 0u) << (2 * (warp - 12));
+        }
+        const char* src = raws + raw * T::kRawBytes;
+        char* dst = stages + slot * T::kBytes;
+        constexpr int kPer = D / 16;  // 16-byte pieces of a token
+  #pragma unroll
+        for (int x = 0; x < kPer; ++x) {
+          // Eight lanes take 128 bytes that lie in 32 different banks, and so do the chunks they write: two
+          // tokens of different parity, of which the swizzle puts even chunks into even and odd places.
+          const int piece = x * kTile + i, swap_half = kPer == 8 ? ((piece >> 2) ^ (piece >> 3)) & 1 : 0;
+          const int tok = kPer == 8 ? (piece >> 4) * 2 + ((piece >> 2) & 1) : piece / kPer, c = kPer == 8 ? swap_half * 4 + (piece & 3) : piece % kPer;
+          const uint4 w = *reinterpret_cast<const uint4*>(src + (tok * kPer + c) * 16);
+          const uint2 a = codes_to_f16(w.x), b = codes_to_f16(w.y), d = codes_to_f16(w.z), e = codes_to_f16(w.w);
+          char* to = dst + (c / 4) * T::kHalfBytes + tok * 128;
+          const int at = (c % 4) * 2;
+          *reinterpret_cast<uint4*>(to + ((at ^ (tok & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
+          *reinterpret_cast<uint4*>(to + (((at + 1) ^ (tok & 7)) << 4)) = make_uint4(d.x, d.y, e.x, e.y);
+        }
+        fence_async();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&s.full[slot]);
+          mbar_arrive(&s.raw_empty[raw]);
+          if (kv == 0) mbar_arrive(&s.info[t % kInfo]);
+        }
+        if (kv == 0) scales_of(t + 1);
+      }
+      __syncwarp();
+    }
+  }
+  __syncthreads();
+  if (warp == 8) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+template <int D, bool INT8>
+cudaError_t launch_tile(const Params& p, const CUtensorMap& map, int chunk, cudaStream_t st) {
+  using T = Tiles<D, INT8>;
+  auto k = prefix_tile_kernel<D, INT8>;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid(p.n_splits, p.h, (p.rows + 2 * kTile - 1) / (2 * kTile));
+  return launch_pdl(k, grid, dim3(T::kThreads), T::kSmem, st, 0, p, map, chunk);
+}
+
+}  // namespace
+
+// One CTA per SM: the number of splits whose waves of CTAs take the least time, a CTA's start and end
+// counted as two tiles of the prefix.
+int tile_splits(int rows, int h, int64_t prefix_len) {
+  const int64_t tiles = (prefix_len + kTile - 1) / kTile, units = (int64_t)h * ((rows + 2 * kTile - 1) / (2 * kTile));
+  int64_t best = 0, best_cost = 0;
+  for (int64_t n = 1; n <= tiles && (n == 1 || units * n <= 4 * kNumSMs); ++n) {
+    const int64_t chunk = (tiles + n - 1) / n, cost = ((units * n + kNumSMs - 1) / kNumSMs) * (chunk + 2);
+    if (best == 0 || cost < best_cost) best = n, best_cost = cost;
+  }
+  const int64_t chunk = (tiles + best - 1) / best;
+  return (int)((tiles + chunk - 1) / chunk);
+}
+
+int run_tiles(const Params& p, int d, bool int8, cudaStream_t st) {
+  static const char* who = "lkv_prefix_attention";
+  const int tiles = (p.prefix_len + kTile - 1) / kTile, chunk = (tiles + p.n_splits - 1) / p.n_splits;
+  if ((p.rows + 2 * kTile - 1) / (2 * kTile) > 65535) return fail(LKV_ERR_ARG, "%s: too many rows", who);
+  CUtensorMap map = {};
+  if (!int8) {
+    const int bs = 1 << p.page_shift;
+    const int64_t rows = (int64_t)p.n_pages * 2 * p.h * bs;
+    if (rows > INT32_MAX) return fail(LKV_ERR_ARG, "%s: %lld rows of pages", who, (long long)rows);
+    if (rows == 0) return fail(LKV_ERR_ARG, "%s: a prefix in a cache without pages", who);
+    const cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)d * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)bs}, ones[2] = {1, 1};
+    const CUresult r = encode_tiled(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p.pages), dims, strides, box, ones,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(LKV_ERR_CUDA, "%s: the pages' tensor map was refused (%d)", who, (int)r);
+  }
+  const cudaError_t e = d == 128 ? (int8 ? launch_tile<128, true>(p, map, chunk, st) : launch_tile<128, false>(p, map, chunk, st))
+                                 : (int8 ? launch_tile<64, true>(p, map, chunk, st) : launch_tile<64, false>(p, map, chunk, st));
+  if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "%s (prefix): %s", who, cudaGetErrorString(e));
+  return LKV_OK;
+}
+
+}  // namespace prefix
+
+cudaError_t prefix_device_status(int* status, int clear) { return tu_device_status(status, clear); }
+cudaError_t prefix_status_attach(int* mirror) { return tu_status_attach(mirror); }
+
+}  // namespace lkv
