@@ -11,18 +11,18 @@
 // one partial (m, l, o) per row, which stream_kernel (prefix.cu) folds into the output.
 //
 // Warps 0-3 and 4-7 are the two tiles' rows, warp 8 issues the matrix products, warp 9 the copies; with
-// int8 pages warps 12-15 turn codes into f16 operands. All of it is joined by mbarriers, every wait
+// int8 pages warps 12-19 turn codes into f16 operands. All of it is joined by mbarriers, every wait
 // bounded (tma.cuh).
 //
 // bf16 pages: P and V are bf16; the pages come by tensor-map TMA straight into the swizzled operand
 // layout (a page that is missing as a row past the tensor's end, that is as zeros).
 // int8 pages: codes are exact in f16, and so is a query row after a power of two that brings its largest
 // element to [1, 2) (smaller ones lose bits below 2^-25 of it). A key's scale multiplies its column of
-// scores in float32. A value's scale multiplies the weight before the rounding to f16: with 2^E the
-// least power of two not below any scale of the tile, the reference that weights are taken from is
-// m + E - 7 instead of m, which keeps weight x scale within 2^15 (the reference may lag by 2^8 before
-// the accumulator is rescaled) and its last bit at 2^-24, 2^-31 of the largest weight: 11 bits for every
-// weight that counts, against the 8 of bf16.
+// scores in float32. A value's scale goes into V: code x (scale / 2^E), rounded to f16 (2^-11 relative,
+// the scale too), with 2^E the least power of two not below any scale of the tile. A weight is then
+// 2^(score - reference + E) and the reference at least the row's maximum + E - 7: weights stay below
+// 2^7 when it is set and may grow to 2^15 before it is set again, and their last bit is 2^-24: 11 bits for
+// every weight that counts, against the 8 of bf16.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -39,7 +39,9 @@ namespace {
 
 constexpr int kTile = 128;       // rows of a tile of queries, tokens of a tile of the prefix
 constexpr int kInfo = 8;         // tiles whose scales and page bits are kept (see the producer)
-constexpr int kLag = 8;          // powers of two that the reference may lag behind the maximum
+// What the sum of a thread's weights may grow to before its references are set again: every weight has to
+// be an f16; a bf16 one has float32's range, of which the accumulated values need the rest.
+constexpr float kMostF16 = 32768.0f, kMostBf16 = 1048576.0f;  // 2^15, 2^20
 
 template <int D, bool INT8>
 struct Tiles {
@@ -49,11 +51,11 @@ struct Tiles {
   static constexpr int kStages = INT8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8);
   static constexpr int kRawBytes = INT8 ? kTile * D : 0; // one tile of codes
   static constexpr int kRaw = INT8 ? 3 : 0;
-  static constexpr int kThreads = INT8 ? 512 : 384;      // four warpgroups, or three
-  // Registers per thread, of the launch's 65,536 / kThreads (128, or 168): the warpgroups that compute
-  // weights take what the others leave, 256 x kMany + (kThreads - 256) x kFew = kThreads x the launch's.
-  static constexpr int kMany = INT8 ? 168 : 208, kFew = 88;
-  static_assert(256 * kMany + (kThreads - 256) * kFew == kThreads * (INT8 ? 128 : 168), "the register split is the launch's own");
+  static constexpr int kThreads = INT8 ? 640 : 384;      // five warpgroups, or three
+  // Registers per thread: the warpgroups that compute weights take what the others leave of the launch's
+  // 96 (or 168) per thread. The split's sum stays within the launch's.
+  static constexpr int kMany = INT8 ? 160 : 208, kFew = INT8 ? 48 : 88;
+  static_assert(256 * kMany + (kThreads - 256) * kFew <= kThreads * (INT8 ? 96 : 168), "the register split is the launch's own");
   static constexpr int kScaleBytes = INT8 ? kInfo * 2 * kTile * 4 : 0;
   static constexpr int kSmem = 2 * kBytes + kStages * kBytes + kRaw * kRawBytes + kScaleBytes + 1024;
 };
@@ -97,6 +99,8 @@ __device__ __forceinline__ bool wait_long(Barriers& s, uint64_t* bar, uint32_t p
   return true;
 }
 __device__ __forceinline__ bool wait_for(Barriers& s, uint64_t* bar, uint32_t parity) { return try_once(bar, parity) || wait_long(s, bar, parity); }
+
+__device__ __forceinline__ int largest(const int32_t (&x)[4]) { return max(max(x[0], x[1]), max(x[2], x[3])); }
 
 // One arrival for the warp, after what all of its lanes did before.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
@@ -194,7 +198,7 @@ __device__ __forceinline__ void ld(Frag& f, uint32_t addr) {
 }
 // The registers pass through the wait, so that no use of them is scheduled before it.
 __device__ __forceinline__ void ld_wait(Frag& f) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;");  // (no clobber: the scales' loads may move over it)
 #pragma unroll
   for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(f.v[i / 8][i % 8]));
 }
@@ -225,6 +229,11 @@ __device__ __forceinline__ uint2 codes_to_f16(uint32_t w) {
   const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
   const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
   return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+__device__ __forceinline__ uint2 times(uint2 x, __half2 by) {
+  const __half2 a = __hmul2(*reinterpret_cast<const __half2*>(&x.x), by), b = __hmul2(*reinterpret_cast<const __half2*>(&x.y), by);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
 // This thread's query row into its place of the operand tile; returns what its scores have to be
@@ -295,14 +304,14 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       mbar_init(&s.p_full[i], 4);
     }
     for (int i = 0; i < T::kStages; ++i) {
-      mbar_init(&s.full[i], INT8 ? 4 : 1);
+      mbar_init(&s.full[i], INT8 ? 8 : 1);
       mbar_init(&s.empty[i], 1);
     }
     for (int i = 0; i < T::kRaw; ++i) {
       mbar_init(&s.raw_full[i], 1);
-      mbar_init(&s.raw_empty[i], 4);
+      mbar_init(&s.raw_empty[i], 8);
     }
-    for (int i = 0; i < kInfo; ++i) mbar_init(&s.info[i], INT8 ? 4 : 1);
+    for (int i = 0; i < kInfo; ++i) mbar_init(&s.info[i], INT8 ? 8 : 1);
     s.quit = 0;
     fence_mbar_init();
   }
@@ -345,118 +354,126 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
     float from[4], l[4];                      // per row: the reference that weights are taken from (log2 domain), their sum
 #pragma unroll
     for (int i = 0; i < 4; ++i) from[i] = -INFINITY, l[i] = 0.0f;
-    bool ok = true;
+    bool ok = true, unset = true;  // has some row no reference yet
     int n_done = 0;
     for (int i = u; i < n_jobs; i += 2, ++n_done) {
       const int t = two ? i >> 1 : i, slot = t % kInfo;
-      ok = wait_for(s, &s.info[slot], (t / kInfo) & 1) && wait_for(s, &s.s_full[u], n_done & 1);
+      ok = wait_for(s, &s.info[slot], (t / kInfo) & 1);
+      const uint32_t have = (s.have[slot][0] | s.have[slot][1]) | (s.have[slot][2] | s.have[slot][3]);
+      const int seen = end - t * kTile;  // tokens of this tile inside the prefix
+      [[maybe_unused]] const uint64_t* ks = reinterpret_cast<const uint64_t*>(scale_ring + slot * 2 * kTile + c2);  // pair 4 k: columns 8 k + c2, + 1
+      float e = 0.0f;  // int8: the exponent of the tile's largest value scale
+      if constexpr (INT8) e = (float)largest(s.top[slot]);
+      ok = ok && wait_for(s, &s.s_full[u], n_done & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_after();
       if (any_live) {
-        const uint32_t have = (s.have[slot][0] | s.have[slot][1]) | (s.have[slot][2] | s.have[slot][3]);
-        const int seen = end - t * kTile;  // tokens of this tile inside the prefix
-        [[maybe_unused]] const uint64_t* ks = reinterpret_cast<const uint64_t*>(scale_ring + slot * 2 * kTile + c2);  // pair 4 k: columns 8 k + c2, + 1
-        [[maybe_unused]] const uint64_t* vs = ks + kTile / 2;
         auto weigh = [&](auto masked) {
           constexpr bool kMasked = decltype(masked)::value;
           constexpr int N = kTile / 16;
           auto sees = [&](int x) { return !kMasked || (x < seen && ((have >> (x / 16)) & 1)); };
+          auto score = [&](const Frag& a, int k, int r) {
+            return pair(__uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1)]), __uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1) + 1]));
+          };
           Frag f[2];
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          ld(f[0], ts);
-          ld_wait(f[0]);
+          // The references that the weights need, from the tile's maxima, and what was summed so far brought to them.
+          auto set_references = [&]() {
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+            for (int n = 0; n < N; ++n) {
+              ld(f[0], ts + 16 * n);
+              ld_wait(f[0]);
 #pragma unroll
-          for (int n = 0; n < N; ++n) {
-            if (n + 1 < N) ld(f[(n + 1) & 1], ts + 16 * (n + 1));
-            const Frag& a = f[n & 1];
+              for (int k = 0; k < 2; ++k) {
+                [[maybe_unused]] uint64_t kk = 0;
+                if constexpr (INT8) kk = ks[4 * (2 * n + k)];
+                const bool s0 = sees(16 * n + 8 * k + c2), s1 = sees(16 * n + 8 * k + c2 + 1);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              [[maybe_unused]] uint64_t kk = 0;
-              if constexpr (INT8) kk = ks[4 * (2 * n + k)];
-              const bool s0 = sees(16 * n + 8 * k + c2), s1 = sees(16 * n + 8 * k + c2 + 1);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                uint64_t z = pair(__uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1)]), __uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1) + 1]));
-                if constexpr (INT8) z = mul2(z, kk);
-                if constexpr (kMasked) {
+                for (int r = 0; r < 4; ++r) {
+                  uint64_t z = score(f[0], k, r);
+                  if constexpr (INT8) z = mul2(z, kk);
                   if (s0) top[r] = fmaxf(top[r], first_of(z));
                   if (s1) top[r] = fmaxf(top[r], second_of(z));
-                } else {
-                  top[r] = fmaxf(fmaxf(top[r], first_of(z)), second_of(z));
                 }
               }
             }
-            if (n + 1 < N) ld_wait(f[(n + 1) & 1]);
-          }
-          ld(f[0], ts);  // the first columns again, while the reference is found
-          float e = 0.0f;
-          if constexpr (INT8) e = (float)(max(max(s.top[slot][0], s.top[slot][1]), max(s.top[slot][2], s.top[slot][3])) - 7);
-          float want[4];
-          bool move = false;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-            want[r] = top[r] == -INFINITY ? -INFINITY : fmaf(top[r], scale[r], e);
-            move = move || want[r] > from[r] + kLag || (from[r] == -INFINITY && want[r] > from[r]);
-          }
-          if (__any_sync(0xffffffffu, move)) {
             float by[4];
+            bool none = false;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float to_ref = fmaxf(from[r], want[r]);
+              top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+              top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+              const float want = top[r] == -INFINITY ? -INFINITY : __fmaf_ru(top[r], scale[r], INT8 ? e - 7.0f : 0.0f), to_ref = fmaxf(from[r], want);
               by[r] = to_ref == -INFINITY ? 1.0f : ex2(from[r] - to_ref);
               from[r] = to_ref;
               l[r] *= by[r];
+              none = none || to_ref == -INFINITY;
             }
+            unset = __any_sync(0xffffffffu, none);
             if (n_done > 0) {  // the products of this row tile's last job are done: its scores came after them
 #pragma unroll 1
               for (int n = 0; n < D / 16; ++n) {
-                ld(f[1], to + 16 * n);
-                ld_wait(f[1]);
+                ld(f[0], to + 16 * n);
+                ld_wait(f[0]);
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                  uint32_t& w = f[1].v[x / 8][x % 8];
+                  uint32_t& w = f[0].v[x / 8][x % 8];
                   w = __float_as_uint(__uint_as_float(w) * by[2 * (x / 8) + (x % 4) / 2]);
                 }
-                st(to + 16 * n, f[1]);
+                st(to + 16 * n, f[0]);
               }
             }
-          }
-          uint64_t ref[4], scale2[4], sum[4] = {0, 0, 0, 0};
+          };
+          if (unset) set_references();
+          // One pass, from the references as they are; again with new ones where a score has outgrown them.
+#pragma unroll 1
+          for (bool again = false;; again = true) {
+            uint64_t ref[4], scale2[4], sum[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float x = from[r] == -INFINITY ? 0.0f : -from[r];
-            ref[r] = pair(x, x), scale2[r] = pair(scale[r], scale[r]);
-          }
-          ld_wait(f[0]);
-#pragma unroll
-          for (int n = 0; n < N; ++n) {
-            if (n + 1 < N) ld(f[(n + 1) & 1], ts + 16 * (n + 1));
-            const Frag& a = f[n & 1];
-            uint32_t w[2][4];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              [[maybe_unused]] uint64_t kk = 0, vv = 0;
-              if constexpr (INT8) kk = ks[4 * (2 * n + k)], vv = vs[4 * (2 * n + k)];
-              const bool s0 = sees(16 * n + 8 * k + c2), s1 = sees(16 * n + 8 * k + c2 + 1);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                uint64_t z = pair(__uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1)]), __uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1) + 1]));
-                if constexpr (INT8) z = mul2(z, kk);
-                z = fma2(z, scale2[r], ref[r]);
-                z = pair(s0 ? ex2(first_of(z)) : 0.0f, s1 ? ex2(second_of(z)) : 0.0f);
-                sum[r] = add2(sum[r], z);
-                if constexpr (INT8) z = mul2(z, vv);
-                w[r / 2][2 * k + (r & 1)] = INT8 ? pack_f16(first_of(z), second_of(z)) : pack_bf16(first_of(z), second_of(z));
-              }
+            for (int r = 0; r < 4; ++r) {
+              const float x = e - (from[r] == -INFINITY ? 0.0f : from[r]);
+              ref[r] = pair(x, x), scale2[r] = pair(scale[r], scale[r]);
             }
-            if (n + 1 < N) ld_wait(f[(n + 1) & 1]);
-            st_packed(ts + 8 * n, w);  // over scores that have been read
-          }
+            uint32_t w[N][2][4];
+            ld(f[0], ts);
+            ld_wait(f[0]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) l[r] += first_of(sum[r]) + second_of(sum[r]);
+            for (int n = 0; n < N; ++n) {
+              if (n + 1 < N) ld(f[(n + 1) & 1], ts + 16 * (n + 1));
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                [[maybe_unused]] uint64_t kk = 0;
+                if constexpr (INT8) kk = ks[4 * (2 * n + k)];
+                const bool s0 = sees(16 * n + 8 * k + c2), s1 = sees(16 * n + 8 * k + c2 + 1);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  uint64_t z = score(f[n & 1], k, r);
+                  if constexpr (INT8) z = mul2(z, kk);
+                  z = fma2(z, scale2[r], ref[r]);
+                  if constexpr (kMasked) z = pair(s0 ? first_of(z) : -INFINITY, s1 ? second_of(z) : -INFINITY);
+                  z = pair(ex2(first_of(z)), ex2(second_of(z)));
+                  sum[r] = add2(sum[r], z);
+                  w[n][r / 2][2 * k + (r & 1)] = INT8 ? pack_f16(first_of(z), second_of(z)) : pack_bf16(first_of(z), second_of(z));
+                }
+              }
+              if (n + 1 < N) ld_wait(f[(n + 1) & 1]);
+            }
+            // No weight is above the sum that it is part of. (Rounded up, a new reference leaves no score above it.)
+            bool over = false;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) over = over || fmaxf(first_of(sum[r]), second_of(sum[r])) > (INT8 ? kMostF16 : kMostBf16);
+            if (!again && __any_sync(0xffffffffu, over)) {
+              set_references();
+              continue;
+            }
+            const float unit = INT8 ? ex2(-e) : 1.0f;
+#pragma unroll
+            for (int n = 0; n < N; ++n) st_packed(ts + 8 * n, w[n]);  // over the scores
+#pragma unroll
+            for (int r = 0; r < 4; ++r) l[r] = fmaf(first_of(sum[r]) + second_of(sum[r]), unit, l[r]);
+            break;
+          }
         };
         if (have != 0xffu || seen < kTile) weigh(std::true_type{});
         else weigh(std::false_type{});
@@ -548,10 +565,17 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
     constexpr uint32_t kQk = instruction<INT8>(kTile, false), kPv = instruction<INT8>(D, true);
     const uint32_t q_u = smem_u32(q_tiles), st_u = smem_u32(stages), mine = elect(), tm = __shfl_sync(0xffffffffu, tmem, 0);
     auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_for(s, bar, parity)) != 0; };
+    // Keys of job i's tile, or its values, are in place (asked once per tile).
+    auto wait_keys = [&](int i) {
+      const int n = 2 * (two ? i >> 1 : i);
+      return i >= n_jobs || (two && (i & 1) != 0) || wait_all(&s.full[n % T::kStages], (n / T::kStages) & 1);
+    };
+    auto wait_values = [&](int i) {
+      const int t = two ? i >> 1 : i, n = 2 * t + 1;
+      return (two && (i & 1) != 0) || (wait_all(&s.full[n % T::kStages], (n / T::kStages) & 1) && (INT8 || end - t * kTile >= kTile || wait_all(&s.tail, 0)));
+    };
     auto qk = [&](int i) {
-      const int t = two ? i >> 1 : i, u = i & 1, n = 2 * t, slot = n % T::kStages;
-      if ((!two || u == 0) && !wait_all(&s.full[slot], (n / T::kStages) & 1)) return false;
-      tc_after();
+      const int t = two ? i >> 1 : i, u = i & 1, slot = 2 * t % T::kStages;
       const uint64_t a = desc_of(q_u + (two ? u * T::kBytes : 0), 16), b = desc_of(st_u + slot * T::kBytes, 16);
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) {  // 16 channels further: 32 bytes, in units of 16
@@ -560,27 +584,34 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       }
       commit(&s.s_full[u], mine);
       if (!two || u == 1) commit(&s.empty[slot], mine);
-      return true;
     };
     auto pv = [&](int i) {
-      const int t = two ? i >> 1 : i, u = i & 1, n = 2 * t + 1, slot = n % T::kStages;
-      if (!wait_all(&s.p_full[u], (i >> 1) & 1)) return false;
-      if ((!two || u == 0) && !wait_all(&s.full[slot], (n / T::kStages) & 1)) return false;
-      if (!INT8 && end - t * kTile < kTile && (!two || u == 0) && !wait_all(&s.tail, 0)) return false;
-      tc_after();
+      const int t = two ? i >> 1 : i, u = i & 1, slot = (2 * t + 1) % T::kStages;
       const uint64_t b = desc_of(st_u + slot * T::kBytes, T::kHalfBytes);
 #pragma unroll
       for (int x = 0; x < kTile / 16; ++x)  // 16 tokens further: 2 KB of V, 8 columns of P
         mma_ts(tm + 2 * kTile + u * D, tm + u * kTile + 8 * x, b + x * (2048 / 16), kPv, x > 0 || i > 1, mine);
       if (!two || u == 1) commit(&s.empty[slot], mine);
       if (i + 2 >= n_jobs) commit(&s.o_full[u], mine);
-      return true;
     };
+    // The scores of job i + 2 follow the output of job i at once (the weights wait for both): their
+    // operands are asked for before the weights are. With three stages and one row tile the next keys
+    // come into the stage that these values leave, so there they are asked for after.
+    const bool early = two || T::kStages > 3;
     bool ok = wait_all(&s.q_full, 0);
-    for (int i = 0; ok && i < 2 && i < n_jobs; ++i) ok = qk(i);
+    for (int i = 0; ok && i < 2 && i < n_jobs; ++i) {
+      ok = wait_keys(i);
+      tc_after();
+      if (ok) qk(i);
+    }
     for (int i = 0; ok && i < n_jobs; ++i) {
-      ok = pv(i);
-      if (ok && i + 2 < n_jobs) ok = qk(i + 2);
+      ok = wait_values(i) && (!early || wait_keys(i + 2)) && wait_all(&s.p_full[i & 1], (i >> 1) & 1);
+      if (!ok) break;
+      tc_after();
+      pv(i);
+      if (!early) ok = wait_keys(i + 2);
+      tc_after();
+      if (ok && i + 2 < n_jobs) qk(i + 2);
     }
     if (!ok) {  // nothing is freed under a product in flight
       commit(&s.drain, mine);
@@ -658,59 +689,81 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
     __syncwarp();
   } else if (warp >= 12) {
     if constexpr (INT8) {
-      // ---- codes to f16 operands: thread i also carries token i's scales --------------------------------
-      const int i = tid - 12 * 32;
+      // ---- codes to f16 operands: thread i also carries token i % 128's key scale, or its value scale ----
+      const int i = tid - 12 * 32, token = i % kTile;
+      const bool values = i >= kTile;
       bool ok = true;
-      float ks = 0.0f, vs = 0.0f;
+      // Scales are loaded a tile ahead, and their page's id (checked where it is used) a tile before that:
+      // neither load is waited for where it is issued.
+      float scale = 0.0f;
       bool there = false;
-      auto scales_of = [&](int t) {  // looked up a tile ahead
-        ks = vs = 0.0f;
-        there = false;
-        const int pos = (first + t) * kTile + i;
-        if (t < n_tiles && pos < p.prefix_len) {
-          const int page = page_at(p.prefix_table, p.prefix_cols, p.n_pages, pos, p.page_shift), bs = 1 << p.page_shift;
-          if (page >= 0) {
-            const float* src = p.scales + (((int64_t)page * p.h + j) * 2) * bs + (pos & (bs - 1));
-            ks = src[0], vs = src[bs];
-            there = true;
-          }
-        }
+      int id = -1;
+      auto page_of = [&](int t) {
+        const int pos = (first + t) * kTile + token, blk = pos >> p.page_shift;
+        id = t < n_tiles && pos < p.prefix_len && blk < p.prefix_cols ? p.prefix_table[blk] : -1;
       };
+      auto scales_of = [&](int t) {
+        scale = 0.0f;
+        there = id >= 0 && id < p.n_pages;
+        if (there) {
+          const int bs = 1 << p.page_shift, pos = (first + t) * kTile + token;
+          scale = p.scales[(((int64_t)id * p.h + j) * 2 + (values ? 1 : 0)) * bs + (pos & (bs - 1))];
+        }
+        page_of(t + 1);
+      };
+      page_of(0);
       scales_of(0);
+      // A thread's pieces of 16 codes, one channel range of every kStep-th token. Eight lanes take 128 bytes
+      // that lie in 32 different banks, and so do the chunks they write: two tokens of different parity, of
+      // which the swizzle puts even chunks into even and odd places.
+      constexpr int kPer = D / 16, kMine = kPer / 2, kStep = 2 * kTile / kPer;  // kStep is a multiple of 8
+      const int odd = (i >> 2) & 1, half = odd ^ ((i >> 3) & 1);
+      const int tok0 = kPer == 8 ? (i >> 4) * 2 + odd : i / kPer, c = kPer == 8 ? half * 4 + (i & 3) : i % kPer;
+      const int from = (tok0 * kPer + c) * 16, row = (c / 4) * T::kHalfBytes + tok0 * 128, at = (c % 4) * 2;
+      const int to0 = row + ((at ^ (tok0 & 7)) << 4), to1 = row + (((at + 1) ^ (tok0 & 7)) << 4);
       for (int n = 0; n < 2 * n_tiles; ++n) {
         const int t = n >> 1, kv = n & 1, raw = n % T::kRaw, slot = n % T::kStages;
-        ok = wait_for(s, &s.raw_full[raw], (n / T::kRaw) & 1);
+        float* ring = scale_ring + (t % kInfo) * 2 * kTile;
+        ok = ok && wait_for(s, &s.raw_full[raw], (n / T::kRaw) & 1);
         if (ok && n >= T::kStages) ok = wait_for(s, &s.empty[slot], (n / T::kStages - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (kv == 0) {
-          float* ring = scale_ring + (t % kInfo) * 2 * kTile;
-          ring[i] = ks;
-          ring[kTile + i] = vs;
-          // vs < 2^e, e from its exponent; what is not finite stays what it is. At least -40, so that the
-          // sum of the weights stays far from float32's end where the values are all but zero.
-          const int bits = (int)((__float_as_uint(vs) >> 23) & 0xffu);
-          const int e = bits == 0xff ? -40 : max(bits - 126, -40);
-          const int top = __reduce_max_sync(0xffffffffu, e);
-          if (lane == 0) s.top[t % kInfo][warp - 12] = top;
-          const uint32_t mask = __ballot_sync(0xffffffffu, there);
-          if (lane == 0) s.have[t % kInfo][warp - 12] = ((mask & 0xffffu) != 0 ? 1u : 0u) << (2 * (warp - 12)) | (mask >> 16 != 0 ? 2u : 0u) << (2 * (warp - 12));
+        if (!ok) {  // given up: no warp is left at the barrier below
+          if (kv == 1) asm volatile("bar.sync 2, 256;" ::: "memory");
+          continue;
         }
-        const char* src = raws + raw * T::kRawBytes;
+        uint4 w[kMine];
+#pragma unroll
+        for (int x = 0; x < kMine; ++x) w[x] = *reinterpret_cast<const uint4*>(raws + raw * T::kRawBytes + from + x * (kStep * kPer * 16));
         char* dst = stages + slot * T::kBytes;
-        constexpr int kPer = D / 16;  // 16-byte pieces of a token
-  #pragma unroll
-        for (int x = 0; x < kPer; ++x) {
-          // Eight lanes take 128 bytes that lie in 32 different banks, and so do the chunks they write: two
-          // tokens of different parity, of which the swizzle puts even chunks into even and odd places.
-          const int piece = x * kTile + i, swap_half = kPer == 8 ? ((piece >> 2) ^ (piece >> 3)) & 1 : 0;
-          const int tok = kPer == 8 ? (piece >> 4) * 2 + ((piece >> 2) & 1) : piece / kPer, c = kPer == 8 ? swap_half * 4 + (piece & 3) : piece % kPer;
-          const uint4 w = *reinterpret_cast<const uint4*>(src + (tok * kPer + c) * 16);
-          const uint2 a = codes_to_f16(w.x), b = codes_to_f16(w.y), d = codes_to_f16(w.z), e = codes_to_f16(w.w);
-          char* to = dst + (c / 4) * T::kHalfBytes + tok * 128;
-          const int at = (c % 4) * 2;
-          *reinterpret_cast<uint4*>(to + ((at ^ (tok & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
-          *reinterpret_cast<uint4*>(to + (((at + 1) ^ (tok & 7)) << 4)) = make_uint4(d.x, d.y, e.x, e.y);
+        if (kv == 0) {
+          ring[i] = scale;
+          if (values) {
+            // scale < 2^e, e from its exponent; what is not finite stays what it is. At least -40, so that the
+            // sum of the weights stays far from float32's end where the values are all but zero.
+            const int bits = (int)((__float_as_uint(scale) >> 23) & 0xffu);
+            const int top = __reduce_max_sync(0xffffffffu, bits == 0xff ? -40 : max(bits - 126, -40));
+            if (lane == 0) s.top[t % kInfo][warp - 16] = top;
+          } else {
+            const uint32_t mask = __ballot_sync(0xffffffffu, there);
+            if (lane == 0) s.have[t % kInfo][warp - 12] = ((mask & 0xffffu) != 0 ? 1u : 0u) << (2 * (warp - 12)) | (mask >> 16 != 0 ? 2u : 0u) << (2 * (warp - 12));
+          }
+#pragma unroll
+          for (int x = 0; x < kMine; ++x) {
+            const uint2 a = codes_to_f16(w[x].x), b = codes_to_f16(w[x].y), d = codes_to_f16(w[x].z), e = codes_to_f16(w[x].w);
+            *reinterpret_cast<uint4*>(dst + to0 + kStep * x * 128) = make_uint4(a.x, a.y, b.x, b.y);
+            *reinterpret_cast<uint4*>(dst + to1 + kStep * x * 128) = make_uint4(d.x, d.y, e.x, e.y);
+          }
+        } else {
+          asm volatile("bar.sync 2, 256;" ::: "memory");  // the tile's scales and exponents, which other warps wrote
+          const float down = __int_as_float((127 - largest(s.top[t % kInfo])) << 23);  // 2^-E
+#pragma unroll
+          for (int x = 0; x < kMine; ++x) {
+            const __half2 by = __float2half2_rn(ring[kTile + tok0 + kStep * x] * down);
+            const uint2 a = times(codes_to_f16(w[x].x), by), b = times(codes_to_f16(w[x].y), by), d = times(codes_to_f16(w[x].z), by),
+                        e = times(codes_to_f16(w[x].w), by);
+            *reinterpret_cast<uint4*>(dst + to0 + kStep * x * 128) = make_uint4(a.x, a.y, b.x, b.y);
+            *reinterpret_cast<uint4*>(dst + to1 + kStep * x * 128) = make_uint4(d.x, d.y, e.x, e.y);
+          }
         }
         fence_async();
         __syncwarp();
