@@ -600,9 +600,9 @@ int lkv_paged_read(const void* pages, int kind, const float* scales, int64_t n_p
  * token without a page is not attended. out [batch, tokens, hq, d] contiguous in out_dtype and lse
  * [batch, tokens, hq] float32; a row that attends nothing gets out = 0, lse = -inf. lens and the tables
  * are read on the device, so a captured graph follows them; prefix_len and the shapes are the call's.
- * The prefix is read once for the batch: partials in the workspace (any contents,
- * lkv_prefix_attention_workspace bytes, 16-byte aligned), folded in by the launch over the sequences'
- * own tokens. Calls that may overlap on the GPU need a workspace each.
+ * The prefix is read once for the batch. Partials go to the workspace (any contents,
+ * lkv_prefix_attention_workspace bytes with own_reach = table_cols * bs, 16-byte aligned) and are merged
+ * by the last of two or three launches. Calls that may overlap on the GPU need a workspace each.
  */
 typedef struct {
   const void* q;
@@ -628,7 +628,7 @@ typedef struct {
   void* workspace;
   size_t workspace_bytes;
 } lkv_prefix_args;
-size_t lkv_prefix_attention_workspace(int batch, int tokens, int hq, int h, int d, int64_t prefix_len);
+size_t lkv_prefix_attention_workspace(int batch, int tokens, int hq, int h, int d, int64_t prefix_len, int kind, int64_t own_reach);
 int lkv_prefix_attention(const lkv_prefix_args* args, void* stream);
 
 /*

@@ -85,7 +85,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                 c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p]),
     "lkv_paged_read": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p,
                                c_void_p, c_void_p, c_int, c_void_p]),
-    "lkv_prefix_attention_workspace": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int64]),
+    "lkv_prefix_attention_workspace": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int64, c_int, c_int64]),
     "lkv_prefix_attention": (c_int, [c_void_p, c_void_p]),
     "lkv_verify_drafts": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int,
                                   c_void_p, c_void_p, c_void_p]),

@@ -2,62 +2,71 @@
 // sequence's, and the prefix's pages are read once for the whole batch.
 //
 // The query rows of KV head j are (b, t, g): sequence, position among the step's tokens, query head of
-// the group. Row (b, t, g) sees the prefix [0, prefix_len) and own tokens 0 .. lens[b] - tokens + t. Two
-// softmaxes over disjoint key sets merge exactly by their maxima and sums, so the work is two launches:
-//   1. the prefix: all rows of the batch against chunks of the prefix, a partial (m, l, o) per chunk;
-//   2. the sequences' own tokens, one cluster of CTAs per (sequence, KV head, row tile), which then
-//      folds the prefix's partials in and writes the output.
-// The second launch starts under the first (programmatic dependent launch) and waits for it only before
-// it folds.
+// the group. Row (b, t, g) sees the prefix [0, prefix_len) and own tokens 0 .. lens[b] - tokens + t.
+// Softmaxes over disjoint key sets merge exactly by their references and sums, so the work is cut into
+// partials (m, l, o), l = sum 2^(s - m), o = sum 2^(s - m) v, s the scores in the log2 domain:
+//   1. stream_kernel: the sequences' own tokens, and the prefix too where the batch has few rows;
+//   2. prefix_tile_kernel (prefix_tile.cu): the prefix for many rows, on tcgen05;
+//   3. combine_kernel: the partials of every row.
+// Each launch starts under the one before it (programmatic dependent launch).
 //
-// prefix_tile.cu does the first launch. stream_kernel does the second, and the first where the batch has
-// few rows: each warp takes a
-// tile of 16 rows through its share of the tokens with mma.sync.m16n8k16 (bf16 operands, float32
-// accumulators). A lane copies by cp.async exactly the bytes that it will hold as mma fragments, into
-// slots of shared memory of its own, so the pipeline needs no barrier and no bank conflicts arise; the
-// channels are permuted so that a fragment's elements are 16 contiguous bytes of a row (a dot product
-// does not mind, and the output's permutation ends in contiguous runs again). int8 codes become bf16
-// exactly in registers; a key's scale multiplies its column of scores, a value's its column of
-// probabilities, both in float32. Probabilities are rounded to bf16 for the second product (2^-9
-// relative, unbiased over the keys, and below the rounding of a bf16 output).
-#include <cooperative_groups.h>
-
+// stream_kernel is bound by the pages' bytes. Its work is one line of stages (prefix.cuh) that all warps
+// of the grid share equally, whatever the sequences' lengths: only the device knows them, and with a CTA
+// or a cluster per (sequence, head) the longest sequence set the time. A warp takes a tile of 16 rows
+// through its stages with mma.sync.m16n8k16 (float32 accumulators). A lane copies by cp.async exactly the
+// bytes that it will hold as mma fragments, into slots of shared memory of its own, so the pipeline needs
+// no barrier and has no bank conflicts; the channels are permuted so that a fragment's elements are 16
+// contiguous bytes of a row (a dot product does not mind, and the output's permutation ends in contiguous
+// runs again).
+//
+// bf16 pages: probabilities are rounded to bf16 for the second product (2^-8 relative at most, unbiased
+// over the keys). int8 pages: codes and queries are f16 (prefix_tile.cu tells how exactly), a key's scale
+// multiplies its column of scores in float32, and a value's scale its column of weights, before they are
+// rounded to f16: with 2^E above every value scale of the stage, references are at least the maximum + E -
+// 7, so weights x scales stay below 2^7 when a reference is set and below 2^15 until it is set again.
 #include "prefix.cuh"
 
 namespace lkv {
 namespace prefix {
 namespace {
 
-namespace cg = cooperative_groups;
-
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kRows = 16;  // rows of an mma tile
-constexpr int kMaxCluster = 8;
+constexpr float kLag = 8.0f;  // powers of two that a reference may lag behind the maximum
 
+template <bool F16>
 __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  if constexpr (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Asynchronous copy of N bytes, or N zeros where !there (nothing is read then).
+template <int N>
+__device__ __forceinline__ void copy(uint32_t dst, const void* src) {
+  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+}
+// N bytes, or N zeros where !there (nothing is read then).
 template <int N>
 __device__ __forceinline__ void copy_or_zero(uint32_t dst, const void* src, bool there) {
   const int n = there ? N : 0;
-  if constexpr (N == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
+  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
 }
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
-constexpr int stage_tokens(int d) { return d == 128 ? 16 : 32; }
+constexpr int stage_shift_of(int d) { return d == 128 ? 4 : 5; }
 
 // Geometry of the stream for one head dimension and cache type.
 template <int D, bool INT8>
 struct Shape {
   static constexpr int kElt = INT8 ? 1 : 2;
-  static constexpr int kTok = stage_tokens(D);                 // tokens per stage
+  static constexpr int kTok = 1 << stage_shift_of(D);          // tokens per stage
   static constexpr int kGran = kTok / 16;                      // 16-token granules per stage
   static constexpr int kKLoads = D * kElt / 64;                // 16-byte loads per lane and 8 keys (4 lanes a row)
   static constexpr int kVBytes = D * kElt / 8 >= 16 ? 16 : 8;  // bytes per lane and load of a value row (8 lanes a row)
@@ -67,10 +76,12 @@ struct Shape {
   static constexpr int kSBytes = INT8 ? 32 : 0;                // the scales of 4 tokens' keys and values
   static constexpr int kGranBytes = (kKBytes + kVAll + kSBytes) * 32;
   static constexpr int kStageBytes = kGran * kGranBytes;
-  static constexpr int kStages = INT8 ? 4 : 3;                 // 72 to 96 KB of copies per CTA, two CTAs an SM
-  static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kVCh = kVBytes / kElt;                  // channels per value load
-  // The channel of column n of the i-th output tile.
+  static constexpr int kStages = 3;
+  static constexpr int kRing = kWarps * kStages * kStageBytes;  // 60 to 96 KB; the warps' states fit too
+  static_assert(kRing >= kWarps * kRows * ((D + 4) * 4 + 8), "the merge is done in the ring");
+  static constexpr int kCtas = INT8 ? 3 : 2;                    // per SM
+  static constexpr int kVCh = kVBytes / kElt;                   // channels per value load
+  // The channel of column n of the i-th output tile: kVCh consecutive ones per column and kVCh tiles.
   __device__ static __forceinline__ int channel(int i, int n) { return (i / kVCh) * (8 * kVCh) + n * kVCh + i % kVCh; }
 };
 
@@ -87,26 +98,39 @@ struct State {
   }
 };
 
-// The A fragments of a 16-row tile of queries, channels permuted as Shape's keys are. Rows without a
-// pointer are zero.
+// The A fragments of a 16-row tile of queries, channels permuted as the keys' are, and per row what its
+// scores have to be multiplied with. Rows without a pointer are zero.
 template <int D, bool INT8>
-__device__ __forceinline__ void load_queries(uint32_t (&qf)[D / 16][4], const __nv_bfloat16* lo, const __nv_bfloat16* hi, int c) {
+__device__ __forceinline__ void load_queries(uint32_t (&qf)[D / 16][4], float (&scale)[2], const __nv_bfloat16* lo, const __nv_bfloat16* hi, int c,
+                                             float scale_log2) {
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const __nv_bfloat16* row = half ? hi : lo;
+    scale[half] = scale_log2;
     if constexpr (INT8) {
+      uint4 w[D / 64][2];
+      uint32_t top = 0;
 #pragma unroll
       for (int x = 0; x < D / 64; ++x) {
-        uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-        if (row != nullptr) {
-          const uint4* p = reinterpret_cast<const uint4*>(row + 64 * x + 16 * c);
-          w[0] = p[0], w[1] = p[1];
-        }
-        const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // k-step 4x + i: channels (0, 2) then (1, 3) of four
-          qf[4 * x + i][half] = __byte_perm(u[2 * i], u[2 * i + 1], 0x5410);
-          qf[4 * x + i][2 + half] = __byte_perm(u[2 * i], u[2 * i + 1], 0x7632);
+        for (int y = 0; y < 2; ++y) {
+          w[x][y] = row != nullptr ? reinterpret_cast<const uint4*>(row + 64 * x + 16 * c)[y] : make_uint4(0, 0, 0, 0);
+          const uint32_t u[4] = {w[x][y].x, w[x][y].y, w[x][y].z, w[x][y].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
+        }
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float2 by = row_scales(top);
+      scale[half] *= by.y;
+#pragma unroll
+      for (int x = 0; x < D / 64; ++x) {
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(w[x]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // k-step 4 x + i: four channels
+          qf[4 * x + i][half] = pack_f16(__uint_as_float(u[2 * i] << 16) * by.x, __uint_as_float(u[2 * i] & 0xffff0000u) * by.x);
+          qf[4 * x + i][2 + half] = pack_f16(__uint_as_float(u[2 * i + 1] << 16) * by.x, __uint_as_float(u[2 * i + 1] & 0xffff0000u) * by.x);
         }
       }
     } else {
@@ -121,59 +145,86 @@ __device__ __forceinline__ void load_queries(uint32_t (&qf)[D / 16][4], const __
   }
 }
 
-// Starts the copies of one stage: tokens first .. first + kTok - 1 of the list, those at or past `end`
-// and those without a page as zeros. `have` gets a bit per granule that has a page.
+// Starts the copies of one stage: tokens first .. first + kTok - 1 of a list that ends at `end`, those at
+// or past it and those without a page as zeros. Returns a bit per granule that has a page.
 template <int D, bool INT8>
-__device__ __forceinline__ uint32_t fill_stage(const Params& p, int j, const int (&page)[Shape<D, INT8>::kGran], int first, int end, uint32_t slot, int lane) {
+__device__ __forceinline__ uint32_t fill_stage(const Params& p, int j, const int (&id)[Shape<D, INT8>::kGran], int first, int end, uint32_t slot, int lane) {
   using S = Shape<D, INT8>;
+  constexpr int kRowBytes = D * S::kElt;
   const int r = lane / 4, c = lane % 4;
   const int bs = 1 << p.page_shift;
   uint32_t have = 0;
 #pragma unroll
   for (int g = 0; g < S::kGran; ++g) {
     const int tok = first + 16 * g;
-    const bool ok = page[g] >= 0;
+    const bool ok = id[g] >= 0 && id[g] < p.n_pages && tok < end;
     have |= (ok ? 1u : 0u) << g;
-    const int64_t krow = (((int64_t)(ok ? page[g] : 0) * p.h + j) * 2) * bs + (tok & (bs - 1));
-    const char* kp = static_cast<const char*>(p.pages) + krow * (D * S::kElt);
-    const char* vp = kp + (int64_t)bs * (D * S::kElt);
-    uint32_t dst = slot + g * S::kGranBytes + lane * 16;
+    const int64_t krow = (((int64_t)(ok ? id[g] : 0) * p.h + j) * 2) * bs + (tok & (bs - 1));
+    const char* kp = static_cast<const char*>(p.pages) + krow * kRowBytes;
+    const char* vp = kp + bs * kRowBytes + 2 * c * kRowBytes + r * S::kVBytes;
+    kp += r * kRowBytes + 16 * c;
+    const uint32_t kd = slot + g * S::kGranBytes + lane * 16, vd = slot + g * S::kGranBytes + S::kKBytes * 32 + lane * S::kVBytes;
+    if (ok && tok + 16 <= end) {
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
+      for (int i = 0; i < 2 * S::kKLoads; ++i) copy<16>(kd + 512 * i, kp + (i / S::kKLoads) * 8 * kRowBytes + 64 * (i % S::kKLoads));
 #pragma unroll
-      for (int x = 0; x < S::kKLoads; ++x, dst += 512) {
-        const int t = 8 * nt + r;
-        copy_or_zero<16>(dst, kp + t * (D * S::kElt) + 64 * x + 16 * c, ok && tok + t < end);
+      for (int i = 0; i < 4 * S::kVLoads; ++i)
+        copy<S::kVBytes>(vd + S::kVBytes * 32 * i, vp + (((i / S::kVLoads) & 1) + 8 * (i / S::kVLoads >> 1)) * kRowBytes + (i % S::kVLoads) * 8 * S::kVBytes);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2 * S::kKLoads; ++i)
+        copy_or_zero<16>(kd + 512 * i, kp + (i / S::kKLoads) * 8 * kRowBytes + 64 * (i % S::kKLoads), ok && tok + 8 * (i / S::kKLoads) + r < end);
+#pragma unroll
+      for (int i = 0; i < 4 * S::kVLoads; ++i) {
+        const int t = ((i / S::kVLoads) & 1) + 8 * (i / S::kVLoads >> 1);
+        copy_or_zero<S::kVBytes>(vd + S::kVBytes * 32 * i, vp + t * kRowBytes + (i % S::kVLoads) * 8 * S::kVBytes, ok && tok + 2 * c + t < end);
       }
-    if constexpr (S::kVBytes == 8) dst = slot + g * S::kGranBytes + S::kKBytes * 32 + lane * 8;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = 2 * c + (i & 1) + 8 * (i >> 1);
-#pragma unroll
-      for (int y = 0; y < S::kVLoads; ++y, dst += S::kVBytes * 32)
-        copy_or_zero<S::kVBytes>(dst, vp + t * (D * S::kElt) + (8 * y + r) * S::kVBytes, ok && tok + t < end);
     }
     if constexpr (INT8) {
-      dst = slot + g * S::kGranBytes + (S::kKBytes + S::kVAll) * 32 + lane * 8;
+      const uint32_t sd = slot + g * S::kGranBytes + (S::kKBytes + S::kVAll) * 32 + lane * 8;
       const float* sp = p.scales + krow + 2 * c;  // two tokens' key scales, then (bs further) their value scales
+      // Past `end` inside a page the scales are read all the same: they exist, and their columns are masked.
 #pragma unroll
-      for (int i = 0; i < 4; ++i, dst += 256) {
-        // Past `end` inside a page the scales are read all the same: they exist, and their columns are masked.
-        copy_or_zero<8>(dst, sp + (i >> 1) * bs + 8 * (i & 1), ok);
-      }
+      for (int i = 0; i < 4; ++i) copy_or_zero<8>(sd + 256 * i, sp + (i >> 1) * bs + 8 * (i & 1), ok);
     }
   }
-  asm volatile("cp.async.commit_group;" ::: "memory");
+  copies_done();
   return have;
 }
 
-// One stage's tokens folded into the warp's state. limit[0/1]: the tokens that rows r and r + 8 see.
-template <int D, bool INT8>
-__device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D / 16][4], const char* slot, int first, const int (&limit)[2], int low,
-                                           uint32_t have, float scale_log2, int lane) {
+// A granule's P V without mma (see fold_stage): weights of zero take nothing from their values.
+template <int D>
+__device__ __forceinline__ void fold_values_singly(State<D>& st, const char* values, const float (&s)[2][4], int lane) {
+  using S = Shape<D, false>;
+  const int c = lane % 4;
+#pragma unroll 1
+  for (int t = 0; t < 16; ++t) {
+    const int c2 = (t & 7) >> 1, owner = (lane & ~3) | c2;  // the lane that holds this token's weights of rows r, r + 8
+    const float x0 = t < 8 ? (t & 1 ? s[0][1] : s[0][0]) : (t & 1 ? s[1][1] : s[1][0]);
+    const float x1 = t < 8 ? (t & 1 ? s[0][3] : s[0][2]) : (t & 1 ? s[1][3] : s[1][2]);
+    const float p0 = bf16_round(__shfl_sync(0xffffffffu, x0, owner)), p1 = bf16_round(__shfl_sync(0xffffffffu, x1, owner));
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      // Column n of output tile i is in what lane (n, c2) copied: load t % 2 + 2 (t / 8), and i / kVCh of it.
+      const char* src = values + (((t & 1) + 2 * (t >> 3)) * S::kVLoads + i / S::kVCh) * (S::kVBytes * 32) + 2 * (i % S::kVCh);
+      const float va = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(src + ((2 * c) * 4 + c2) * S::kVBytes));
+      const float vb = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(src + ((2 * c + 1) * 4 + c2) * S::kVBytes));
+      if (p0 != 0.0f) st.o[i][0] += p0 * va, st.o[i][1] += p0 * vb;
+      if (p1 != 0.0f) st.o[i][2] += p1 * va, st.o[i][3] += p1 * vb;
+    }
+  }
+  __syncwarp();  // these slots are other lanes' to fill again
+}
+
+// One stage's tokens folded into the warp's state. limit[0/1]: the tokens that rows r and r + 8 see. MASKED:
+// some row's sight ends in this stage, or a page is missing.
+template <int D, bool INT8, bool MASKED>
+__device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D / 16][4], const float (&scale)[2], const char* slot, int first,
+                                           const int (&limit)[2], uint32_t have, int lane) {
   using S = Shape<D, INT8>;
   const int c = lane % 4;
   float s[2 * S::kGran][4];
+  float2 vs[2 * S::kGran];  // int8: the value scales of this lane's columns
 #pragma unroll
   for (int g = 0; g < S::kGran; ++g) {
     const char* base = slot + g * S::kGranBytes + lane * 16;
@@ -187,25 +238,26 @@ __device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D 
         if constexpr (INT8) {
           const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma16816(x, qf[4 * i + k], codes_to_bf16(u[k]), codes_to_bf16(u[k] >> 8));
+          for (int k = 0; k < 4; ++k) {
+            const uint2 b = codes_to_f16(u[k]);
+            mma16816<true>(x, qf[4 * i + k], b.x, b.y);
+          }
         } else {
-          mma16816(x, qf[2 * i], w.x, w.y);
-          mma16816(x, qf[2 * i + 1], w.z, w.w);
+          mma16816<false>(x, qf[2 * i], w.x, w.y);
+          mma16816<false>(x, qf[2 * i + 1], w.z, w.w);
         }
       }
       if constexpr (INT8) {
-        const float2 ks = *reinterpret_cast<const float2*>(slot + g * S::kGranBytes + (S::kKBytes + S::kVAll) * 32 + nt * 256 + lane * 8);
-        x[0] *= ks.x * scale_log2, x[1] *= ks.y * scale_log2;
-        x[2] *= ks.x * scale_log2, x[3] *= ks.y * scale_log2;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] *= scale_log2;
+        const char* sp = slot + g * S::kGranBytes + (S::kKBytes + S::kVAll) * 32 + nt * 256 + lane * 8;
+        const float2 ks = *reinterpret_cast<const float2*>(sp);
+        vs[2 * g + nt] = *reinterpret_cast<const float2*>(sp + 512);
+        x[0] *= ks.x, x[1] *= ks.y, x[2] *= ks.x, x[3] *= ks.y;
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] *= scale[e >> 1];
     }
   }
-  // The mask, where a row's sight ends inside this stage or a page is missing (the same for the warp).
-  const bool masked = low < first + S::kTok || have != (1u << S::kGran) - 1;
-  if (masked) {
+  if constexpr (MASKED) {
 #pragma unroll
     for (int n = 0; n < 2 * S::kGran; ++n)
 #pragma unroll
@@ -214,28 +266,42 @@ __device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D 
         if (tok >= limit[e >> 1] || !((have >> (n / 2)) & 1)) s[n][e] = -INFINITY;
       }
   }
-  float top[2] = {st.m[0], st.m[1]};
+  float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
   for (int n = 0; n < 2 * S::kGran; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+  float above = 0.0f;  // int8: E - 7
+  if constexpr (INT8) {
+    // Scales are below 2^E, E from the largest finite one's exponent; at least 2^-40, so that the sums stay
+    // far from float32's end where the values are all but zero.
+    int bits = 87;  // of 2^-40
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+    for (int n = 0; n < 2 * S::kGran; ++n) {
+      const int x = (__float_as_int(vs[n].x) >> 23) & 0xff, y = (__float_as_int(vs[n].y) >> 23) & 0xff;
+      const bool on = !MASKED || ((have >> (n / 2)) & 1);
+      if (on && x != 0xff) bits = max(bits, x);
+      if (on && y != 0xff) bits = max(bits, y);
+    }
+    above = (float)(bits - 126 - 7);
   }
-  if (__any_sync(0xffffffffu, top[0] > st.m[0] || top[1] > st.m[1])) {
+  // A reference moves where a lane sees it outgrown (or has none yet), for the four lanes of the row alike.
+  const float grown[2] = {top[0] + above, top[1] + above};
+  if (__any_sync(0xffffffffu, grown[0] > st.m[0] + kLag || grown[1] > st.m[1] + kLag)) {
     float f[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      f[i] = top[i] > st.m[i] ? ex2(st.m[i] - top[i]) : 1.0f;  // 0 where nothing was seen before
+      float want = grown[i];
+      want = fmaxf(want, __shfl_xor_sync(0xffffffffu, want, 1));
+      want = fmaxf(want, __shfl_xor_sync(0xffffffffu, want, 2));
+      f[i] = want > st.m[i] ? ex2(st.m[i] - want) : 1.0f;  // 0 where nothing was seen before
+      st.m[i] = fmaxf(st.m[i], want);
       st.l[i] *= f[i];
-      st.m[i] = top[i];
     }
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) st.o[i][0] *= f[0], st.o[i][1] *= f[0], st.o[i][2] *= f[1], st.o[i][3] *= f[1];
   }
-  // A row that has seen nothing keeps m = -inf: its weights come from a maximum of 0, ex2(-inf) = 0.
+  // A row that has seen nothing keeps m = -inf: its weights come from a reference of 0, ex2(-inf) = 0.
   const float m0 = st.m[0] == -INFINITY ? 0.0f : st.m[0], m1 = st.m[1] == -INFINITY ? 0.0f : st.m[1];
 #pragma unroll
   for (int n = 0; n < 2 * S::kGran; ++n) {
@@ -244,293 +310,474 @@ __device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D 
     st.l[0] += s[n][0] + s[n][1];
     st.l[1] += s[n][2] + s[n][3];
     if constexpr (INT8) {
-      const float2 vs = *reinterpret_cast<const float2*>(slot + (n / 2) * S::kGranBytes + (S::kKBytes + S::kVAll) * 32 + (2 + n % 2) * 256 + lane * 8);
-      // A weight of zero stays zero whatever the scale (a masked token's may be NaN).
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = s[n][e] == 0.0f ? 0.0f : s[n][e] * ((e & 1) ? vs.y : vs.x);
+      for (int e = 0; e < 4; ++e) {
+        const float by = (e & 1) ? vs[n].y : vs[n].x;
+        s[n][e] = MASKED && s[n][e] == 0.0f ? 0.0f : s[n][e] * by;  // a masked token's scale may be a NaN
+      }
     }
   }
 #pragma unroll
   for (int g = 0; g < S::kGran; ++g) {
-    const char* base = slot + g * S::kGranBytes + S::kKBytes * 32 + lane * S::kVBytes;
-    const uint32_t a[4] = {pack_bf16(s[2 * g][0], s[2 * g][1]), pack_bf16(s[2 * g][2], s[2 * g][3]), pack_bf16(s[2 * g + 1][0], s[2 * g + 1][1]),
-                           pack_bf16(s[2 * g + 1][2], s[2 * g + 1][3])};
+    const char* values = slot + g * S::kGranBytes + S::kKBytes * 32;
+    uint32_t w[S::kVLoads][4][S::kVBytes / 4];
 #pragma unroll
-    for (int y = 0; y < S::kVLoads; ++y) {
-      constexpr int kWords = S::kVBytes / 4;
-      uint32_t w[4][kWords];
+    for (int y = 0; y < S::kVLoads; ++y)
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const char* src = base + (t * S::kVLoads + y) * (S::kVBytes * 32);
-        if constexpr (kWords == 4) {
+        const char* src = values + lane * S::kVBytes + (t * S::kVLoads + y) * (S::kVBytes * 32);
+        if constexpr (S::kVBytes == 16) {
           const uint4 x = *reinterpret_cast<const uint4*>(src);
-          w[t][0] = x.x, w[t][1] = x.y, w[t][2] = x.z, w[t][3] = x.w;
+          w[y][t][0] = x.x, w[y][t][1] = x.y, w[y][t][2] = x.z, w[y][t][3] = x.w;
         } else {
           const uint2 x = *reinterpret_cast<const uint2*>(src);
-          w[t][0] = x.x, w[t][1] = x.y;
+          w[y][t][0] = x.x, w[y][t][1] = x.y;
         }
       }
-      if constexpr (!INT8) {
-        if (masked) {
-          // 0 x infinity is NaN: a token that some rows do not see must not reach them through a value
-          // that is not finite. Such a stage (the step's own last tokens only) is summed without mma.
-          bool odd = false;
+    if constexpr (MASKED && !INT8) {
+      // 0 x infinity is NaN: a token that some rows do not see must not reach them through a value that is
+      // not finite.
+      bool odd = false;
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
+      for (int y = 0; y < S::kVLoads; ++y)
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) odd |= (w[t][i] & 0x7f80u) == 0x7f80u || (w[t][i] & 0x7f800000u) == 0x7f800000u;
-          if (__any_sync(0xffffffffu, odd)) {
-#pragma unroll 1
-            for (int t = 0; t < 16; ++t) {
-              const int e = t & 1, owner = (lane & ~3) | ((t & 7) >> 1);  // the lane that holds this token's weights for rows r, r + 8
-              const float x0 = t < 8 ? (e ? s[2 * g][1] : s[2 * g][0]) : (e ? s[2 * g + 1][1] : s[2 * g + 1][0]);
-              const float x1 = t < 8 ? (e ? s[2 * g][3] : s[2 * g][2]) : (e ? s[2 * g + 1][3] : s[2 * g + 1][2]);
-              const float p0 = bf16_round(__shfl_sync(0xffffffffu, x0, owner)), p1 = bf16_round(__shfl_sync(0xffffffffu, x1, owner));
-              const int slot_t = e + 2 * (t >> 3);
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-              for (int i = 0; i < S::kVCh; ++i) {
-                // Column n of output tile (y, i) is channel(., n), which lane (n, owner's c) copied.
-                const char* src = slot + g * S::kGranBytes + S::kKBytes * 32 + (slot_t * S::kVLoads + y) * (S::kVBytes * 32);
-                const int c2 = (t & 7) >> 1;
-                const __nv_bfloat16 va = *reinterpret_cast<const __nv_bfloat16*>(src + ((2 * c) * 4 + c2) * S::kVBytes + 2 * i);
-                const __nv_bfloat16 vb = *reinterpret_cast<const __nv_bfloat16*>(src + ((2 * c + 1) * 4 + c2) * S::kVBytes + 2 * i);
-                float* o = st.o[S::kVCh * y + i];
-                if (p0 != 0.0f) o[0] += p0 * __bfloat162float(va), o[1] += p0 * __bfloat162float(vb);
-                if (p1 != 0.0f) o[2] += p1 * __bfloat162float(va), o[3] += p1 * __bfloat162float(vb);
-              }
-            }
-            __syncwarp();  // these slots are other lanes' to fill again
-            continue;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-          mma16816(st.o[S::kVCh * y + 2 * i], a, __byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x5410));
-          mma16816(st.o[S::kVCh * y + 2 * i + 1], a, __byte_perm(w[0][i], w[1][i], 0x7632), __byte_perm(w[2][i], w[3][i], 0x7632));
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-          // Bytes (0, 1) of two tokens, then (2, 3): the even bytes of a word are two tokens' same channel.
-          const uint32_t lo01 = __byte_perm(w[0][i], w[1][i], 0x5410), hi01 = __byte_perm(w[0][i], w[1][i], 0x7632);
-          const uint32_t lo23 = __byte_perm(w[2][i], w[3][i], 0x5410), hi23 = __byte_perm(w[2][i], w[3][i], 0x7632);
-          float(*o)[4] = &st.o[S::kVCh * y + 4 * i];
-          mma16816(o[0], a, codes_to_bf16(lo01), codes_to_bf16(lo23));
-          mma16816(o[1], a, codes_to_bf16(lo01 >> 8), codes_to_bf16(lo23 >> 8));
-          mma16816(o[2], a, codes_to_bf16(hi01), codes_to_bf16(hi23));
-          mma16816(o[3], a, codes_to_bf16(hi01 >> 8), codes_to_bf16(hi23 >> 8));
-        }
+          for (int i = 0; i < S::kVBytes / 4; ++i) odd = odd || (w[y][t][i] & 0x7f80u) == 0x7f80u || (w[y][t][i] & 0x7f800000u) == 0x7f800000u;
+      if (__any_sync(0xffffffffu, odd)) {
+        const float weights[2][4] = {{s[2 * g][0], s[2 * g][1], s[2 * g][2], s[2 * g][3]}, {s[2 * g + 1][0], s[2 * g + 1][1], s[2 * g + 1][2], s[2 * g + 1][3]}};
+        fold_values_singly<D>(st, values, weights, lane);
+        continue;
       }
     }
+    auto packed = [](float x, float y) { return INT8 ? pack_f16(x, y) : pack_bf16(x, y); };
+    const uint32_t a[4] = {packed(s[2 * g][0], s[2 * g][1]), packed(s[2 * g][2], s[2 * g][3]), packed(s[2 * g + 1][0], s[2 * g + 1][1]),
+                           packed(s[2 * g + 1][2], s[2 * g + 1][3])};
+#pragma unroll
+    for (int y = 0; y < S::kVLoads; ++y)
+#pragma unroll
+      for (int i = 0; i < S::kVBytes / 4; ++i) {
+        const uint32_t(&v)[4][S::kVBytes / 4] = w[y];
+        if constexpr (INT8) {
+          // Bytes of two tokens by turns: (0, 1) of both, then (2, 3).
+          const uint2 lo01 = codes_to_f16(__byte_perm(v[0][i], v[1][i], 0x5140)), hi01 = codes_to_f16(__byte_perm(v[0][i], v[1][i], 0x7362));
+          const uint2 lo23 = codes_to_f16(__byte_perm(v[2][i], v[3][i], 0x5140)), hi23 = codes_to_f16(__byte_perm(v[2][i], v[3][i], 0x7362));
+          float(*o)[4] = &st.o[S::kVCh * y + 4 * i];
+          mma16816<true>(o[0], a, lo01.x, lo23.x);
+          mma16816<true>(o[1], a, lo01.y, lo23.y);
+          mma16816<true>(o[2], a, hi01.x, hi23.x);
+          mma16816<true>(o[3], a, hi01.y, hi23.y);
+        } else {
+          mma16816<false>(st.o[S::kVCh * y + 2 * i], a, __byte_perm(v[0][i], v[1][i], 0x5410), __byte_perm(v[2][i], v[3][i], 0x5410));
+          mma16816<false>(st.o[S::kVCh * y + 2 * i + 1], a, __byte_perm(v[0][i], v[1][i], 0x7632), __byte_perm(v[2][i], v[3][i], 0x7632));
+        }
+      }
   }
 }
 
-// PREFIX: grid (row tile, split, head); the tokens are the prefix's, the rows the whole batch's.
-// Otherwise: grid (row tile and, within its cluster of n_ctas, split; head; sequence); own tokens.
-template <int D, bool INT8, bool PREFIX>
-__global__ void __launch_bounds__(kThreads, 2) stream_kernel(const Params p, int n_ctas) {
+// The line, as a warp sees it: a lane has the length on it of the sequences before its slice of sequences
+// (of one head's and row tile's units), and the length of all.
+struct Line {
+  int64_t before, all;
+};
+__device__ __forceinline__ int slice_of(const Params& p) { return (p.batch + 31) / 32; }
+
+__device__ __forceinline__ Line sum_line(const Params& p, int lane) {
+  const int n = slice_of(p);
+  int64_t mine = 0;
+  for (int b = lane * n; b < min(p.batch, (lane + 1) * n); ++b) mine += length_of(stages_of(p, p.lens[b]));
+  int64_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  return {upto - mine, __shfl_sync(0xffffffffu, upto, 31)};
+}
+// Lengths of the prefix's part, of the whole line, and of each warp's piece of it.
+__device__ __forceinline__ int64_t prefix_length(const Params& p) { return (int64_t)length_of(p.prefix_stages) * p.h * p.prefix_row_tiles; }
+__device__ __forceinline__ int64_t line_length(const Params& p, const Line& line) {
+  return prefix_length(p) + line.all * p.h * p.own_row_tiles;
+}
+__device__ __forceinline__ int64_t piece_length(const Params& p, const Line& line) {
+  return max(quotient(line_length(p, line) + p.n_warps - 1, p.n_warps), (int64_t)kMinStages);
+}
+
+// A place on the line, `x` further than the warp's first: stage s of the n of unit `unit` of sequence b (-1:
+// of the prefix), units of one list counted head by head, row tile by row tile.
+struct Place {
+  int64_t x;
+  int b, unit, s, n, len;
+};
+// To the first stage of the next unit, which lies `skip` further.
+__device__ __forceinline__ void next_unit(const Params& p, Place& at, int skip) {
+  at.x += skip;
+  at.s = 0;
+  if (++at.unit < p.h * (at.b < 0 ? p.prefix_row_tiles : p.own_row_tiles)) return;
+  at.unit = 0;
+  do {
+    if (++at.b >= p.batch) {
+      at.x = INT64_MAX;  // the line's end
+      return;
+    }
+    at.len = own_len(p, p.lens[at.b]);
+    at.n = stages_of(p, at.len);
+  } while (at.n == 0);
+}
+__device__ __forceinline__ void advance(const Params& p, Place& at) {
+  ++at.x;
+  if (++at.s == at.n) next_unit(p, at, kUnitStages);
+}
+// The first stage at or past place x of the line (x inside it).
+__device__ __forceinline__ Place place_at(const Params& p, const Line& line, int64_t x) {
+  Place at;
+  at.x = 0;
+  const int64_t prefix = prefix_length(p);
+  int64_t rest = x;
+  if (x < prefix) {
+    at.b = -1, at.n = p.prefix_stages, at.len = p.prefix_len;
+  } else {
+    x -= prefix;
+    const int per = p.h * p.own_row_tiles;
+    const int lo = 31 - __clz(__ballot_sync(0xffffffffu, line.before * per <= x));  // the last slice that begins at or before x
+    int64_t before = __shfl_sync(0xffffffffu, line.before, lo);
+    for (at.b = lo * slice_of(p);; ++at.b) {
+      at.len = own_len(p, p.lens[at.b]);
+      at.n = stages_of(p, at.len);
+      if (x < (before + length_of(at.n)) * per) break;
+      before += length_of(at.n);
+    }
+    rest = x - before * per;
+  }
+  const int length = length_of(at.n);
+  at.unit = (int)quotient(rest, length);
+  at.s = (int)(rest - (int64_t)at.unit * length);
+  if (at.s >= at.n) next_unit(p, at, length - at.s);
+  return at;
+}
+
+template <int D, bool INT8>
+__global__ void __launch_bounds__(kThreads, (Shape<D, INT8>::kCtas)) stream_kernel(const Params p) {
   using S = Shape<D, INT8>;
   extern __shared__ __align__(128) char ring[];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, r = lane / 4, c = lane % 4;
-  // Launched after the prefix's kernel, which itself waited for what ran before it and only then let
-  // this one start, so the inputs are in place; alone, this one has to wait.
-  if (PREFIX || p.n_splits == 0) pdl_wait();
-  int tile, split, j, b = 0;
-  if constexpr (PREFIX) {
-    tile = blockIdx.x, split = blockIdx.y, j = blockIdx.z;
-    pdl_release();
-  } else {
-    split = blockIdx.x % n_ctas, tile = blockIdx.x / n_ctas, j = blockIdx.y, b = blockIdx.z;
+  pdl_wait();
+  pdl_release();
+  const Line line = sum_line(p, lane);
+  const int w = blockIdx.x * kWarps + warp;
+  const int64_t piece = piece_length(p, line), length = line_length(p, line);
+  const int64_t x0 = w * piece, n = min(piece, length - x0);  // this warp's places: x0 .. x0 + n - 1
+  // One unit's stages may fill the pieces of all four warps: then they are merged here.
+  bool whole = false;
+  Place at;
+  if ((w - warp) * piece < length) {
+    at = place_at(p, line, (w - warp) * piece);
+    whole = at.x == 0 && at.n - at.s >= kWarps * piece;
+    if (whole) at.s += (int)(warp * piece);
+    else if (warp > 0 && n > 0) at = place_at(p, line, x0);
   }
-  const int unit_rows = PREFIX ? p.rows : p.tokens * p.group;
-  const int row0 = tile * kRows, n_rows = min(kRows, unit_rows - row0);
-  // Tokens of the list that each of this lane's rows sees, the most that any row of the tile sees and the least.
-  const int32_t* table = PREFIX ? p.prefix_table : p.table + (int64_t)b * p.table_ld;
-  const int cols = PREFIX ? p.prefix_cols : p.table_cols;
-  int limit[2], end, low;
-  if constexpr (PREFIX) {
-    limit[0] = limit[1] = low = end = p.prefix_len;
-  } else {
-    const int64_t room = (int64_t)p.table_cols << p.page_shift;
-    const int len = (int)min((int64_t)max(p.lens[b], 0), room);
+  if (!whole && n <= 0) return;
+  Place ahead = at;
+  const uint32_t slots = (uint32_t)__cvta_generic_to_shared(ring) + warp * (S::kStages * S::kStageBytes);
+  const char* slots_p = ring + warp * (S::kStages * S::kStageBytes);
+  // Pages are looked up one stage before their copies start.
+  int id[S::kGran];
+  auto look_up = [&]() {
+    const int32_t* table = ahead.b < 0 ? p.prefix_table : p.table + (int64_t)ahead.b * p.table_ld;
+    const int cols = ahead.b < 0 ? p.prefix_cols : p.table_cols;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int t = min(row0 + r + 8 * i, unit_rows - 1) / p.group;
-      limit[i] = max(0, len - p.tokens + t + 1);
+    for (int g = 0; g < S::kGran; ++g) {
+      const int blk = (ahead.s * S::kTok + 16 * g) >> p.page_shift;
+      id[g] = blk < cols ? table[blk] : -1;
     }
-    low = max(0, len - p.tokens + row0 / p.group + 1);
-    end = max(0, len - p.tokens + (row0 + n_rows - 1) / p.group + 1);
-  }
-  // This CTA's stages; its warps take them in turn.
-  const int n_stages = (end + S::kTok - 1) / S::kTok;
-  const int share = max((n_stages + n_ctas - 1) / n_ctas, kWarps);
-  const int s_lo = min(split * share, n_stages), s_hi = min(s_lo + share, n_stages);
-  uint32_t qf[D / 16][4];
-  {
-    const __nv_bfloat16* at[2];
+  };
+  uint32_t have = 0;  // kGran bits per stage in flight, the oldest lowest
+  auto fetch = [&](int slot, int place) {
+    if (ahead.x >= n) {
+      copies_done();
+      return;
+    }
+    const int tiles = ahead.b < 0 ? p.prefix_row_tiles : p.own_row_tiles, j = tiles == 1 ? ahead.unit : ahead.unit / tiles;
+    have |= fill_stage<D, INT8>(p, j, id, ahead.s * S::kTok, ahead.len, slots + slot * S::kStageBytes, lane) << (place * S::kGran);
+    advance(p, ahead);
+    if (ahead.x < n) look_up();
+  };
+  if (ahead.x < n) look_up();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = r + 8 * i;
-      at[i] = nullptr;
-      if (row < n_rows) {
-        const int x = row0 + row, g = x % p.group, bt = x / p.group;
-        const int t = PREFIX ? bt % p.tokens : bt, bb = PREFIX ? bt / p.tokens : b;
-        at[i] = p.q + bb * p.q_sb + t * p.q_st + (int64_t)(j * p.group + g) * p.q_sh;
-      }
-    }
-    load_queries<D, INT8>(qf, at[0], at[1], c);
-  }
+  for (int i = 0; i < S::kStages - 1; ++i) fetch(i, i);
   State<D> st;
-  st.clear();
-  {
-    const char* mine = ring + warp * (S::kStages * S::kStageBytes);
-    const uint32_t mine_u = (uint32_t)__cvta_generic_to_shared(mine);
-    // Pages are looked up one stage before their copies start.
-    int page[S::kGran];
-    auto look_up = [&](int s) {
+  uint32_t qf[D / 16][4];
+  float scale[2];
+  int limit[2], low = 0, n_rows = 0, unit = 0;
+  bool fresh = true;
+  int slot = 0;
+  while (at.x < n) {
+    if (fresh) {
+      // The unit's rows, and the tokens that each of this lane's two sees.
+      const bool pre = at.b < 0;
+      const int tiles = pre ? p.prefix_row_tiles : p.own_row_tiles, j = at.unit / tiles, row0 = (at.unit % tiles) * kRows;
+      const int rows = pre ? p.rows : p.tokens * p.group;
+      n_rows = min(kRows, rows - row0);
+      unit = pre ? at.unit : p.h * p.prefix_row_tiles + at.b * p.h * p.own_row_tiles + at.unit;
+      const __nv_bfloat16* src[2];
 #pragma unroll
-      for (int g = 0; g < S::kGran; ++g) page[g] = s < s_hi && s * S::kTok + 16 * g < end ? page_at(table, cols, p.n_pages, s * S::kTok + 16 * g, p.page_shift) : -1;
-    };
-    uint32_t have[S::kStages];
-    int s = s_lo + warp;
-    look_up(s);
-#pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) {
-      have[i] = 0;
-      if (s + i * kWarps < s_hi) have[i] = fill_stage<D, INT8>(p, j, page, (s + i * kWarps) * S::kTok, end, mine_u + i * S::kStageBytes, lane);
-      else asm volatile("cp.async.commit_group;" ::: "memory");
-      look_up(s + (i + 1) * kWarps);
+      for (int k = 0; k < 2; ++k) {
+        const int x = min(row0 + r + 8 * k, rows - 1), g = x % p.group, bt = x / p.group, t = bt % p.tokens, b = pre ? bt / p.tokens : at.b;
+        src[k] = r + 8 * k < n_rows ? p.q + b * p.q_sb + t * p.q_st + (int64_t)(j * p.group + g) * p.q_sh : nullptr;
+        limit[k] = pre ? at.len : max(0, at.len - p.tokens + t + 1);
+      }
+      low = pre ? at.len : max(0, at.len - p.tokens + row0 / p.group + 1);
+      load_queries<D, INT8>(qf, scale, src[0], src[1], c, p.scale_log2);
+      st.clear();
+      fresh = false;
     }
-    have[S::kStages - 1] = 0;
-    int slot = 0;
-    for (; s < s_hi; s += kWarps) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
-      const int ahead = s + (S::kStages - 1) * kWarps, to = slot == 0 ? S::kStages - 1 : slot - 1;
-      uint32_t got = 0;
-      if (ahead < s_hi) got = fill_stage<D, INT8>(p, j, page, ahead * S::kTok, end, mine_u + to * S::kStageBytes, lane);
-      else asm volatile("cp.async.commit_group;" ::: "memory");
-      look_up(ahead + kWarps);
-      fold_stage<D, INT8>(st, qf, mine + slot * S::kStageBytes, s * S::kTok, limit, low, have[0], p.scale_log2, lane);
+    asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+    fetch(slot == 0 ? S::kStages - 1 : slot - 1, S::kStages - 1);
+    const uint32_t has = have & ((1u << S::kGran) - 1);
+    const int first = at.s * S::kTok;
+    if (low < first + S::kTok || has != (1u << S::kGran) - 1)
+      fold_stage<D, INT8, true>(st, qf, scale, slots_p + slot * S::kStageBytes, first, limit, has, lane);
+    else
+      fold_stage<D, INT8, false>(st, qf, scale, slots_p + slot * S::kStageBytes, first, limit, has, lane);
+    have >>= S::kGran;
+    slot = slot + 1 == S::kStages ? 0 : slot + 1;
+    if (at.s + 1 == at.n || at.x + 1 >= n) {
+      // The unit, or this warp's part of it, is done.
 #pragma unroll
-      for (int i = 0; i + 1 < S::kStages - 1; ++i) have[i] = have[i + 1];
-      have[S::kStages - 2] = got;
-      slot = slot + 1 == S::kStages ? 0 : slot + 1;
+      for (int k = 0; k < 2; ++k) {
+        st.l[k] += __shfl_xor_sync(0xffffffffu, st.l[k], 1);
+        st.l[k] += __shfl_xor_sync(0xffffffffu, st.l[k], 2);
+      }
+      if (whole) break;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int row = r + 8 * k;
+        if (row < n_rows) {
+          const int64_t to = (int64_t)(w + unit) * p.slot_rows + row;
+          if (c == 0) p.slot_ml[to] = make_float2(st.m[k], st.l[k]);
+          // Tiles kVCh y .. kVCh y + kVCh - 1 of columns 2 c and 2 c + 1 are 2 kVCh consecutive channels.
+#pragma unroll
+          for (int x = 0; x < D / 8; x += 4)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              *reinterpret_cast<float4*>(p.slot_o + to * D + S::channel(x, 2 * c + e)) =
+                  make_float4(st.o[x][2 * k + e], st.o[x + 1][2 * k + e], st.o[x + 2][2 * k + e], st.o[x + 3][2 * k + e]);
+        }
+      }
+      fresh = true;
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    advance(p, at);
   }
-  // The warps' states, then one per CTA: rows of D + 4 floats (o), and (m, l).
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (!whole) return;
+  // The four warps' states, in the ring, as one partial.
   __syncthreads();
   constexpr int kLd = D + 4;
-  float* po = reinterpret_cast<float*>(ring);                        // [kWarps][16][kLd]
-  float2* pml = reinterpret_cast<float2*>(po + kWarps * kRows * kLd);  // [kWarps][16]
-  float2* cml = pml + kWarps * kRows;                                 // [16], the CTA's
+  float* po = reinterpret_cast<float*>(ring);                          // [kWarps][kRows][kLd]
+  float2* pml = reinterpret_cast<float2*>(po + kWarps * kRows * kLd);  // [kWarps][kRows]
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 1);
-    st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 2);
-    if (c == 0) pml[warp * kRows + r + 8 * i] = make_float2(st.m[i], st.l[i]);
+  for (int k = 0; k < 2; ++k) {
+    const int row = warp * kRows + r + 8 * k;
+    if (c == 0) pml[row] = make_float2(st.m[k], st.l[k]);
+#pragma unroll
+    for (int x = 0; x < D / 8; x += 4)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        *reinterpret_cast<float4*>(po + row * kLd + S::channel(x, 2 * c + e)) =
+            make_float4(st.o[x][2 * k + e], st.o[x + 1][2 * k + e], st.o[x + 2][2 * k + e], st.o[x + 3][2 * k + e]);
   }
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) po[(warp * kRows + r + 8 * (e >> 1)) * kLd + S::channel(i, 2 * c + (e & 1))] = st.o[i][e];
   __syncthreads();
-  constexpr int kPer = D / 4;  // threads per row, a float4 each
-  for (int x = tid; x < n_rows * kPer; x += kThreads) {
-    const int row = x / kPer, ch = (x % kPer) * 4;
-    float m = -INFINITY;
+  for (int x = tid; x < n_rows * (D / 4); x += kThreads) {
+    const int row = x / (D / 4), ch = x % (D / 4) * 4;
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, pml[w * kRows + row].x);
-    const float from = m == -INFINITY ? 0.0f : m;  // nothing seen: every weight below is 0 (or NaN, which stays)
-    float l = 0.0f;
+    for (int i = 0; i < kWarps; ++i) m = fmaxf(m, pml[i * kRows + row].x);
+    const float from = m == -INFINITY ? 0.0f : m;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float2 ml = pml[w * kRows + row];
+    for (int i = 0; i < kWarps; ++i) {
+      const float2 ml = pml[i * kRows + row];
       const float f = ex2(ml.x - from);
-      const float4 v = *reinterpret_cast<const float4*>(po + (w * kRows + row) * kLd + ch);
+      const float4 v = *reinterpret_cast<const float4*>(po + (i * kRows + row) * kLd + ch);
       l += ml.y * f;
       o.x += v.x * f, o.y += v.y * f, o.z += v.z * f, o.w += v.w * f;
     }
-    if constexpr (PREFIX) {
-      const int64_t at = ((int64_t)split * p.h + j) * p.rows + row0 + row;
-      *reinterpret_cast<float4*>(p.part_o + at * D + ch) = o;
-      if (ch == 0) p.part_ml[at] = make_float2(m, l);
-    } else {
-      *reinterpret_cast<float4*>(po + row * kLd + ch) = o;  // warp 0's place: only this thread reads it
-      if (ch == 0) cml[row] = make_float2(m, l);
-    }
-  }
-  if constexpr (!PREFIX) {
-    cg::cluster_group cluster = cg::this_cluster();
-    if (n_ctas > 1) cluster.sync();
-    else __syncthreads();
-    if (p.n_splits > 0) pdl_wait();  // the prefix's partials
-    pdl_release();
-    for (int x = split * kThreads + tid; x < n_rows * kPer; x += n_ctas * kThreads) {
-      const int row = x / kPer, ch = (x % kPer) * 4, u = row0 + row;
-      float m = -INFINITY, l = 0.0f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      auto fold = [&](float2 ml, float4 v) {
-        const float top = fmaxf(m, ml.x), from = top == -INFINITY ? 0.0f : top, f = ex2(m - from), e = ex2(ml.x - from);
-        m = top;
-        l = l * f + ml.y * e;
-        o.x = o.x * f + v.x * e, o.y = o.y * f + v.y * e, o.z = o.z * f + v.z * e, o.w = o.w * f + v.w * e;
-      };
-      for (int i = 0; i < n_ctas; ++i) {
-        const float* src = n_ctas > 1 ? cluster.map_shared_rank(po, i) : po;
-        const float2* sml = n_ctas > 1 ? cluster.map_shared_rank(cml, i) : cml;
-        fold(sml[row], *reinterpret_cast<const float4*>(src + row * kLd + ch));
-      }
-      const int64_t prow = (int64_t)b * unit_rows + u, step = (int64_t)p.h * p.rows;
-      const float2* ml = p.part_ml + (int64_t)j * p.rows + prow;
-      const float* po2 = p.part_o + ((int64_t)j * p.rows + prow) * D + ch;
-      int i = 0;
-      for (; i + 8 <= p.n_splits; i += 8) {
-        float2 a[8];
-        float4 v[8];
-#pragma unroll
-        for (int y = 0; y < 8; ++y) a[y] = ml[(i + y) * step], v[y] = *reinterpret_cast<const float4*>(po2 + (i + y) * step * D);
-#pragma unroll
-        for (int y = 0; y < 8; ++y) fold(a[y], v[y]);
-      }
-      for (; i < p.n_splits; ++i) fold(ml[i * step], *reinterpret_cast<const float4*>(po2 + i * step * D));
-      const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // no key at all: 0; a NaN stays one
-      const int64_t at = ((int64_t)b * p.tokens + u / p.group) * (p.h * p.group) + j * p.group + u % p.group;
-      if (p.out_f32)
-        *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at * D + ch) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-      else
-        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at * D + ch) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
-      if (ch == 0) p.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
-    }
-    if (n_ctas > 1) cluster.sync();  // no CTA leaves while another reads its shared memory
+    const int64_t to = (int64_t)(w - warp + unit) * p.slot_rows + row;
+    if (ch == 0) p.slot_ml[to] = make_float2(m, l);
+    *reinterpret_cast<float4*>(p.slot_o + to * D + ch) = o;
   }
 }
 
-template <int D, bool INT8, bool PREFIX>
-cudaError_t launch_stream(const Params& p, dim3 grid, int cluster, int n_ctas, cudaStream_t st) {
+// A warp's sum over some partials of a row: lane `lane` has channels 4 (lane % (D / 4)) .., and where D is 64
+// one of the warp's halves every second partial.
+struct Sum {
+  float m, l;
+  float4 o;
+};
+__device__ __forceinline__ void fold(Sum& a, float m, float l, float4 o) {
+  const float top = fmaxf(a.m, m), from = top == -INFINITY ? 0.0f : top, f = ex2(a.m - from), e = ex2(m - from);
+  a.m = top;
+  a.l = a.l * f + l * e;
+  a.o.x = a.o.x * f + o.x * e, a.o.y = a.o.y * f + o.y * e, a.o.z = a.o.z * f + o.z * e, a.o.w = a.o.w * f + o.w * e;
+}
+
+// The slots of one unit, stages [x, x + n) of the line in pieces of `piece`: a warp each up to the first CTA
+// that the unit fills, then a slot per CTA (every kWarps), then a warp each again.
+struct Slots {
+  int first, heads, ctas, tails;
+};
+__device__ __forceinline__ Slots slots_of(int64_t x, int n, int64_t piece, int unit) {
+  if (n <= 0) return {0, 0, 0, 0};
+  const int w0 = (int)quotient(x, piece), w1 = (int)quotient(x + n - 1, piece);
+  const int c0 = (int)quotient(x + kWarps * piece - 1, kWarps * piece), c1 = (int)quotient(x + n, kWarps * piece);  // CTAs filled: c0 .. c1 - 1
+  if (c1 <= c0) return {w0 + unit, w1 - w0 + 1, 0, 0};
+  return {w0 + unit, c0 * kWarps - w0, c1 - c0, w1 + 1 - c1 * kWarps};
+}
+
+// The partials of every row: `team` warps (1, 2 or 4) per row of (sequence, KV head), kWarps / team rows a
+// CTA. Grid: (rows of a sequence and head by CTAs, head, sequence).
+template <int D>
+__global__ void __launch_bounds__(kThreads, 4) combine_kernel(const Params p, int team) {
+  __shared__ Sum sums[kWarps][32];
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int j = blockIdx.y, b = blockIdx.z, unit_rows = p.tokens * p.group;
+  const int row = blockIdx.x * (kWarps / team) + warp / team, part = warp % team;
+  const bool live = row < unit_rows;
+  // The lengths are this call's input, in place since before the launches in front of this one began
+  // (where there are none, they have to be waited for).
+  const bool alone = p.n_warps == 0 && p.n_splits == 0;
+  if (alone) pdl_wait();
+  Slots own = {0, 0, 0, 0}, pre = {0, 0, 0, 0};  // the row's own unit, and the prefix's where that is streamed
+  if (p.n_warps > 0) {
+    const Line line = sum_line(p, lane);
+    const int64_t piece = piece_length(p, line);
+    const int n = stages_of(p, p.lens[b]), slice = b / slice_of(p);
+    int64_t before = __shfl_sync(0xffffffffu, line.before, slice);
+    for (int i = slice * slice_of(p); i < b; ++i) before += length_of(stages_of(p, p.lens[i]));
+    int unit = j * p.own_row_tiles + row / kRows;
+    own = slots_of(prefix_length(p) + before * p.h * p.own_row_tiles + (int64_t)unit * length_of(n), n, piece,
+                   p.h * p.prefix_row_tiles + b * p.h * p.own_row_tiles + unit);
+    unit = j * p.prefix_row_tiles + (b * unit_rows + row) / kRows;
+    pre = slots_of((int64_t)unit * length_of(p.prefix_stages), p.prefix_stages, piece, unit);
+  }
+  if (!alone) pdl_wait();
+  pdl_release();
+  // All partials of the row as one list: the tiled prefix's, the own ones, the streamed prefix's. Partial
+  // rows are numbered through the workspace, the tiled ones first.
+  const int64_t tiled = (int64_t)p.n_splits * p.h * p.rows;
+  auto row_of = [&](int i) -> int64_t {
+    if (i < p.n_splits) return ((int64_t)i * p.h + j) * p.rows + (int64_t)b * unit_rows + row;
+    i -= p.n_splits;
+    const int n_own = own.heads + own.ctas + own.tails;
+    const bool mine = i < n_own;
+    const Slots x = mine ? own : pre;
+    if (!mine) i -= n_own;
+    if (i >= x.heads) i = i < x.heads + x.ctas ? x.heads + (i - x.heads) * kWarps : i + x.ctas * (kWarps - 1);
+    return tiled + (int64_t)(x.first + i) * p.slot_rows + (mine ? row : b * unit_rows + row) % kRows;
+  };
+  const int n_parts = p.n_splits + own.heads + own.ctas + own.tails + pre.heads + pre.ctas + pre.tails;
+  constexpr int kLanes = D / 4, kTogether = 32 / kLanes;  // partials side by side in the warp
+  const int ch = 4 * (lane % kLanes), side = lane / kLanes;
+  Sum a = {-INFINITY, 0.0f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  // 32 at a time: references and sums, one per lane, then the outputs with weights that are known.
+  for (int base = part; live && base < n_parts; base += 32 * team) {
+    const int mine = base + lane * team;
+    const int64_t from_row = row_of(min(mine, n_parts - 1));
+    float2 x = make_float2(-INFINITY, 0.0f);
+    if (mine < n_parts) x = p.tile_ml[from_row];
+    const int count = min(32, (n_parts - base + team - 1) / team);
+    float top = x.x;
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+    top = fmaxf(top, a.m);
+    const float from = top == -INFINITY ? 0.0f : top, f = ex2(a.m - from), by = ex2(x.x - from);
+    float l = x.y * by;
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+    a.m = top;
+    a.l = a.l * f + l;
+    a.o.x *= f, a.o.y *= f, a.o.z *= f, a.o.w *= f;
+#pragma unroll 1
+    for (int i = 0; i < count; i += 8 * kTogether) {
+      float4 v[8];
+      float weight[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int which = i + k * kTogether + side;
+        const int64_t at = __shfl_sync(0xffffffffu, from_row, which & 31);
+        weight[k] = __shfl_sync(0xffffffffu, by, which & 31);
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (which < count) v[k] = *reinterpret_cast<const float4*>(p.tile_o + at * D + ch);
+        else weight[k] = 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        a.o.x += v[k].x * weight[k], a.o.y += v[k].y * weight[k], a.o.z += v[k].z * weight[k], a.o.w += v[k].w * weight[k];
+    }
+  }
+  if constexpr (D == 64) {  // the two halves of the warp share m and l and have half of the outputs each
+    a.o.x += __shfl_xor_sync(0xffffffffu, a.o.x, 16), a.o.y += __shfl_xor_sync(0xffffffffu, a.o.y, 16);
+    a.o.z += __shfl_xor_sync(0xffffffffu, a.o.z, 16), a.o.w += __shfl_xor_sync(0xffffffffu, a.o.w, 16);
+  }
+  if (team > 1) {
+    sums[warp][lane] = a;
+    __syncthreads();
+    if (part == 0)
+      for (int i = 1; i < team; ++i) {
+        const Sum x = sums[warp + i][lane];
+        fold(a, x.m, x.l, x.o);
+      }
+  }
+  if (!live || part != 0 || lane >= D / 4) return;
+  const float inv = a.l > 0.0f ? 1.0f / a.l : a.l == 0.0f ? 0.0f : a.l;  // no key at all: 0; a NaN stays one
+  const int64_t at = ((int64_t)b * p.tokens + row / p.group) * (p.h * p.group) + j * p.group + row % p.group;
+  const float4 o = make_float4(a.o.x * inv, a.o.y * inv, a.o.z * inv, a.o.w * inv);
+  if (p.out_f32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at * D + 4 * lane) = o;
+  else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at * D + 4 * lane) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+  if (lane == 0) p.lse[at] = a.l == 0.0f ? -INFINITY : (a.m + log2f(a.l)) * kLn2;
+}
+
+template <int D, bool INT8>
+cudaError_t launch_stream(const Params& p, cudaStream_t st) {
   using S = Shape<D, INT8>;
-  constexpr int kMerge = kWarps * kRows * (D + 4) * 4 + (kWarps + 1) * kRows * 8;
-  constexpr int kSmem = S::kRing > kMerge ? S::kRing : kMerge;
-  auto k = stream_kernel<D, INT8, PREFIX>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  auto k = stream_kernel<D, INT8>;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kRing);
   if (e != cudaSuccess) return e;
-  return launch_pdl(k, grid, dim3(kThreads), kSmem, st, cluster, p, n_ctas);
+  return launch_pdl(k, dim3(p.n_warps / kWarps), dim3(kThreads), S::kRing, st, 0, p);
 }
 
-// Batches of at most this many rows per KV head take the prefix through stream_kernel, one row tile.
-bool streams(int rows) { return rows <= kRows; }
+// Batches of at most this many rows per KV head stream the prefix, one row tile.
+bool streams(int64_t rows) { return rows <= kRows; }
 
-// Splits of the prefix: enough CTAs for two on each SM, no split shorter than two stages per warp.
-int prefix_splits(int rows, int h, int64_t prefix_len, int d) {
-  if (prefix_len <= 0) return 0;
-  if (!streams(rows)) return tile_splits(rows, h, prefix_len);
-  const int tok = stage_tokens(d);
-  const int64_t tiles = (rows + kRows - 1) / kRows, most = (prefix_len + 2 * kWarps * tok - 1) / (2 * kWarps * tok);
-  int64_t n = (2 * kNumSMs) / (tiles * h);
-  if (n < 1) n = 1;
-  if (n > most) n = most;
-  return (int)n;
+// How a call is cut up: Params' numbers that follow from the shapes alone, and the workspace they take.
+struct Plan {
+  int n_splits, prefix_stages, prefix_row_tiles, own_row_tiles, n_warps, slot_rows;
+  size_t tile_floats, slot_count;
+  size_t bytes(int d, int64_t rows, int h) const {
+    return (size_t)n_splits * h * rows * ((size_t)d * 4 + 8) + slot_count * slot_rows * ((size_t)d * 4 + 8);
+  }
+};
+
+Plan plan_of(int batch, int tokens, int hq, int h, int d, int64_t prefix_len, int kind, int64_t own_reach) {
+  Plan x = {};
+  const int64_t unit = (int64_t)tokens * (hq / h), rows = batch * unit;
+  const int shift = stage_shift_of(d);
+  const bool stream_prefix = prefix_len > 0 && streams(rows);
+  if (prefix_len > 0 && !stream_prefix) x.n_splits = tile_splits((int)rows, h, prefix_len);
+  x.own_row_tiles = (int)((unit + kRows - 1) / kRows);
+  if (stream_prefix) {
+    x.prefix_stages = (int)((prefix_len + (1 << shift) - 1) >> shift);
+    x.prefix_row_tiles = (int)((rows + kRows - 1) / kRows);
+  }
+  // Warps for as many stages as there can be, up to all that the GPU holds at once.
+  const int64_t most = (int64_t)x.prefix_stages * h * x.prefix_row_tiles + ((own_reach + (1 << shift) - 1) >> shift) * batch * h * x.own_row_tiles;
+  const int64_t room = (int64_t)kNumSMs * (kind == LKV_CACHE_INT8 ? 3 : 2) * kWarps;
+  int64_t warps = (most + kMinStages - 1) / kMinStages;
+  warps = warps < room ? (warps + kWarps - 1) / kWarps * kWarps : room;
+  x.n_warps = (int)warps;
+  x.slot_rows = (int)(stream_prefix && rows > unit ? (rows < kRows ? rows : kRows) : (unit < kRows ? unit : kRows));
+  x.slot_count = x.n_warps == 0 ? 0 : (size_t)x.n_warps + (size_t)h * x.prefix_row_tiles + (size_t)batch * h * x.own_row_tiles;
+  return x;
 }
 
 }  // namespace
@@ -542,10 +789,9 @@ using namespace lkv::prefix;
 
 extern "C" {
 
-size_t lkv_prefix_attention_workspace(int batch, int tokens, int hq, int h, int d, int64_t prefix_len) {
-  if (batch < 1 || tokens < 1 || h < 1 || hq < h || prefix_len < 1) return 0;
-  const int64_t rows = (int64_t)batch * tokens * (hq / h);
-  return (size_t)prefix_splits((int)rows, h, prefix_len, d) * h * rows * ((size_t)d * 4 + 8);
+size_t lkv_prefix_attention_workspace(int batch, int tokens, int hq, int h, int d, int64_t prefix_len, int kind, int64_t own_reach) {
+  if (batch < 1 || tokens < 1 || h < 1 || hq < h || prefix_len < 0 || own_reach < 0 || (d != 64 && d != 128)) return 0;
+  return plan_of(batch, tokens, hq, h, d, prefix_len, kind, own_reach).bytes(d, (int64_t)batch * tokens * (hq / h), h);
 }
 
 int lkv_prefix_attention(const lkv_prefix_args* a, void* stream) {
@@ -590,39 +836,45 @@ int lkv_prefix_attention(const lkv_prefix_args* a, void* stream) {
   p.prefix_len = (int)a->prefix_len;
   p.scale_log2 = a->scale * kLog2e;
   p.rows = (int)rows;
-  p.n_splits = prefix_splits(p.rows, a->h, a->prefix_len, a->d);
+  const int64_t reach = (int64_t)a->table_cols * a->bs;
+  const Plan plan = plan_of(a->batch, a->tokens, a->hq, a->h, a->d, a->prefix_len, a->kind, reach);
+  p.n_splits = plan.n_splits;
+  p.stage_shift = stage_shift_of(a->d);
+  p.prefix_stages = plan.prefix_stages;
+  p.prefix_row_tiles = plan.prefix_row_tiles;
+  p.own_row_tiles = plan.own_row_tiles;
+  p.n_warps = plan.n_warps;
+  p.slot_rows = plan.slot_rows;
   p.out = a->out;
   p.out_f32 = a->out_dtype == LKV_F32;
   p.lse = a->lse;
-  if (p.n_splits > 0) {
-    const size_t need = lkv_prefix_attention_workspace(a->batch, a->tokens, a->hq, a->h, a->d, a->prefix_len);
+  const size_t need = plan.bytes(a->d, rows, a->h);
+  if (need > 0) {
     if (a->workspace_bytes < need) return fail(LKV_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, a->workspace_bytes, need);
     if (a->workspace == nullptr || !aligned(a->workspace, 16)) return fail(LKV_ERR_PTR, "%s: workspace must be 16-byte aligned", who);
-    p.part_o = static_cast<float*>(a->workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)p.n_splits * a->h * rows * a->d);
+    const size_t tiled = (size_t)p.n_splits * a->h * rows, slots = plan.slot_count * plan.slot_rows;
+    p.tile_o = static_cast<float*>(a->workspace);
+    p.slot_o = p.tile_o + tiled * a->d;
+    p.tile_ml = reinterpret_cast<float2*>(p.slot_o + slots * a->d);
+    p.slot_ml = p.tile_ml + tiled;
   }
   cudaStream_t st = as_stream(stream);
   const bool int8 = a->kind == LKV_CACHE_INT8, wide = a->d == 128;
   cudaError_t e = cudaSuccess;
-  if (p.n_splits > 0 && !streams(p.rows)) {
-    if (int rc = run_tiles(p, a->d, int8, st)) return rc;
-  } else if (p.n_splits > 0) {
-    const int tiles = (p.rows + kRows - 1) / kRows;
-    if (p.n_splits > 65535) return fail(LKV_ERR_ARG, "%s: prefix too long", who);
-    const dim3 grid(tiles, p.n_splits, a->h);
-    e = wide ? (int8 ? launch_stream<128, true, true>(p, grid, 0, p.n_splits, st) : launch_stream<128, false, true>(p, grid, 0, p.n_splits, st))
-             : (int8 ? launch_stream<64, true, true>(p, grid, 0, p.n_splits, st) : launch_stream<64, false, true>(p, grid, 0, p.n_splits, st));
-    if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "%s (prefix): %s", who, cudaGetErrorString(e));
+  if (p.n_warps > 0) {
+    e = wide ? (int8 ? launch_stream<128, true>(p, st) : launch_stream<128, false>(p, st))
+             : (int8 ? launch_stream<64, true>(p, st) : launch_stream<64, false>(p, st));
+    if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "%s (stream): %s", who, cudaGetErrorString(e));
+    p.stream_first = 1;
   }
-  const int unit = a->tokens * group, tiles = (unit + kRows - 1) / kRows;
-  // Own tokens: more CTAs per (sequence, head, row tile) while they all stay resident and the tables
-  // could hold at least 512 tokens for each; how many tokens there are only the device knows.
-  int c = 1;
-  while (c < kMaxCluster && (int64_t)a->batch * a->h * tiles * c * 2 <= 2 * kNumSMs && (int64_t)a->table_cols * a->bs >= 512 * 2 * c) c *= 2;
-  const dim3 grid(tiles * c, a->h, a->batch);
-  e = wide ? (int8 ? launch_stream<128, true, false>(p, grid, c > 1 ? c : 0, c, st) : launch_stream<128, false, false>(p, grid, c > 1 ? c : 0, c, st))
-           : (int8 ? launch_stream<64, true, false>(p, grid, c > 1 ? c : 0, c, st) : launch_stream<64, false, false>(p, grid, c > 1 ? c : 0, c, st));
-  if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+  if (p.n_splits > 0)
+    if (int rc = run_tiles(p, a->d, int8, st)) return rc;
+  // Several warps to a row where it has many partials.
+  const int parts = p.n_splits + (p.prefix_stages > 0 ? p.n_warps / (kWarps * a->h) : 0), team = parts > 16 ? 4 : parts > 8 ? 2 : 1;
+  const int unit = a->tokens * group, per = kWarps / team;
+  const dim3 grid((unit + per - 1) / per, a->h, a->batch);
+  e = wide ? launch_pdl(combine_kernel<128>, grid, dim3(kThreads), 0, st, 0, p, team) : launch_pdl(combine_kernel<64>, grid, dim3(kThreads), 0, st, 0, p, team);
+  if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "%s (combine): %s", who, cudaGetErrorString(e));
   return LKV_OK;
 }
 

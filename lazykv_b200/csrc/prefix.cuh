@@ -1,6 +1,8 @@
-// What the kernels of the shared-prefix attention have in common: the call's parameters, the layout of
-// the prefix's partials, and small device helpers.
+// What the kernels of the shared-prefix attention have in common: the call's parameters, the order of the
+// streamed work, the layout of the partials, and small device helpers.
 #pragma once
+
+#include <cuda_fp16.h>
 
 #include "common.cuh"
 
@@ -9,7 +11,17 @@ namespace prefix {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kRows = 16;       // rows of an mma.sync tile
+constexpr int kMinStages = 2;   // stages of the stream that a warp takes at least
+// A unit's start (its queries) and end (its partial) count as this many stages more on the line, or the
+// warps that get many short lists would set the time.
+constexpr int kUnitStages = 3;
 
+// The streamed work (prefix.cu). A unit is one tile of kRows query rows of one KV head against one list
+// of tokens: first the prefix's units (head, row tile of the whole batch), where the prefix is streamed,
+// then the sequences' own (sequence, head, row tile). A unit has a stage per 2^stage_shift tokens. All
+// units in this order are one line, of which every warp takes an equal piece; a unit is as long on it as
+// its stages and kUnitStages, an empty list's has no length.
 struct Params {
   const __nv_bfloat16* q;  // [batch, tokens, hq, d], element strides, channels contiguous
   int64_t q_sb, q_st, q_sh;
@@ -25,14 +37,25 @@ struct Params {
   int prefix_cols;
   int prefix_len;
   float scale_log2;  // the softmax scale times log2(e): scores live in the log2 domain
-  // Partials of the prefix, per (split, KV head, row): row r = (b * tokens + t) * group + g.
-  int rows;        // batch * tokens * group
-  int n_splits;    // 0: no prefix
-  float* part_o;   // [n_splits][h][rows][d], not yet divided by the sum
-  float2* part_ml; // [n_splits][h][rows]: (running maximum in the log2 domain, sum)
-  void* out;       // [batch, tokens, hq, d]
+  int rows;          // batch * tokens * group; row (b * tokens + t) * group + g
+  // Tiled prefix (prefix_tile.cu): partials per (split, KV head, row).
+  int n_splits;  // 0: no prefix, or a streamed one
+  float* tile_o;    // [n_splits][h][rows][d], not yet divided by the sum
+  float2* tile_ml;  // [n_splits][h][rows]: (reference in the log2 domain, sum)
+  // Streamed work: a partial per (warp, unit) that meet, in slot warp + unit; where one unit fills the four
+  // warps of a CTA, one partial for all of them, in its first warp's slot.
+  int stage_shift;       // log2 of the tokens per stage
+  int prefix_stages;     // stages of a streamed prefix (0: tiled, or none)
+  int prefix_row_tiles;  // row tiles of the whole batch, of a streamed prefix
+  int own_row_tiles;     // row tiles of a sequence's tokens * group rows
+  int n_warps;           // 0: nothing is streamed
+  int slot_rows;         // rows a slot holds
+  float* slot_o;         // [slots][slot_rows][d]
+  float2* slot_ml;       // [slots][slot_rows]
+  void* out;             // [batch, tokens, hq, d]
   int out_f32;
-  float* lse;      // [batch, tokens, hq]
+  float* lse;            // [batch, tokens, hq]
+  int stream_first;      // the tiled prefix runs behind a stream launch
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -45,22 +68,40 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&b);
 }
-
-// Two int8 codes as bf16, exactly: bytes 0 and 2 of `w` (the others are ignored). With c = l - 128 f,
-// l the low seven bits and f the sign bit, 0x4300 | l is 128 + l and 0x4300 | (f << 7) is 128 + 128 f.
-__device__ __forceinline__ uint32_t codes_to_bf16(uint32_t w) {
-  const uint32_t a = (w & 0x007f007fu) | 0x43004300u, s = (w & 0x00800080u) | 0x43004300u;
-  const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&s));
-  return *reinterpret_cast<const uint32_t*>(&x);
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 b = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
 }
 
-// The page of token pos of a page list, or -1 where it has none.
-__device__ __forceinline__ int page_at(const int32_t* table, int cols, int n_pages, int pos, int shift) {
-  const int blk = pos >> shift;
-  if (blk >= cols) return -1;
-  const int id = table[blk];
-  return id < n_pages ? id : -1;
+// Four int8 codes as f16, exactly: byte b with its sign bit turned is u = code + 128, and 0x6400 | u is
+// 1024 + u. `u`: four such bytes.
+__device__ __forceinline__ uint2 biased_to_f16(uint32_t u) {
+  const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+  const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
+__device__ __forceinline__ uint2 codes_to_f16(uint32_t w) { return biased_to_f16(w ^ 0x80808080u); }
+
+// For queries against int8 pages: the power of two 2^-e that brings a row's largest magnitude (its bf16
+// bits) to [1, 2), and 2^e, which its scores have to be multiplied with. Both are normal numbers; an
+// infinity or a NaN is what it is at any scale.
+__device__ __forceinline__ float2 row_scales(uint32_t top_bits) {
+  int e = (int)(top_bits >> 7) - 127;
+  e = e > 126 ? 126 : e < -126 ? -126 : e;
+  return make_float2(__int_as_float((127 - e) << 23), __int_as_float((127 + e) << 23));
+}
+
+// Stages of sequence b's own tokens (lens may lie outside [0, the table's reach]).
+__device__ __forceinline__ int own_len(const Params& p, int len) {
+  return (int)min((int64_t)max(len, 0), (int64_t)p.table_cols << p.page_shift);
+}
+__device__ __forceinline__ int stages_of(const Params& p, int len) { return (own_len(p, len) + (1 << p.stage_shift) - 1) >> p.stage_shift; }
+// a / b for 0 <= a, 0 < b (the line is rarely longer than 2^32 stages).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+__device__ __forceinline__ int length_of(int stages) { return stages > 0 ? stages + kUnitStages : 0; }
 
 // prefix_tile.cu: the prefix's partials for many rows, and how many splits of the prefix they take.
 int tile_splits(int rows, int h, int64_t prefix_len);

@@ -8,7 +8,7 @@
 // memory, V from shared memory) accumulates in tensor memory. The two tiles alternate, so that one
 // computes weights while the tensor core works for the other. With 128 rows or fewer both tiles are the
 // same queries and take the prefix's tiles in turn; their results are merged at the end. Each CTA writes
-// one partial (m, l, o) per row, which stream_kernel (prefix.cu) folds into the output.
+// one partial (m, l, o) per row, which combine_kernel (prefix.cu) folds into the output.
 //
 // Warps 0-3 and 4-7 are the two tiles' rows, warp 8 issues the matrix products, warp 9 the copies; with
 // int8 pages warps 12-19 turn codes into f16 operands. All of it is joined by mbarriers, every wait
@@ -101,6 +101,14 @@ __device__ __forceinline__ bool wait_long(Barriers& s, uint64_t* bar, uint32_t p
 __device__ __forceinline__ bool wait_for(Barriers& s, uint64_t* bar, uint32_t parity) { return try_once(bar, parity) || wait_long(s, bar, parity); }
 
 __device__ __forceinline__ int largest(const int32_t (&x)[4]) { return max(max(x[0], x[1]), max(x[2], x[3])); }
+
+// The page of token pos of a page list, or -1 where it has none.
+__device__ __forceinline__ int page_at(const int32_t* table, int cols, int n_pages, int pos, int shift) {
+  const int blk = pos >> shift;
+  if (blk >= cols) return -1;
+  const int id = table[blk];
+  return id < n_pages ? id : -1;
+}
 
 // One arrival for the warp, after what all of its lanes did before.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
@@ -217,20 +225,6 @@ __device__ __forceinline__ void st_packed(uint32_t addr, const uint32_t (&w)[2][
 }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 b = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&b);
-}
-
-// Four int8 codes as f16, exactly: byte b with its sign bit turned is u = code + 128, and 0x6400 | u is
-// 1024 + u.
-__device__ __forceinline__ uint2 codes_to_f16(uint32_t w) {
-  const uint32_t u = w ^ 0x80808080u, a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-  const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
-  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
-  return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-}
-
 __device__ __forceinline__ uint2 times(uint2 x, __half2 by) {
   const __half2 a = __hmul2(*reinterpret_cast<const __half2*>(&x.x), by), b = __hmul2(*reinterpret_cast<const __half2*>(&x.y), by);
   return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
@@ -255,12 +249,9 @@ __device__ __forceinline__ float stage_query(const __nv_bfloat16* row, char* til
 #pragma unroll
       for (int k = 0; k < 4; ++k) top = max(top, max(x[k] & 0x7fffu, (x[k] >> 16) & 0x7fffu));
     }
-    // The exponent e of the largest magnitude, kept where both 2^-e and 2^e are normal numbers. An
-    // infinity or NaN is what it is at any scale.
-    int e = (int)(top >> 7) - 127;
-    e = e > 126 ? 126 : e < -126 ? -126 : e;
-    const float down = __int_as_float((127 - e) << 23);
-    back = __int_as_float((127 + e) << 23);
+    const float2 by = row_scales(top);
+    const float down = by.x;
+    back = by.y;
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) {
       uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
@@ -323,7 +314,9 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
   __syncthreads();
   tc_after();
   const uint32_t tmem = s.tmem;  // columns: S or P of the two row tiles at 0 and 128, O at 256 and 256 + D
-  pdl_wait();
+  // Behind the stream's launch, which itself waited for what ran before it and only then let this one
+  // start, the inputs are in place; first of all, this launch has to wait. The stream is waited for at the end.
+  if (!p.stream_first) pdl_wait();
   pdl_release();
 
   if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kMany));
@@ -548,7 +541,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
             const float2 other = *reinterpret_cast<const float2*>(swap + (base + 8 * i) * kLd + ch);
             o.x = o.x * f0[i] + other.x * f1[i], o.y = o.y * f0[i] + other.y * f1[i];
           }
-          if (base + 8 * i < n_rows) *reinterpret_cast<float2*>(p.part_o + (at + 8 * i) * D + ch) = o;
+          if (base + 8 * i < n_rows) *reinterpret_cast<float2*>(p.tile_o + (at + 8 * i) * D + ch) = o;
         }
       }
       ok = ok && *static_cast<volatile int*>(&s.quit) == 0;
@@ -556,7 +549,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       if (c2 == 0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (base + 8 * i < n_rows) p.part_ml[at + 8 * i] = ok ? make_float2(from[i], l[i]) : make_float2(0.0f, __uint_as_float(0x7fc00000u));
+          if (base + 8 * i < n_rows) p.tile_ml[at + 8 * i] = ok ? make_float2(from[i], l[i]) : make_float2(0.0f, __uint_as_float(0x7fc00000u));
       }
     }
     tc_before();
@@ -778,6 +771,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
     }
   }
   __syncthreads();
+  if (p.stream_first) pdl_wait();  // what comes after this launch may read the stream's partials too
   if (warp == 8) {
     tc_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");

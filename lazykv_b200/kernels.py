@@ -537,7 +537,7 @@ def prefix_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tens
                      scale: float, scales: torch.Tensor | None = None, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
                      lse: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Attention of query [batch, T, hq, d] (bfloat16) for a batch that shares a prefix, whose pages are
-    read once for all (lkv_prefix_attention, two launches). Query t of sequence b attends the prefix_len
+    read once for all (lkv_prefix_attention, two or three launches). Query t of sequence b attends the prefix_len
     tokens of the pages that prefix_table [columns] lists, and the first lens[b] - T + t + 1 of its own
     lens[b] tokens in the pages of table[b]: the step's T tokens (drafted ones included) are written
     before the call and are the last of lens[b].
@@ -570,7 +570,7 @@ def prefix_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tens
         lse = torch.empty((batch, t, hq), dtype=torch.float32, device=dev)
     elif lse.shape != (batch, t, hq) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise ValueError(f"prefix_attention: lse must be a contiguous float32 {(batch, t, hq)}")
-    nbytes = L.lib().lkv_prefix_attention_workspace(batch, t, hq, h, d, prefix_len)
+    nbytes = L.lib().lkv_prefix_attention_workspace(batch, t, hq, h, d, prefix_len, kind, table.shape[1] * bs)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     args = L.PrefixArgs(query.data_ptr(), L.LKV_BF16, query.stride(0), query.stride(1), query.stride(2), pages.data_ptr(), kind, ptr(scales), n, bs,
                         batch, t, hq, h, d, table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(), prefix_table.data_ptr(), cols,

@@ -92,10 +92,11 @@ def test_attention_of_nothing_and_its_workspace(lib) -> None:  # noqa: ANN001
     assert lib.lkv_prefix_attention(None, None) == 2 and "null" in _lib.last_error()
     assert lib.lkv_prefix_attention(ctypes.byref(_args(batch=0)), None) == 0
     assert lib.lkv_prefix_attention(ctypes.byref(_args(tokens=0)), None) == 0
-    assert lib.lkv_prefix_attention_workspace(4, 1, 32, 8, 128, 0) == 0  # no prefix, no partials
-    one = lib.lkv_prefix_attention_workspace(4, 1, 32, 8, 128, 1)
+    assert lib.lkv_prefix_attention_workspace(4, 1, 32, 8, 128, 0, 0, 0) == 0  # nothing to attend, no partials
+    one = lib.lkv_prefix_attention_workspace(4, 1, 32, 8, 128, 1, 0, 0)
     assert one >= 4 * 32 * (128 * 4 + 8)
-    assert lib.lkv_prefix_attention_workspace(4, 1, 32, 8, 128, 100_000) > one
+    assert lib.lkv_prefix_attention_workspace(4, 1, 32, 8, 128, 1, 0, 1000) > one
+    assert lib.lkv_prefix_attention_workspace(4, 1, 32, 8, 128, 100_000, 0, 0) > one
 
 
 def _verify(lib, target=FAKE, tokens=FAKE, uniforms=FAKE, batch=2, k=3, vocab=100, kept=FAKE, token=FAKE):  # noqa: ANN001, ANN202
