@@ -579,18 +579,35 @@ typedef enum { LKV_CACHE_MODEL = 0, LKV_CACHE_INT8 = 1 } lkv_cache_kind;
  * FLT_MIN), at most what keeps 127 s finite, and its codes the whole numbers nearest to x / s (halfway: even); a row that holds an
  * infinity or a NaN gets the scale NaN. Model dtype: copied. batch * tokens * h < 2^31.
  */
-int lkv_paged_write(const void* keys, int64_t k_sb, int64_t k_st, int64_t k_sh, const void* values, int64_t v_sb, int64_t v_st, int64_t v_sh,
-                    int dtype, int batch, int tokens, int h, int d, void* pages, int kind, float* scales, int64_t n_pages, int bs,
-                    const int32_t* table, int64_t table_ld, int table_cols, const int32_t* starts, void* stream);
+typedef struct {
+  /* The tokens written: [batch, tokens, h, d], element strides, channels contiguous. */
+  const void* keys;
+  const void* values;
+  int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  int dtype; /* of the tokens written or read back, and of model-dtype pages */
+  int batch, tokens, h, d;
+  void* pages;
+  int kind;
+  float* scales;
+  int64_t n_pages;
+  int bs;
+  const int32_t* table;
+  int64_t table_ld;
+  int table_cols;
+  const int32_t* starts;
+  /* The tokens read back. */
+  const int32_t* lens;
+  void* out_k;
+  void* out_v;
+} lkv_paged_args;
+int lkv_paged_write(const lkv_paged_args* args, void* stream);
 
 /*
  * Reads tokens starts[b] .. starts[b] + tokens - 1 of every sequence back as out_k, out_v [batch,
- * tokens, h, d] in dtype (model-dtype pages: that dtype): code * scale, rounded once. Tokens at or past
+ * tokens, h, d], contiguous, in dtype (model-dtype pages: that dtype): code * scale, rounded once. Tokens at or past
  * lens[b] (where lens is given) and tokens without a page are zeros.
  */
-int lkv_paged_read(const void* pages, int kind, const float* scales, int64_t n_pages, int bs, int batch, int tokens, int h, int d,
-                   const int32_t* table, int64_t table_ld, int table_cols, const int32_t* starts, const int32_t* lens, void* out_k, void* out_v,
-                   int dtype, void* stream);
+int lkv_paged_read(const lkv_paged_args* args, void* stream);
 
 /*
  * Attention of a batch whose sequences share a prefix (no reference counterpart). Query t of sequence b
@@ -642,9 +659,20 @@ int lkv_prefix_attention(const lkv_prefix_args* args, void* stream);
  * [0, vocab) ends its sequence's drafts (as if all before it had been all). token[b] = -1 where the
  * weights are all 0 or have no finite sum. vocab <= 4,194,304.
  */
-int lkv_verify_drafts(const float* target, int64_t p_sb, int64_t p_st, const float* draft, int64_t q_sb, int64_t q_st, const int64_t* tokens,
-                      int64_t t_sb, const float* uniforms, int64_t u_sb, int batch, int k, int vocab, int32_t* kept, int64_t* token,
-                      void* stream);
+typedef struct {
+  const float* target;
+  int64_t p_sb, p_st;
+  const float* draft;
+  int64_t q_sb, q_st;
+  const int64_t* tokens;
+  int64_t t_sb;
+  const float* uniforms;
+  int64_t u_sb;
+  int batch, k, vocab;
+  int32_t* kept;
+  int64_t* token;
+} lkv_verify_args;
+int lkv_verify_drafts(const lkv_verify_args* args, void* stream);
 
 #ifdef __cplusplus
 }

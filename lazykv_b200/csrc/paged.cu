@@ -230,6 +230,46 @@ cudaError_t launch_read(const PagedParams& p, bool int8, unsigned grid, cudaStre
               : launch_pdl(paged_read_kernel<T, D, false>, dim3(grid), dim3(kThreads), 0, st, 0, p);
 }
 
+// What write and read check alike; `rows` gets batch * tokens * h.
+int check_call(const char* who, const lkv_paged_args* a, int64_t* rows) {
+  if (a == nullptr) return fail(LKV_ERR_PTR, "%s: null arguments", who);
+  if (int rc = check_cache(who, a->kind, a->dtype, a->h, a->bs, a->d, a->n_pages, a->pages, a->scales)) return rc;
+  if (a->batch < 0 || a->tokens < 0 || a->table_cols < 0 || (a->batch > 1 && a->table_ld < a->table_cols))
+    return fail(LKV_ERR_ARG, "%s: bad shape (batch %d, tokens %d, table of %d columns)", who, a->batch, a->tokens, a->table_cols);
+  if ((int64_t)a->batch * a->tokens > INT32_MAX || (int64_t)a->batch * a->tokens * a->h > INT32_MAX)
+    return fail(LKV_ERR_ARG, "%s: %d x %d x %d rows of one call", who, a->batch, a->tokens, a->h);
+  *rows = (int64_t)a->batch * a->tokens * a->h;
+  return LKV_OK;
+}
+
+PagedParams params_of(const lkv_paged_args* a, int64_t rows) {
+  PagedParams p = {};
+  p.keys = a->keys;
+  p.values = a->values;
+  p.k_sb = a->k_sb, p.k_st = a->k_st, p.k_sh = a->k_sh;
+  p.v_sb = a->v_sb, p.v_st = a->v_st, p.v_sh = a->v_sh;
+  p.pages = a->pages;
+  p.scales = a->scales;
+  p.n_pages = a->n_pages;
+  p.table = a->table;
+  p.table_ld = a->table_ld;
+  p.table_cols = a->table_cols;
+  p.starts = a->starts;
+  p.lens = a->lens;
+  p.rows = (uint32_t)rows;
+  p.tokens = a->tokens;
+  p.h = a->h;
+  p.page_shift = shift_of(a->bs);
+  p.out_k = a->out_k;
+  p.out_v = a->out_v;
+  return p;
+}
+
+unsigned grid_of(int64_t rows, int d) {
+  const unsigned per_cta = kThreads / (d / kCh);
+  return (unsigned)((rows + per_cta - 1) / per_cta);
+}
+
 }  // namespace
 }  // namespace lkv
 
@@ -237,84 +277,47 @@ using namespace lkv;
 
 extern "C" {
 
-int lkv_paged_write(const void* keys, int64_t k_sb, int64_t k_st, int64_t k_sh, const void* values, int64_t v_sb, int64_t v_st, int64_t v_sh,
-                    int dtype, int batch, int tokens, int h, int d, void* pages, int kind, float* scales, int64_t n_pages, int bs,
-                    const int32_t* table, int64_t table_ld, int table_cols, const int32_t* starts, void* stream) {
-  if (int rc = check_cache("lkv_paged_write", kind, dtype, h, bs, d, n_pages, pages, scales)) return rc;
-  if (batch < 0 || tokens < 0 || table_cols < 0 || (batch > 1 && table_ld < table_cols))
-    return fail(LKV_ERR_ARG, "lkv_paged_write: bad shape (batch %d, tokens %d, table of %d columns)", batch, tokens, table_cols);
-  const int64_t rows = (int64_t)batch * tokens * h;
-  if (rows > INT32_MAX) return fail(LKV_ERR_ARG, "lkv_paged_write: %lld rows of one call", (long long)rows);
-  if (rows == 0 || n_pages == 0 || table_cols == 0) return LKV_OK;
-  if (keys == nullptr || values == nullptr || table == nullptr || starts == nullptr) return fail(LKV_ERR_PTR, "lkv_paged_write: null pointer");
-  const int size = (int)dtype_size(dtype), per = 16 / size;
-  if (!aligned(keys, size) || !aligned(values, size)) return fail(LKV_ERR_PTR, "lkv_paged_write: misaligned keys or values");
-  const bool vec = aligned(keys, 16) && aligned(values, 16) && k_sb % per == 0 && k_st % per == 0 && k_sh % per == 0 && v_sb % per == 0 &&
-                   v_st % per == 0 && v_sh % per == 0;
-  PagedParams p = {};
-  p.keys = keys;
-  p.values = values;
-  p.k_sb = k_sb, p.k_st = k_st, p.k_sh = k_sh;
-  p.v_sb = v_sb, p.v_st = v_st, p.v_sh = v_sh;
-  p.pages = pages;
-  p.scales = scales;
-  p.n_pages = n_pages;
-  p.table = table;
-  p.table_ld = table_ld;
-  p.table_cols = table_cols;
-  p.starts = starts;
-  p.rows = (uint32_t)rows;
-  p.tokens = tokens;
-  p.h = h;
-  p.page_shift = shift_of(bs);
-  const unsigned per_cta = kThreads / (d / kCh), grid = (unsigned)((rows + per_cta - 1) / per_cta);
-  const bool int8 = kind == LKV_CACHE_INT8;
+int lkv_paged_write(const lkv_paged_args* a, void* stream) {
+  static const char* who = "lkv_paged_write";
+  int64_t rows = 0;
+  if (int rc = check_call(who, a, &rows)) return rc;
+  if (rows == 0 || a->n_pages == 0 || a->table_cols == 0) return LKV_OK;
+  if (a->keys == nullptr || a->values == nullptr || a->table == nullptr || a->starts == nullptr) return fail(LKV_ERR_PTR, "%s: null pointer", who);
+  const int size = (int)dtype_size(a->dtype), per = 16 / size;
+  if (!aligned(a->keys, size) || !aligned(a->values, size)) return fail(LKV_ERR_PTR, "%s: misaligned keys or values", who);
+  const bool vec = aligned(a->keys, 16) && aligned(a->values, 16) && a->k_sb % per == 0 && a->k_st % per == 0 && a->k_sh % per == 0 &&
+                   a->v_sb % per == 0 && a->v_st % per == 0 && a->v_sh % per == 0;
+  const PagedParams p = params_of(a, rows);
+  const unsigned grid = grid_of(rows, a->d);
+  const bool int8 = a->kind == LKV_CACHE_INT8;
   cudaStream_t st = as_stream(stream);
   cudaError_t e;
-  if (dtype == LKV_BF16)
-    e = d == 64 ? launch_write<__nv_bfloat16, 64>(p, int8, vec, grid, st) : launch_write<__nv_bfloat16, 128>(p, int8, vec, grid, st);
+  if (a->dtype == LKV_BF16)
+    e = a->d == 64 ? launch_write<__nv_bfloat16, 64>(p, int8, vec, grid, st) : launch_write<__nv_bfloat16, 128>(p, int8, vec, grid, st);
   else
-    e = d == 64 ? launch_write<float, 64>(p, int8, vec, grid, st) : launch_write<float, 128>(p, int8, vec, grid, st);
-  if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "lkv_paged_write: %s", cudaGetErrorString(e));
+    e = a->d == 64 ? launch_write<float, 64>(p, int8, vec, grid, st) : launch_write<float, 128>(p, int8, vec, grid, st);
+  if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
   return LKV_OK;
 }
 
-int lkv_paged_read(const void* pages, int kind, const float* scales, int64_t n_pages, int bs, int batch, int tokens, int h, int d,
-                   const int32_t* table, int64_t table_ld, int table_cols, const int32_t* starts, const int32_t* lens, void* out_k, void* out_v,
-                   int dtype, void* stream) {
-  if (int rc = check_cache("lkv_paged_read", kind, dtype, h, bs, d, n_pages, pages, scales)) return rc;
-  if (batch < 0 || tokens < 0 || table_cols < 0 || (batch > 1 && table_ld < table_cols))
-    return fail(LKV_ERR_ARG, "lkv_paged_read: bad shape (batch %d, tokens %d, table of %d columns)", batch, tokens, table_cols);
-  const int64_t rows = (int64_t)batch * tokens * h;
-  if (rows > INT32_MAX) return fail(LKV_ERR_ARG, "lkv_paged_read: %lld rows of one call", (long long)rows);
+int lkv_paged_read(const lkv_paged_args* a, void* stream) {
+  static const char* who = "lkv_paged_read";
+  int64_t rows = 0;
+  if (int rc = check_call(who, a, &rows)) return rc;
   if (rows == 0) return LKV_OK;
-  if ((table == nullptr && table_cols > 0) || starts == nullptr || out_k == nullptr || out_v == nullptr)
-    return fail(LKV_ERR_PTR, "lkv_paged_read: null pointer");
-  if (!aligned(out_k, 16) || !aligned(out_v, 16)) return fail(LKV_ERR_PTR, "lkv_paged_read: outputs must be 16-byte aligned");
-  PagedParams p = {};
-  p.pages = const_cast<void*>(pages);
-  p.scales = const_cast<float*>(scales);
-  p.n_pages = n_pages;
-  p.table = table;
-  p.table_ld = table_ld;
-  p.table_cols = table_cols;
-  p.starts = starts;
-  p.lens = lens;
-  p.rows = (uint32_t)rows;
-  p.tokens = tokens;
-  p.h = h;
-  p.page_shift = shift_of(bs);
-  p.out_k = out_k;
-  p.out_v = out_v;
-  const unsigned per_cta = kThreads / (d / kCh), grid = (unsigned)((rows + per_cta - 1) / per_cta);
-  const bool int8 = kind == LKV_CACHE_INT8;
+  if ((a->table == nullptr && a->table_cols > 0) || a->starts == nullptr || a->out_k == nullptr || a->out_v == nullptr)
+    return fail(LKV_ERR_PTR, "%s: null pointer", who);
+  if (!aligned(a->out_k, 16) || !aligned(a->out_v, 16)) return fail(LKV_ERR_PTR, "%s: outputs must be 16-byte aligned", who);
+  const PagedParams p = params_of(a, rows);
+  const unsigned grid = grid_of(rows, a->d);
+  const bool int8 = a->kind == LKV_CACHE_INT8;
   cudaStream_t st = as_stream(stream);
   cudaError_t e;
-  if (dtype == LKV_BF16)
-    e = d == 64 ? launch_read<__nv_bfloat16, 64>(p, int8, grid, st) : launch_read<__nv_bfloat16, 128>(p, int8, grid, st);
+  if (a->dtype == LKV_BF16)
+    e = a->d == 64 ? launch_read<__nv_bfloat16, 64>(p, int8, grid, st) : launch_read<__nv_bfloat16, 128>(p, int8, grid, st);
   else
-    e = d == 64 ? launch_read<float, 64>(p, int8, grid, st) : launch_read<float, 128>(p, int8, grid, st);
-  if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "lkv_paged_read: %s", cudaGetErrorString(e));
+    e = a->d == 64 ? launch_read<float, 64>(p, int8, grid, st) : launch_read<float, 128>(p, int8, grid, st);
+  if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
   return LKV_OK;
 }
 

@@ -741,7 +741,8 @@ template <int D, bool INT8>
 cudaError_t launch_stream(const Params& p, cudaStream_t st) {
   using S = Shape<D, INT8>;
   auto k = stream_kernel<D, INT8>;
-  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kRing);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(k, S::kRing, done);
   if (e != cudaSuccess) return e;
   return launch_pdl(k, dim3(p.n_warps / kWarps), dim3(kThreads), S::kRing, st, 0, p);
 }

@@ -4,6 +4,8 @@
 
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace lkv {
@@ -102,6 +104,17 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 __device__ __forceinline__ int length_of(int stages) { return stages > 0 ? stages + kUnitStages : 0; }
+
+// Dynamic shared memory above 48 KB, asked for once per kernel and device (`done`: a bit per device).
+template <typename K>
+inline cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
+}
 
 // prefix_tile.cu: the prefix's partials for many rows, and how many splits of the prefix they take.
 int tile_splits(int rows, int h, int64_t prefix_len);

@@ -782,7 +782,8 @@ template <int D, bool INT8>
 cudaError_t launch_tile(const Params& p, const CUtensorMap& map, int chunk, cudaStream_t st) {
   using T = Tiles<D, INT8>;
   auto k = prefix_tile_kernel<D, INT8>;
-  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(k, T::kSmem, done);
   if (e != cudaSuccess) return e;
   const dim3 grid(p.n_splits, p.h, (p.rows + 2 * kTile - 1) / (2 * kTile));
   return launch_pdl(k, grid, dim3(T::kThreads), T::kSmem, st, 0, p, map, chunk);

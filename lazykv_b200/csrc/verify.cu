@@ -220,15 +220,15 @@ using namespace lkv;
 
 extern "C" {
 
-int lkv_verify_drafts(const float* target, int64_t p_sb, int64_t p_st, const float* draft, int64_t q_sb, int64_t q_st, const int64_t* tokens,
-                      int64_t t_sb, const float* uniforms, int64_t u_sb, int batch, int k, int vocab, int32_t* kept, int64_t* token,
-                      void* stream) {
-  if (batch < 0 || k < 0 || vocab < 1 || vocab > (1 << 22))
-    return fail(LKV_ERR_ARG, "lkv_verify_drafts: bad shape (batch %d, drafted %d, vocabulary %d of at most 4,194,304)", batch, k, vocab);
+int lkv_verify_drafts(const lkv_verify_args* a, void* stream) {
+  if (a == nullptr) return fail(LKV_ERR_PTR, "lkv_verify_drafts: null arguments");
+  const int batch = a->batch, vocab = a->vocab;
+  if (batch < 0 || a->k < 0 || vocab < 1 || vocab > (1 << 22))
+    return fail(LKV_ERR_ARG, "lkv_verify_drafts: bad shape (batch %d, drafted %d, vocabulary %d of at most 4,194,304)", batch, a->k, vocab);
   if (batch == 0) return LKV_OK;
-  if (target == nullptr || (k > 0 && tokens == nullptr) || uniforms == nullptr || kept == nullptr || token == nullptr)
+  if (a->target == nullptr || (a->k > 0 && a->tokens == nullptr) || a->uniforms == nullptr || a->kept == nullptr || a->token == nullptr)
     return fail(LKV_ERR_PTR, "lkv_verify_drafts: null pointer");
-  if (!aligned(target, 4) || !aligned(draft, 4) || !aligned(tokens, 8) || !aligned(uniforms, 4) || !aligned(kept, 4) || !aligned(token, 8))
+  if (!aligned(a->target, 4) || !aligned(a->draft, 4) || !aligned(a->tokens, 8) || !aligned(a->uniforms, 4) || !aligned(a->kept, 4) || !aligned(a->token, 8))
     return fail(LKV_ERR_PTR, "lkv_verify_drafts: misaligned pointer");
   // As many CTAs per sequence (a power of two, 8 at most) as keep all of them resident at four to an
   // SM, and no more than a slice of one tile per warp fills; always enough that the tile sums fit.
@@ -236,21 +236,22 @@ int lkv_verify_drafts(const float* target, int64_t p_sb, int64_t p_st, const flo
   while (c < 8 && (int64_t)batch * c * 2 <= 4 * kNumSMs && (int64_t)kTile * kWarps * c < vocab) c *= 2;
   while (c < 8 && (int64_t)kTile * kMaxTiles * c < vocab) c *= 2;
   VerifyParams p = {};
-  p.target = target;
-  p.p_sb = p_sb, p.p_st = p_st;
-  p.draft = draft;
-  p.q_sb = q_sb, p.q_st = q_st;
-  p.tokens = tokens;
-  p.t_sb = t_sb;
-  p.uniforms = uniforms;
-  p.u_sb = u_sb;
-  p.k = k;
+  p.target = a->target;
+  p.p_sb = a->p_sb, p.p_st = a->p_st;
+  p.draft = a->draft;
+  p.q_sb = a->q_sb, p.q_st = a->q_st;
+  p.tokens = a->tokens;
+  p.t_sb = a->t_sb;
+  p.uniforms = a->uniforms;
+  p.u_sb = a->u_sb;
+  p.k = a->k;
   p.vocab = vocab;
   p.per_cta = ((vocab + c - 1) / c + kTile - 1) / kTile * kTile;
-  p.kept = kept;
-  p.token = token;
+  p.kept = a->kept;
+  p.token = a->token;
   if ((int64_t)batch * c > INT32_MAX) return fail(LKV_ERR_ARG, "lkv_verify_drafts: batch of %d", batch);
-  const bool vec = aligned(target, 16) && p_sb % 4 == 0 && p_st % 4 == 0 && (draft == nullptr || (aligned(draft, 16) && q_sb % 4 == 0 && q_st % 4 == 0));
+  const bool vec = aligned(a->target, 16) && a->p_sb % 4 == 0 && a->p_st % 4 == 0 &&
+                   (a->draft == nullptr || (aligned(a->draft, 16) && a->q_sb % 4 == 0 && a->q_st % 4 == 0));
   const cudaError_t e = vec ? launch_pdl(verify_kernel<true>, dim3((unsigned)(batch * c)), dim3(kThreads), 0, as_stream(stream), c, p)
                             : launch_pdl(verify_kernel<false>, dim3((unsigned)(batch * c)), dim3(kThreads), 0, as_stream(stream), c, p);
   if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "lkv_verify_drafts: %s", cudaGetErrorString(e));

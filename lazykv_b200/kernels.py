@@ -7,6 +7,7 @@ tensors (or device views of pinned host memory); there is no CPU path.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -440,40 +441,59 @@ def quest_topk_admit(query: torch.Tensor, kmin: torch.Tensor, kmax: torch.Tensor
 # -- the paged cache of a batch, the attention over a shared prefix, and draft verification --------------
 
 
-def _on(dev: torch.device, name: str, *args: object) -> None:
-    """call(name, *args, the current stream of `dev`) with `dev` current."""
-    if dev.index == torch.cuda.current_device():
-        call(name, *args, stream_handle(dev))
+_device_of = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+def _run(name: str, args: bytes, index: int) -> None:
+    """Entry `name` (an args struct and a stream) on the current stream of device `index`, which is made current."""
+    fn = getattr(L.lib(), name)
+    if index == _device_of():
+        rc = fn(args, L._RAW_STREAM(index) if L._RAW_STREAM is not None else stream_handle(torch.device("cuda", index)))
     else:
-        with torch.cuda.device(dev):
-            call(name, *args, stream_handle(dev))
+        with torch.cuda.device(index):
+            rc = fn(args, stream_handle(torch.device("cuda", index)))
+    if rc != 0:
+        raise L.LkvError(f"{name} failed ({rc}): {L.last_error()}")
 
 
-def _one_device(who: str, *tensors: torch.Tensor | None) -> torch.device:
-    dev = require_cuda(*tensors)
+def _one_device(who: str, *tensors: torch.Tensor | None) -> int:
+    """The index of the one CUDA device that all tensors are on."""
+    index = -1
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{who}: tensors on {dev} and {t.device}")
-    return dev
+        if t is not None:
+            at = t.get_device()
+            if at < 0:
+                require_cuda(t)
+            if index < 0:
+                index = at
+            elif at != index:
+                raise ValueError(f"{who}: tensors on cuda:{index} and cuda:{at}")
+    return index
 
 
-def _cache_geometry(who: str, pages: torch.Tensor, scales: torch.Tensor | None, table: torch.Tensor) -> tuple[int, int, int, int, int]:
-    """(n_pages, h, bs, d, cache kind) of pages [n_pages, h, 2, bs, d] and their page table."""
-    if pages.dim() != 5 or pages.shape[2] != 2 or not pages.is_contiguous():
+def _cache_geometry(who: str, pages: torch.Tensor, scales: torch.Tensor | None, table: torch.Tensor) -> tuple[int, int, int, int, int, int, int, int]:
+    """(n_pages, h, bs, d, cache kind) of pages [n_pages, h, 2, bs, d], and (batch, row stride, columns) of their table."""
+    if pages.dim() != 5 or not pages.is_contiguous() or pages.shape[2] != 2:
         raise ValueError(f"{who}: pages must be a contiguous [n_pages, h, 2, block_size, head_dim], got {tuple(pages.shape)}")
     n, h, _, bs, d = pages.shape
-    int8 = pages.dtype == torch.int8
-    if int8 and (scales is None or scales.dtype != torch.float32 or scales.shape != (n, h, 2, bs) or not scales.is_contiguous()):
-        raise ValueError(f"{who}: int8 pages need contiguous float32 scales [{n}, {h}, 2, {bs}]")
-    if not int8 and scales is not None:
-        raise ValueError(f"{who}: scales belong to int8 pages, these are {pages.dtype}")
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+    if pages.dtype == torch.int8:
+        kind = L.LKV_CACHE_INT8
+        if scales is None or scales.dtype != torch.float32 or scales.shape != (n, h, 2, bs) or not scales.is_contiguous():
+            raise ValueError(f"{who}: int8 pages need contiguous float32 scales [{n}, {h}, 2, {bs}]")
+    else:
+        kind = L.LKV_CACHE_MODEL
+        if scales is not None:
+            raise ValueError(f"{who}: scales belong to int8 pages, these are {pages.dtype}")
+    if table.dtype != torch.int32 or table.dim() != 2:
         raise ValueError(f"{who}: the page table must be int32 [batch, columns] with unit column stride")
-    return n, h, bs, d, L.LKV_CACHE_INT8 if int8 else L.LKV_CACHE_MODEL
+    (batch, cols), (ld, unit) = table.shape, table.stride()
+    if unit != 1 and cols > 1:
+        raise ValueError(f"{who}: the page table must be int32 [batch, columns] with unit column stride")
+    return n, h, bs, d, kind, batch, ld, cols
 
 
 def _per_sequence(who: str, name: str, t: torch.Tensor, batch: int) -> None:
-    if t.dtype != torch.int32 or t.shape != (batch,) or (batch > 1 and t.stride(0) != 1):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != batch or not t.is_contiguous():
         raise ValueError(f"{who}: {name} must be a contiguous int32 [{batch}]")
 
 
@@ -487,19 +507,22 @@ def paged_write(keys: torch.Tensor, values: torch.Tensor, pages: torch.Tensor, t
     int32 lists each sequence's pages; a token whose page is missing (past the table, an id outside
     [0, n_pages)) is not written, so a batch may be padded. Two tokens must not share a row.
     """
-    dev = _one_device("paged_write", keys, values, pages, table, starts, scales)
-    if keys.dim() != 4 or values.shape != keys.shape or values.dtype != keys.dtype:
+    who = "paged_write"
+    index = _one_device(who, keys, values, pages, table, starts, scales)
+    dtype = keys.dtype
+    if keys.dim() != 4 or values.shape != keys.shape or values.dtype != dtype:
         raise ValueError(f"paged_write: keys and values must be alike, [batch, T, h, d]; got {tuple(keys.shape)} and {tuple(values.shape)}")
     batch, t, h, d = keys.shape
-    n, ph, bs, pd, kind = _cache_geometry("paged_write", pages, scales, table)
-    if (ph, pd) != (h, d) or (kind == L.LKV_CACHE_MODEL and pages.dtype != keys.dtype):
-        raise ValueError(f"paged_write: {tuple(keys.shape)} {keys.dtype} tokens do not fit pages {tuple(pages.shape)} {pages.dtype}")
-    if table.shape[0] != batch or keys.stride(3) != 1 or values.stride(3) != 1:
+    n, ph, bs, pd, kind, rows, ld, cols = _cache_geometry(who, pages, scales, table)
+    if ph != h or pd != d or (kind == L.LKV_CACHE_MODEL and pages.dtype != dtype):
+        raise ValueError(f"paged_write: {tuple(keys.shape)} {dtype} tokens do not fit pages {tuple(pages.shape)} {pages.dtype}")
+    (kb, kt, kh, kc), (vb, vt, vh, vc) = keys.stride(), values.stride()
+    if rows != batch or kc != 1 or vc != 1:
         raise ValueError("paged_write: one table row per sequence, and contiguous channels")
-    _per_sequence("paged_write", "starts", starts, batch)
-    _on(dev, "lkv_paged_write", keys.data_ptr(), keys.stride(0), keys.stride(1), keys.stride(2), values.data_ptr(), values.stride(0), values.stride(1),
-        values.stride(2), dtype_code(keys.dtype), batch, t, h, d, pages.data_ptr(), kind, ptr(scales), n, bs, table.data_ptr(), table.stride(0),
-        table.shape[1], starts.data_ptr())
+    _per_sequence(who, "starts", starts, batch)
+    _run("lkv_paged_write", L.PAGED_ARGS.pack(
+        keys.data_ptr(), values.data_ptr(), kb, kt, kh, vb, vt, vh, dtype_code(dtype), batch, t, h, d, pages.data_ptr(), kind,
+        0 if scales is None else scales.data_ptr(), n, bs, table.data_ptr(), ld, cols, starts.data_ptr(), 0, 0, 0), index)
 
 
 def paged_read(pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, n_tokens: int, lens: torch.Tensor | None = None,
@@ -510,27 +533,39 @@ def paged_read(pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, n
     by default; model-dtype pages are copied). Tokens at or past lens[b] (int32 [batch], optional) and
     tokens without a page are zeros.
     """
-    dev = _one_device("paged_read", pages, table, starts, lens, scales)
-    n, h, bs, d, kind = _cache_geometry("paged_read", pages, scales, table)
-    batch = table.shape[0]
-    if dtype is None:
-        dtype = pages.dtype if kind == L.LKV_CACHE_MODEL else torch.bfloat16
-    if kind == L.LKV_CACHE_MODEL and dtype != pages.dtype:
-        raise ValueError(f"paged_read: {pages.dtype} pages are read back as {pages.dtype}, not {dtype}")
+    who = "paged_read"
+    index = _one_device(who, pages, table, starts, lens, scales)
+    n, h, bs, d, kind, batch, ld, cols = _cache_geometry(who, pages, scales, table)
+    if kind == L.LKV_CACHE_MODEL:
+        if dtype is not None and dtype != pages.dtype:
+            raise ValueError(f"paged_read: {pages.dtype} pages are read back as {pages.dtype}, not {dtype}")
+        dtype = pages.dtype
+    elif dtype is None:
+        dtype = torch.bfloat16
+    code = dtype_code(dtype)
     if n_tokens < 0:
         raise ValueError(f"paged_read: {n_tokens} tokens")
-    _per_sequence("paged_read", "starts", starts, batch)
+    _per_sequence(who, "starts", starts, batch)
     if lens is not None:
-        _per_sequence("paged_read", "lens", lens, batch)
+        _per_sequence(who, "lens", lens, batch)
     shape = (batch, n_tokens, h, d)
     if out is None:
-        out = (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
-    for o in out:
-        if o.shape != shape or o.dtype != dtype or o.device != dev or not o.is_contiguous():
-            raise ValueError(f"paged_read: out must be two contiguous {dtype} {shape} on {dev}")
-    _on(dev, "lkv_paged_read", pages.data_ptr(), kind, ptr(scales), n, bs, batch, n_tokens, h, d, table.data_ptr(), table.stride(0), table.shape[1],
-        starts.data_ptr(), ptr(lens), out[0].data_ptr(), out[1].data_ptr(), dtype_code(dtype))
+        k, v = pages.new_empty(shape, dtype=dtype), pages.new_empty(shape, dtype=dtype)
+        out = k, v
+    else:
+        k, v = out
+        for o in out:
+            if o.shape != shape or o.dtype != dtype or o.get_device() != index or not o.is_contiguous():
+                raise ValueError(f"paged_read: out must be two contiguous {dtype} {shape} on cuda:{index}")
+    _run("lkv_paged_read", L.PAGED_ARGS.pack(
+        0, 0, 0, 0, 0, 0, 0, 0, code, batch, n_tokens, h, d, pages.data_ptr(), kind, 0 if scales is None else scales.data_ptr(), n, bs,
+        table.data_ptr(), ld, cols, starts.data_ptr(), 0 if lens is None else lens.data_ptr(), k.data_ptr(), v.data_ptr()), index)
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _prefix_workspace(batch: int, tokens: int, hq: int, h: int, d: int, prefix_len: int, kind: int, reach: int) -> int:
+    return int(L.lib().lkv_prefix_attention_workspace(batch, tokens, hq, h, d, prefix_len, kind, reach))
 
 
 def prefix_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, prefix_table: torch.Tensor, prefix_len: int,
@@ -549,33 +584,36 @@ def prefix_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tens
     The partials' workspace comes from torch's allocator call by call, so calls on several streams and
     several captured graphs do not share it.
     """
-    dev = _one_device("prefix_attention", query, pages, table, lens, prefix_table, scales, out, lse)
+    who = "prefix_attention"
+    index = _one_device(who, query, pages, table, lens, prefix_table, scales, out, lse)
     if query.dim() != 4 or query.dtype != torch.bfloat16:
         raise ValueError(f"prefix_attention: query must be bfloat16 [batch, T, hq, d], got {query.dtype} {tuple(query.shape)}")
     batch, t, hq, d = query.shape
-    n, h, bs, pd, kind = _cache_geometry("prefix_attention", pages, scales, table)
-    if pd != d or hq % h or table.shape[0] != batch or (kind == L.LKV_CACHE_MODEL and pages.dtype != torch.bfloat16):
+    n, h, bs, pd, kind, rows, ld, cols = _cache_geometry(who, pages, scales, table)
+    if pd != d or h < 1 or hq % h or rows != batch or (kind == L.LKV_CACHE_MODEL and pages.dtype != torch.bfloat16):
         raise ValueError(f"prefix_attention: query {tuple(query.shape)} and table {tuple(table.shape)} do not fit {pages.dtype} pages {tuple(pages.shape)}")
-    _per_sequence("prefix_attention", "lens", lens, batch)
-    cols = prefix_table.numel()
-    if prefix_table.dtype != torch.int32 or prefix_table.dim() != 1 or (cols > 1 and prefix_table.stride(0) != 1) or not 0 <= prefix_len <= cols * bs:
+    _per_sequence(who, "lens", lens, batch)
+    pcols = prefix_table.numel()
+    if prefix_table.dtype != torch.int32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous() or not 0 <= prefix_len <= pcols * bs:
         raise ValueError(f"prefix_attention: prefix_table must be a contiguous int32 [columns] holding the {prefix_len} tokens of the prefix")
-    if query.stride(3) != 1 or query.stride(0) % 8 or query.stride(1) % 8 or query.stride(2) % 8 or query.data_ptr() % 16:
+    sb, st, sh, sc = query.stride()
+    if sc != 1 or (sb | st | sh) & 7 or query.data_ptr() & 15:
         query = query.clone(memory_format=torch.contiguous_format)
+        sb, st, sh, _ = query.stride()
     if out is None:
-        out = torch.empty((batch, t, hq, d), dtype=out_dtype or torch.bfloat16, device=dev)
-    elif out.shape != query.shape or not out.is_contiguous() or out.dtype != (out_dtype or out.dtype):
+        out = query.new_empty((batch, t, hq, d)) if out_dtype is None else query.new_empty((batch, t, hq, d), dtype=out_dtype)
+    elif out.shape != query.shape or not out.is_contiguous() or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"prefix_attention: out must be a contiguous {tuple(query.shape)}")
     if lse is None:
-        lse = torch.empty((batch, t, hq), dtype=torch.float32, device=dev)
+        lse = query.new_empty((batch, t, hq), dtype=torch.float32)
     elif lse.shape != (batch, t, hq) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise ValueError(f"prefix_attention: lse must be a contiguous float32 {(batch, t, hq)}")
-    nbytes = L.lib().lkv_prefix_attention_workspace(batch, t, hq, h, d, prefix_len, kind, table.shape[1] * bs)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    args = L.PrefixArgs(query.data_ptr(), L.LKV_BF16, query.stride(0), query.stride(1), query.stride(2), pages.data_ptr(), kind, ptr(scales), n, bs,
-                        batch, t, hq, h, d, table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(), prefix_table.data_ptr(), cols,
-                        prefix_len, scale, out.data_ptr(), dtype_code(out.dtype), lse.data_ptr(), ptr(ws), nbytes)
-    _on(dev, "lkv_prefix_attention", ctypes.byref(args))
+    nbytes = _prefix_workspace(batch, t, hq, h, d, prefix_len, kind, cols * bs)
+    ws = query.new_empty((nbytes + 1) // 2) if nbytes else None
+    _run("lkv_prefix_attention", L.PREFIX_ARGS.pack(
+        query.data_ptr(), L.LKV_BF16, sb, st, sh, pages.data_ptr(), kind, 0 if scales is None else scales.data_ptr(), n, bs, batch, t, hq, h, d,
+        table.data_ptr(), ld, cols, lens.data_ptr(), prefix_table.data_ptr(), pcols, prefix_len, scale, out.data_ptr(), dtype_code(out.dtype),
+        lse.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes), index)
     return out, lse
 
 
@@ -592,22 +630,24 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     target there. Returns (kept [batch] int32, token [batch] int64); token is -1 where the weights are all
     zero or have no finite sum.
     """
-    dev = _one_device("verify_drafts", target, draft, tokens, uniforms)
+    index = _one_device("verify_drafts", target, draft, tokens, uniforms)
     if target.dim() != 3 or tokens.dim() != 2:
         raise ValueError("verify_drafts: target must be [batch, k + 1, vocab] and tokens [batch, k]")
     batch, k = tokens.shape
     vocab = target.shape[2]
-    if target.shape[:2] != (batch, k + 1) or uniforms.shape != (batch, k + 1) or (draft is not None and draft.shape != (batch, k, vocab)):
+    if target.shape != (batch, k + 1, vocab) or uniforms.shape != (batch, k + 1) or (draft is not None and draft.shape != (batch, k, vocab)):
         raise ValueError(f"verify_drafts: {k} tokens drafted for {batch} sequences do not fit target {tuple(target.shape)}, uniforms "
                          f"{tuple(uniforms.shape)}, draft {None if draft is None else tuple(draft.shape)}")
-    if target.dtype != torch.float32 or uniforms.dtype != torch.float32 or tokens.dtype != torch.int64 or (draft is not None and draft.dtype != torch.float32):
+    f32 = torch.float32
+    if target.dtype != f32 or uniforms.dtype != f32 or tokens.dtype != torch.int64 or (draft is not None and draft.dtype != f32):
         raise ValueError("verify_drafts: probabilities and uniforms are float32, tokens int64")
-    for t in (target, draft, tokens, uniforms):
-        if t is not None and t.shape[-1] > 1 and t.stride(-1) != 1:
-            raise ValueError("verify_drafts: rows must be contiguous")
-    kept = torch.empty((batch,), dtype=torch.int32, device=dev)
-    token = torch.empty((batch,), dtype=torch.int64, device=dev)
-    _on(dev, "lkv_verify_drafts", target.data_ptr(), target.stride(0), target.stride(1), ptr(draft), 0 if draft is None else draft.stride(0),
-        0 if draft is None else draft.stride(1), tokens.data_ptr(), tokens.stride(0), uniforms.data_ptr(), uniforms.stride(0), batch, k, vocab,
-        kept.data_ptr(), token.data_ptr())
+    (pb, pt, pv), (tb, tk), (ub, uk) = target.stride(), tokens.stride(), uniforms.stride()
+    qb, qt, qv = (0, 0, 1) if draft is None else draft.stride()
+    if (vocab > 1 and (pv != 1 or qv != 1)) or (k > 1 and tk != 1) or (k > 0 and uk != 1):
+        raise ValueError("verify_drafts: rows must be contiguous")
+    token = tokens.new_empty(batch)
+    kept = tokens.new_empty(batch, dtype=torch.int32)
+    _run("lkv_verify_drafts", L.VERIFY_ARGS.pack(
+        target.data_ptr(), pb, pt, 0 if draft is None else draft.data_ptr(), qb, qt, tokens.data_ptr(), tb, uniforms.data_ptr(), ub, batch, k, vocab,
+        kept.data_ptr(), token.data_ptr()), index)
     return kept, token
