@@ -7,14 +7,17 @@
 // are quantised per channel over a whole block, a row's scale needs that row only, so a token is
 // final as soon as it is written.
 //
-// The row's code: s = max(max_c |x_c| / 127, FLT_MIN) (at most what keeps 127 s finite), code_c = the whole number nearest to x_c / s
-// (halfway: the even one), value code_c * s. The quotient is never rounded before the rounding to a
-// whole number: k = rint(x * (1 / s)) is within one of it, the remainder x - k s is exact in one fused
-// multiply-add, and k moves by one where the remainder passes s / 2. A row that holds an infinity or a
-// NaN has no scale: it gets s = NaN and codes 0 and reads back as NaN throughout.
+// The row's code: s = max(max_c |x_c| / 127, FLT_MIN) (at most what keeps 127 s finite), code_c = the whole
+// number nearest to x_c / s (halfway: the even one), value code_c * s. The quotient is never rounded before
+// the rounding to a whole number: k, x * (1 / s) rounded to one in a fused multiply-add, is within one of
+// it, the remainder x - k s is exact in another, and where one reaches s / 2 (next to never) k is put
+// right. A row that holds an infinity or a NaN has no scale: it gets s = NaN and codes 0 and reads back as
+// NaN throughout.
 //
-// What bounds both kernels is memory: every byte moves once. A thread carries 16 channels of one
-// token's key row and of its value row (64 bytes in flight per thread for bf16), d / 16 threads a row.
+// What bounds both kernels is memory: every byte moves once. A thread carries 16 bytes of the model's type
+// (8 channels of bf16, 4 of float32) of a token's key row and of its value row, so that a warp reads and
+// writes whole runs; with 32 bytes a thread, two stores a sector each, a read wrote 4.8 TB/s. Reading, a
+// thread carries several tokens, since its loads wait for the page's id and that for the table's row.
 #include <float.h>
 
 #include "common.cuh"
@@ -23,7 +26,6 @@ namespace lkv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kCh = 16;  // channels per thread
 constexpr float kMaxScale = 0x1.020406p+121f;  // the largest whose 127-fold is finite
 
 struct PagedParams {
@@ -38,31 +40,32 @@ struct PagedParams {
   int table_cols;
   const int32_t* starts;
   const int32_t* lens;  // read: tokens a sequence has (null: as many as its table)
-  uint32_t rows;        // batch * tokens * h
+  uint32_t rows;  // batch * tokens * h
   uint32_t tokens, h;
   int page_shift;
   void* out_k;  // read: contiguous [b, n, h, d]
   void* out_v;
 };
 
-// 16 consecutive elements as float; VEC: 16-byte aligned. Plain loads: the read-only path may serve a
+// Channels per thread: 16 bytes of the model's type.
+template <typename T>
+constexpr int kCh = 16 / (int)sizeof(T);
+
+// A thread's consecutive elements as float; VEC: 16-byte aligned. Plain loads: the read-only path may serve a
 // line that the kernel before this one, still running when this one started, has written since.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load16(const T* p, float* x) {
+__device__ __forceinline__ void load(const T* p, float* x) {
   if constexpr (!VEC) {
 #pragma unroll
-    for (int i = 0; i < kCh; ++i) x[i] = to_f32<T>(p[i]);
+    for (int i = 0; i < kCh<T>; ++i) x[i] = to_f32<T>(p[i]);
   } else if constexpr (sizeof(T) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float4 a = reinterpret_cast<const float4*>(p)[i];
-      x[4 * i] = a.x, x[4 * i + 1] = a.y, x[4 * i + 2] = a.z, x[4 * i + 3] = a.w;
-    }
-  } else {
-    const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
-    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
       x[2 * i] = __uint_as_float(w[i] << 16);
       x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
@@ -70,19 +73,17 @@ __device__ __forceinline__ void load16(const T* p, float* x) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store16(T* p, const float* x) {
+__device__ __forceinline__ void store(T* p, const float* x) {
   if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
   } else {
-    uint32_t w[8];
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
       w[i] = *reinterpret_cast<const uint32_t*>(&b);
     }
-    reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -95,112 +96,158 @@ __device__ __forceinline__ int64_t page_of(const PagedParams& p, uint32_t b, int
   return id < p.n_pages ? id : -1;
 }
 
-// One quantised row, 16 channels per lane of a group of L lanes: the codes and the row's scale.
-template <int L>
-__device__ __forceinline__ uint4 quantise_row(const float* x, float& scale) {
+// One quantised row, C channels per lane of a group of L lanes: the codes (4 to a word) and the row's scale.
+template <int L, int C>
+__device__ __forceinline__ void quantise_row(const float* x, uint32_t (&w)[C / 4], float& scale) {
   uint32_t top = 0;  // magnitudes compare as their bits; infinities and NaN come out above FLT_MAX
 #pragma unroll
-  for (int i = 0; i < kCh; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  for (int i = 0; i < C; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (top >= 0x7f800000u) {
     scale = __uint_as_float(0x7fc00000u);
-    return make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < C / 4; ++i) w[i] = 0;
+    return;
   }
   const float s = fminf(fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), FLT_MIN), kMaxScale), inv = 1.0f / s, half = 0.5f * s;
   scale = s;
-  uint32_t w[4] = {0, 0, 0, 0};
+  constexpr float kWhole = 12582912.0f;  // 1.5 x 2^23: a sum with it has the whole number in its low bits
+  float k[C], far = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kCh; ++i) {
-    float k = rintf(x[i] * inv);
-    const float r = fmaf(-k, s, x[i]);
-    // A remainder of exactly half a step belongs to the even neighbour.
-    const bool odd = (static_cast<int>(k) & 1) != 0;
-    if (r > half || (r == half && odd)) k += 1.0f;
-    if (r < -half || (r == -half && odd)) k -= 1.0f;
-    w[i / 4] |= (static_cast<uint32_t>(static_cast<int>(k)) & 0xffu) << (8 * (i % 4));
+  for (int i = 0; i < C; ++i) {
+    k[i] = fmaf(x[i], inv, kWhole);
+    far = fmaxf(far, fabsf(fmaf(kWhole - k[i], s, x[i])));
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  if (far >= half) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const float r = fmaf(kWhole - k[i], s, x[i]);
+      // A remainder of exactly half a step belongs to the even neighbour.
+      const bool odd = (__float_as_uint(k[i]) & 1u) != 0;
+      if (r > half || (r == half && odd)) k[i] += 1.0f;
+      else if (r < -half || (r == -half && odd)) k[i] -= 1.0f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < C / 4; ++i) {
+    const uint32_t lo = __byte_perm(__float_as_uint(k[4 * i]), __float_as_uint(k[4 * i + 1]), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(k[4 * i + 2]), __float_as_uint(k[4 * i + 3]), 0x0040);
+    w[i] = __byte_perm(lo, hi, 0x5410);
+  }
 }
 
-// Grid: rows of (sequence, token, head), D / 16 threads each.
+// Grid: rows of (sequence, token, head), D / kCh threads each.
 template <typename T, int D, bool INT8, bool VEC>
 __global__ void __launch_bounds__(kThreads) paged_write_kernel(const PagedParams p) {
-  constexpr int L = D / kCh;
+  constexpr int C = kCh<T>, L = D / C;
   pdl_wait();
   pdl_release();
   const uint32_t row = blockIdx.x * (kThreads / L) + threadIdx.x / L;
-  const int c = (threadIdx.x % L) * kCh;
+  const int c = (threadIdx.x % L) * C;
   const bool live = row < p.rows;
   const uint32_t j = row % p.h, bt = row / p.h, t = bt % p.tokens, b = bt / p.tokens;
   int64_t page = -1, pos = 0;
-  float k[kCh], v[kCh];
+  float k[C], v[C];
   if (live) {
-    load16<T, VEC>(static_cast<const T*>(p.keys) + b * p.k_sb + t * p.k_st + j * p.k_sh + c, k);
-    load16<T, VEC>(static_cast<const T*>(p.values) + b * p.v_sb + t * p.v_st + j * p.v_sh + c, v);
+    load<T, VEC>(static_cast<const T*>(p.keys) + b * p.k_sb + t * p.k_st + j * p.k_sh + c, k);
+    load<T, VEC>(static_cast<const T*>(p.values) + b * p.v_sb + t * p.v_st + j * p.v_sh + c, v);
     pos = (int64_t)p.starts[b] + t;
     page = page_of(p, b, pos);
   } else {
 #pragma unroll
-    for (int i = 0; i < kCh; ++i) k[i] = v[i] = 0.0f;
+    for (int i = 0; i < C; ++i) k[i] = v[i] = 0.0f;
   }
   const int bs = 1 << p.page_shift, at = (int)(pos & (bs - 1));
   const int64_t kr = ((page * p.h + j) * 2) * bs + at, vr = kr + bs;  // rows of the page's keys and values
   if constexpr (INT8) {
     float ks, vs;
-    const uint4 kq = quantise_row<L>(k, ks), vq = quantise_row<L>(v, vs);
+    uint32_t kq[C / 4], vq[C / 4];
+    quantise_row<L, C>(k, kq, ks);
+    quantise_row<L, C>(v, vq, vs);
     if (page < 0) return;
-    *reinterpret_cast<uint4*>(static_cast<int8_t*>(p.pages) + kr * D + c) = kq;
-    *reinterpret_cast<uint4*>(static_cast<int8_t*>(p.pages) + vr * D + c) = vq;
+    int8_t* pages = static_cast<int8_t*>(p.pages);
+    if constexpr (C == 8) {
+      *reinterpret_cast<uint2*>(pages + kr * D + c) = make_uint2(kq[0], kq[1]);
+      *reinterpret_cast<uint2*>(pages + vr * D + c) = make_uint2(vq[0], vq[1]);
+    } else {
+      *reinterpret_cast<uint32_t*>(pages + kr * D + c) = kq[0];
+      *reinterpret_cast<uint32_t*>(pages + vr * D + c) = vq[0];
+    }
     if (c == 0) {
       p.scales[kr] = ks;
       p.scales[vr] = vs;
     }
   } else {
     if (page < 0) return;
-    store16<T>(static_cast<T*>(p.pages) + kr * D + c, k);
-    store16<T>(static_cast<T*>(p.pages) + vr * D + c, v);
+    store<T>(static_cast<T*>(p.pages) + kr * D + c, k);
+    store<T>(static_cast<T*>(p.pages) + vr * D + c, v);
   }
 }
 
-// 16 codes and their scale as values.
-__device__ __forceinline__ void dequantise16(const int8_t* p, float s, float* x) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  const int8_t* q = reinterpret_cast<const int8_t*>(&w);
-#pragma unroll
-  for (int i = 0; i < kCh; ++i) x[i] = (float)q[i] * s;
-}
-
+// Grid: as for the write, kReads tokens of the grid's span apart per thread.
+template <bool INT8>
+constexpr int kReads = INT8 ? 4 : 2;
 template <typename T, int D, bool INT8>
 __global__ void __launch_bounds__(kThreads) paged_read_kernel(const PagedParams p) {
-  constexpr int L = D / kCh;
+  constexpr int C = kCh<T>, L = D / C, R = kReads<INT8>, kWords = INT8 ? C / 4 : 4;
   pdl_wait();
   pdl_release();
-  const uint32_t row = blockIdx.x * (kThreads / L) + threadIdx.x / L;
-  if (row >= p.rows) return;
-  const int c = (threadIdx.x % L) * kCh;
-  const uint32_t j = row % p.h, bt = row / p.h, t = bt % p.tokens, b = bt / p.tokens;
-  const int64_t pos = (int64_t)p.starts[b] + t;
-  int64_t page = -1;
-  if (p.lens == nullptr || pos < p.lens[b]) page = page_of(p, b, pos);
-  float k[kCh], v[kCh];
-  if (page < 0) {
+  const uint32_t span = gridDim.x * (kThreads / L), first = blockIdx.x * (kThreads / L) + threadIdx.x / L;
+  const int c = (threadIdx.x % L) * C, bs = 1 << p.page_shift;
+  int64_t from[R];  // the key's row of the pages, or -1
 #pragma unroll
-    for (int i = 0; i < kCh; ++i) k[i] = v[i] = 0.0f;
-  } else {
-    const int bs = 1 << p.page_shift, at = (int)(pos & (bs - 1));
-    const int64_t kr = ((page * p.h + j) * 2) * bs + at, vr = kr + bs;
-    if constexpr (INT8) {
-      const int8_t* pages = static_cast<const int8_t*>(p.pages);
-      dequantise16(pages + kr * D + c, p.scales[kr], k);
-      dequantise16(pages + vr * D + c, p.scales[vr], v);
-    } else {
-      load16<T, true>(static_cast<const T*>(p.pages) + kr * D + c, k);
-      load16<T, true>(static_cast<const T*>(p.pages) + vr * D + c, v);
+  for (int i = 0; i < R; ++i) {
+    const uint32_t row = first + i * span;
+    const uint32_t j = row % p.h, bt = row / p.h, t = bt % p.tokens, b = bt / p.tokens;
+    int64_t page = -1, pos = 0;
+    if (row < p.rows) {
+      pos = (int64_t)p.starts[b] + t;
+      if (p.lens == nullptr || pos < p.lens[b]) page = page_of(p, b, pos);
+    }
+    from[i] = page < 0 ? -1 : (page * p.h + j) * 2 * bs + (pos & (bs - 1));
+  }
+  uint32_t w[R][2][kWords];
+  float s[R][2];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const int64_t at = from[i] + kv * bs;
+      const char* src = static_cast<const char*>(p.pages) + (at * D + c) * (INT8 ? 1 : (int)sizeof(T));
+      s[i][kv] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) w[i][kv][k] = 0;
+      if (from[i] >= 0) {
+        if constexpr (kWords == 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(src);
+          w[i][kv][0] = x.x, w[i][kv][1] = x.y, w[i][kv][2] = x.z, w[i][kv][3] = x.w;
+        } else if constexpr (kWords == 2) {
+          const uint2 x = *reinterpret_cast<const uint2*>(src);
+          w[i][kv][0] = x.x, w[i][kv][1] = x.y;
+        } else {
+          w[i][kv][0] = *reinterpret_cast<const uint32_t*>(src);
+        }
+        if (INT8) s[i][kv] = p.scales[at];
+      }
+    }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const uint32_t row = first + i * span;
+    if (row >= p.rows) return;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      T* to = static_cast<T*>(kv ? p.out_v : p.out_k) + (int64_t)row * D + c;
+      if constexpr (INT8) {
+        float x[C];
+#pragma unroll
+        for (int k = 0; k < C; ++k) x[k] = (float)(int8_t)(w[i][kv][k / 4] >> (8 * (k % 4))) * s[i][kv];
+        store<T>(to, x);
+      } else {
+        *reinterpret_cast<uint4*>(to) = make_uint4(w[i][kv][0], w[i][kv][1], w[i][kv][2], w[i][kv][3]);
+      }
     }
   }
-  store16<T>(static_cast<T*>(p.out_k) + (int64_t)row * D + c, k);
-  store16<T>(static_cast<T*>(p.out_v) + (int64_t)row * D + c, v);
 }
 
 int check_cache(const char* who, int kind, int dtype, int h, int bs, int d, int64_t n_pages, const void* pages, const void* scales) {
@@ -265,8 +312,8 @@ PagedParams params_of(const lkv_paged_args* a, int64_t rows) {
   return p;
 }
 
-unsigned grid_of(int64_t rows, int d) {
-  const unsigned per_cta = kThreads / (d / kCh);
+unsigned grid_of(int64_t rows, int d, int dtype, int per_thread) {
+  const unsigned per_cta = kThreads / (d * (unsigned)dtype_size(dtype) / 16) * per_thread;
   return (unsigned)((rows + per_cta - 1) / per_cta);
 }
 
@@ -288,7 +335,7 @@ int lkv_paged_write(const lkv_paged_args* a, void* stream) {
   const bool vec = aligned(a->keys, 16) && aligned(a->values, 16) && a->k_sb % per == 0 && a->k_st % per == 0 && a->k_sh % per == 0 &&
                    a->v_sb % per == 0 && a->v_st % per == 0 && a->v_sh % per == 0;
   const PagedParams p = params_of(a, rows);
-  const unsigned grid = grid_of(rows, a->d);
+  const unsigned grid = grid_of(rows, a->d, a->dtype, 1);
   const bool int8 = a->kind == LKV_CACHE_INT8;
   cudaStream_t st = as_stream(stream);
   cudaError_t e;
@@ -309,8 +356,8 @@ int lkv_paged_read(const lkv_paged_args* a, void* stream) {
     return fail(LKV_ERR_PTR, "%s: null pointer", who);
   if (!aligned(a->out_k, 16) || !aligned(a->out_v, 16)) return fail(LKV_ERR_PTR, "%s: outputs must be 16-byte aligned", who);
   const PagedParams p = params_of(a, rows);
-  const unsigned grid = grid_of(rows, a->d);
   const bool int8 = a->kind == LKV_CACHE_INT8;
+  const unsigned grid = grid_of(rows, a->d, a->dtype, int8 ? kReads<true> : kReads<false>);
   cudaStream_t st = as_stream(stream);
   cudaError_t e;
   if (a->dtype == LKV_BF16)

@@ -21,7 +21,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTile = 512;        // elements a warp sums at a time
 constexpr int kMaxTiles = 1024;   // tile sums a CTA keeps
@@ -64,7 +64,7 @@ struct Weights {
 template <bool VEC>
 __device__ __forceinline__ double tile_sum(const Weights& w, int base, int lane) {
   double s = 0.0;
-  if (VEC && base + kTile <= w.vocab) {
+  if (VEC && base + kTile <= w.vocab && w.struck < 0) {
     float4 a[4], b[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = reinterpret_cast<const float4*>(w.p + base)[i * 32 + lane];
@@ -75,11 +75,19 @@ __device__ __forceinline__ double tile_sum(const Weights& w, int base, int lane)
 #pragma unroll
       for (int i = 0; i < 4; ++i) b[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
+    // A positive difference of two float32 as d + r, exactly: d rounded, r what that lost. The d are summed
+    // in float64, the r, 2^-24 of them, in float32: half the conversions, and 2^-48 of the sum is still there.
+    float lost = 0.0f;
+    auto add = [&](float x, float y) {
+      const float d = x - y;
+      if (d > 0.0f) {
+        s += (double)d;
+        lost += (x - d) - y;
+      }
+    };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int v = base + (i * 32 + lane) * 4;
-      s += (w.one(a[i].x, b[i].x, v) + w.one(a[i].y, b[i].y, v + 1)) + (w.one(a[i].z, b[i].z, v + 2) + w.one(a[i].w, b[i].w, v + 3));
-    }
+    for (int i = 0; i < 4; ++i) add(a[i].x, b[i].x), add(a[i].y, b[i].y), add(a[i].z, b[i].z), add(a[i].w, b[i].w);
+    s += (double)lost;
   } else {
     for (int i = lane; i < kTile; i += 32) s += w.at(base + i);
   }
@@ -87,7 +95,7 @@ __device__ __forceinline__ double tile_sum(const Weights& w, int base, int lane)
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads, 1) verify_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kThreads, 4) verify_kernel(const VerifyParams p) {
   __shared__ double tiles[kMaxTiles];
   __shared__ double total;
   __shared__ int first_bad;
