@@ -28,6 +28,18 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kMaxScale = 0x1.020406p+121f;  // the largest whose 127-fold is finite
 
+// Division by a number that is known when the kernel is launched: n / d for n < 2^31 (d < 2^31) as the high
+// half of a product and a shift, with m = floor(2^32 (2^s - d) / d) + 1 and s the least for which 2^s >= d.
+struct Divisor {
+  uint32_t d, m, s;
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
+Divisor divisor(uint32_t d) {
+  uint32_t s = 0;
+  while ((1ull << s) < d) ++s;
+  return {d, (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
+}
+
 struct PagedParams {
   const void* keys;    // write: [b, t, h, d] with these element strides (channels contiguous)
   const void* values;
@@ -41,7 +53,7 @@ struct PagedParams {
   const int32_t* starts;
   const int32_t* lens;  // read: tokens a sequence has (null: as many as its table)
   uint32_t rows;  // batch * tokens * h
-  uint32_t tokens, h;
+  Divisor tokens, h;
   int page_shift;
   void* out_k;  // read: contiguous [b, n, h, d]
   void* out_v;
@@ -96,30 +108,45 @@ __device__ __forceinline__ int64_t page_of(const PagedParams& p, uint32_t b, int
   return id < p.n_pages ? id : -1;
 }
 
-// One quantised row, C channels per lane of a group of L lanes: the codes (4 to a word) and the row's scale.
-template <int L, int C>
-__device__ __forceinline__ void quantise_row(const float* x, uint32_t (&w)[C / 4], float& scale) {
-  uint32_t top = 0;  // magnitudes compare as their bits; infinities and NaN come out above FLT_MAX
+// The largest magnitudes of a key row and a value row, C channels per lane of a group of L lanes, as float32
+// bits: magnitudes compare as their bits, and infinities and NaN come out above FLT_MAX.
+template <typename T, int L, int C>
+__device__ __forceinline__ uint2 row_tops(const float* k, const float* v) {
+  uint32_t a = 0, b = 0;
 #pragma unroll
-  for (int i = 0; i < C; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  for (int i = 0; i < C; ++i) a = max(a, __float_as_uint(k[i]) & 0x7fffffffu), b = max(b, __float_as_uint(v[i]) & 0x7fffffffu);
+  if constexpr (sizeof(T) == 2) {  // two bf16 travel as one word
+    uint32_t both = (a >> 16) | b;
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (top >= 0x7f800000u) {
-    scale = __uint_as_float(0x7fc00000u);
+    for (int o = L / 2; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
+    return make_uint2(both << 16, both & 0xffff0000u);
+  } else {
 #pragma unroll
-    for (int i = 0; i < C / 4; ++i) w[i] = 0;
-    return;
+    for (int o = L / 2; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o)), b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+    return make_uint2(a, b);
   }
-  const float s = fminf(fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), FLT_MIN), kMaxScale), inv = 1.0f / s, half = 0.5f * s;
-  scale = s;
+}
+
+// The scale of a row whose largest magnitude has these bits.
+__device__ __forceinline__ float scale_of(uint32_t top) {
+  if (top >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  return fminf(fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), FLT_MIN), kMaxScale);
+}
+
+// A lane's codes (4 to a word) of a row with scale s; a NaN scale has codes 0.
+template <int C>
+__device__ __forceinline__ void quantise(const float* x, float s, uint32_t (&w)[C / 4]) {
   constexpr float kWhole = 12582912.0f;  // 1.5 x 2^23: a sum with it has the whole number in its low bits
+  float inv;  // good to a few ulp, which the remainder makes up for
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  const float half = 0.5f * s;
   float k[C], far = 0.0f;
 #pragma unroll
   for (int i = 0; i < C; ++i) {
     k[i] = fmaf(x[i], inv, kWhole);
     far = fmaxf(far, fabsf(fmaf(kWhole - k[i], s, x[i])));
   }
-  if (far >= half) {
+  if (!(far < half)) {  // next to never, or s is a NaN
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       const float r = fmaf(kWhole - k[i], s, x[i]);
@@ -127,6 +154,7 @@ __device__ __forceinline__ void quantise_row(const float* x, uint32_t (&w)[C / 4
       const bool odd = (__float_as_uint(k[i]) & 1u) != 0;
       if (r > half || (r == half && odd)) k[i] += 1.0f;
       else if (r < -half || (r == -half && odd)) k[i] -= 1.0f;
+      if (isnan(s)) k[i] = kWhole;
     }
   }
 #pragma unroll
@@ -146,7 +174,7 @@ __global__ void __launch_bounds__(kThreads) paged_write_kernel(const PagedParams
   const uint32_t row = blockIdx.x * (kThreads / L) + threadIdx.x / L;
   const int c = (threadIdx.x % L) * C;
   const bool live = row < p.rows;
-  const uint32_t j = row % p.h, bt = row / p.h, t = bt % p.tokens, b = bt / p.tokens;
+  const uint32_t bt = p.h.of(row), j = row - bt * p.h.d, b = p.tokens.of(bt), t = bt - b * p.tokens.d;
   int64_t page = -1, pos = 0;
   float k[C], v[C];
   if (live) {
@@ -159,12 +187,16 @@ __global__ void __launch_bounds__(kThreads) paged_write_kernel(const PagedParams
     for (int i = 0; i < C; ++i) k[i] = v[i] = 0.0f;
   }
   const int bs = 1 << p.page_shift, at = (int)(pos & (bs - 1));
-  const int64_t kr = ((page * p.h + j) * 2) * bs + at, vr = kr + bs;  // rows of the page's keys and values
+  const int64_t kr = ((page * p.h.d + j) * 2) * bs + at, vr = kr + bs;  // rows of the page's keys and values
   if constexpr (INT8) {
-    float ks, vs;
+    // Even lanes divide for the key's scale, odd ones for the value's.
+    const uint2 tops = row_tops<T, L, C>(k, v);
+    const int lane = threadIdx.x % 32;
+    const float mine = scale_of((lane & 1) ? tops.y : tops.x);
+    const float ks = __shfl_sync(0xffffffffu, mine, lane & ~1), vs = __shfl_sync(0xffffffffu, mine, lane | 1);
     uint32_t kq[C / 4], vq[C / 4];
-    quantise_row<L, C>(k, kq, ks);
-    quantise_row<L, C>(v, vq, vs);
+    quantise<C>(k, ks, kq);
+    quantise<C>(v, vs, vq);
     if (page < 0) return;
     int8_t* pages = static_cast<int8_t*>(p.pages);
     if constexpr (C == 8) {
@@ -199,13 +231,13 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(const PagedParams 
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const uint32_t row = first + i * span;
-    const uint32_t j = row % p.h, bt = row / p.h, t = bt % p.tokens, b = bt / p.tokens;
+    const uint32_t bt = p.h.of(row), j = row - bt * p.h.d, b = p.tokens.of(bt), t = bt - b * p.tokens.d;
     int64_t page = -1, pos = 0;
     if (row < p.rows) {
       pos = (int64_t)p.starts[b] + t;
       if (p.lens == nullptr || pos < p.lens[b]) page = page_of(p, b, pos);
     }
-    from[i] = page < 0 ? -1 : (page * p.h + j) * 2 * bs + (pos & (bs - 1));
+    from[i] = page < 0 ? -1 : (page * p.h.d + j) * 2 * bs + (pos & (bs - 1));
   }
   uint32_t w[R][2][kWords];
   float s[R][2];
@@ -304,8 +336,8 @@ PagedParams params_of(const lkv_paged_args* a, int64_t rows) {
   p.starts = a->starts;
   p.lens = a->lens;
   p.rows = (uint32_t)rows;
-  p.tokens = a->tokens;
-  p.h = a->h;
+  p.tokens = divisor(a->tokens);
+  p.h = divisor(a->h);
   p.page_shift = shift_of(a->bs);
   p.out_k = a->out_k;
   p.out_v = a->out_v;

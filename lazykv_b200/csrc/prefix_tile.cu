@@ -11,7 +11,7 @@
 // one partial (m, l, o) per row, which combine_kernel (prefix.cu) folds into the output.
 //
 // Warps 0-3 and 4-7 are the two tiles' rows, warp 8 issues the matrix products, warp 9 the copies; with
-// int8 pages warps 12-19 turn codes into f16 operands. All of it is joined by mbarriers, every wait
+// int8 pages warps 12-15 turn codes of keys into f16 operands and warps 16-19 those of values. All of it is joined by mbarriers, every wait
 // bounded (tma.cuh).
 //
 // bf16 pages: P and V are bf16; the pages come by tensor-map TMA straight into the swizzled operand
@@ -295,12 +295,12 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       mbar_init(&s.p_full[i], 4);
     }
     for (int i = 0; i < T::kStages; ++i) {
-      mbar_init(&s.full[i], INT8 ? 8 : 1);
+      mbar_init(&s.full[i], INT8 ? 4 : 1);
       mbar_init(&s.empty[i], 1);
     }
     for (int i = 0; i < T::kRaw; ++i) {
       mbar_init(&s.raw_full[i], 1);
-      mbar_init(&s.raw_empty[i], 8);
+      mbar_init(&s.raw_empty[i], 4);
     }
     for (int i = 0; i < kInfo; ++i) mbar_init(&s.info[i], INT8 ? 8 : 1);
     s.quit = 0;
@@ -682,9 +682,8 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
     __syncwarp();
   } else if (warp >= 12) {
     if constexpr (INT8) {
-      // ---- codes to f16 operands: thread i also carries token i % 128's key scale, or its value scale ----
-      const int i = tid - 12 * 32, token = i % kTile;
-      const bool values = i >= kTile;
+      // ---- codes to f16 operands: warps 12-15 the keys', 16-19 the values'; thread i carries token i's scale --
+      const int i = tid % kTile, kv = (tid - 12 * 32) / kTile;
       bool ok = true;
       // Scales are loaded a tile ahead, and their page's id (checked where it is used) a tile before that:
       // neither load is waited for where it is issued.
@@ -692,15 +691,15 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       bool there = false;
       int id = -1;
       auto page_of = [&](int t) {
-        const int pos = (first + t) * kTile + token, blk = pos >> p.page_shift;
+        const int pos = (first + t) * kTile + i, blk = pos >> p.page_shift;
         id = t < n_tiles && pos < p.prefix_len && blk < p.prefix_cols ? p.prefix_table[blk] : -1;
       };
       auto scales_of = [&](int t) {
         scale = 0.0f;
         there = id >= 0 && id < p.n_pages;
         if (there) {
-          const int bs = 1 << p.page_shift, pos = (first + t) * kTile + token;
-          scale = p.scales[(((int64_t)id * p.h + j) * 2 + (values ? 1 : 0)) * bs + (pos & (bs - 1))];
+          const int bs = 1 << p.page_shift, pos = (first + t) * kTile + i;
+          scale = p.scales[(((int64_t)id * p.h + j) * 2 + kv) * bs + (pos & (bs - 1))];
         }
         page_of(t + 1);
       };
@@ -709,63 +708,61 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       // A thread's pieces of 16 codes, one channel range of every kStep-th token. Eight lanes take 128 bytes
       // that lie in 32 different banks, and so do the chunks they write: two tokens of different parity, of
       // which the swizzle puts even chunks into even and odd places.
-      constexpr int kPer = D / 16, kMine = kPer / 2, kStep = 2 * kTile / kPer;  // kStep is a multiple of 8
+      constexpr int kPer = D / 16, kStep = kTile / kPer;  // kStep is a multiple of 8
       const int odd = (i >> 2) & 1, half = odd ^ ((i >> 3) & 1);
       const int tok0 = kPer == 8 ? (i >> 4) * 2 + odd : i / kPer, c = kPer == 8 ? half * 4 + (i & 3) : i % kPer;
       const int from = (tok0 * kPer + c) * 16, row = (c / 4) * T::kHalfBytes + tok0 * 128, at = (c % 4) * 2;
       const int to0 = row + ((at ^ (tok0 & 7)) << 4), to1 = row + (((at + 1) ^ (tok0 & 7)) << 4);
-      for (int n = 0; n < 2 * n_tiles; ++n) {
-        const int t = n >> 1, kv = n & 1, raw = n % T::kRaw, slot = n % T::kStages;
-        float* ring = scale_ring + (t % kInfo) * 2 * kTile;
+      for (int t = 0; t < n_tiles; ++t) {
+        const int n = 2 * t + kv, raw = n % T::kRaw, slot = n % T::kStages, info = t % kInfo;
+        // The ring entry's last reader is more than two tiles behind (see the copies): it is free.
+        float* ring = scale_ring + (info * 2 + kv) * kTile;
+        ring[i] = scale;
+        if (kv == 1) {
+          // scale < 2^e, e from its exponent; what is not finite stays what it is. At least -40, so that the
+          // sum of the weights stays far from float32's end where the values are all but zero.
+          const int bits = (int)((__float_as_uint(scale) >> 23) & 0xffu);
+          const int top = __reduce_max_sync(0xffffffffu, bits == 0xff ? -40 : max(bits - 126, -40));
+          if (lane == 0) s.top[info][warp - 16] = top;
+        } else {
+          const uint32_t mask = __ballot_sync(0xffffffffu, there);
+          if (lane == 0) s.have[info][warp - 12] = ((mask & 0xffffu) != 0 ? 1u : 0u) << (2 * (warp - 12)) | (mask >> 16 != 0 ? 2u : 0u) << (2 * (warp - 12));
+        }
+        warp_arrive(&s.info[info], lane);
+        float down = 1.0f;  // 2^-E
+        if (kv == 1) {
+          asm volatile("bar.sync 2, 128;" ::: "memory");  // the tile's scales and exponents, of all four warps
+          down = __int_as_float((127 - largest(s.top[info])) << 23);
+        }
+        scales_of(t + 1);
         ok = ok && wait_for(s, &s.raw_full[raw], (n / T::kRaw) & 1);
         if (ok && n >= T::kStages) ok = wait_for(s, &s.empty[slot], (n / T::kStages - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) {  // given up: no warp is left at the barrier below
-          if (kv == 1) asm volatile("bar.sync 2, 256;" ::: "memory");
-          continue;
-        }
-        uint4 w[kMine];
-#pragma unroll
-        for (int x = 0; x < kMine; ++x) w[x] = *reinterpret_cast<const uint4*>(raws + raw * T::kRawBytes + from + x * (kStep * kPer * 16));
+        if (!ok) continue;  // given up; no warp is left at the barrier above
+        const char* src = raws + raw * T::kRawBytes + from;
         char* dst = stages + slot * T::kBytes;
-        if (kv == 0) {
-          ring[i] = scale;
-          if (values) {
-            // scale < 2^e, e from its exponent; what is not finite stays what it is. At least -40, so that the
-            // sum of the weights stays far from float32's end where the values are all but zero.
-            const int bits = (int)((__float_as_uint(scale) >> 23) & 0xffu);
-            const int top = __reduce_max_sync(0xffffffffu, bits == 0xff ? -40 : max(bits - 126, -40));
-            if (lane == 0) s.top[t % kInfo][warp - 16] = top;
-          } else {
-            const uint32_t mask = __ballot_sync(0xffffffffu, there);
-            if (lane == 0) s.have[t % kInfo][warp - 12] = ((mask & 0xffffu) != 0 ? 1u : 0u) << (2 * (warp - 12)) | (mask >> 16 != 0 ? 2u : 0u) << (2 * (warp - 12));
+#pragma unroll
+        for (int x0 = 0; x0 < kPer; x0 += 4) {
+          uint4 w[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) w[x] = *reinterpret_cast<const uint4*>(src + (x0 + x) * (kStep * kPer * 16));
+          if (x0 + 4 >= kPer) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.raw_empty[raw]);
           }
 #pragma unroll
-          for (int x = 0; x < kMine; ++x) {
-            const uint2 a = codes_to_f16(w[x].x), b = codes_to_f16(w[x].y), d = codes_to_f16(w[x].z), e = codes_to_f16(w[x].w);
-            *reinterpret_cast<uint4*>(dst + to0 + kStep * x * 128) = make_uint4(a.x, a.y, b.x, b.y);
-            *reinterpret_cast<uint4*>(dst + to1 + kStep * x * 128) = make_uint4(d.x, d.y, e.x, e.y);
-          }
-        } else {
-          asm volatile("bar.sync 2, 256;" ::: "memory");  // the tile's scales and exponents, which other warps wrote
-          const float down = __int_as_float((127 - largest(s.top[t % kInfo])) << 23);  // 2^-E
-#pragma unroll
-          for (int x = 0; x < kMine; ++x) {
-            const __half2 by = __float2half2_rn(ring[kTile + tok0 + kStep * x] * down);
-            const uint2 a = times(codes_to_f16(w[x].x), by), b = times(codes_to_f16(w[x].y), by), d = times(codes_to_f16(w[x].z), by),
-                        e = times(codes_to_f16(w[x].w), by);
-            *reinterpret_cast<uint4*>(dst + to0 + kStep * x * 128) = make_uint4(a.x, a.y, b.x, b.y);
-            *reinterpret_cast<uint4*>(dst + to1 + kStep * x * 128) = make_uint4(d.x, d.y, e.x, e.y);
+          for (int x = 0; x < 4; ++x) {
+            uint2 a = codes_to_f16(w[x].x), b = codes_to_f16(w[x].y), d = codes_to_f16(w[x].z), e = codes_to_f16(w[x].w);
+            if (kv == 1) {
+              const __half2 by = __float2half2_rn(ring[tok0 + kStep * (x0 + x)] * down);
+              a = times(a, by), b = times(b, by), d = times(d, by), e = times(e, by);
+            }
+            *reinterpret_cast<uint4*>(dst + to0 + kStep * (x0 + x) * 128) = make_uint4(a.x, a.y, b.x, b.y);
+            *reinterpret_cast<uint4*>(dst + to1 + kStep * (x0 + x) * 128) = make_uint4(d.x, d.y, e.x, e.y);
           }
         }
         fence_async();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&s.full[slot]);
-          mbar_arrive(&s.raw_empty[raw]);
-          if (kv == 0) mbar_arrive(&s.info[t % kInfo]);
-        }
-        if (kv == 0) scales_of(t + 1);
+        warp_arrive(&s.full[slot], lane);
       }
       __syncwarp();
     }
