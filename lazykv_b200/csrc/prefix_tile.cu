@@ -62,7 +62,7 @@ struct Tiles {
 
 struct Barriers {
   uint64_t q_full, o_full[2], s_full[2], p_full[2], tail, drain;
-  uint64_t full[8], empty[8], raw_full[3], raw_empty[3], info[kInfo];
+  uint64_t full[9], empty[9], raw_full[3], raw_empty[3], info[kInfo];
   uint32_t have[kInfo][4];   // together, bit g: tokens 16 g .. 16 g + 15 of the tile have a page
   int32_t top[kInfo][4];     // largest exponent of a finite value scale, per warp of converters
   float back[2][kTile];      // int8: what a row's scores are multiplied with (stage_query)
@@ -98,7 +98,13 @@ __device__ __forceinline__ bool wait_long(Barriers& s, uint64_t* bar, uint32_t p
   }
   return true;
 }
-__device__ __forceinline__ bool wait_for(Barriers& s, uint64_t* bar, uint32_t parity) { return try_once(bar, parity) || wait_long(s, bar, parity); }
+// For the whole warp, every lane for itself (each needs what the barrier makes visible); the warp leaves it
+// together, with one answer.
+__device__ __forceinline__ bool wait_for(Barriers& s, uint64_t* bar, uint32_t parity) {
+  const bool ok = __all_sync(0xffffffffu, try_once(bar, parity) || wait_long(s, bar, parity)) != 0;
+  __syncwarp();
+  return ok;
+}
 
 __device__ __forceinline__ int largest(const int32_t (&x)[4]) { return max(max(x[0], x[1]), max(x[2], x[3])); }
 
@@ -274,13 +280,15 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
   __shared__ Barriers s;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   char* q_tiles = smem;
-  char* stages = q_tiles + 2 * T::kBytes;
-  char* raws = stages + T::kStages * T::kBytes;
+  char* raws = q_tiles + (2 + T::kStages) * T::kBytes;
   float* scale_ring = reinterpret_cast<float*>(raws + T::kRaw * T::kRawBytes);  // [kInfo][2][kTile]: keys', values'
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int split = blockIdx.x, j = blockIdx.y, row0 = blockIdx.z * 2 * kTile;
   const int n_rows = min(2 * kTile, p.rows - row0);
   const bool two = n_rows > kTile;
+  // The second tile of queries is one stage more where there is none.
+  const int n_stages = T::kStages + (two ? 0 : 1);
+  char* stages = q_tiles + (two ? 2 : 1) * T::kBytes;
   const int first = split * chunk;                                               // this CTA's tiles of the prefix
   const int n_tiles = min(chunk, (p.prefix_len + kTile - 1) / kTile - first);
   const int n_jobs = two ? 2 * n_tiles : n_tiles;                                // job i: rows i % 2, tile two ? i / 2 : i
@@ -294,7 +302,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.p_full[i], 4);
     }
-    for (int i = 0; i < T::kStages; ++i) {
+    for (int i = 0; i <= T::kStages; ++i) {
       mbar_init(&s.full[i], INT8 ? 4 : 1);
       mbar_init(&s.empty[i], 1);
     }
@@ -358,7 +366,6 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       float e = 0.0f;  // int8: the exponent of the tile's largest value scale
       if constexpr (INT8) e = (float)largest(s.top[slot]);
       ok = ok && wait_for(s, &s.s_full[u], n_done & 1);
-      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_after();
       if (any_live) {
@@ -478,7 +485,6 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
     // ---- the rows' partials -------------------------------------------------------------------------
     const bool any_job = n_done > 0;
     if (ok && any_job) ok = wait_for(s, &s.o_full[u], 0);
-    ok = __all_sync(0xffffffffu, ok);
     tc_after();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -557,18 +563,17 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
     // ---- matrix products: issued by one lane, in order -----------------------------------------------
     constexpr uint32_t kQk = instruction<INT8>(kTile, false), kPv = instruction<INT8>(D, true);
     const uint32_t q_u = smem_u32(q_tiles), st_u = smem_u32(stages), mine = elect(), tm = __shfl_sync(0xffffffffu, tmem, 0);
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_for(s, bar, parity)) != 0; };
     // Keys of job i's tile, or its values, are in place (asked once per tile).
     auto wait_keys = [&](int i) {
       const int n = 2 * (two ? i >> 1 : i);
-      return i >= n_jobs || (two && (i & 1) != 0) || wait_all(&s.full[n % T::kStages], (n / T::kStages) & 1);
+      return i >= n_jobs || (two && (i & 1) != 0) || wait_for(s, &s.full[n % n_stages], (n / n_stages) & 1);
     };
     auto wait_values = [&](int i) {
       const int t = two ? i >> 1 : i, n = 2 * t + 1;
-      return (two && (i & 1) != 0) || (wait_all(&s.full[n % T::kStages], (n / T::kStages) & 1) && (INT8 || end - t * kTile >= kTile || wait_all(&s.tail, 0)));
+      return (two && (i & 1) != 0) || (wait_for(s, &s.full[n % n_stages], (n / n_stages) & 1) && (INT8 || end - t * kTile >= kTile || wait_for(s, &s.tail, 0)));
     };
     auto qk = [&](int i) {
-      const int t = two ? i >> 1 : i, u = i & 1, slot = 2 * t % T::kStages;
+      const int t = two ? i >> 1 : i, u = i & 1, slot = 2 * t % n_stages;
       const uint64_t a = desc_of(q_u + (two ? u * T::kBytes : 0), 16), b = desc_of(st_u + slot * T::kBytes, 16);
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) {  // 16 channels further: 32 bytes, in units of 16
@@ -579,7 +584,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       if (!two || u == 1) commit(&s.empty[slot], mine);
     };
     auto pv = [&](int i) {
-      const int t = two ? i >> 1 : i, u = i & 1, slot = (2 * t + 1) % T::kStages;
+      const int t = two ? i >> 1 : i, u = i & 1, slot = (2 * t + 1) % n_stages;
       const uint64_t b = desc_of(st_u + slot * T::kBytes, T::kHalfBytes);
 #pragma unroll
       for (int x = 0; x < kTile / 16; ++x)  // 16 tokens further: 2 KB of V, 8 columns of P
@@ -588,23 +593,19 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       if (i + 2 >= n_jobs) commit(&s.o_full[u], mine);
     };
     // The scores of job i + 2 follow the output of job i at once (the weights wait for both): their
-    // operands are asked for before the weights are. With three stages and one row tile the next keys
-    // come into the stage that these values leave, so there they are asked for after.
-    const bool early = two || T::kStages > 3;
-    bool ok = wait_all(&s.q_full, 0);
+    // operands are asked for before the weights are.
+    bool ok = wait_for(s, &s.q_full, 0);
     for (int i = 0; ok && i < 2 && i < n_jobs; ++i) {
       ok = wait_keys(i);
       tc_after();
       if (ok) qk(i);
     }
     for (int i = 0; ok && i < n_jobs; ++i) {
-      ok = wait_values(i) && (!early || wait_keys(i + 2)) && wait_all(&s.p_full[i & 1], (i >> 1) & 1);
+      ok = wait_values(i) && wait_keys(i + 2) && wait_for(s, &s.p_full[i & 1], (i >> 1) & 1);
       if (!ok) break;
       tc_after();
       pv(i);
-      if (!early) ok = wait_keys(i + 2);
-      tc_after();
-      if (ok && i + 2 < n_jobs) qk(i + 2);
+      if (i + 2 < n_jobs) qk(i + 2);
     }
     if (!ok) {  // nothing is freed under a product in flight
       commit(&s.drain, mine);
@@ -613,18 +614,17 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
     __syncwarp();
   } else if (warp == 9) {
     // ---- copies: the pages of one operand tile at a time, keys then values ----------------------------
-    // An entry of the info ring is written again kInfo tiles later. The keys of that tile need a stage
-    // that the keys of a tile at most kStages / 2 + 1 earlier have left, and those products follow the
-    // weights of all but the two jobs before them: more than that many tiles lie between.
+    // An entry of the info ring is written again kInfo = 8 tiles later. That tile's keys, or the tile's before
+    // it, have a stage that a tile's at most (n_stages + 1) / 2 = 5 before has left, and its products follow the
+    // weights of all but the two jobs before them: the entry's last reader is done.
     const int bs = 1 << p.page_shift, per = kTile >> p.page_shift;  // pages per tile
     int filled = 0;
     bool ok = true;
     for (int n = 0; ok && n < 2 * n_tiles; ++n) {
       const int t = n >> 1, kv = n & 1, pos = (first + t) * kTile;
       if constexpr (!INT8) {
-        const int slot = n % T::kStages;
-        if (n >= T::kStages) ok = wait_for(s, &s.empty[slot], (n / T::kStages - 1) & 1);
-        ok = __all_sync(0xffffffffu, ok);
+        const int slot = n % n_stages;
+        if (n >= n_stages) ok = wait_for(s, &s.empty[slot], (n / n_stages - 1) & 1);
         if (!ok) break;
         const int tok = pos + lane * bs;
         int page = -1;
@@ -649,8 +649,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
         const int seen = end - t * kTile;
         if (kv == 1 && seen < kTile) {
           // Rows of the last page past the prefix hold anything, a NaN too, and 0 x NaN is NaN.
-          ok = wait_for(s, &s.full[slot], (n / T::kStages) & 1);
-          ok = __all_sync(0xffffffffu, ok);
+          ok = wait_for(s, &s.full[slot], (n / n_stages) & 1);
           if (!ok) break;
           for (int h2 = 0; h2 < T::kHalves; ++h2)
             for (int x = seen * 8 + lane; x < kTile * 8; x += 32)
@@ -661,7 +660,6 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       } else {
         const int slot = n % T::kRaw;
         if (n >= T::kRaw) ok = wait_for(s, &s.raw_empty[slot], (n / T::kRaw - 1) & 1);
-        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const int tok = pos + lane * bs;
         int page = -1;
@@ -676,7 +674,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       }
     }
     if (!ok) {  // no copy may land after the CTA has gone
-      constexpr int kSlots = INT8 ? T::kRaw : T::kStages;
+      const int kSlots = INT8 ? T::kRaw : n_stages;
       for (int n = max(0, filled - kSlots); n < filled; ++n) mbar_wait(INT8 ? &s.raw_full[n % kSlots] : &s.full[n % kSlots], (n / kSlots) & 1);
     }
     __syncwarp();
@@ -714,7 +712,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       const int from = (tok0 * kPer + c) * 16, row = (c / 4) * T::kHalfBytes + tok0 * 128, at = (c % 4) * 2;
       const int to0 = row + ((at ^ (tok0 & 7)) << 4), to1 = row + (((at + 1) ^ (tok0 & 7)) << 4);
       for (int t = 0; t < n_tiles; ++t) {
-        const int n = 2 * t + kv, raw = n % T::kRaw, slot = n % T::kStages, info = t % kInfo;
+        const int n = 2 * t + kv, raw = n % T::kRaw, slot = n % n_stages, info = t % kInfo;
         // The ring entry's last reader is more than two tiles behind (see the copies): it is free.
         float* ring = scale_ring + (info * 2 + kv) * kTile;
         ring[i] = scale;
@@ -736,8 +734,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
         }
         scales_of(t + 1);
         ok = ok && wait_for(s, &s.raw_full[raw], (n / T::kRaw) & 1);
-        if (ok && n >= T::kStages) ok = wait_for(s, &s.empty[slot], (n / T::kStages - 1) & 1);
-        ok = __all_sync(0xffffffffu, ok);
+        if (ok && n >= n_stages) ok = wait_for(s, &s.empty[slot], (n / n_stages - 1) & 1);
         if (!ok) continue;  // given up; no warp is left at the barrier above
         const char* src = raws + raw * T::kRawBytes + from;
         char* dst = stages + slot * T::kBytes;
