@@ -27,8 +27,8 @@
 #include <cudaTypedefs.h>
 
 #include <cuda_fp16.h>
+#include <float.h>
 
-#include <type_traits>
 
 #include "prefix.cuh"
 #include "tma.cuh"
@@ -348,7 +348,8 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
     }
     float scale[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) scale[i] = p.scale_log2 * sign * (INT8 ? s.back[u][(warp % 4) * 32 + g + 8 * i] : 1.0f);  // this warp's own rows
+    // (At least a number: a score of -infinity stays one under a softmax scale of zero.)
+    for (int i = 0; i < 4; ++i) scale[i] = (p.scale_log2 == 0.0f ? FLT_MIN : p.scale_log2 * sign) * (INT8 ? s.back[u][(warp % 4) * 32 + g + 8 * i] : 1.0f);  // this warp's own rows
     const uint32_t lanes = (uint32_t)(warp % 4) << 21;  // lane 32 (warp % 4) of tensor memory
     const uint32_t ts = tmem + lanes + u * kTile, to = tmem + lanes + 2 * kTile + u * D;
     const bool any_live = base - g < n_rows;  // does this warp hold a row at all
@@ -369,16 +370,31 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       if (!ok) break;
       tc_after();
       if (any_live) {
-        auto weigh = [&](auto masked) {
-          constexpr bool kMasked = decltype(masked)::value;
-          constexpr int N = kTile / 16;
-          auto sees = [&](int x) { return !kMasked || (x < seen && ((have >> (x / 16)) & 1)); };
-          auto score = [&](const Frag& a, int k, int r) {
-            return pair(__uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1)]), __uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1) + 1]));
-          };
-          Frag f[2];
-          // The references that the weights need, from the tile's maxima, and what was summed so far brought to them.
-          auto set_references = [&]() {
+        constexpr int N = kTile / 16;
+        Frag f[2];
+        if (have != 0xffu || seen < kTile) {
+          // Columns without a token, or past the prefix's end, get scores of -infinity (their key scales are 1).
+#pragma unroll 1
+          for (int n = 0; n < N; ++n) {
+            ld(f[0], ts + 16 * n);
+            ld_wait(f[0]);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              const int col = 16 * n + 8 * ((x % 8) / 4) + c2 + (x & 1);
+              if (col >= seen || !((have >> n) & 1)) f[0].v[x / 8][x % 8] = 0xff800000u;
+            }
+            st(ts + 16 * n, f[0]);
+          }
+          st_wait();
+        }
+        auto score = [&](const Frag& a, int k, int r) {
+          return pair(__uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1)]), __uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1) + 1]));
+        };
+        // One pass, from the references as they are; where there are none yet or a score has outgrown them, they
+        // are set from the tile's maxima first. (One copy of each loop: the kernel's first jobs wait for code.)
+#pragma unroll 1
+        for (bool set = unset, again = false;; again = true) {
+          if (set) {
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
             for (int n = 0; n < N; ++n) {
@@ -388,13 +404,11 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
               for (int k = 0; k < 2; ++k) {
                 [[maybe_unused]] uint64_t kk = 0;
                 if constexpr (INT8) kk = ks[4 * (2 * n + k)];
-                const bool s0 = sees(16 * n + 8 * k + c2), s1 = sees(16 * n + 8 * k + c2 + 1);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                   uint64_t z = score(f[0], k, r);
                   if constexpr (INT8) z = mul2(z, kk);
-                  if (s0) top[r] = fmaxf(top[r], first_of(z));
-                  if (s1) top[r] = fmaxf(top[r], second_of(z));
+                  top[r] = fmaxf(fmaxf(top[r], first_of(z)), second_of(z));
                 }
               }
             }
@@ -404,6 +418,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
             for (int r = 0; r < 4; ++r) {
               top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
               top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+              // Rounded up, a reference leaves no score above it.
               const float want = top[r] == -INFINITY ? -INFINITY : __fmaf_ru(top[r], scale[r], INT8 ? e - 7.0f : 0.0f), to_ref = fmaxf(from[r], want);
               by[r] = to_ref == -INFINITY ? 1.0f : ex2(from[r] - to_ref);
               from[r] = to_ref;
@@ -424,59 +439,48 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
                 st(to + 16 * n, f[0]);
               }
             }
-          };
-          if (unset) set_references();
-          // One pass, from the references as they are; again with new ones where a score has outgrown them.
-#pragma unroll 1
-          for (bool again = false;; again = true) {
-            uint64_t ref[4], scale2[4], sum[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float x = e - (from[r] == -INFINITY ? 0.0f : from[r]);
-              ref[r] = pair(x, x), scale2[r] = pair(scale[r], scale[r]);
-            }
-            uint32_t w[N][2][4];
-            ld(f[0], ts);
-            ld_wait(f[0]);
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-              if (n + 1 < N) ld(f[(n + 1) & 1], ts + 16 * (n + 1));
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                [[maybe_unused]] uint64_t kk = 0;
-                if constexpr (INT8) kk = ks[4 * (2 * n + k)];
-                const bool s0 = sees(16 * n + 8 * k + c2), s1 = sees(16 * n + 8 * k + c2 + 1);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  uint64_t z = score(f[n & 1], k, r);
-                  if constexpr (INT8) z = mul2(z, kk);
-                  z = fma2(z, scale2[r], ref[r]);
-                  if constexpr (kMasked) z = pair(s0 ? first_of(z) : -INFINITY, s1 ? second_of(z) : -INFINITY);
-                  z = pair(ex2(first_of(z)), ex2(second_of(z)));
-                  sum[r] = add2(sum[r], z);
-                  w[n][r / 2][2 * k + (r & 1)] = INT8 ? pack_f16(first_of(z), second_of(z)) : pack_bf16(first_of(z), second_of(z));
-                }
-              }
-              if (n + 1 < N) ld_wait(f[(n + 1) & 1]);
-            }
-            // No weight is above the sum that it is part of. (Rounded up, a new reference leaves no score above it.)
-            bool over = false;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) over = over || fmaxf(first_of(sum[r]), second_of(sum[r])) > (INT8 ? kMostF16 : kMostBf16);
-            if (!again && __any_sync(0xffffffffu, over)) {
-              set_references();
-              continue;
-            }
-            const float unit = INT8 ? ex2(-e) : 1.0f;
-#pragma unroll
-            for (int n = 0; n < N; ++n) st_packed(ts + 8 * n, w[n]);  // over the scores
-#pragma unroll
-            for (int r = 0; r < 4; ++r) l[r] = fmaf(first_of(sum[r]) + second_of(sum[r]), unit, l[r]);
-            break;
           }
-        };
-        if (have != 0xffu || seen < kTile) weigh(std::true_type{});
-        else weigh(std::false_type{});
+          uint64_t ref[4], scale2[4], sum[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float x = e - (from[r] == -INFINITY ? 0.0f : from[r]);
+            ref[r] = pair(x, x), scale2[r] = pair(scale[r], scale[r]);
+          }
+          uint32_t w[N][2][4];
+          ld(f[0], ts);
+          ld_wait(f[0]);
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            if (n + 1 < N) ld(f[(n + 1) & 1], ts + 16 * (n + 1));
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              [[maybe_unused]] uint64_t kk = 0;
+              if constexpr (INT8) kk = ks[4 * (2 * n + k)];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                uint64_t z = score(f[n & 1], k, r);
+                if constexpr (INT8) z = mul2(z, kk);
+                z = fma2(z, scale2[r], ref[r]);
+                z = pair(ex2(first_of(z)), ex2(second_of(z)));
+                sum[r] = add2(sum[r], z);
+                w[n][r / 2][2 * k + (r & 1)] = INT8 ? pack_f16(first_of(z), second_of(z)) : pack_bf16(first_of(z), second_of(z));
+              }
+            }
+            if (n + 1 < N) ld_wait(f[(n + 1) & 1]);
+          }
+          // No weight is above the sum that it is part of.
+          bool over = false;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) over = over || fmaxf(first_of(sum[r]), second_of(sum[r])) > (INT8 ? kMostF16 : kMostBf16);
+          set = !again && __any_sync(0xffffffffu, over);
+          if (set) continue;
+          const float unit = INT8 ? ex2(-e) : 1.0f;
+#pragma unroll
+          for (int n = 0; n < N; ++n) st_packed(ts + 8 * n, w[n]);  // over the scores
+#pragma unroll
+          for (int r = 0; r < 4; ++r) l[r] = fmaf(first_of(sum[r]) + second_of(sum[r]), unit, l[r]);
+          break;
+        }
         st_wait();
       }
       tc_before();
@@ -693,7 +697,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
         id = t < n_tiles && pos < p.prefix_len && blk < p.prefix_cols ? p.prefix_table[blk] : -1;
       };
       auto scales_of = [&](int t) {
-        scale = 0.0f;
+        scale = kv == 0 ? 1.0f : 0.0f;  // of a token that is not there
         there = id >= 0 && id < p.n_pages;
         if (there) {
           const int bs = 1 << p.page_shift, pos = (first + t) * kTile + i;
