@@ -108,14 +108,6 @@ __device__ __forceinline__ bool wait_for(Barriers& s, uint64_t* bar, uint32_t pa
 
 __device__ __forceinline__ int largest(const int32_t (&x)[4]) { return max(max(x[0], x[1]), max(x[2], x[3])); }
 
-// The page of token pos of a page list, or -1 where it has none.
-__device__ __forceinline__ int page_at(const int32_t* table, int cols, int n_pages, int pos, int shift) {
-  const int blk = pos >> shift;
-  if (blk >= cols) return -1;
-  const int id = table[blk];
-  return id < n_pages ? id : -1;
-}
-
 // One arrival for the warp, after what all of its lanes did before.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   __syncwarp();
@@ -624,15 +616,23 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
     const int bs = 1 << p.page_shift, per = kTile >> p.page_shift;  // pages per tile
     int filled = 0;
     bool ok = true;
+    // Lane i has page i of the tile, looked up a tile ahead (its id, checked where it is used).
+    int page = -1, next = -1;
+    auto look_up = [&](int t) {
+      const int tok = (first + t) * kTile + lane * bs, blk = tok >> p.page_shift;
+      next = t < n_tiles && lane < per && tok < p.prefix_len && blk < p.prefix_cols ? p.prefix_table[blk] : -1;
+    };
+    look_up(0);
     for (int n = 0; ok && n < 2 * n_tiles; ++n) {
-      const int t = n >> 1, kv = n & 1, pos = (first + t) * kTile;
+      const int t = n >> 1, kv = n & 1;
+      if (kv == 0) {
+        page = next < p.n_pages ? next : -1;
+        look_up(t + 1);
+      }
       if constexpr (!INT8) {
         const int slot = n % n_stages;
         if (n >= n_stages) ok = wait_for(s, &s.empty[slot], (n / n_stages - 1) & 1);
         if (!ok) break;
-        const int tok = pos + lane * bs;
-        int page = -1;
-        if (lane < per && tok < p.prefix_len) page = page_at(p.prefix_table, p.prefix_cols, p.n_pages, tok, p.page_shift);
         const uint32_t granules = lane < per && page >= 0 ? ((1u << (bs / 16)) - 1) << (lane * (bs / 16)) : 0u;
         const uint32_t have = __reduce_or_sync(0xffffffffu, granules);
         if (lane == 0) mbar_arrive_expect_tx(&s.full[slot], T::kBytes);
@@ -665,9 +665,6 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
         const int slot = n % T::kRaw;
         if (n >= T::kRaw) ok = wait_for(s, &s.raw_empty[slot], (n / T::kRaw - 1) & 1);
         if (!ok) break;
-        const int tok = pos + lane * bs;
-        int page = -1;
-        if (lane < per && tok < p.prefix_len) page = page_at(p.prefix_table, p.prefix_cols, p.n_pages, tok, p.page_shift);
         const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, page >= 0));
         if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[slot], n_copies * bs * D);
         __syncwarp();
