@@ -471,29 +471,32 @@ def _one_device(who: str, *tensors: torch.Tensor | None) -> int:
     return index
 
 
-def _cache_geometry(who: str, pages: torch.Tensor, scales: torch.Tensor | None, table: torch.Tensor) -> tuple[int, int, int, int, int, int, int, int]:
-    """(n_pages, h, bs, d, cache kind) of pages [n_pages, h, 2, bs, d], and (batch, row stride, columns) of their table."""
-    if pages.dim() != 5 or not pages.is_contiguous() or pages.shape[2] != 2:
+def _cache_geometry(who: str, pages: torch.Tensor, scales: torch.Tensor | None, table: torch.Tensor) -> tuple[int, int, int, int, int, int, int, int, int]:
+    """(n_pages, h, bs, d, cache kind, scales' address) of pages [n_pages, h, 2, bs, d], and (batch, row stride,
+    columns) of their table."""
+    if pages.dim() != 5 or not pages.is_contiguous():
         raise ValueError(f"{who}: pages must be a contiguous [n_pages, h, 2, block_size, head_dim], got {tuple(pages.shape)}")
-    n, h, _, bs, d = pages.shape
-    if pages.dtype == torch.int8:
-        kind = L.LKV_CACHE_INT8
-        if scales is None or scales.dtype != torch.float32 or scales.shape != (n, h, 2, bs) or not scales.is_contiguous():
+    n, h, two, bs, d = pages.shape
+    if two != 2:
+        raise ValueError(f"{who}: pages must be a contiguous [n_pages, h, 2, block_size, head_dim], got {tuple(pages.shape)}")
+    if pages.dtype is torch.int8:
+        if scales is None or scales.dtype is not torch.float32 or scales.shape != (n, h, 2, bs) or not scales.is_contiguous():
             raise ValueError(f"{who}: int8 pages need contiguous float32 scales [{n}, {h}, 2, {bs}]")
+        kind, at = 1, scales.data_ptr()  # LKV_CACHE_INT8
+    elif scales is not None:
+        raise ValueError(f"{who}: scales belong to int8 pages, these are {pages.dtype}")
     else:
-        kind = L.LKV_CACHE_MODEL
-        if scales is not None:
-            raise ValueError(f"{who}: scales belong to int8 pages, these are {pages.dtype}")
-    if table.dtype != torch.int32 or table.dim() != 2:
+        kind, at = 0, 0  # LKV_CACHE_MODEL
+    if table.dtype is not torch.int32 or table.dim() != 2:
         raise ValueError(f"{who}: the page table must be int32 [batch, columns] with unit column stride")
     (batch, cols), (ld, unit) = table.shape, table.stride()
     if unit != 1 and cols > 1:
         raise ValueError(f"{who}: the page table must be int32 [batch, columns] with unit column stride")
-    return n, h, bs, d, kind, batch, ld, cols
+    return n, h, bs, d, kind, at, batch, ld, cols
 
 
 def _per_sequence(who: str, name: str, t: torch.Tensor, batch: int) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != batch or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != batch or not t.is_contiguous():
         raise ValueError(f"{who}: {name} must be a contiguous int32 [{batch}]")
 
 
@@ -508,21 +511,24 @@ def paged_write(keys: torch.Tensor, values: torch.Tensor, pages: torch.Tensor, t
     [0, n_pages)) is not written, so a batch may be padded. Two tokens must not share a row.
     """
     who = "paged_write"
-    index = _one_device(who, keys, values, pages, table, starts, scales)
-    dtype = keys.dtype
-    if keys.dim() != 4 or values.shape != keys.shape or values.dtype != dtype:
-        raise ValueError(f"paged_write: keys and values must be alike, [batch, T, h, d]; got {tuple(keys.shape)} and {tuple(values.shape)}")
-    batch, t, h, d = keys.shape
-    n, ph, bs, pd, kind, rows, ld, cols = _cache_geometry(who, pages, scales, table)
-    if ph != h or pd != d or (kind == L.LKV_CACHE_MODEL and pages.dtype != dtype):
-        raise ValueError(f"paged_write: {tuple(keys.shape)} {dtype} tokens do not fit pages {tuple(pages.shape)} {pages.dtype}")
+    index = keys.get_device()
+    if index < 0 or not (values.get_device() == pages.get_device() == table.get_device() == starts.get_device() == index) or (
+            scales is not None and scales.get_device() != index):
+        index = _one_device(who, keys, values, pages, table, starts, scales)
+    dtype, shape = keys.dtype, keys.shape
+    if keys.dim() != 4 or values.shape != shape or values.dtype is not dtype:
+        raise ValueError(f"paged_write: keys and values must be alike, [batch, T, h, d]; got {tuple(shape)} and {tuple(values.shape)}")
+    batch, t, h, d = shape
+    n, ph, bs, pd, kind, at, rows, ld, cols = _cache_geometry(who, pages, scales, table)
+    if ph != h or pd != d or (kind == 0 and pages.dtype is not dtype):
+        raise ValueError(f"paged_write: {tuple(shape)} {dtype} tokens do not fit pages {tuple(pages.shape)} {pages.dtype}")
     (kb, kt, kh, kc), (vb, vt, vh, vc) = keys.stride(), values.stride()
     if rows != batch or kc != 1 or vc != 1:
         raise ValueError("paged_write: one table row per sequence, and contiguous channels")
     _per_sequence(who, "starts", starts, batch)
     _run("lkv_paged_write", L.PAGED_ARGS.pack(
-        keys.data_ptr(), values.data_ptr(), kb, kt, kh, vb, vt, vh, dtype_code(dtype), batch, t, h, d, pages.data_ptr(), kind,
-        0 if scales is None else scales.data_ptr(), n, bs, table.data_ptr(), ld, cols, starts.data_ptr(), 0, 0, 0), index)
+        keys.data_ptr(), values.data_ptr(), kb, kt, kh, vb, vt, vh, dtype_code(dtype), batch, t, h, d, pages.data_ptr(), kind, at, n, bs,
+        table.data_ptr(), ld, cols, starts.data_ptr(), 0, 0, 0), index)
 
 
 def paged_read(pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, n_tokens: int, lens: torch.Tensor | None = None,
@@ -534,10 +540,13 @@ def paged_read(pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, n
     tokens without a page are zeros.
     """
     who = "paged_read"
-    index = _one_device(who, pages, table, starts, lens, scales)
-    n, h, bs, d, kind, batch, ld, cols = _cache_geometry(who, pages, scales, table)
-    if kind == L.LKV_CACHE_MODEL:
-        if dtype is not None and dtype != pages.dtype:
+    index = pages.get_device()
+    if index < 0 or not (table.get_device() == starts.get_device() == index) or (lens is not None and lens.get_device() != index) or (
+            scales is not None and scales.get_device() != index):
+        index = _one_device(who, pages, table, starts, lens, scales)
+    n, h, bs, d, kind, at, batch, ld, cols = _cache_geometry(who, pages, scales, table)
+    if kind == 0:
+        if dtype is not None and dtype is not pages.dtype:
             raise ValueError(f"paged_read: {pages.dtype} pages are read back as {pages.dtype}, not {dtype}")
         dtype = pages.dtype
     elif dtype is None:
@@ -548,18 +557,18 @@ def paged_read(pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, n
     _per_sequence(who, "starts", starts, batch)
     if lens is not None:
         _per_sequence(who, "lens", lens, batch)
-    shape = (batch, n_tokens, h, d)
     if out is None:
-        k, v = pages.new_empty(shape, dtype=dtype), pages.new_empty(shape, dtype=dtype)
+        k = pages.new_empty((batch, n_tokens, h, d), dtype=dtype)
+        v = torch.empty_like(k)
         out = k, v
     else:
         k, v = out
         for o in out:
-            if o.shape != shape or o.dtype != dtype or o.get_device() != index or not o.is_contiguous():
-                raise ValueError(f"paged_read: out must be two contiguous {dtype} {shape} on cuda:{index}")
+            if o.shape != (batch, n_tokens, h, d) or o.dtype is not dtype or o.get_device() != index or not o.is_contiguous():
+                raise ValueError(f"paged_read: out must be two contiguous {dtype} {(batch, n_tokens, h, d)} on cuda:{index}")
     _run("lkv_paged_read", L.PAGED_ARGS.pack(
-        0, 0, 0, 0, 0, 0, 0, 0, code, batch, n_tokens, h, d, pages.data_ptr(), kind, 0 if scales is None else scales.data_ptr(), n, bs,
-        table.data_ptr(), ld, cols, starts.data_ptr(), 0 if lens is None else lens.data_ptr(), k.data_ptr(), v.data_ptr()), index)
+        0, 0, 0, 0, 0, 0, 0, 0, code, batch, n_tokens, h, d, pages.data_ptr(), kind, at, n, bs, table.data_ptr(), ld, cols, starts.data_ptr(),
+        0 if lens is None else lens.data_ptr(), k.data_ptr(), v.data_ptr()), index)
     return out
 
 
@@ -585,35 +594,41 @@ def prefix_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tens
     several captured graphs do not share it.
     """
     who = "prefix_attention"
-    index = _one_device(who, query, pages, table, lens, prefix_table, scales, out, lse)
-    if query.dim() != 4 or query.dtype != torch.bfloat16:
+    index = query.get_device()
+    if index < 0 or not (pages.get_device() == table.get_device() == lens.get_device() == prefix_table.get_device() == index) or (
+            scales is not None and scales.get_device() != index):
+        index = _one_device(who, query, pages, table, lens, prefix_table, scales)
+    if query.dim() != 4 or query.dtype is not torch.bfloat16:
         raise ValueError(f"prefix_attention: query must be bfloat16 [batch, T, hq, d], got {query.dtype} {tuple(query.shape)}")
     batch, t, hq, d = query.shape
-    n, h, bs, pd, kind, rows, ld, cols = _cache_geometry(who, pages, scales, table)
-    if pd != d or h < 1 or hq % h or rows != batch or (kind == L.LKV_CACHE_MODEL and pages.dtype != torch.bfloat16):
+    n, h, bs, pd, kind, at, rows, ld, cols = _cache_geometry(who, pages, scales, table)
+    if pd != d or h < 1 or hq % h or rows != batch or (kind == 0 and pages.dtype is not torch.bfloat16):
         raise ValueError(f"prefix_attention: query {tuple(query.shape)} and table {tuple(table.shape)} do not fit {pages.dtype} pages {tuple(pages.shape)}")
     _per_sequence(who, "lens", lens, batch)
     pcols = prefix_table.numel()
-    if prefix_table.dtype != torch.int32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous() or not 0 <= prefix_len <= pcols * bs:
+    if prefix_table.dtype is not torch.int32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous() or not 0 <= prefix_len <= pcols * bs:
         raise ValueError(f"prefix_attention: prefix_table must be a contiguous int32 [columns] holding the {prefix_len} tokens of the prefix")
     sb, st, sh, sc = query.stride()
     if sc != 1 or (sb | st | sh) & 7 or query.data_ptr() & 15:
         query = query.clone(memory_format=torch.contiguous_format)
         sb, st, sh, _ = query.stride()
     if out is None:
-        out = query.new_empty((batch, t, hq, d)) if out_dtype is None else query.new_empty((batch, t, hq, d), dtype=out_dtype)
-    elif out.shape != query.shape or not out.is_contiguous() or (out_dtype is not None and out.dtype != out_dtype):
-        raise ValueError(f"prefix_attention: out must be a contiguous {tuple(query.shape)}")
+        if out_dtype is None:
+            out = torch.empty_like(query) if query.is_contiguous() else query.new_empty((batch, t, hq, d))
+        else:
+            out = query.new_empty((batch, t, hq, d), dtype=out_dtype)
+    elif out.shape != query.shape or not out.is_contiguous() or (out_dtype is not None and out.dtype is not out_dtype) or out.get_device() != index:
+        raise ValueError(f"prefix_attention: out must be a contiguous {tuple(query.shape)} on cuda:{index}")
     if lse is None:
         lse = query.new_empty((batch, t, hq), dtype=torch.float32)
-    elif lse.shape != (batch, t, hq) or lse.dtype != torch.float32 or not lse.is_contiguous():
-        raise ValueError(f"prefix_attention: lse must be a contiguous float32 {(batch, t, hq)}")
+    elif lse.shape != (batch, t, hq) or lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.get_device() != index:
+        raise ValueError(f"prefix_attention: lse must be a contiguous float32 {(batch, t, hq)} on cuda:{index}")
+    code = dtype_code(out.dtype)
     nbytes = _prefix_workspace(batch, t, hq, h, d, prefix_len, kind, cols * bs)
     ws = query.new_empty((nbytes + 1) // 2) if nbytes else None
     _run("lkv_prefix_attention", L.PREFIX_ARGS.pack(
-        query.data_ptr(), L.LKV_BF16, sb, st, sh, pages.data_ptr(), kind, 0 if scales is None else scales.data_ptr(), n, bs, batch, t, hq, h, d,
-        table.data_ptr(), ld, cols, lens.data_ptr(), prefix_table.data_ptr(), pcols, prefix_len, scale, out.data_ptr(), dtype_code(out.dtype),
-        lse.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes), index)
+        query.data_ptr(), 1, sb, st, sh, pages.data_ptr(), kind, at, n, bs, batch, t, hq, h, d, table.data_ptr(), ld, cols, lens.data_ptr(),
+        prefix_table.data_ptr(), pcols, prefix_len, scale, out.data_ptr(), code, lse.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes), index)
     return out, lse
 
 
@@ -630,7 +645,9 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     target there. Returns (kept [batch] int32, token [batch] int64); token is -1 where the weights are all
     zero or have no finite sum.
     """
-    index = _one_device("verify_drafts", target, draft, tokens, uniforms)
+    index = target.get_device()
+    if index < 0 or not (tokens.get_device() == uniforms.get_device() == index) or (draft is not None and draft.get_device() != index):
+        index = _one_device("verify_drafts", target, draft, tokens, uniforms)
     if target.dim() != 3 or tokens.dim() != 2:
         raise ValueError("verify_drafts: target must be [batch, k + 1, vocab] and tokens [batch, k]")
     batch, k = tokens.shape
@@ -639,7 +656,7 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
         raise ValueError(f"verify_drafts: {k} tokens drafted for {batch} sequences do not fit target {tuple(target.shape)}, uniforms "
                          f"{tuple(uniforms.shape)}, draft {None if draft is None else tuple(draft.shape)}")
     f32 = torch.float32
-    if target.dtype != f32 or uniforms.dtype != f32 or tokens.dtype != torch.int64 or (draft is not None and draft.dtype != f32):
+    if target.dtype is not f32 or uniforms.dtype is not f32 or tokens.dtype is not torch.int64 or (draft is not None and draft.dtype is not f32):
         raise ValueError("verify_drafts: probabilities and uniforms are float32, tokens int64")
     (pb, pt, pv), (tb, tk), (ub, uk) = target.stride(), tokens.stride(), uniforms.stride()
     qb, qt, qv = (0, 0, 1) if draft is None else draft.stride()
