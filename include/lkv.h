@@ -617,7 +617,7 @@ int lkv_paged_read(const lkv_paged_args* args, void* stream);
  * token without a page is not attended. out [batch, tokens, hq, d] contiguous in out_dtype and lse
  * [batch, tokens, hq] float32; a row that attends nothing gets out = 0, lse = -inf. lens and the tables
  * are read on the device, so a captured graph follows them; prefix_len and the shapes are the call's.
- * The prefix is read once for the batch. Partials go to the workspace (any contents,
+ * The prefix is read once for up to 256 query rows per KV head (batch * tokens * hq / h). Partials go to the workspace (any contents,
  * lkv_prefix_attention_workspace bytes with own_reach = table_cols * bs, 16-byte aligned) and are merged
  * by the last of two or three launches. Calls that may overlap on the GPU need a workspace each.
  */

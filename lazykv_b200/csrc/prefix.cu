@@ -273,9 +273,9 @@ __device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D 
     for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
   float above = 0.0f;  // int8: E - 7
   if constexpr (INT8) {
-    // Scales are below 2^E, E from the largest finite one's exponent; at least 2^-40, so that the sums stay
+    // Scales are below 2^E, E from the largest finite one's exponent; at least -64, so that the sums stay
     // far from float32's end where the values are all but zero.
-    int bits = 87;  // of 2^-40
+    int bits = 62;  // E = -64
 #pragma unroll
     for (int n = 0; n < 2 * S::kGran; ++n) {
       const int x = (__float_as_int(vs[n].x) >> 23) & 0xff, y = (__float_as_int(vs[n].y) >> 23) & 0xff;
@@ -815,6 +815,8 @@ int lkv_prefix_attention(const lkv_prefix_args* a, void* stream) {
   const int group = a->hq / a->h;
   const int64_t rows = (int64_t)a->batch * a->tokens * group;
   if (a->batch > 65535 || a->h > 65535 || rows > (1 << 24)) return fail(LKV_ERR_ARG, "%s: a batch of %d with %lld rows per KV head", who, a->batch, (long long)rows);
+  const int64_t own_units = (int64_t)a->batch * a->h * (((int64_t)a->tokens * group + kRows - 1) / kRows);
+  if (own_units > (1 << 30)) return fail(LKV_ERR_ARG, "%s: a batch of %d with %lld row tiles", who, a->batch, (long long)own_units);
   if (a->q == nullptr || a->out == nullptr || a->lse == nullptr || a->lens == nullptr || a->pages == nullptr ||
       (a->kind == LKV_CACHE_INT8 && a->scales == nullptr) || (a->table_cols > 0 && a->table == nullptr) || (a->prefix_len > 0 && a->prefix_table == nullptr))
     return fail(LKV_ERR_PTR, "%s: null pointer", who);

@@ -718,10 +718,10 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
         float* ring = scale_ring + (info * 2 + kv) * kTile;
         ring[i] = scale;
         if (kv == 1) {
-          // scale < 2^e, e from its exponent; what is not finite stays what it is. At least -40, so that the
+          // scale < 2^e, e from its exponent; what is not finite stays what it is. At least -64, so that the
           // sum of the weights stays far from float32's end where the values are all but zero.
           const int bits = (int)((__float_as_uint(scale) >> 23) & 0xffu);
-          const int top = __reduce_max_sync(0xffffffffu, bits == 0xff ? -40 : max(bits - 126, -40));
+          const int top = __reduce_max_sync(0xffffffffu, bits == 0xff ? -64 : max(bits - 126, -64));
           if (lane == 0) s.top[info][warp - 16] = top;
         } else {
           const uint32_t mask = __ballot_sync(0xffffffffu, there);

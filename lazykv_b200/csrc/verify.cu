@@ -64,7 +64,7 @@ struct Weights {
 template <bool VEC>
 __device__ __forceinline__ double tile_sum(const Weights& w, int base, int lane) {
   double s = 0.0;
-  if (VEC && base + kTile <= w.vocab && w.struck < 0) {
+  if (VEC && base + kTile <= w.vocab && (w.struck < base || w.struck >= base + kTile)) {
     float4 a[4], b[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = reinterpret_cast<const float4*>(w.p + base)[i * 32 + lane];

@@ -581,7 +581,7 @@ def prefix_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tens
                      scale: float, scales: torch.Tensor | None = None, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
                      lse: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Attention of query [batch, T, hq, d] (bfloat16) for a batch that shares a prefix, whose pages are
-    read once for all (lkv_prefix_attention, two or three launches). Query t of sequence b attends the prefix_len
+    read once for all, up to 256 query rows per KV head (lkv_prefix_attention, two or three launches). Query t of sequence b attends the prefix_len
     tokens of the pages that prefix_table [columns] lists, and the first lens[b] - T + t + 1 of its own
     lens[b] tokens in the pages of table[b]: the step's T tokens (drafted ones included) are written
     before the call and are the last of lens[b].

@@ -46,6 +46,7 @@ class PagedBatch:
         self.table = torch.full((max_seqs, self.cols), -1, dtype=torch.int32, device=self.dev)
         self.prefix_table = torch.empty(0, dtype=torch.int32, device=self.dev)
         self.prefix_len = 0
+        K.status_attach(self.pages.device)
         self._prefix_pages: list[int] = []
         self._free_pages = list(range(n_pages - 1, -1, -1))
         self._free_seqs = list(range(max_seqs - 1, -1, -1))
@@ -121,6 +122,7 @@ class PagedBatch:
         """T new tokens of every sequence: keys / values [n, T, h, d] are written, and query [n, T, h * g, d]
         attends the prefix and the sequences' own tokens, each position those up to itself. Returns
         (out [n, T, h * g, d], lse [n, T, h * g] float32)."""
+        K.raise_on_status("PagedBatch.step")  # an earlier step's wait that ran out (not synchronised)
         n = len(seq_ids)
         if len(set(seq_ids)) != n:
             raise ValueError(f"a sequence is named twice in {seq_ids}")

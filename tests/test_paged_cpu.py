@@ -105,7 +105,7 @@ def _attend(lib, **over: object) -> int:  # noqa: ANN001
     (dict(kind=4), 1, "cache kind"), (dict(dtype=0), 1, "dtype"), (dict(out_dtype=9), 1, "dtype"), (dict(d=32), 1, "head_dim"), (dict(bs=8), 1, "pages of 8"),
     (dict(hq=7), 1, "do not group"), (dict(h=0), 1, "do not group"), (dict(batch=-2), 1, "bad shape"), (dict(table_ld=2), 1, "bad shape"),
     (dict(prefix_len=-1), 1, "bad shape"), (dict(prefix_len=65), 1, "a prefix of 65"), (dict(batch=70000), 1, "a batch of 70000"),
-    (dict(tokens=2**23, batch=1), 1, "a batch of 1"), (dict(table_cols=2**28, table_ld=2**28), 1, "2^30"), (dict(q=0), 2, "null"), (dict(lens=0), 2, "null"),
+    (dict(tokens=2**23, batch=1), 1, "a batch of 1"), (dict(table_cols=2**28, table_ld=2**28), 1, "2^30"), (dict(batch=60000, h=60000, hq=60000), 1, "row tiles"), (dict(q=0), 2, "null"), (dict(lens=0), 2, "null"),
     (dict(scales=0), 2, "null"), (dict(prefix_table=0), 2, "null"), (dict(out=0), 2, "null"), (dict(lse=0), 2, "null"),
     (dict(q=4104), 2, "aligned"), (dict(q_sh=68), 2, "aligned"), (dict(workspace_bytes=64), 4, "workspace"), (dict(workspace=0), 2, "workspace"),
 ])

@@ -6,7 +6,15 @@ sum p. A score is a float32 sum of d products (two more roundings for the scales
 delta = (d + 4) 2^-24 reach with reach = max over keys of sum |q k| scale, which moves every weight by a
 factor within e^(+-delta), and so do exp2's own error (2^-22) and the float32 sums of n keys (at most
 n 2^-24, their worst case): out is off by (2^-8 + 2 (delta + 2^-22 + n 2^-24)) mass, plus half a step of a
-bfloat16 output. lse is off by delta + 2^-22 + n 2^-24, plus float32's roundings of its own size."""
+bfloat16 output. lse is off by delta + 2^-22 + n 2^-24, plus float32's roundings of its own size.
+
+int8 pages: weights and the scales of values are rounded to f16 instead, relative 2^-11 each (three of them,
+with the product of a code and its scale: less than 2^-8), but with a last bit. A reference is set so that the
+largest weight times the largest value scale 2^E is 2^7, and f16 steps by 2^-24 at least: a weight times its
+scale is off by up to 2^-25 = 2^-32 of that, which a code of 127 makes 2^-32 127 2^E <= 2^-31 vmax (2^E is less
+than twice the largest scale, and 127 times that is vmax, the largest magnitude of a value). n keys: at most
+n 2^-31 vmax, the sum of the weights being at least the largest. A scale below 2^-14 of 2^E is off by up to
+2^-25 of it: weights that sum to one make that 2^-24 vmax."""
 
 from __future__ import annotations
 
@@ -52,6 +60,9 @@ def check(cache: Cache, query: torch.Tensor, tables, lens, prefix_table, prefix:
     delta = (d + 4) * 2.0**-24 * reach
     sums = delta + 2.0**-22 + n * 2.0**-24
     bound = (2.0**-8 + 2 * sums[..., None]) * mass + (2.0**-8 if out.dtype == torch.bfloat16 else 2.0**-23) * want.abs()
+    if cache.int8:
+        vmax = float((cache.scales[:, :, 1].nan_to_num(0.0) * 127).amax())
+        bound = bound + (n * 2.0**-31 + 2.0**-24) * vmax
     err = (out.double().cpu() - want).abs()
     nan, lost = want.isnan(), wlse.isnan()  # where a row attends a NaN it is one
     assert bool(((err <= bound) | nan).all()), (float(err[~nan].max()), float((err / bound.clamp_min(1e-30))[~nan].max()))
@@ -77,6 +88,9 @@ CASES = [
     (2, 1, 1, 16, 3000, [1]),  # one row: the prefix split over many CTAs
     (1, 8, 1, 32, 513, [20 + i for i in range(40)]),  # 320 rows: more than one tile of 256
     (2, 4, 7, 16, 640, [7 + 3 * i for i in range(10)]),  # 280 rows, odd numbers of tokens
+    (1, 8, 1, 128, 385, [1] * 50),  # 400 rows: a second block of more than one tile; one token in the last tile
+    (1, 4, 1, 64, 384, [3] * 20),  # whole tiles only
+    (1, 17, 1, 16, 5000, [2]),  # 17 rows: the fewest that take the tiled prefix; many splits
 ]
 
 
@@ -243,6 +257,45 @@ def test_strides_streams_given_outputs_and_graphs(b: int) -> None:
     torch.cuda.synchronize()
     for o, l in outs:
         assert torch.equal(o, again) and torch.equal(l, again_lse)
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("b", [3, 40])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1.5])
+def test_any_softmax_scale(scale: float, b: int, int8: bool) -> None:
+    from lazykv_b200 import kernels as K
+
+    gen = torch.Generator().manual_seed(31)
+    lens = [9 + i % 5 for i in range(b)]
+    cache, prefix_table, tables = build(gen, 1, 64, 16, int8, 200, lens)
+    prefix_table[3] = -1  # missing pages and a last tile that is not full, under a scale of zero too
+    pages, scales, ptab, table, n = on_gpu(cache, prefix_table, tables, lens)
+    query = torch.randn((b, 1, 4, 64), generator=gen).bfloat16()
+    out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, 200, scale, scales=scales, out_dtype=torch.float32)
+    check(cache, query, tables, lens, prefix_table, 200, scale, out, lse)
+
+
+@pytest.mark.parametrize("b", [3, 40])
+@pytest.mark.parametrize("up", [-60, 0, 60])
+def test_int8_pages_of_any_magnitude(b: int, up: int) -> None:
+    """Queries times 2^up under a softmax scale of 2^-up, values times 2^up or 2^-up: powers of two change no
+    rounding of float32, and those of the f16 operands are taken from them."""
+    from lazykv_b200 import kernels as K
+
+    gen = torch.Generator().manual_seed(32)
+    lens = [9 + i % 5 for i in range(b)]
+    cache, prefix_table, tables = build(gen, 1, 64, 16, True, 200, lens, fill=0.0)
+    pages, scales, ptab, table, n = on_gpu(cache, prefix_table, tables, lens)
+    query = torch.randn((b, 1, 4, 64), generator=gen).bfloat16()
+    base = K.prefix_attention(query.cuda(), pages, table, n, ptab, 200, 0.125, scales=scales, out_dtype=torch.float32)
+    big = (query.float() * 2.0**up).bfloat16().cuda()
+    out, lse = K.prefix_attention(big, pages, table, n, ptab, 200, 0.125 * 2.0**-up, scales=scales, out_dtype=torch.float32)
+    assert torch.equal(out, base[0]) and torch.equal(lse, base[1])
+    scales[:, :, 1] *= 2.0**up  # the references move with the values: their sums are rounded at other places
+    out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, 200, 0.125, scales=scales, out_dtype=torch.float32)
+    assert bool(((out * 2.0**-up - base[0]).abs() <= 2.0**-10 * base[0].abs().amax()).all())
+    # lse is a difference of two numbers of up to 70: their float32 roundings
+    assert bool(((lse - base[1]).abs() <= 6 * 70 * 2.0**-24).all())
 
 
 def test_one_result_for_one_input() -> None:
