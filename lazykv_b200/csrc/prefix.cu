@@ -5,10 +5,11 @@
 // the group. Row (b, t, g) sees the prefix [0, prefix_len) and own tokens 0 .. lens[b] - tokens + t.
 // Softmaxes over disjoint key sets merge exactly by their references and sums, so the work is cut into
 // partials (m, l, o), l = sum 2^(s - m), o = sum 2^(s - m) v, s the scores in the log2 domain:
-//   1. stream_kernel: the sequences' own tokens, and the prefix too where the batch has few rows;
-//   2. prefix_tile_kernel (prefix_tile.cu): the prefix for many rows, on tcgen05;
+//   1. prefix_tile_kernel (prefix_tile.cu): the prefix for many rows, on tcgen05;
+//   2. stream_kernel: the sequences' own tokens, and the prefix too where the batch has few rows;
 //   3. combine_kernel: the partials of every row.
-// Each launch starts under the one before it (programmatic dependent launch).
+// Each launch starts under the one before it (programmatic dependent launch): the stream's CTAs take the
+// SMs that the tiles leave, or never had (32 rows on 32K int8 tokens: 38 us, the other way about 44).
 //
 // stream_kernel is bound by the pages' bytes. Its work is one line of stages (prefix.cuh) that all warps
 // of the grid share equally, whatever the sequences' lengths: only the device knows them, and with a CTA
@@ -457,12 +458,9 @@ __device__ __forceinline__ Place place_at(const Params& p, const Line& line, int
 }
 
 template <int D, bool INT8>
-__global__ void __launch_bounds__(kThreads, (Shape<D, INT8>::kCtas)) stream_kernel(const Params p) {
+__device__ __forceinline__ void stream(const Params& p, char* ring) {
   using S = Shape<D, INT8>;
-  extern __shared__ __align__(128) char ring[];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, r = lane / 4, c = lane % 4;
-  pdl_wait();
-  pdl_release();
   const Line line = sum_line(p, lane);
   const int w = blockIdx.x * kWarps + warp;
   const int64_t piece = piece_length(p, line), length = line_length(p, line);
@@ -606,6 +604,17 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, INT8>::kCtas)) stream_kern
     if (ch == 0) p.slot_ml[to] = make_float2(m, l);
     *reinterpret_cast<float4*>(p.slot_o + to * D + ch) = o;
   }
+}
+
+template <int D, bool INT8>
+__global__ void __launch_bounds__(kThreads, (Shape<D, INT8>::kCtas)) stream_kernel(const Params p) {
+  extern __shared__ __align__(128) char ring[];
+  // Behind the tiles' launch, which itself waited for what ran before it and only then let this one start,
+  // the inputs are in place; otherwise this one has to wait for them.
+  if (!p.tile_first) pdl_wait();
+  pdl_release();
+  stream<D, INT8>(p, ring);
+  if (p.tile_first) pdl_wait();  // what comes after this launch may read the tiles' partials too
 }
 
 // A warp's sum over some partials of a row: lane `lane` has channels 4 (lane % (D / 4)) .., and where D is 64
@@ -864,14 +873,15 @@ int lkv_prefix_attention(const lkv_prefix_args* a, void* stream) {
   cudaStream_t st = as_stream(stream);
   const bool int8 = a->kind == LKV_CACHE_INT8, wide = a->d == 128;
   cudaError_t e = cudaSuccess;
+  if (p.n_splits > 0) {
+    if (int rc = run_tiles(p, a->d, int8, st)) return rc;
+    p.tile_first = 1;
+  }
   if (p.n_warps > 0) {
     e = wide ? (int8 ? launch_stream<128, true>(p, st) : launch_stream<128, false>(p, st))
              : (int8 ? launch_stream<64, true>(p, st) : launch_stream<64, false>(p, st));
     if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "%s (stream): %s", who, cudaGetErrorString(e));
-    p.stream_first = 1;
   }
-  if (p.n_splits > 0)
-    if (int rc = run_tiles(p, a->d, int8, st)) return rc;
   // Several warps to a row where it has many partials.
   const int parts = p.n_splits + (p.prefix_stages > 0 ? p.n_warps / (kWarps * a->h) : 0), team = parts > 16 ? 4 : parts > 8 ? 2 : 1;
   const int unit = a->tokens * group, per = kWarps / team;

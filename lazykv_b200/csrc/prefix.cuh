@@ -57,7 +57,7 @@ struct Params {
   void* out;             // [batch, tokens, hq, d]
   int out_f32;
   float* lse;            // [batch, tokens, hq]
-  int stream_first;      // the tiled prefix runs behind a stream launch
+  int tile_first;        // the stream's launch is behind the tiled prefix's
 };
 
 __device__ __forceinline__ float ex2(float x) {

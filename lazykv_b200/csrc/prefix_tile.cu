@@ -314,9 +314,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
   __syncthreads();
   tc_after();
   const uint32_t tmem = s.tmem;  // columns: S or P of the two row tiles at 0 and 128, O at 256 and 256 + D
-  // Behind the stream's launch, which itself waited for what ran before it and only then let this one
-  // start, the inputs are in place; first of all, this launch has to wait. The stream is waited for at the end.
-  if (!p.stream_first) pdl_wait();
+  pdl_wait();
   pdl_release();
 
   if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kMany));
@@ -766,7 +764,6 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
     }
   }
   __syncthreads();
-  if (p.stream_first) pdl_wait();  // what comes after this launch may read the stream's partials too
   if (warp == 8) {
     tc_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
