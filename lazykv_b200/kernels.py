@@ -442,16 +442,21 @@ def quest_topk_admit(query: torch.Tensor, kmin: torch.Tensor, kmax: torch.Tensor
 
 
 _device_of = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_stream_of = L._RAW_STREAM if L._RAW_STREAM is not None else lambda index: torch.cuda.current_stream(index).cuda_stream
+_ENTRY: dict[str, object] = {}  # entries that have been called
+_F32, _BF16, _I8, _I32, _I64 = torch.float32, torch.bfloat16, torch.int8, torch.int32, torch.int64
 
 
 def _run(name: str, args: bytes, index: int) -> None:
     """Entry `name` (an args struct and a stream) on the current stream of device `index`, which is made current."""
-    fn = getattr(L.lib(), name)
+    fn = _ENTRY.get(name)
+    if fn is None:
+        fn = _ENTRY[name] = getattr(L.lib(), name)
     if index == _device_of():
-        rc = fn(args, L._RAW_STREAM(index) if L._RAW_STREAM is not None else stream_handle(torch.device("cuda", index)))
+        rc = fn(args, _stream_of(index))  # type: ignore[operator]
     else:
         with torch.cuda.device(index):
-            rc = fn(args, stream_handle(torch.device("cuda", index)))
+            rc = fn(args, _stream_of(index))  # type: ignore[operator]
     if rc != 0:
         raise L.LkvError(f"{name} failed ({rc}): {L.last_error()}")
 
@@ -479,15 +484,15 @@ def _cache_geometry(who: str, pages: torch.Tensor, scales: torch.Tensor | None, 
     n, h, two, bs, d = pages.shape
     if two != 2:
         raise ValueError(f"{who}: pages must be a contiguous [n_pages, h, 2, block_size, head_dim], got {tuple(pages.shape)}")
-    if pages.dtype is torch.int8:
-        if scales is None or scales.dtype is not torch.float32 or scales.shape != (n, h, 2, bs) or not scales.is_contiguous():
+    if pages.dtype is _I8:
+        if scales is None or scales.dtype is not _F32 or scales.shape != (n, h, 2, bs) or not scales.is_contiguous():
             raise ValueError(f"{who}: int8 pages need contiguous float32 scales [{n}, {h}, 2, {bs}]")
         kind, at = 1, scales.data_ptr()  # LKV_CACHE_INT8
     elif scales is not None:
         raise ValueError(f"{who}: scales belong to int8 pages, these are {pages.dtype}")
     else:
         kind, at = 0, 0  # LKV_CACHE_MODEL
-    if table.dtype is not torch.int32 or table.dim() != 2:
+    if table.dtype is not _I32 or table.dim() != 2:
         raise ValueError(f"{who}: the page table must be int32 [batch, columns] with unit column stride")
     (batch, cols), (ld, unit) = table.shape, table.stride()
     if unit != 1 and cols > 1:
@@ -496,7 +501,7 @@ def _cache_geometry(who: str, pages: torch.Tensor, scales: torch.Tensor | None, 
 
 
 def _per_sequence(who: str, name: str, t: torch.Tensor, batch: int) -> None:
-    if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != batch or not t.is_contiguous():
+    if t.dtype is not _I32 or t.dim() != 1 or t.numel() != batch or not t.is_contiguous():
         raise ValueError(f"{who}: {name} must be a contiguous int32 [{batch}]")
 
 
@@ -527,7 +532,7 @@ def paged_write(keys: torch.Tensor, values: torch.Tensor, pages: torch.Tensor, t
         raise ValueError("paged_write: one table row per sequence, and contiguous channels")
     _per_sequence(who, "starts", starts, batch)
     _run("lkv_paged_write", L.PAGED_ARGS.pack(
-        keys.data_ptr(), values.data_ptr(), kb, kt, kh, vb, vt, vh, dtype_code(dtype), batch, t, h, d, pages.data_ptr(), kind, at, n, bs,
+        keys.data_ptr(), values.data_ptr(), kb, kt, kh, vb, vt, vh, 1 if dtype is _BF16 else dtype_code(dtype), batch, t, h, d, pages.data_ptr(), kind, at, n, bs,
         table.data_ptr(), ld, cols, starts.data_ptr(), 0, 0, 0), index)
 
 
@@ -550,8 +555,8 @@ def paged_read(pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, n
             raise ValueError(f"paged_read: {pages.dtype} pages are read back as {pages.dtype}, not {dtype}")
         dtype = pages.dtype
     elif dtype is None:
-        dtype = torch.bfloat16
-    code = dtype_code(dtype)
+        dtype = _BF16
+    code = 1 if dtype is _BF16 else dtype_code(dtype)
     if n_tokens < 0:
         raise ValueError(f"paged_read: {n_tokens} tokens")
     _per_sequence(who, "starts", starts, batch)
@@ -598,15 +603,15 @@ def prefix_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tens
     if index < 0 or not (pages.get_device() == table.get_device() == lens.get_device() == prefix_table.get_device() == index) or (
             scales is not None and scales.get_device() != index):
         index = _one_device(who, query, pages, table, lens, prefix_table, scales)
-    if query.dim() != 4 or query.dtype is not torch.bfloat16:
+    if query.dim() != 4 or query.dtype is not _BF16:
         raise ValueError(f"prefix_attention: query must be bfloat16 [batch, T, hq, d], got {query.dtype} {tuple(query.shape)}")
     batch, t, hq, d = query.shape
     n, h, bs, pd, kind, at, rows, ld, cols = _cache_geometry(who, pages, scales, table)
-    if pd != d or h < 1 or hq % h or rows != batch or (kind == 0 and pages.dtype is not torch.bfloat16):
+    if pd != d or h < 1 or hq % h or rows != batch or (kind == 0 and pages.dtype is not _BF16):
         raise ValueError(f"prefix_attention: query {tuple(query.shape)} and table {tuple(table.shape)} do not fit {pages.dtype} pages {tuple(pages.shape)}")
     _per_sequence(who, "lens", lens, batch)
     pcols = prefix_table.numel()
-    if prefix_table.dtype is not torch.int32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous() or not 0 <= prefix_len <= pcols * bs:
+    if prefix_table.dtype is not _I32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous() or not 0 <= prefix_len <= pcols * bs:
         raise ValueError(f"prefix_attention: prefix_table must be a contiguous int32 [columns] holding the {prefix_len} tokens of the prefix")
     sb, st, sh, sc = query.stride()
     if sc != 1 or (sb | st | sh) & 7 or query.data_ptr() & 15:
@@ -620,10 +625,10 @@ def prefix_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tens
     elif out.shape != query.shape or not out.is_contiguous() or (out_dtype is not None and out.dtype is not out_dtype) or out.get_device() != index:
         raise ValueError(f"prefix_attention: out must be a contiguous {tuple(query.shape)} on cuda:{index}")
     if lse is None:
-        lse = query.new_empty((batch, t, hq), dtype=torch.float32)
-    elif lse.shape != (batch, t, hq) or lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.get_device() != index:
+        lse = query.new_empty((batch, t, hq), dtype=_F32)
+    elif lse.shape != (batch, t, hq) or lse.dtype is not _F32 or not lse.is_contiguous() or lse.get_device() != index:
         raise ValueError(f"prefix_attention: lse must be a contiguous float32 {(batch, t, hq)} on cuda:{index}")
-    code = dtype_code(out.dtype)
+    code = 1 if out.dtype is _BF16 else dtype_code(out.dtype)
     nbytes = _prefix_workspace(batch, t, hq, h, d, prefix_len, kind, cols * bs)
     ws = query.new_empty((nbytes + 1) // 2) if nbytes else None
     _run("lkv_prefix_attention", L.PREFIX_ARGS.pack(
@@ -655,15 +660,14 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     if target.shape != (batch, k + 1, vocab) or uniforms.shape != (batch, k + 1) or (draft is not None and draft.shape != (batch, k, vocab)):
         raise ValueError(f"verify_drafts: {k} tokens drafted for {batch} sequences do not fit target {tuple(target.shape)}, uniforms "
                          f"{tuple(uniforms.shape)}, draft {None if draft is None else tuple(draft.shape)}")
-    f32 = torch.float32
-    if target.dtype is not f32 or uniforms.dtype is not f32 or tokens.dtype is not torch.int64 or (draft is not None and draft.dtype is not f32):
+    if target.dtype is not _F32 or uniforms.dtype is not _F32 or tokens.dtype is not _I64 or (draft is not None and draft.dtype is not _F32):
         raise ValueError("verify_drafts: probabilities and uniforms are float32, tokens int64")
     (pb, pt, pv), (tb, tk), (ub, uk) = target.stride(), tokens.stride(), uniforms.stride()
     qb, qt, qv = (0, 0, 1) if draft is None else draft.stride()
     if (vocab > 1 and (pv != 1 or qv != 1)) or (k > 1 and tk != 1) or (k > 0 and uk != 1):
         raise ValueError("verify_drafts: rows must be contiguous")
     token = tokens.new_empty(batch)
-    kept = tokens.new_empty(batch, dtype=torch.int32)
+    kept = tokens.new_empty(batch, dtype=_I32)
     _run("lkv_verify_drafts", L.VERIFY_ARGS.pack(
         target.data_ptr(), pb, pt, 0 if draft is None else draft.data_ptr(), qb, qt, tokens.data_ptr(), tb, uniforms.data_ptr(), ub, batch, k, vocab,
         kept.data_ptr(), token.data_ptr()), index)
