@@ -272,22 +272,31 @@ __device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D 
   for (int n = 0; n < 2 * S::kGran; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
-  float above = 0.0f;  // int8: E - 7
+  float above[2] = {0.0f, 0.0f};  // int8: E - 7, of the tokens that each of the two rows sees
   if constexpr (INT8) {
     // Scales are below 2^E, E from the largest finite one's exponent; at least -64, so that the sums stay
-    // far from float32's end where the values are all but zero.
-    int bits = 62;  // E = -64
+    // far from float32's end where the values are all but zero. What a row does not see must not raise its
+    // reference: rows of a page behind a list's end hold any scale.
+    int bits[2] = {62, 62};  // E = -64
 #pragma unroll
-    for (int n = 0; n < 2 * S::kGran; ++n) {
-      const int x = (__float_as_int(vs[n].x) >> 23) & 0xff, y = (__float_as_int(vs[n].y) >> 23) & 0xff;
-      const bool on = !MASKED || ((have >> (n / 2)) & 1);
-      if (on && x != 0xff) bits = max(bits, x);
-      if (on && y != 0xff) bits = max(bits, y);
-    }
-    above = (float)(bits - 126 - 7);
+    for (int n = 0; n < 2 * S::kGran; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int x = (__float_as_int(e ? vs[n].y : vs[n].x) >> 23) & 0xff;
+        if constexpr (MASKED) {
+          const int tok = first + 8 * n + 2 * c + e;
+          const bool on = x != 0xff && ((have >> (n / 2)) & 1);
+          if (on && tok < limit[0]) bits[0] = max(bits[0], x);
+          if (on && tok < limit[1]) bits[1] = max(bits[1], x);
+        } else {
+          if (x != 0xff) bits[0] = max(bits[0], x);
+        }
+      }
+    if constexpr (!MASKED) bits[1] = bits[0];
+    above[0] = (float)(bits[0] - 126 - 7), above[1] = (float)(bits[1] - 126 - 7);
   }
   // A reference moves where a lane sees it outgrown (or has none yet), for the four lanes of the row alike.
-  const float grown[2] = {top[0] + above, top[1] + above};
+  const float grown[2] = {top[0] + above[0], top[1] + above[1]};
   if (__any_sync(0xffffffffu, grown[0] > st.m[0] + kLag || grown[1] > st.m[1] + kLag)) {
     float f[2];
 #pragma unroll

@@ -298,6 +298,48 @@ def test_int8_pages_of_any_magnitude(b: int, up: int) -> None:
     assert bool(((lse - base[1]).abs() <= 6 * 70 * 2.0**-24).all())
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,t", [(2, 1), (3, 4), (40, 1)])
+def test_scales_of_unseen_rows_do_not_count(b: int, t: int, d: int) -> None:
+    """int8 pages whose rows past the lists' ends hold scales that are numbers, huge ones: the same bits as with NaN."""
+    from lazykv_b200 import kernels as K
+
+    got = []
+    for fill in (math.nan, 1e30):
+        gen = torch.Generator().manual_seed(b)
+        lens = [5 + 7 * i for i in range(b)]
+        cache, prefix_table, tables = build(gen, 2, d, 16, True, 203, lens, fill=fill)
+        pages, scales, ptab, table, n = on_gpu(cache, prefix_table, tables, lens)
+        q = torch.randn((b, t, 2, d), generator=gen).bfloat16().cuda()
+        got.append(K.prefix_attention(q, pages, table, n, ptab, 203, d**-0.5, scales=scales, out_dtype=torch.float32))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b", [1, 40])
+def test_a_drafted_token_counts_for_no_row_before_it(b: int, d: int) -> None:
+    """int8: the step's last token has values 2^40 times the others'; the rows before it keep the others' bound."""
+    from lazykv_b200 import kernels as K
+
+    gen = torch.Generator().manual_seed(d)
+    t, lens = 3, [3 + i for i in range(b)]
+    cache, prefix_table, tables = build(gen, 2, d, 16, True, 90, lens)
+    pages, scales, ptab, table, n = on_gpu(cache, prefix_table, tables, lens)
+    ordinary = float((cache.scales[:, :, 1].nan_to_num(0.0) * 127).amax())
+    for i, m in enumerate(lens):
+        page = tables[i][(m - 1) // 16]
+        scales[page, :, 1, (m - 1) % 16] *= 2.0**40
+        cache.scales[page, :, 1, (m - 1) % 16] *= 2.0**40
+    query = torch.randn((b, t, 4, d), generator=gen).bfloat16()
+    out, _ = K.prefix_attention(query.cuda(), pages, table, n, ptab, 90, d**-0.5, scales=scales, out_dtype=torch.float32)
+    want, _, mass, reach = attend(cache, query, tables, lens, prefix_table, 90, d**-0.5)
+    keys = 90 + max(lens)
+    sums = (d + 4) * 2.0**-24 * reach + 2.0**-22 + keys * 2.0**-24
+    bound = (2.0**-8 + 2 * sums[..., None]) * mass + 2.0**-23 * want.abs() + (keys * 2.0**-31 + 2.0**-24) * ordinary
+    err = (out.double().cpu() - want).abs()[:, : t - 1]
+    assert bool((err <= bound[:, : t - 1]).all()), float((err / bound[:, : t - 1]).max())
+
+
 def test_one_result_for_one_input() -> None:
     """The same call gives the same bits every time (no atomics order its sums)."""
     from lazykv_b200 import kernels as K
