@@ -136,9 +136,10 @@ class PagedBatch:
         host = torch.tensor([seq_ids, [self.lengths[s] for s in seq_ids], [self.lengths[s] + t for s in seq_ids]], dtype=torch.int32).to(self.dev)
         table = self.table.index_select(0, host[0])
         K.paged_write(keys, values, self.pages, table, host[1], scales=self.scales)
-        for s in seq_ids:
+        done = K.prefix_attention(query, self.pages, table, host[2], self.prefix_table, self.prefix_len, scale, scales=self.scales, out_dtype=out_dtype)
+        for s in seq_ids:  # behind the calls: a refused step leaves the sequences as they were
             self.lengths[s] += t
-        return K.prefix_attention(query, self.pages, table, host[2], self.prefix_table, self.prefix_len, scale, scales=self.scales, out_dtype=out_dtype)
+        return done
 
     def take_back(self, s: int, tokens: int) -> None:
         """Forget the last `tokens` own tokens of sequence `s` (drafted ones that were rejected); their pages stay

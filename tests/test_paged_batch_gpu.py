@@ -124,6 +124,21 @@ def test_what_the_paged_batch_refuses() -> None:
         batch.step([a], q[:1].repeat(1, 2, 1, 1), kv[:1].repeat(1, 2, 1, 1), kv[:1].repeat(1, 2, 1, 1), 1.0)
 
 
+def test_a_refused_step_leaves_the_sequences_as_they_were() -> None:
+    from lazykv_b200.paged import PagedBatch
+
+    batch = PagedBatch(H, G, D, max_seqs=1, max_tokens=40, n_pages=4)
+    a = batch.fork()
+    q, kv = torch.zeros((1, 2, H * G, D), dtype=torch.bfloat16, device="cuda"), torch.zeros((1, 2, H, D), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="bfloat16"):
+        batch.step([a], q.float(), kv, kv, 1.0)
+    with pytest.raises((ValueError, TypeError)):
+        batch.step([a], q, kv, kv, 1.0, out_dtype=torch.int8)
+    assert batch.lengths == {a: 0}
+    batch.step([a], q, kv, kv, 1.0)
+    assert batch.lengths == {a: 2}
+
+
 def test_the_wrappers_refuse_what_does_not_fit() -> None:
     from lazykv_b200 import kernels as K
 
