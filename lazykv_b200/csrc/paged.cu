@@ -14,10 +14,15 @@
 // right. A row that holds an infinity or a NaN has no scale: it gets s = NaN and codes 0 and reads back as
 // NaN throughout.
 //
-// What bounds both kernels is memory: every byte moves once. A thread carries 16 bytes of the model's type
-// (8 channels of bf16, 4 of float32) of a token's key row and of its value row, so that a warp reads and
-// writes whole runs; with 32 bytes a thread, two stores a sector each, a read wrote 4.8 TB/s. Reading, a
-// thread carries several tokens, since its loads wait for the page's id and that for the table's row.
+// Every byte moves once. A thread carries 16 bytes of the model's type (8 channels of bf16, 4 of float32) of a
+// token's key row and of its value row, so that a warp reads and writes whole runs; with 32 bytes a thread, two
+// stores a sector each, a read wrote 4.8 TB/s. Reading, a thread carries several tokens, since its loads wait
+// for the page's id and that for the table's row.
+//
+// Measured (8 heads, d 128, bf16 tokens, int8 pages): 12 x up to 16,000 tokens read back at 6.0 TB/s, 0.94 of a
+// plain copy (989 MB, 163 us): memory bounds it. 65,536 tokens of a prompt written at 3.7 TB/s, 0.57 of a copy
+// (407 MB, 110 us): quantising bounds it, 74% of the issue slots. A token of each of 64 sequences written and
+// read back: 5.9 us, two launches of three dependent loads each.
 #include <float.h>
 
 #include "common.cuh"

@@ -11,7 +11,7 @@
 // Each launch starts under the one before it (programmatic dependent launch): the stream's CTAs take the
 // SMs that the tiles leave, or never had (32 rows on 32K int8 tokens: 38 us, the other way about 44).
 //
-// stream_kernel is bound by the pages' bytes. Its work is one line of stages (prefix.cuh) that all warps
+// stream_kernel's work is one line of stages (prefix.cuh) that all warps
 // of the grid share equally, whatever the sequences' lengths: only the device knows them, and with a CTA
 // or a cluster per (sequence, head) the longest sequence set the time. A warp takes a tile of 16 rows
 // through its stages with mma.sync.m16n8k16 (float32 accumulators). A lane copies by cp.async exactly the
@@ -23,8 +23,13 @@
 // bf16 pages: probabilities are rounded to bf16 for the second product (2^-8 relative at most, unbiased
 // over the keys). int8 pages: codes and queries are f16 (prefix_tile.cu tells how exactly), a key's scale
 // multiplies its column of scores in float32, and a value's scale its column of weights, before they are
-// rounded to f16: with 2^E above every value scale of the stage, references are at least the maximum + E -
-// 7, so weights x scales stay below 2^7 when a reference is set and below 2^15 until it is set again.
+// rounded to f16: with 2^E above every value scale that the row sees in the stage, references are at least the
+// maximum + E - 7, so weights x scales stay below 2^7 when a reference is set and below 2^15 until it is set again.
+//
+// Measured: 6 sequences on 32,768 bf16 tokens, 16 KV heads, d 128: 276 MB in 63 us, 4.4 TB/s; each further
+// token moves at 5.8 TB/s, the rest is the start, the last stages and the merge (13 us). int8 pages are bound by
+// issue slots instead, some 600 instructions of a warp per 16 tokens and head (codes to f16, products, softmax):
+// 64 sequences' own 0 .. 2,000 tokens take 48 us at 36% of the memory's cycles.
 #include "prefix.cuh"
 
 namespace lkv {

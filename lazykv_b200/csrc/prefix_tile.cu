@@ -3,7 +3,7 @@
 //
 // A CTA holds up to 256 query rows of one KV head as two tiles of 128 and takes a chunk of the prefix
 // through them, 128 tokens at a time. Per tile of rows: S = Q K^T (tcgen05.mma, both operands in shared
-// memory, S in tensor memory), one thread per row turns its 128 scores into weights (running maximum and
+// memory, S in tensor memory), each warp turns its 32 rows' 128 scores into weights (running maximum and
 // sum in registers, float32), writes them back as 16-bit P over S, and O += P V (P read from tensor
 // memory, V from shared memory) accumulates in tensor memory. The two tiles alternate, so that one
 // computes weights while the tensor core works for the other. With 128 rows or fewer both tiles are the
@@ -11,8 +11,15 @@
 // one partial (m, l, o) per row, which combine_kernel (prefix.cu) folds into the output.
 //
 // Warps 0-3 and 4-7 are the two tiles' rows, warp 8 issues the matrix products, warp 9 the copies; with
-// int8 pages warps 12-15 turn codes of keys into f16 operands and warps 16-19 those of values. All of it is joined by mbarriers, every wait
-// bounded (tma.cuh).
+// int8 pages warps 12-15 turn codes of keys into f16 operands and warps 16-19 those of values. All of it is
+// joined by mbarriers, every wait bounded.
+//
+// Measured at 512 rows of a KV head on 32,768 tokens, d 128: int8 100 us, the tensor cores busy 33% of the time
+// and the exponentials' unit 40%; bf16 78 us, 43% and 50%. 128 sequences of 8 KV heads with 4 query heads each
+// on 131,072 int8 tokens, with their own tokens: 391 us, 0.71 PFLOP/s. What bounds it is the chain of one tile
+// of rows, scores -> weights -> products -> next scores: S and P share 128 columns of tensor memory (two tiles
+// of S and O of d 128 fill it), so a tile's next scores wait for its present product, and two tiles do not
+// fill each other's gaps. Short prefixes add a start of 5 to 8 us (tensor memory, queries, the first pages).
 //
 // bf16 pages: P and V are bf16; the pages come by tensor-map TMA straight into the swizzled operand
 // layout (a page that is missing as a row past the tensor's end, that is as zeros).
@@ -28,7 +35,6 @@
 
 #include <cuda_fp16.h>
 #include <float.h>
-
 
 #include "prefix.cuh"
 #include "tma.cuh"

@@ -8,10 +8,14 @@
 // one are distributed as samples of the target. Differences and sums are float64: a vocabulary's
 // float32 sum would move the border between neighbouring tokens by more than a token's own weight.
 //
-// Only one row (or pair of rows) of the vocabulary is read per sequence, which is what bounds it: one
-// cluster of CTAs per sequence, a slice of the row each. A slice's sums per tile of 512 stay in shared
+// Only one row (or pair of rows) of the vocabulary is read per sequence: one cluster of CTAs per
+// sequence, a slice of the row each. A slice's sums per tile of 512 stay in shared
 // memory, the cluster exchanges the slices' totals, and the CTA whose slice holds the border finds the
 // tile, then reads that tile once more and finds the element.
+//
+// Measured: 64 sequences, 7 drafted, a vocabulary of 128,256: 20 us, 3.3 TB/s (the floor at a copy's rate is
+// 10 us): one wave of reads stands between the chain that decides n (three loads in turn) and two cluster
+// barriers, and is not overlapped with either. One sequence, 4 drafted, 32,000: 7.5 us, those chains alone.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
