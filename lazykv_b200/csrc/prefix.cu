@@ -531,14 +531,16 @@ __device__ __forceinline__ void stream(const Params& p, char* ring) {
       const int rows = pre ? p.rows : p.tokens * p.group;
       n_rows = min(kRows, rows - row0);
       unit = pre ? at.unit : p.h * p.prefix_row_tiles + at.b * p.h * p.own_row_tiles + at.unit;
+      // Rows count their sight from the length as given, which may lie past the list's end.
+      const int given = pre ? 0 : max(p.lens[at.b], 0);
       const __nv_bfloat16* src[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int x = min(row0 + r + 8 * k, rows - 1), g = x % p.group, bt = x / p.group, t = bt % p.tokens, b = pre ? bt / p.tokens : at.b;
         src[k] = r + 8 * k < n_rows ? p.q + b * p.q_sb + t * p.q_st + (int64_t)(j * p.group + g) * p.q_sh : nullptr;
-        limit[k] = pre ? at.len : max(0, at.len - p.tokens + t + 1);
+        limit[k] = pre ? at.len : min(at.len, max(0, given - p.tokens + t + 1));
       }
-      low = pre ? at.len : max(0, at.len - p.tokens + row0 / p.group + 1);
+      low = pre ? at.len : min(at.len, max(0, given - p.tokens + row0 / p.group + 1));
       load_queries<D, INT8>(qf, scale, src[0], src[1], c, p.scale_log2);
       st.clear();
       fresh = false;
