@@ -23,8 +23,8 @@
 // bf16 pages: probabilities are rounded to bf16 for the second product (2^-8 relative at most, unbiased
 // over the keys). int8 pages: codes and queries are f16 (prefix_tile.cu tells how exactly), a key's scale
 // multiplies its column of scores in float32, and a value's scale its column of weights, before they are
-// rounded to f16: with 2^E above every value scale that the row sees in the stage, references are at least the
-// maximum + E - 7, so weights x scales stay below 2^7 when a reference is set and below 2^15 until it is set again.
+// rounded to f16, the only rounding of the second product's operands (prefix.cuh, weight_room: 2^-11 relative,
+// and an absolute 2^-31 of the largest weight times scale).
 //
 // Measured: 6 sequences on 32,768 bf16 tokens, 16 KV heads, d 128: 276 MB in 63 us, 4.4 TB/s; each further
 // token moves at 5.8 TB/s, the rest is the start, the last stages and the merge (13 us). int8 pages are bound by
@@ -274,44 +274,24 @@ __device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D 
   }
   float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-  for (int n = 0; n < 2 * S::kGran; ++n)
+  for (int n = 0; n < 2 * S::kGran; ++n) {
+    // int8: a weight is rounded together with its token's value scale, so the largest product sets the reference,
+    // not the largest weight, and what a row does not see (a score of -infinity) has no part in it.
+    const float up[2] = {INT8 ? weight_room(vs[n].x) : 0.0f, INT8 ? weight_room(vs[n].y) : 0.0f};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
-  float above[2] = {0.0f, 0.0f};  // int8: E - 7, of the tokens that each of the two rows sees
-  if constexpr (INT8) {
-    // Scales are below 2^E, E from the largest finite one's exponent; at least -64, so that the sums stay
-    // far from float32's end where the values are all but zero. What a row does not see must not raise its
-    // reference: rows of a page behind a list's end hold any scale.
-    int bits[2] = {62, 62};  // E = -64
-#pragma unroll
-    for (int n = 0; n < 2 * S::kGran; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int x = (__float_as_int(e ? vs[n].y : vs[n].x) >> 23) & 0xff;
-        if constexpr (MASKED) {
-          const int tok = first + 8 * n + 2 * c + e;
-          const bool on = x != 0xff && ((have >> (n / 2)) & 1);
-          if (on && tok < limit[0]) bits[0] = max(bits[0], x);
-          if (on && tok < limit[1]) bits[1] = max(bits[1], x);
-        } else {
-          if (x != 0xff) bits[0] = max(bits[0], x);
-        }
-      }
-    if constexpr (!MASKED) bits[1] = bits[0];
-    above[0] = (float)(bits[0] - 126 - 7), above[1] = (float)(bits[1] - 126 - 7);
+    for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], INT8 ? s[n][e] + up[e & 1] : s[n][e]);
   }
   // A reference moves where a lane sees it outgrown (or has none yet), for the four lanes of the row alike.
-  const float grown[2] = {top[0] + above[0], top[1] + above[1]};
-  if (__any_sync(0xffffffffu, grown[0] > st.m[0] + kLag || grown[1] > st.m[1] + kLag)) {
+  if (__any_sync(0xffffffffu, top[0] > st.m[0] + kLag || top[1] > st.m[1] + kLag)) {
     float f[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      float want = grown[i];
+      float want = top[i];
       want = fmaxf(want, __shfl_xor_sync(0xffffffffu, want, 1));
       want = fmaxf(want, __shfl_xor_sync(0xffffffffu, want, 2));
       f[i] = want > st.m[i] ? ex2(st.m[i] - want) : 1.0f;  // 0 where nothing was seen before
+      st.l[i] = INT8 && want > st.m[i] ? times_ex2(st.l[i], st.m[i] - want) : st.l[i] * f[i];
       st.m[i] = fmaxf(st.m[i], want);
-      st.l[i] *= f[i];
     }
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) st.o[i][0] *= f[0], st.o[i][1] *= f[0], st.o[i][2] *= f[1], st.o[i][3] *= f[1];
@@ -325,9 +305,10 @@ __device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D 
     st.l[0] += s[n][0] + s[n][1];
     st.l[1] += s[n][2] + s[n][3];
     if constexpr (INT8) {
+      const float by2[2] = {vs[n].x * kScaleDown, vs[n].y * kScaleDown};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float by = (e & 1) ? vs[n].y : vs[n].x;
+        const float by = by2[e & 1];
         s[n][e] = MASKED && s[n][e] == 0.0f ? 0.0f : s[n][e] * by;  // a masked token's scale may be a NaN
       }
     }
@@ -561,6 +542,7 @@ __device__ __forceinline__ void stream(const Params& p, char* ring) {
       for (int k = 0; k < 2; ++k) {
         st.l[k] += __shfl_xor_sync(0xffffffffu, st.l[k], 1);
         st.l[k] += __shfl_xor_sync(0xffffffffu, st.l[k], 2);
+        if (INT8) st.m[k] += kScaleShift, st.l[k] *= kScaleDown;  // o is in units of 2^(m + kScaleShift)
       }
       if (whole) break;
 #pragma unroll
@@ -613,7 +595,7 @@ __device__ __forceinline__ void stream(const Params& p, char* ring) {
       const float2 ml = pml[i * kRows + row];
       const float f = ex2(ml.x - from);
       const float4 v = *reinterpret_cast<const float4*>(po + (i * kRows + row) * kLd + ch);
-      l += ml.y * f;
+      l += times_ex2(ml.y, ml.x - from);
       o.x += v.x * f, o.y += v.y * f, o.z += v.z * f, o.w += v.w * f;
     }
     const int64_t to = (int64_t)(w - warp + unit) * p.slot_rows + row;
@@ -641,8 +623,8 @@ struct Sum {
 };
 __device__ __forceinline__ void fold(Sum& a, float m, float l, float4 o) {
   const float top = fmaxf(a.m, m), from = top == -INFINITY ? 0.0f : top, f = ex2(a.m - from), e = ex2(m - from);
+  a.l = times_ex2(a.l, a.m - from) + times_ex2(l, m - from);
   a.m = top;
-  a.l = a.l * f + l * e;
   a.o.x = a.o.x * f + o.x * e, a.o.y = a.o.y * f + o.y * e, a.o.z = a.o.z * f + o.z * e, a.o.w = a.o.w * f + o.w * e;
 }
 
@@ -716,11 +698,11 @@ __global__ void __launch_bounds__(kThreads, 4) combine_kernel(const Params p, in
     for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
     top = fmaxf(top, a.m);
     const float from = top == -INFINITY ? 0.0f : top, f = ex2(a.m - from), by = ex2(x.x - from);
-    float l = x.y * by;
+    float l = times_ex2(x.y, x.x - from);
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+    a.l = times_ex2(a.l, a.m - from) + l;
     a.m = top;
-    a.l = a.l * f + l;
     a.o.x *= f, a.o.y *= f, a.o.z *= f, a.o.w *= f;
 #pragma unroll 1
     for (int i = 0; i < count; i += 8 * kTogether) {

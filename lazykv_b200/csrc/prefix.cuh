@@ -66,6 +66,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// x 2^e, e <= 0, also where 2^e alone is too small for a float32 (two references as far apart as value scales may be).
+__device__ __forceinline__ float times_ex2(float x, float e) {
+  if (e >= -120.0f || e == -INFINITY) return x * ex2(e);
+  const float half = ex2(0.5f * e);
+  return x * half * half;
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&b);
@@ -92,6 +99,20 @@ __device__ __forceinline__ float2 row_scales(uint32_t top_bits) {
   int e = (int)(top_bits >> 7) - 127;
   e = e > 126 ? 126 : e < -126 ? -126 : e;
   return make_float2(__int_as_float((127 - e) << 23), __int_as_float((127 + e) << 23));
+}
+
+// int8 pages: codes of values are exact in f16, and a weight is rounded to f16 once, as the product with its
+// token's value scale: w = 2^(s - m) x scale x 2^-kScaleShift, s the score and m the row's reference. With
+// scale < 2^E, m >= max(s + E) - kScaleShift - 7 over the tokens that the row sees makes w < 2^7 when m is set
+// (half that for the token that set it, at least) and w < 2^15 until m is set again, and f16's last bit, 2^-24,
+// is 2^-30 of the largest w: a token keeps 11 bits however its scale and weight make the product up, and none
+// counts by a scale without its weight. The sum of the weights is float32, of 2^(s - m), whose range the shift
+// lets scales from 2^-64 (smaller ones count as that, and lose bits below 2^-90) to float32's end share. o and
+// the weights' sum l are an ordinary partial as (m + kScaleShift, l x 2^-kScaleShift, o).
+constexpr float kScaleShift = 16.0f, kScaleDown = 1.0f / 65536.0f;
+__device__ __forceinline__ float weight_room(float scale) {  // E - kScaleShift - 7; a scale that is not finite claims nothing
+  const int bits = (__float_as_int(scale) >> 23) & 0xff;
+  return (float)(bits == 0xff ? -64 : max(bits - 126, -64)) - (kScaleShift + 7.0f);
 }
 
 // Stages of sequence b's own tokens (lens may lie outside [0, the table's reach]).

@@ -71,3 +71,72 @@ def test_several_queries_of_a_length_past_the_table(b: int, t: int, g: int, int8
     query = torch.randn((b, t, h * g, d), generator=gen).bfloat16()
     out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, prefix, d**-0.5, scales=scales, out_dtype=torch.float32)
     near(cache, query, tables, lens, prefix_table, prefix, d**-0.5, out, lse)
+
+
+def near_int8(cache: Cache, query: torch.Tensor, tables, lens, prefix_table, prefix: int, scale: float, out: torch.Tensor, lse: torch.Tensor) -> None:
+    """int8 pages, each row on its own: a weight times its value's scale is rounded to f16 once, 2^-11 of it or 2^-25
+    of a unit of which the row's largest such product has 2^6 at least: n keys, codes up to 127, make that at most
+    n 2^-31 top, top = max p max |v| / sum p over the row's keys. The rest as in `near`, with four more float32 roundings."""
+    want, wlse, mass, reach = attend(cache, query, tables, lens, prefix_table, prefix, scale)
+    b, t, hq, d = query.shape
+    h = cache.pages.shape[1]
+    n = prefix + max(len(x) for x in tables) * cache.bs
+    kp, vp, okp = cache.read(prefix_table, list(range(prefix)))
+    top = torch.zeros((b, t, hq), dtype=torch.float64)
+    for i in range(b):
+        ko, vo, oko = cache.read(tables[i], list(range(len(tables[i]) * cache.bs)))
+        for step in range(t):
+            m = min(ko.shape[0], max(0, lens[i] - t + step + 1))
+            k, v = torch.cat([kp[okp], ko[:m][oko[:m]]]), torch.cat([vp[okp], vo[:m][oko[:m]]])
+            if k.shape[0] > 0:
+                p = torch.softmax(torch.einsum("hgd,nhd->hgn", query[i, step].double().cpu().view(h, hq // h, d), k) * scale, -1)
+                top[i, step] = (p * v.abs().amax(-1).T[:, None]).amax(-1).reshape(hq)
+    sums = (d + 4) * 2.0**-24 * reach + 2.0**-22 + n * 2.0**-24
+    bound = (2.0**-11 + 2 * sums[..., None] + 4 * 2.0**-24) * mass + n * 2.0**-31 * top[..., None] + 2.0**-23 * want.abs()
+    err, lerr = (out.double().cpu() - want).abs(), (lse.double().cpu() - wlse).abs()
+    empty = wlse == -math.inf
+    assert bool((err <= bound).all()), float((err / bound.clamp_min(1e-300)).max())
+    assert bool((lerr <= sums + 4 * 2.0**-24 * (wlse.abs() + 1))[~empty].all()), float(lerr[~empty].max())
+
+
+def rescale(cache: Cache, prefix_table: list[int], prefix: int, every: int, first: int, values: float, keys: float) -> None:
+    """Every `every`-th token of the prefix from `first` on: values times `values`, keys times `keys` (powers of two, or 0)."""
+    for pos in range(first, prefix, every):
+        page, at = prefix_table[pos // cache.bs], pos % cache.bs
+        cache.scales[page, :, 1, at] = (cache.scales[page, :, 1, at].double() * values).float()  # (2^170 is no float32)
+        cache.scales[page, :, 0, at] *= keys
+
+
+# Some tokens' values are many powers of two times the others', (every, first, power, what their keys are multiplied
+# with, power of all values): with the others' weights (keys as they are, or all zero: one score for all), far less (a
+# score some tens lower: negated keys of a query that points along them), from the first token on or late in the list.
+SPREADS = [(50, 0, 20, 1.0, 0), (50, 49, 40, 1.0, 0), (13, 5, -20, 1.0, 0), (200, 7, 27, -1.0, 0), (200, 150, 27, -1.0, 0), (64, 63, 60, -1.0, 0),
+           (5, 3, 100, 0.0, 0), (7, 2, -60, 0.0, 0), (90, 80, 170, 0.0, -60), (90, 0, 170, 0.0, -60)]
+
+
+def spread_case(b: int, d: int, spread, bs: int, prefix: int, h: int = 2):  # noqa: ANN001, ANN201
+    every, first, power, keys, all_of_them = spread
+    gen = torch.Generator().manual_seed(b + power + d)
+    lens = [3 + i % 9 for i in range(b)]
+    cache, prefix_table, tables = build(gen, h, d, bs, True, prefix, lens, fill=0.0)
+    # All keys point along one direction per head and queries too: scores around 25 with the keys as they are.
+    along = torch.randn((1, h, d), generator=gen)
+    k = (along + 0.1 * torch.randn((prefix, h, d), generator=gen)).bfloat16()
+    cache.write(prefix_table, 0, k, torch.randn((prefix, h, d), generator=gen).bfloat16())
+    cache.scales[:, :, 1] *= 2.0**all_of_them
+    rescale(cache, prefix_table, prefix, every, first, 2.0**power, keys)
+    if keys == 0.0:
+        cache.scales[:, :, 0] = 0.0
+    query = (along.transpose(0, 1).expand(h, 2, d).reshape(1, 1, 2 * h, d) * 3 * 64**0.5 / d**0.5 + 0.1 * torch.randn((b, 1, 2 * h, d), generator=gen)).bfloat16()
+    return cache, prefix_table, tables, lens, query
+
+
+@pytest.mark.parametrize("spread", SPREADS, ids=str)
+@pytest.mark.parametrize("d", [64, 128])
+def test_int8_values_beside_far_larger_ones_in_the_stream(d: int, spread) -> None:  # noqa: ANN001
+    from lazykv_b200 import kernels as K
+
+    cache, prefix_table, tables, lens, query = spread_case(3, d, spread, 16, 400)
+    pages, scales, ptab, table, n = on_gpu(cache, prefix_table, tables, lens)
+    out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, 400, d**-0.5, scales=scales, out_dtype=torch.float32)
+    near_int8(cache, query, tables, lens, prefix_table, 400, d**-0.5, out, lse)
