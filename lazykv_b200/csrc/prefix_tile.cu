@@ -25,11 +25,8 @@
 // layout (a page that is missing as a row past the tensor's end, that is as zeros).
 // int8 pages: codes are exact in f16, and so is a query row after a power of two that brings its largest
 // element to [1, 2) (smaller ones lose bits below 2^-25 of it). A key's scale multiplies its column of
-// scores in float32. A value's scale goes into V: code x (scale / 2^E), rounded to f16 (2^-11 relative,
-// the scale too), with 2^E the least power of two not below any scale of the tile. A weight is then
-// 2^(score - reference + E) and the reference at least the row's maximum + E - 7: weights stay below
-// 2^7 when it is set and may grow to 2^15 before it is set again, and their last bit is 2^-24: 11 bits for
-// every weight that counts, against the 8 of bf16.
+// scores in float32 and a value's scale its column of weights, which are then rounded to f16: the one rounding
+// of the second product's operands (prefix.cuh, weight_room, says what is left of it).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -45,9 +42,12 @@ namespace {
 
 constexpr int kTile = 128;       // rows of a tile of queries, tokens of a tile of the prefix
 constexpr int kInfo = 8;         // tiles whose scales and page bits are kept (see the producer)
-// What the sum of a thread's weights may grow to before its references are set again: every weight has to
-// be an f16; a bf16 one has float32's range, of which the accumulated values need the rest.
-constexpr float kMostF16 = 32768.0f, kMostBf16 = 1048576.0f;  // 2^15, 2^20
+// What the sum of a thread's weights may grow to before its references are set again: a bf16 weight has
+// float32's range, of which the accumulated values need the rest.
+constexpr float kMostBf16 = 1048576.0f;  // 2^20
+// int8: a weight times its value's scale has to stay below 2^kMostF16. That is asked of the sum and the tile's
+// largest scale: where a token of little weight has that scale, references are looked up for nothing.
+constexpr int kMostF16 = 15;
 
 template <int D, bool INT8>
 struct Tiles {
@@ -70,7 +70,7 @@ struct Barriers {
   uint64_t q_full, o_full[2], s_full[2], p_full[2], tail, drain;
   uint64_t full[9], empty[9], raw_full[3], raw_empty[3], info[kInfo];
   uint32_t have[kInfo][4];   // together, bit g: tokens 16 g .. 16 g + 15 of the tile have a page
-  int32_t top[kInfo][4];     // largest exponent of a finite value scale, per warp of converters
+  int32_t top[kInfo][4];     // int8: 2^top is above every finite value scale x kScaleDown, per warp of converters
   float back[2][kTile];      // int8: what a row's scores are multiplied with (stage_query)
   uint32_t tmem;
   int quit;
@@ -112,13 +112,19 @@ __device__ __forceinline__ bool wait_for(Barriers& s, uint64_t* bar, uint32_t pa
   return ok;
 }
 
-__device__ __forceinline__ int largest(const int32_t (&x)[4]) { return max(max(x[0], x[1]), max(x[2], x[3])); }
-
 // One arrival for the warp, after what all of its lanes did before.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   __syncwarp();
   if (lane == 0) mbar_arrive(bar);
 }
+
+// A value scale that kScaleDown has multiplied is below 2^scaled_top, one that is not finite claims nothing;
+// weight_room is 7 less.
+__device__ __forceinline__ int scaled_top(float scaled) {
+  const int bits = (__float_as_int(scaled) >> 23) & 0xff;
+  return bits == 0xff ? -80 : max(bits - 126, -80);
+}
+__device__ __forceinline__ float scaled_room(float scaled) { return (float)scaled_top(scaled) - 7.0f; }
 
 // Packed float32 pairs.
 __device__ __forceinline__ uint64_t pair(float a, float b) { return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32); }
@@ -229,11 +235,6 @@ __device__ __forceinline__ void st_packed(uint32_t addr, const uint32_t (&w)[2][
 }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ uint2 times(uint2 x, __half2 by) {
-  const __half2 a = __hmul2(*reinterpret_cast<const __half2*>(&x.x), by), b = __hmul2(*reinterpret_cast<const __half2*>(&x.y), by);
-  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-}
-
 // This thread's query row into its place of the operand tile; returns what its scores have to be
 // multiplied with for int8 pages (a power of two). `flip`: negated (a negative softmax scale).
 template <int D, bool INT8>
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   char* q_tiles = smem;
   char* raws = q_tiles + (2 + T::kStages) * T::kBytes;
-  float* scale_ring = reinterpret_cast<float*>(raws + T::kRaw * T::kRawBytes);  // [kInfo][2][kTile]: keys', values'
+  float* scale_ring = reinterpret_cast<float*>(raws + T::kRaw * T::kRawBytes);  // [kInfo][2][kTile]: keys', values' x kScaleDown
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int split = blockIdx.x, j = blockIdx.y, row0 = blockIdx.z * 2 * kTile;
   const int n_rows = min(2 * kTile, p.rows - row0);
@@ -359,9 +360,10 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       ok = wait_for(s, &s.info[slot], (t / kInfo) & 1);
       const uint32_t have = (s.have[slot][0] | s.have[slot][1]) | (s.have[slot][2] | s.have[slot][3]);
       const int seen = end - t * kTile;  // tokens of this tile inside the prefix
-      [[maybe_unused]] const uint64_t* ks = reinterpret_cast<const uint64_t*>(scale_ring + slot * 2 * kTile + c2);  // pair 4 k: columns 8 k + c2, + 1
-      float e = 0.0f;  // int8: the exponent of the tile's largest value scale
-      if constexpr (INT8) e = (float)largest(s.top[slot]);
+      // Pair 4 k: columns 8 k + c2, + 1.
+      [[maybe_unused]] const uint64_t* ks = reinterpret_cast<const uint64_t*>(scale_ring + slot * 2 * kTile + c2);
+      [[maybe_unused]] const uint64_t* vs = ks + kTile / 2;
+      const float most = INT8 ? __int_as_float((127 + kMostF16 - max(max(s.top[slot][0], s.top[slot][1]), max(s.top[slot][2], s.top[slot][3]))) << 23) : kMostBf16;
       ok = ok && wait_for(s, &s.s_full[u], n_done & 1);
       if (!ok) break;
       tc_after();
@@ -398,12 +400,16 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
               ld_wait(f[0]);
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                [[maybe_unused]] uint64_t kk = 0;
-                if constexpr (INT8) kk = ks[4 * (2 * n + k)];
+                [[maybe_unused]] uint64_t kk = 0, up = 0;
+                if constexpr (INT8) {
+                  kk = ks[4 * (2 * n + k)];
+                  const uint64_t v = vs[4 * (2 * n + k)];
+                  up = pair(scaled_room(first_of(v)), scaled_room(second_of(v)));
+                }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                   uint64_t z = score(f[0], k, r);
-                  if constexpr (INT8) z = mul2(z, kk);
+                  if constexpr (INT8) z = fma2(mul2(z, kk), pair(scale[r], scale[r]), up);
                   top[r] = fmaxf(fmaxf(top[r], first_of(z)), second_of(z));
                 }
               }
@@ -415,10 +421,10 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
               top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
               top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
               // Rounded up, a reference leaves no score above it.
-              const float want = top[r] == -INFINITY ? -INFINITY : __fmaf_ru(top[r], scale[r], INT8 ? e - 7.0f : 0.0f), to_ref = fmaxf(from[r], want);
+              const float want = INT8 || top[r] == -INFINITY ? top[r] : __fmul_ru(top[r], scale[r]), to_ref = fmaxf(from[r], want);
               by[r] = to_ref == -INFINITY ? 1.0f : ex2(from[r] - to_ref);
+              l[r] = INT8 && to_ref > from[r] ? times_ex2(l[r], from[r] - to_ref) : l[r] * by[r];
               from[r] = to_ref;
-              l[r] *= by[r];
               none = none || to_ref == -INFINITY;
             }
             unset = __any_sync(0xffffffffu, none);
@@ -439,7 +445,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
           uint64_t ref[4], scale2[4], sum[4] = {0, 0, 0, 0};
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float x = e - (from[r] == -INFINITY ? 0.0f : from[r]);
+            const float x = from[r] == -INFINITY ? 0.0f : -from[r];
             ref[r] = pair(x, x), scale2[r] = pair(scale[r], scale[r]);
           }
           uint32_t w[N][2][4];
@@ -450,8 +456,8 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
             if (n + 1 < N) ld(f[(n + 1) & 1], ts + 16 * (n + 1));
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              [[maybe_unused]] uint64_t kk = 0;
-              if constexpr (INT8) kk = ks[4 * (2 * n + k)];
+              [[maybe_unused]] uint64_t kk = 0, vv = 0;
+              if constexpr (INT8) kk = ks[4 * (2 * n + k)], vv = vs[4 * (2 * n + k)];
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 uint64_t z = score(f[n & 1], k, r);
@@ -459,6 +465,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
                 z = fma2(z, scale2[r], ref[r]);
                 z = pair(ex2(first_of(z)), ex2(second_of(z)));
                 sum[r] = add2(sum[r], z);
+                if constexpr (INT8) z = mul2(z, vv);
                 w[n][r / 2][2 * k + (r & 1)] = INT8 ? pack_f16(first_of(z), second_of(z)) : pack_bf16(first_of(z), second_of(z));
               }
             }
@@ -467,14 +474,13 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
           // No weight is above the sum that it is part of.
           bool over = false;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) over = over || fmaxf(first_of(sum[r]), second_of(sum[r])) > (INT8 ? kMostF16 : kMostBf16);
+          for (int r = 0; r < 4; ++r) over = over || fmaxf(first_of(sum[r]), second_of(sum[r])) > most;
           set = !again && __any_sync(0xffffffffu, over);
           if (set) continue;
-          const float unit = INT8 ? ex2(-e) : 1.0f;
 #pragma unroll
           for (int n = 0; n < N; ++n) st_packed(ts + 8 * n, w[n]);  // over the scores
 #pragma unroll
-          for (int r = 0; r < 4; ++r) l[r] = fmaf(first_of(sum[r]) + second_of(sum[r]), unit, l[r]);
+          for (int r = 0; r < 4; ++r) l[r] += first_of(sum[r]) + second_of(sum[r]);
           break;
         }
         st_wait();
@@ -528,8 +534,8 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
           const float2 other = swap_ml[base + 8 * i];
           const float both = fmaxf(from[i], other.x), ref = both == -INFINITY ? 0.0f : both;
           f0[i] = ex2(from[i] - ref), f1[i] = ex2(other.x - ref);
+          l[i] = INT8 ? times_ex2(l[i], from[i] - ref) + times_ex2(other.y, other.x - ref) : l[i] * f0[i] + other.y * f1[i];
           from[i] = both;
-          l[i] = l[i] * f0[i] + other.y * f1[i];
         }
       }
     }
@@ -555,7 +561,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       if (c2 == 0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (base + 8 * i < n_rows) p.tile_ml[at + 8 * i] = ok ? make_float2(from[i], l[i]) : make_float2(0.0f, __uint_as_float(0x7fc00000u));
+          if (base + 8 * i < n_rows) p.tile_ml[at + 8 * i] = ok ? (INT8 ? make_float2(from[i] + kScaleShift, l[i] * kScaleDown) : make_float2(from[i], l[i])) : make_float2(0.0f, __uint_as_float(0x7fc00000u));
       }
     }
     tc_before();
@@ -720,27 +726,19 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
         const int n = 2 * t + kv, raw = n % T::kRaw, slot = n % n_stages, info = t % kInfo;
         // The ring entry's last reader is more than two tiles behind (see the copies): it is free.
         float* ring = scale_ring + (info * 2 + kv) * kTile;
-        ring[i] = scale;
+        ring[i] = kv == 1 ? scale * kScaleDown : scale;
         if (kv == 1) {
-          // scale < 2^e, e from its exponent; what is not finite stays what it is. At least -64, so that the
-          // sum of the weights stays far from float32's end where the values are all but zero.
-          const int bits = (int)((__float_as_uint(scale) >> 23) & 0xffu);
-          const int top = __reduce_max_sync(0xffffffffu, bits == 0xff ? -64 : max(bits - 126, -64));
+          const int top = __reduce_max_sync(0xffffffffu, scaled_top(scale * kScaleDown));
           if (lane == 0) s.top[info][warp - 16] = top;
         } else {
           const uint32_t mask = __ballot_sync(0xffffffffu, there);
           if (lane == 0) s.have[info][warp - 12] = ((mask & 0xffffu) != 0 ? 1u : 0u) << (2 * (warp - 12)) | (mask >> 16 != 0 ? 2u : 0u) << (2 * (warp - 12));
         }
         warp_arrive(&s.info[info], lane);
-        float down = 1.0f;  // 2^-E
-        if (kv == 1) {
-          asm volatile("bar.sync 2, 128;" ::: "memory");  // the tile's scales and exponents, of all four warps
-          down = __int_as_float((127 - largest(s.top[info])) << 23);
-        }
         scales_of(t + 1);
         ok = ok && wait_for(s, &s.raw_full[raw], (n / T::kRaw) & 1);
         if (ok && n >= n_stages) ok = wait_for(s, &s.empty[slot], (n / n_stages - 1) & 1);
-        if (!ok) continue;  // given up; no warp is left at the barrier above
+        if (!ok) break;
         const char* src = raws + raw * T::kRawBytes + from;
         char* dst = stages + slot * T::kBytes;
 #pragma unroll
@@ -754,11 +752,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
           }
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            uint2 a = codes_to_f16(w[x].x), b = codes_to_f16(w[x].y), d = codes_to_f16(w[x].z), e = codes_to_f16(w[x].w);
-            if (kv == 1) {
-              const __half2 by = __float2half2_rn(ring[tok0 + kStep * (x0 + x)] * down);
-              a = times(a, by), b = times(b, by), d = times(d, by), e = times(e, by);
-            }
+            const uint2 a = codes_to_f16(w[x].x), b = codes_to_f16(w[x].y), d = codes_to_f16(w[x].z), e = codes_to_f16(w[x].w);
             *reinterpret_cast<uint4*>(dst + to0 + kStep * (x0 + x) * 128) = make_uint4(a.x, a.y, b.x, b.y);
             *reinterpret_cast<uint4*>(dst + to1 + kStep * (x0 + x) * 128) = make_uint4(d.x, d.y, e.x, e.y);
           }

@@ -14,45 +14,73 @@ from tests.test_prefix_attention_gpu import build, on_gpu
 pytestmark = pytest.mark.gpu
 
 
-def attend(cache: Cache, query: torch.Tensor, tables: list[list[int]], lens: list[int], prefix_table: list[int], prefix_len: int,
-           scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(out, lse, mass, reach) in float64: query t of sequence b sees the prefix and own tokens 0 .. lens[b] - T + t, those
-    of them that have a page; mass = sum p |v| / sum p, reach = the largest sum |q k| scale of a row."""
+def tokens(pages: torch.Tensor, scales: torch.Tensor | None, j: int, table: torch.Tensor, n: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Head j's keys and values [..., n, d] of the first n tokens of page lists `table` [..., columns] in float64, and which
+    of them have a page."""
+    bs = pages.shape[3]
+    at = torch.arange(n, device=pages.device)
+    ids = table.long()[..., at // bs]
+    there = (ids >= 0) & (ids < pages.shape[0])
+    take = torch.where(there, ids, 0)
+    x = pages[take, j, :, at % bs].double()  # [..., n, 2, d]
+    if scales is not None:
+        x = x * scales[take, j, :, at % bs].double()[..., None]
+    return x[..., 0, :], x[..., 1, :], there
+
+
+def attend(query: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor | None, tables: list[list[int]], lens: list[int], prefix_table: list[int], prefix_len: int,
+           scale: float) -> tuple[torch.Tensor, ...]:
+    """(out, lse, mass, reach, top) in float64: query t of sequence b sees the prefix and own tokens 0 .. lens[b] - T + t,
+    those of them that have a page. mass = sum p |v| / sum p per output element; reach = the largest sum |q k| scale and
+    top = the largest p max |v| / sum p of a row's keys."""
     b, t, hq, d = query.shape
-    h = cache.pages.shape[1]
-    q = query.double().cpu()
-    out, mass = torch.zeros((b, t, hq, d), dtype=torch.float64), torch.zeros((b, t, hq, d), dtype=torch.float64)
-    lse, reach = torch.full((b, t, hq), -math.inf, dtype=torch.float64), torch.zeros((b, t, hq), dtype=torch.float64)
-    kp, vp, okp = cache.read(prefix_table, list(range(prefix_len)))
-    for i in range(b):
-        room = len(tables[i]) * cache.bs  # no token past the table has a page
-        ko, vo, oko = cache.read(tables[i], list(range(room)))
-        for step in range(t):
-            m = min(room, max(0, lens[i] - t + step + 1))
-            k, v = torch.cat([kp[okp], ko[:m][oko[:m]]]), torch.cat([vp[okp], vo[:m][oko[:m]]])
-            if k.shape[0] == 0:
-                continue
-            rows = q[i, step].view(h, hq // h, d)
-            s = torch.einsum("hgd,nhd->hgn", rows, k) * scale
-            reach[i, step] = (torch.einsum("hgd,nhd->hgn", rows.abs(), k.abs()) * abs(scale)).amax(-1).reshape(hq)
-            lse[i, step] = torch.logsumexp(s, -1).reshape(hq)
-            p = torch.softmax(s, -1)
-            out[i, step] = torch.einsum("hgn,nhd->hgd", p, v).reshape(hq, d)
-            mass[i, step] = torch.einsum("hgn,nhd->hgd", p, v.abs()).reshape(hq, d)
-    return out, lse, mass, reach
+    h, bs = pages.shape[1], pages.shape[3]
+    g = hq // h
+    table, ptab = torch.tensor(tables, device="cuda").view(b, -1), torch.tensor(prefix_table, device="cuda")
+    room = table.shape[1] * bs  # no token past the table has a page
+    sight = torch.tensor([[min(room, max(0, n - t + i + 1)) for i in range(t)] for n in lens], device="cuda")  # [b, t]
+    unseen = torch.arange(room, device="cuda") >= sight[..., None]  # [b, t, room]
+    q = query.cuda().double().view(b, t, h, g, d)
+    out, mass = (torch.zeros((b, t, h, g, d), dtype=torch.float64, device="cuda") for _ in range(2))
+    lse, reach, top = (torch.zeros((b, t, h, g), dtype=torch.float64, device="cuda") for _ in range(3))
+    for j in range(h):
+        kp, vp, okp = tokens(pages, scales, j, ptab, prefix_len)
+        ko, vo, oko = tokens(pages, scales, j, table, room)
+        rows = q[:, :, j]  # [b, t, g, d]
+        gone = torch.cat([(~okp).expand(b, t, g, -1), (unseen | ~oko[:, None])[:, :, None].expand(b, t, g, room)], -1)
+        vp, vo = torch.where(okp[:, None], vp, 0.0), torch.where((oko & ~unseen.all(1))[..., None], vo, 0.0)  # what no row sees may hold anything
+        s = torch.cat([rows @ kp.T, torch.einsum("btgd,bnd->btgn", rows, ko)], -1) * scale
+        size = torch.cat([rows.abs() @ kp.abs().T, torch.einsum("btgd,bnd->btgn", rows.abs(), ko.abs())], -1) * abs(scale)
+        s = torch.where(gone, -math.inf, s)
+        lse[:, :, j] = torch.logsumexp(s, -1)
+        p = torch.where(gone, 0.0, torch.exp(s - torch.where(lse[:, :, j] == -math.inf, 0.0, lse[:, :, j])[..., None]))
+        reach[:, :, j] = torch.where(gone, 0.0, size).amax(-1)
+        p1, p2 = p[..., :prefix_len], p[..., prefix_len:]
+        out[:, :, j] = p1 @ vp + torch.einsum("btgn,bnd->btgd", p2, vo)
+        mass[:, :, j] = p1 @ vp.abs() + torch.einsum("btgn,bnd->btgd", p2, vo.abs())
+        most = torch.cat([vp.abs().amax(-1).expand(b, -1), vo.abs().amax(-1)], -1)  # [b, keys]
+        top[:, :, j] = (p * most[:, None, None]).amax(-1)
+    return out.view(b, t, hq, d), lse.view(b, t, hq), mass.view(b, t, hq, d), reach.view(b, t, hq), top.view(b, t, hq)
 
 
 def near(cache: Cache, query: torch.Tensor, tables, lens, prefix_table, prefix: int, scale: float, out: torch.Tensor, lse: torch.Tensor) -> None:
-    """out (float32) and lse within what a weight's one rounding to bfloat16 or f16 and the scores' float32 sums leave
-    (tests/test_prefix_attention_gpu.py derives the terms): 2^-8 of sum p |v|, and 2 (d + 4) 2^-24 reach and n 2^-24 of it."""
-    want, wlse, mass, reach = attend(cache, query, tables, lens, prefix_table, prefix, scale)
-    n = prefix + max(len(t) for t in tables) * cache.bs
+    """out (float32) and lse against `attend`. A score is a float32 sum of d products (two more roundings for the scales):
+    off by at most delta = (d + 4) 2^-24 reach, which moves a weight by a factor within e^(+-delta); exp2 is off by 2^-22 and
+    the sums over n keys by n 2^-24 at most. bf16 pages: a weight is rounded to bfloat16, 2^-8 of it. int8 pages: a weight
+    times its value's scale is rounded to f16, 2^-11 of it or 2^-25 of a unit of which the row's largest such product has
+    2^6 at least; codes go up to 127, so n keys make that n 2^-31 top at most; four more float32 roundings."""
+    pages, scales = cache.pages.cuda(), None if cache.scales is None else cache.scales.cuda()
+    want, wlse, mass, reach, top = attend(query, pages, scales, tables, lens, prefix_table, prefix, scale)
+    n = prefix + max(len(x) for x in tables) * cache.bs
     sums = (query.shape[-1] + 4) * 2.0**-24 * reach + 2.0**-22 + n * 2.0**-24
-    err, lerr = (out.double().cpu() - want).abs(), (lse.double().cpu() - wlse).abs()
-    bound = (2.0**-8 + 2 * sums[..., None]) * mass + 2.0**-23 * want.abs()
+    if cache.int8:
+        bound = (2.0**-11 + 2 * sums[..., None] + 4 * 2.0**-24) * mass + n * 2.0**-31 * top[..., None] + 2.0**-23 * want.abs()
+    else:
+        bound = (2.0**-8 + 2 * sums[..., None]) * mass + 2.0**-23 * want.abs()
     empty = wlse == -math.inf
-    assert bool((err <= bound).all()), float((err / bound.clamp_min(1e-30)).max())
-    assert bool((lse.cpu()[empty] == -math.inf).all())
+    err, lerr = (out.double() - want).abs(), (lse.double() - wlse).abs()
+    assert bool((err <= bound).all()), float((err / bound.clamp_min(1e-300)).max())
+    assert bool((lse[empty] == -math.inf).all())
     assert bool((lerr <= sums + 4 * 2.0**-24 * (wlse.abs() + 1))[~empty].all()), float(lerr[~empty].max())
 
 
@@ -71,32 +99,6 @@ def test_several_queries_of_a_length_past_the_table(b: int, t: int, g: int, int8
     query = torch.randn((b, t, h * g, d), generator=gen).bfloat16()
     out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, prefix, d**-0.5, scales=scales, out_dtype=torch.float32)
     near(cache, query, tables, lens, prefix_table, prefix, d**-0.5, out, lse)
-
-
-def near_int8(cache: Cache, query: torch.Tensor, tables, lens, prefix_table, prefix: int, scale: float, out: torch.Tensor, lse: torch.Tensor) -> None:
-    """int8 pages, each row on its own: a weight times its value's scale is rounded to f16 once, 2^-11 of it or 2^-25
-    of a unit of which the row's largest such product has 2^6 at least: n keys, codes up to 127, make that at most
-    n 2^-31 top, top = max p max |v| / sum p over the row's keys. The rest as in `near`, with four more float32 roundings."""
-    want, wlse, mass, reach = attend(cache, query, tables, lens, prefix_table, prefix, scale)
-    b, t, hq, d = query.shape
-    h = cache.pages.shape[1]
-    n = prefix + max(len(x) for x in tables) * cache.bs
-    kp, vp, okp = cache.read(prefix_table, list(range(prefix)))
-    top = torch.zeros((b, t, hq), dtype=torch.float64)
-    for i in range(b):
-        ko, vo, oko = cache.read(tables[i], list(range(len(tables[i]) * cache.bs)))
-        for step in range(t):
-            m = min(ko.shape[0], max(0, lens[i] - t + step + 1))
-            k, v = torch.cat([kp[okp], ko[:m][oko[:m]]]), torch.cat([vp[okp], vo[:m][oko[:m]]])
-            if k.shape[0] > 0:
-                p = torch.softmax(torch.einsum("hgd,nhd->hgn", query[i, step].double().cpu().view(h, hq // h, d), k) * scale, -1)
-                top[i, step] = (p * v.abs().amax(-1).T[:, None]).amax(-1).reshape(hq)
-    sums = (d + 4) * 2.0**-24 * reach + 2.0**-22 + n * 2.0**-24
-    bound = (2.0**-11 + 2 * sums[..., None] + 4 * 2.0**-24) * mass + n * 2.0**-31 * top[..., None] + 2.0**-23 * want.abs()
-    err, lerr = (out.double().cpu() - want).abs(), (lse.double().cpu() - wlse).abs()
-    empty = wlse == -math.inf
-    assert bool((err <= bound).all()), float((err / bound.clamp_min(1e-300)).max())
-    assert bool((lerr <= sums + 4 * 2.0**-24 * (wlse.abs() + 1))[~empty].all()), float(lerr[~empty].max())
 
 
 def rescale(cache: Cache, prefix_table: list[int], prefix: int, every: int, first: int, values: float, keys: float) -> None:
@@ -139,4 +141,17 @@ def test_int8_values_beside_far_larger_ones_in_the_stream(d: int, spread) -> Non
     cache, prefix_table, tables, lens, query = spread_case(3, d, spread, 16, 400)
     pages, scales, ptab, table, n = on_gpu(cache, prefix_table, tables, lens)
     out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, 400, d**-0.5, scales=scales, out_dtype=torch.float32)
-    near_int8(cache, query, tables, lens, prefix_table, 400, d**-0.5, out, lse)
+    near(cache, query, tables, lens, prefix_table, 400, d**-0.5, out, lse)
+
+
+@pytest.mark.parametrize("spread", SPREADS, ids=str)
+@pytest.mark.parametrize("b,h", [(40, 2), (150, 1), (24, 160)], ids=["one row tile", "two row tiles", "several tiles of the prefix a CTA"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_int8_values_beside_far_larger_ones_in_the_tiles(d: int, b: int, h: int, spread) -> None:  # noqa: ANN001
+    from lazykv_b200 import kernels as K
+
+    cache, prefix_table, tables, lens, query = spread_case(b, d, spread, 32, 700, h)
+    pages, scales, ptab, table, n = on_gpu(cache, prefix_table, tables, lens)
+    out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, 700, d**-0.5, scales=scales, out_dtype=torch.float32)
+    near(cache, query, tables, lens, prefix_table, 700, d**-0.5, out, lse)
+    assert K.device_status() == 0
