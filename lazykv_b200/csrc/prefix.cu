@@ -203,6 +203,7 @@ template <int D>
 __device__ __forceinline__ void fold_values_singly(State<D>& st, const char* values, const float (&s)[2][4], int lane) {
   using S = Shape<D, false>;
   const int c = lane % 4;
+  __syncwarp();  // a lane has waited for its own copies; here it reads other lanes' too
 #pragma unroll 1
   for (int t = 0; t < 16; ++t) {
     const int c2 = (t & 7) >> 1, owner = (lane & ~3) | c2;  // the lane that holds this token's weights of rows r, r + 8

@@ -63,8 +63,9 @@ def attend(query: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor | None
     return out.view(b, t, hq, d), lse.view(b, t, hq), mass.view(b, t, hq, d), reach.view(b, t, hq), top.view(b, t, hq)
 
 
-def near(cache: Cache, query: torch.Tensor, tables, lens, prefix_table, prefix: int, scale: float, out: torch.Tensor, lse: torch.Tensor) -> None:
-    """out (float32) and lse against `attend`. A score is a float32 sum of d products (two more roundings for the scales):
+def near(cache: Cache, query: torch.Tensor, tables, lens, prefix_table, prefix: int, scale: float, out: torch.Tensor, lse: torch.Tensor,
+         queries: slice = slice(None)) -> None:
+    """out (float32) and lse, of some of a step's queries, against `attend`. A score is a float32 sum of d products (two more roundings for the scales):
     off by at most delta = (d + 4) 2^-24 reach, which moves a weight by a factor within e^(+-delta); exp2 is off by 2^-22 and
     the sums over n keys by n 2^-24 at most. bf16 pages: a weight is rounded to bfloat16, 2^-8 of it. int8 pages: a weight
     times its value's scale is rounded to f16, 2^-11 of it or 2^-25 of a unit of which the row's largest such product has
@@ -77,6 +78,7 @@ def near(cache: Cache, query: torch.Tensor, tables, lens, prefix_table, prefix: 
         bound = (2.0**-11 + 2 * sums[..., None] + 4 * 2.0**-24) * mass + n * 2.0**-31 * top[..., None] + 2.0**-23 * want.abs()
     else:
         bound = (2.0**-8 + 2 * sums[..., None]) * mass + 2.0**-23 * want.abs()
+    want, wlse, bound, sums, out, lse = (x[:, queries] for x in (want, wlse, bound, sums, out, lse))
     empty = wlse == -math.inf
     err, lerr = (out.double() - want).abs(), (lse.double() - wlse).abs()
     assert bool((err <= bound).all()), float((err / bound.clamp_min(1e-300)).max())
@@ -155,3 +157,27 @@ def test_int8_values_beside_far_larger_ones_in_the_tiles(d: int, b: int, h: int,
     out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, 700, d**-0.5, scales=scales, out_dtype=torch.float32)
     near(cache, query, tables, lens, prefix_table, 700, d**-0.5, out, lse)
     assert K.device_status() == 0
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_values_that_are_not_finite_in_many_sequences_last_tokens(d: int, int8: bool) -> None:
+    """Every sequence's last token is infinite or NaN here and there: the queries before it get what they get with
+    that token's row all zeros, at every place of a list's end in its stage."""
+    from lazykv_b200 import kernels as K
+
+    h, g, bs, t, b = 2, 4, 16, 3, 60
+    gen = torch.Generator().manual_seed(d)
+    lens = [t + i for i in range(b)]
+    cache, prefix_table, tables = build(gen, h, d, bs, int8, 20, lens)
+    for i, n in enumerate(lens):
+        x = torch.randn((1, h, d), generator=gen).bfloat16()
+        x[..., i % d] = (torch.inf, -torch.inf, torch.nan)[i % 3]
+        cache.write(tables[i], n - 1, x, x)
+    pages, scales, ptab, table, n = on_gpu(cache, prefix_table, tables, lens)
+    query = torch.randn((b, t, h * g, d), generator=gen).bfloat16()
+    out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, 20, d**-0.5, scales=scales, out_dtype=torch.float32)
+    zero = torch.zeros((1, h, d), dtype=torch.bfloat16)
+    for i, m in enumerate(lens):
+        cache.write(tables[i], m - 1, zero, zero)
+    near(cache, query, tables, lens, prefix_table, 20, d**-0.5, out, lse, slice(0, t - 1))
