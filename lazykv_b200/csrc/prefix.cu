@@ -198,9 +198,9 @@ __device__ __forceinline__ uint32_t fill_stage(const Params& p, int j, const int
   return have;
 }
 
-// A granule's P V without mma (see fold_stage): weights of zero take nothing from their values.
+// A granule's P V without mma (see fold_stage), token by token; seen: how many of them rows r and r + 8 see.
 template <int D>
-__device__ __forceinline__ void fold_values_singly(State<D>& st, const char* values, const float (&s)[2][4], int lane) {
+__device__ __forceinline__ void fold_values_singly(State<D>& st, const char* values, const float (&s)[2][4], const int (&seen)[2], int lane) {
   using S = Shape<D, false>;
   const int c = lane % 4;
   __syncwarp();  // a lane has waited for its own copies; here it reads other lanes' too
@@ -216,8 +216,8 @@ __device__ __forceinline__ void fold_values_singly(State<D>& st, const char* val
       const char* src = values + (((t & 1) + 2 * (t >> 3)) * S::kVLoads + i / S::kVCh) * (S::kVBytes * 32) + 2 * (i % S::kVCh);
       const float va = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(src + ((2 * c) * 4 + c2) * S::kVBytes));
       const float vb = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(src + ((2 * c + 1) * 4 + c2) * S::kVBytes));
-      if (p0 != 0.0f) st.o[i][0] += p0 * va, st.o[i][1] += p0 * vb;
-      if (p1 != 0.0f) st.o[i][2] += p1 * va, st.o[i][3] += p1 * vb;
+      if (t < seen[0]) st.o[i][0] += p0 * va, st.o[i][1] += p0 * vb;
+      if (t < seen[1]) st.o[i][2] += p1 * va, st.o[i][3] += p1 * vb;
     }
   }
   __syncwarp();  // these slots are other lanes' to fill again
@@ -309,8 +309,9 @@ __device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D 
       const float by2[2] = {vs[n].x * kScaleDown, vs[n].y * kScaleDown};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float by = by2[e & 1];
-        s[n][e] = MASKED && s[n][e] == 0.0f ? 0.0f : s[n][e] * by;  // a masked token's scale may be a NaN
+        // What a row does not see is nothing whatever its scale; what it sees counts, a NaN under a weight of zero too.
+        const bool unseen = MASKED && (first + 8 * n + 2 * c + (e & 1) >= limit[e >> 1] || !((have >> (n / 2)) & 1));
+        s[n][e] = unseen ? 0.0f : s[n][e] * by2[e & 1];
       }
     }
   }
@@ -343,7 +344,9 @@ __device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D 
           for (int i = 0; i < S::kVBytes / 4; ++i) odd = odd || (w[y][t][i] & 0x7f80u) == 0x7f80u || (w[y][t][i] & 0x7f800000u) == 0x7f800000u;
       if (__any_sync(0xffffffffu, odd)) {
         const float weights[2][4] = {{s[2 * g][0], s[2 * g][1], s[2 * g][2], s[2 * g][3]}, {s[2 * g + 1][0], s[2 * g + 1][1], s[2 * g + 1][2], s[2 * g + 1][3]}};
-        fold_values_singly<D>(st, values, weights, lane);
+        const bool page = (have >> g) & 1;
+        const int seen[2] = {page ? limit[0] - first - 16 * g : 0, page ? limit[1] - first - 16 * g : 0};
+        fold_values_singly<D>(st, values, weights, seen, lane);
         continue;
       }
     }

@@ -181,3 +181,29 @@ def test_values_that_are_not_finite_in_many_sequences_last_tokens(d: int, int8: 
     for i, m in enumerate(lens):
         cache.write(tables[i], m - 1, zero, zero)
     near(cache, query, tables, lens, prefix_table, 20, d**-0.5, out, lse, slice(0, t - 1))
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("b,prefix,at", [(2, 0, 5), (2, 300, 299), (2, 300, 5), (40, 300, 299), (40, 300, 5)])
+def test_a_value_that_is_not_finite_counts_under_any_weight(b: int, prefix: int, at: int, int8: bool, bad: float) -> None:
+    """A token that every row sees, whose score is hundreds below the others' (its weight is 0 in float32), has a value
+    that is not finite: exp(-500) infinity is infinite in the definition, and no row is finite there, wherever the token
+    lies: at a list's end or before, in the own tokens, the streamed prefix or the tiled one."""
+    from lazykv_b200 import kernels as K
+
+    d, bs, n_own = 64, 16, 9
+    gen = torch.Generator().manual_seed(at)
+    cache, prefix_table, tables = build(gen, 1, d, bs, int8, prefix, [n_own] * b)
+    key, value = torch.full((1, 1, d), -8.0).bfloat16(), torch.randn((1, 1, d), generator=gen).bfloat16()
+    value[..., 3] = bad
+    for table in [prefix_table] if prefix else tables:
+        cache.write(table, at, key, value)
+        if int8:
+            cache.pages[table[at // bs], 0, 0, at % bs], cache.scales[table[at // bs], 0, 0, at % bs] = -127, 8 / 127
+    pages, scales, ptab, table, n = on_gpu(cache, prefix_table, tables, [n_own] * b)
+    query = torch.full((b, 1, 4, d), 8.0).bfloat16()
+    out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, prefix, d**-0.5, scales=scales, out_dtype=torch.float32)
+    assert not bool(out[..., 3].isfinite().any()) and bool(lse.isfinite().all())
+    if not int8:  # (int8: one scale for the whole row)
+        assert bool(out[..., :3].isfinite().all()) and bool(out[..., 4:].isfinite().all())
