@@ -172,9 +172,11 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const VerifyParams 
   const double at = fmin(fmax((double)p.uniforms[b * p.u_sb + p.k], 0.0), kBelowOne) * all;
   const bool last = rank == n_ranks - 1;
   if (warp != 0 || !(at >= before && (at < before + mine || last))) return;
-  // This CTA's slice holds the border. Lanes take consecutive tiles, then consecutive elements.
+  // This CTA's slice holds the border. Lanes take consecutive tiles, then consecutive elements. Sums in another order
+  // may round to the border's other side: only what weighs something is ever taken, and the last of it where no
+  // sum passes the border.
   double base = before;
-  int tile = n_tiles - 1;
+  int tile = 0;
   const int share = (n_tiles + 31) / 32;
   {
     double s = 0.0;
@@ -185,10 +187,11 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const VerifyParams 
       const double y = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += y;
     }
-    const uint32_t over = __ballot_sync(0xffffffffu, before + upto > at);
-    const int who = over != 0 ? __ffs(over) - 1 : 31;
+    const uint32_t some = __ballot_sync(0xffffffffu, s > 0.0), over = some & __ballot_sync(0xffffffffu, before + upto > at);
+    const int who = over != 0 ? __ffs(over) - 1 : 31 - __clz(some);
     double run = before + __shfl_sync(0xffffffffu, upto - s, who);
     for (int i = who * share; i < min((who + 1) * share, n_tiles); ++i) {
+      if (!(tiles[i] > 0.0)) continue;
       tile = i;
       base = run;
       run += tiles[i];
@@ -208,7 +211,6 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const VerifyParams 
     const double y = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += y;
   }
-  // The last element that weighs anything stands in where rounding leaves the border past the tile.
   int found = -1, heaviest = -1;
   double run = base + (upto - s);
 #pragma unroll
