@@ -73,12 +73,17 @@ class PagedBatch:
         n = -(-keys.shape[1] // self.page)
         if n > len(self._free_pages) + len(self._prefix_pages):
             raise RuntimeError(f"cache full: {n} pages wanted, {len(self._free_pages) + len(self._prefix_pages)} free")
+        free = list(self._free_pages)
         self._free_pages.extend(reversed(self._prefix_pages))
-        self._prefix_pages = self._take(n)
-        self.prefix_table = torch.tensor(self._prefix_pages, dtype=torch.int32, device=self.dev)
-        self.prefix_len = keys.shape[1]
-        if n:
-            self._write(keys, values, self.prefix_table.view(1, n))
+        try:
+            pages = self._take(n)
+            table = torch.tensor(pages, dtype=torch.int32, device=self.dev)
+            if n:
+                self._write(keys, values, table.view(1, n))
+        except BaseException:  # refused before anything was written: the earlier prompt stays
+            self._free_pages = free
+            raise
+        self._prefix_pages, self.prefix_table, self.prefix_len = pages, table, keys.shape[1]
 
     def _write(self, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor) -> None:
         zero = torch.zeros(1, dtype=torch.int32, device=self.dev)

@@ -1,0 +1,39 @@
+"""PagedBatch and speculative decoding around refused calls, and where a step's work is ordered."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+H, G, D = 2, 4, 64
+
+
+@pytest.mark.parametrize("quant", ["int8", None])
+def test_a_refused_prefix_leaves_the_earlier_one(quant: str | None) -> None:
+    from lazykv_b200.paged import PagedBatch
+
+    gen = torch.Generator().manual_seed(1)
+    rand = lambda *s: torch.randn(s, generator=gen).bfloat16().cuda()  # noqa: E731
+    batch = PagedBatch(H, G, D, max_seqs=2, max_tokens=40, n_pages=8, quant=quant)
+    batch.set_prefix(rand(H, 50, D), rand(H, 50, D))
+    q, k, v = rand(1, 1, H * G, D), rand(1, 1, H, D), rand(1, 1, H, D)
+
+    def step() -> tuple[torch.Tensor, torch.Tensor]:
+        s = batch.fork()
+        done = batch.step([s], q, k, v, 0.125)
+        batch.drop(s)
+        return done
+
+    want, table, free = step(), batch.prefix_table.tolist(), sorted(batch._free_pages)
+    x = rand(H, 37, D)
+    turned = rand(H, D, 37).transpose(1, 2)  # channels that are not contiguous
+    for keys, values in ((x, x.float()), (turned, x), (x, turned)):
+        with pytest.raises(ValueError):
+            batch.set_prefix(keys, values)
+        assert batch.prefix_len == 50 and batch.prefix_table.tolist() == table and sorted(batch._free_pages) == free
+        got = step()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    batch.set_prefix(x, x)
+    assert batch.prefix_len == 37 and len(batch._free_pages) == 5
