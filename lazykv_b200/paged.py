@@ -117,8 +117,12 @@ class PagedBatch:
             new = self._take(len(rows))
             for s, page in zip(rows, new):
                 self._pages_of[s].append(page)
-            at = torch.tensor([rows, cols, new], device=self.dev)
+            at = self._to_device(torch.tensor([rows, cols, new], pin_memory=True))
             self.table[at[0], at[1]] = at[2].to(torch.int32)
+
+    def _to_device(self, pinned: torch.Tensor) -> torch.Tensor:
+        """A copy that the stream orders and the host does not wait for (torch keeps the pinned block until it is done)."""
+        return pinned.to(self.dev, non_blocking=True)
 
     # -- the decode step ----------------------------------------------------------------------------------
 
@@ -138,10 +142,11 @@ class PagedBatch:
             raise ValueError(f"expected query [{n}, {t}, {self.h * self.g}, {self.d}], got {tuple(query.shape)}")
         require_cuda(query, keys, values)
         self._reserve(seq_ids, t)
-        host = torch.tensor([seq_ids, [self.lengths[s] for s in seq_ids], [self.lengths[s] + t for s in seq_ids]], dtype=torch.int32).to(self.dev)
-        table = self.table.index_select(0, host[0])
-        K.paged_write(keys, values, self.pages, table, host[1], scales=self.scales)
-        done = K.prefix_attention(query, self.pages, table, host[2], self.prefix_table, self.prefix_len, scale, scales=self.scales, out_dtype=out_dtype)
+        lens = [self.lengths[s] for s in seq_ids]
+        ints = self._to_device(torch.tensor([seq_ids, lens, [x + t for x in lens]], dtype=torch.int32, pin_memory=True))
+        table = self.table.index_select(0, ints[0])
+        K.paged_write(keys, values, self.pages, table, ints[1], scales=self.scales)
+        done = K.prefix_attention(query, self.pages, table, ints[2], self.prefix_table, self.prefix_len, scale, scales=self.scales, out_dtype=out_dtype)
         for s in seq_ids:  # behind the calls: a refused step leaves the sequences as they were
             self.lengths[s] += t
         return done

@@ -37,3 +37,36 @@ def test_a_refused_prefix_leaves_the_earlier_one(quant: str | None) -> None:
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     batch.set_prefix(x, x)
     assert batch.prefix_len == 37 and len(batch._free_pages) == 5
+
+
+def test_a_step_does_not_wait_for_the_stream() -> None:
+    """Steps that take new pages and steps that do not, behind work that is still running: none synchronises, and each
+    result is the one that the same steps give when every one is waited for."""
+    from lazykv_b200.paged import PagedBatch
+
+    gen = torch.Generator().manual_seed(2)
+    rand = lambda *s: torch.randn(s, generator=gen).bfloat16().cuda()  # noqa: E731
+    pk, pv = rand(H, 100, D), rand(H, 100, D)
+    steps = [(rand(3, t, H * G, D), rand(3, t, H, D), rand(3, t, H, D)) for t in (1, 15, 1, 4, 30, 1)]
+    big = torch.randn((4096, 4096), device="cuda")
+    results = []
+    for waited in (True, False):
+        batch = PagedBatch(H, G, D, max_seqs=3, max_tokens=64, n_pages=30)
+        batch.set_prefix(pk, pv)
+        ids = [batch.fork() for _ in range(3)]
+        got = []
+        torch.cuda.synchronize()
+        torch.cuda.set_sync_debug_mode("default" if waited else "error")
+        try:
+            for x in steps:
+                if not waited:
+                    big = big @ big * 1e-4
+                got.append(batch.step(ids, *x, 0.125))
+                if waited:
+                    torch.cuda.synchronize()
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+        torch.cuda.synchronize()
+        results.append(got)
+    for (a, c), (e, f) in zip(*results):
+        assert torch.equal(a, e) and torch.equal(c, f)
