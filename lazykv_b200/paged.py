@@ -38,7 +38,10 @@ class PagedBatch:
         if min(heads, group, max_seqs, max_tokens, n_pages) < 1:
             raise ValueError("heads, group, max_seqs, max_tokens and n_pages are at least 1")
         self.h, self.g, self.d, self.page = heads, group, head_dim, page
-        self.dev, self.dtype = torch.device(device), dtype
+        dev = torch.device(device)
+        if dev.type == "cuda" and dev.index is None:  # the current device now, whichever is current at a later call
+            dev = torch.device("cuda", torch.cuda.current_device())
+        self.dev, self.dtype = dev, dtype
         self.max_seqs, self.max_tokens = max_seqs, max_tokens
         self.cols = -(-max_tokens // page)
         self.pages = torch.zeros((n_pages, heads, 2, page, head_dim), dtype=torch.int8 if quant else dtype, device=self.dev)

@@ -70,3 +70,10 @@ def test_a_step_does_not_wait_for_the_stream() -> None:
         results.append(got)
     for (a, c), (e, f) in zip(*results):
         assert torch.equal(a, e) and torch.equal(c, f)
+
+
+def test_a_batch_stays_on_the_device_that_was_current_when_it_was_made() -> None:
+    from lazykv_b200.paged import PagedBatch
+
+    batch = PagedBatch(H, G, D, max_seqs=1, max_tokens=16, n_pages=2, device="cuda")
+    assert batch.dev == batch.pages.device == batch.table.device and batch.dev.index == torch.cuda.current_device()
