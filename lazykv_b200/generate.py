@@ -144,7 +144,8 @@ def speculative_decode(model: PreTrainedModel, cache: Cache, draft_model: PreTra
     Both caches hold the same context, up to but without first_token, and are left holding it with
     first_token and every returned token but the last, so a call can go on from there. A round feeds the target the last token and the drafted ones in
     one forward pass, and kernels.verify_drafts decides how many of them are kept and which token follows;
-    the caches forget the others, so they need truncate() (FullGPUCache). `generator` (on the model's
+    the caches forget the others, so they need truncate() (FullGPUCache) and, for a while, room for one token
+    more than they are left with. Where the call fails they are left as they were. `generator` (on the model's
     device) draws the proposals and the uniforms.
     """
     for name, c in (("cache", cache), ("draft_cache", draft_cache)):
@@ -166,36 +167,41 @@ def speculative_decode(model: PreTrainedModel, cache: Cache, draft_model: PreTra
         return torch.softmax(logits.float() / temperature, dim=-1)
 
     res = SpeculativeResult(tokens=[])
-    dev = model.device
+    dev, start = model.device, cache.get_seq_length()
     behind = [first_token]  # returned tokens that the draft's cache does not hold yet, the target's but the last
-    while len(res.tokens) < n_tokens:
-        held = cache.get_seq_length()
-        k = min(n_draft, n_tokens - len(res.tokens))
-        fed, rows, drafted = torch.tensor([behind], dtype=torch.long, device=dev), [], []
-        for _ in range(k):
-            rows.append(probabilities(draft_model, draft_cache, fed, 1)[:, -1])
-            fed = torch.multinomial(rows[-1], 1, generator=generator)
-            drafted.append(fed)
-        tokens = torch.cat(drafted, dim=1)
-        target = probabilities(model, cache, torch.cat([torch.tensor([behind[-1:]], dtype=torch.long, device=dev), tokens], dim=1), k + 1)
-        uniforms = torch.rand((1, k + 1), device=dev, generator=generator)
-        kept, following = kernels.verify_drafts(target, torch.stack(rows, dim=1), tokens, uniforms)
-        decided = torch.cat([kept.long(), following, tokens[0]]).tolist()  # one copy to the host per round
-        n, nxt = decided[0], decided[1]
-        if nxt < 0:
-            raise RuntimeError("the target's probabilities have no finite, positive sum")
-        res.drafted += k
-        res.kept += n
-        new = decided[2 : 2 + n] + [nxt]
-        cache.truncate(held + 1 + n)  # the last token of the round before, and the drafted tokens that were kept
-        draft_cache.truncate(min(held + 1 + n, draft_cache.get_seq_length()))
-        # With all k kept the draft has not seen the last of them.
-        behind = new[-2:] if n == k else new[-1:]
-        res.tokens += new
-    if len(res.tokens) > n_tokens:  # the token after n_tokens kept ones
-        res.tokens = res.tokens[:n_tokens]
-        cache.truncate(cache.get_seq_length() - 1)
-        draft_cache.truncate(cache.get_seq_length())
-    if draft_cache.get_seq_length() < cache.get_seq_length():
-        probabilities(draft_model, draft_cache, torch.tensor([behind[:1]], dtype=torch.long, device=dev), 1)
+    try:
+        while len(res.tokens) < n_tokens:
+            held = cache.get_seq_length()
+            k = min(n_draft, n_tokens - len(res.tokens))
+            fed, rows, drafted = torch.tensor([behind], dtype=torch.long, device=dev), [], []
+            for _ in range(k):
+                rows.append(probabilities(draft_model, draft_cache, fed, 1)[:, -1])
+                fed = torch.multinomial(rows[-1], 1, generator=generator)
+                drafted.append(fed)
+            tokens = torch.cat(drafted, dim=1)
+            target = probabilities(model, cache, torch.cat([torch.tensor([behind[-1:]], dtype=torch.long, device=dev), tokens], dim=1), k + 1)
+            uniforms = torch.rand((1, k + 1), device=dev, generator=generator)
+            kept, following = kernels.verify_drafts(target, torch.stack(rows, dim=1), tokens, uniforms)
+            decided = torch.cat([kept.long(), following, tokens[0]]).tolist()  # one copy to the host per round
+            n, nxt = decided[0], decided[1]
+            if nxt < 0:
+                raise RuntimeError("the target's probabilities have no finite, positive sum")
+            res.drafted += k
+            res.kept += n
+            new = decided[2 : 2 + n] + [nxt]
+            cache.truncate(held + 1 + n)  # the last token of the round before, and the drafted tokens that were kept
+            draft_cache.truncate(min(held + 1 + n, draft_cache.get_seq_length()))
+            # With all k kept the draft has not seen the last of them.
+            behind = new[-2:] if n == k else new[-1:]
+            res.tokens += new
+        if len(res.tokens) > n_tokens:  # the token after n_tokens kept ones
+            res.tokens = res.tokens[:n_tokens]
+            cache.truncate(cache.get_seq_length() - 1)
+            draft_cache.truncate(cache.get_seq_length())
+        if draft_cache.get_seq_length() < cache.get_seq_length():
+            probabilities(draft_model, draft_cache, torch.tensor([behind[:1]], dtype=torch.long, device=dev), 1)
+    except BaseException:
+        for c in (cache, draft_cache):
+            c.truncate(start)
+        raise
     return res

@@ -77,3 +77,62 @@ def test_a_batch_stays_on_the_device_that_was_current_when_it_was_made() -> None
 
     batch = PagedBatch(H, G, D, max_seqs=1, max_tokens=16, n_pages=2, device="cuda")
     assert batch.dev == batch.pages.device == batch.table.device and batch.dev.index == torch.cuda.current_device()
+
+
+def test_speculative_decoding_that_fails_leaves_the_caches_as_they_were(monkeypatch) -> None:  # noqa: ANN001
+    """A draft of another vocabulary, a cache without room, a verification that finds no weight after some rounds: the
+    caches hold the context again, and the call that follows returns what it returns without the failed one."""
+    from transformers import LlamaForCausalLM
+
+    from lazykv_b200 import kernels
+    from lazykv_b200.cache import FullGPUCache
+    from lazykv_b200.generate import prefill, speculative_decode
+    from tests.tiny_model import CAP, make_tiny, prefilled
+
+    cfg, model = make_tiny()
+    wide = type(cfg)(**{**cfg.to_dict(), "vocab_size": cfg.vocab_size + 8})
+    torch.manual_seed(6)
+    other = LlamaForCausalLM(wide)
+    other.set_attn_implementation(model.config._attn_implementation)
+    other = other.to(dtype=torch.bfloat16).cuda().eval()
+
+    def caches(draft, room: int = CAP):  # noqa: ANN001, ANN202
+        ids, full, _ = prefilled(model, cfg)
+        n = full.get_seq_length()
+        cache = FullGPUCache(cfg.num_hidden_layers, room)
+        prefill(draft, cache, ids[:, :n], chunk_size=32)
+        return int(ids[0, n]), n, full, cache
+
+    def decode(first: int, full, draft, cache):  # noqa: ANN001, ANN202
+        return speculative_decode(model, full, draft, cache, first, 9, 3, generator=torch.Generator(device="cuda").manual_seed(1)).tokens
+
+    first, n, full, cache = caches(model)
+    want = decode(first, full, model, cache)
+
+    first, n, full, cache = caches(other)
+    with pytest.raises(ValueError, match="vocabularies"):  # refused before any token reaches the other's embedding
+        decode(first, full, other, cache)
+    assert full.get_seq_length() == n and cache.get_seq_length() == n
+    own = FullGPUCache(cfg.num_hidden_layers, CAP)
+    prefill(model, own, prefilled(model, cfg)[0][:, :n], chunk_size=32)
+    assert decode(first, full, model, own) == want
+
+    first, n, full, cache = caches(model, room=prefilled(model, cfg)[1].get_seq_length() + 4)
+    with pytest.raises(Exception):  # noqa: B017 - the draft's cache is full after a round or two
+        decode(first, full, model, cache)
+    assert full.get_seq_length() == n and cache.get_seq_length() == n
+
+    first, n, full, cache = caches(model)
+    rounds, real = [], kernels.verify_drafts
+
+    def runs_out(*args):  # noqa: ANN002, ANN202
+        rounds.append(1)
+        kept, token = real(*args)
+        return kept, token if len(rounds) < 2 else torch.full_like(token, -1)
+
+    monkeypatch.setattr(kernels, "verify_drafts", runs_out)
+    with pytest.raises(RuntimeError, match="positive sum"):
+        decode(first, full, model, cache)
+    monkeypatch.undo()
+    assert full.get_seq_length() == n and cache.get_seq_length() == n
+    assert decode(first, full, model, cache) == want
