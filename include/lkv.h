@@ -514,9 +514,18 @@ int lkv_status_poll(int* status, int clear);
  * selection first wait on a barrier that nothing completes, so that the wait runs out and the
  * failure path runs (status 1, poisoned output) with the GPU left usable.
  * LKV_DEBUG_EXCHANGE_WAIT_ITERS sets the bound (polls, 1 .. 2^22) of lkv_exchange_merge's wait for
- * its peers. Not for production use; not thread-safe.
+ * its peers. LKV_DEBUG_PREFIX_WAIT_NS sets the bound (nanoseconds, 1 .. 2 x 10^9) of the waits of
+ * lkv_prefix_attention's tiled prefix; LKV_DEBUG_PREFIX_STALL_NEXT makes a warp of every CTA of the next
+ * call with a tiled prefix withhold its arrival for the queries (1) or for the weights (2), so that the
+ * waits run out: status 1, and NaN in every row. Not for production use; not thread-safe.
  */
-enum { LKV_DEBUG_SELECT_WAIT_ITERS = 1, LKV_DEBUG_SELECT_STALL_NEXT = 2, LKV_DEBUG_EXCHANGE_WAIT_ITERS = 3 };
+enum {
+  LKV_DEBUG_SELECT_WAIT_ITERS = 1,
+  LKV_DEBUG_SELECT_STALL_NEXT = 2,
+  LKV_DEBUG_EXCHANGE_WAIT_ITERS = 3,
+  LKV_DEBUG_PREFIX_WAIT_NS = 4,
+  LKV_DEBUG_PREFIX_STALL_NEXT = 5
+};
 int lkv_debug_set(int key, int64_t value);
 
 /*

@@ -21,6 +21,7 @@ LKV_COLD_INT8, LKV_COLD_PAIRS = 0, 1
 LKV_ORDER_BOUND, LKV_ORDER_BLOCK = 0, 1
 LKV_CACHE_MODEL, LKV_CACHE_INT8 = 0, 1
 LKV_DEBUG_SELECT_WAIT_ITERS, LKV_DEBUG_SELECT_STALL_NEXT, LKV_DEBUG_EXCHANGE_WAIT_ITERS = 1, 2, 3
+LKV_DEBUG_PREFIX_WAIT_NS, LKV_DEBUG_PREFIX_STALL_NEXT = 4, 5
 LKV_DEV_WAIT_TIMEOUT, LKV_DEV_LIST_OVERFLOW = 1, 2
 
 _lib: ctypes.CDLL | None = None

@@ -32,6 +32,11 @@ cudaError_t select_status_attach(int* mirror);
 // The status word of prefix_tile.cu's kernels and its host mirror.
 cudaError_t prefix_device_status(int* status, int clear);
 cudaError_t prefix_status_attach(int* mirror);
+// Test hooks of those kernels' waits (prefix_tile.cu).
+namespace prefix {
+int set_tile_wait(int64_t ns);
+int set_tile_stall(int64_t which);
+}
 // The exchange's status word (exchange.cu), its host mirror, and the bound of its wait.
 cudaError_t exchange_device_status(int* status, int clear);
 cudaError_t exchange_status_attach(int* mirror);

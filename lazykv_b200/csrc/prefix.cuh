@@ -58,6 +58,9 @@ struct Params {
   int out_f32;
   float* lse;            // [batch, tokens, hq]
   int tile_first;        // the stream's launch is behind the tiled prefix's
+  // Test hooks of the tiles' waits (lkv_debug_set): how long one may last, and which arrival is withheld (0: none).
+  uint64_t max_wait_ns;
+  int stall;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -139,7 +142,7 @@ inline cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) 
 
 // prefix_tile.cu: the prefix's partials for many rows, and how many splits of the prefix they take.
 int tile_splits(int rows, int h, int64_t prefix_len);
-int run_tiles(const Params& p, int d, bool int8, cudaStream_t st);
+int run_tiles(Params p, int d, bool int8, cudaStream_t st);
 
 }  // namespace prefix
 }  // namespace lkv

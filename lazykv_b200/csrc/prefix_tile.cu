@@ -72,13 +72,14 @@ struct Barriers {
   uint32_t have[kInfo][4];   // together, bit g: tokens 16 g .. 16 g + 15 of the tile have a page
   int32_t top[kInfo][4];     // int8: 2^top is above every finite value scale x kScaleDown, per warp of converters
   float back[2][kTile];      // int8: what a row's scores are multiplied with (stage_query)
+  uint64_t max_wait_ns;
   uint32_t tmem;
   int quit;
 };
 
-// Waits for the phase of `bar` with the given parity, two seconds at most, or until another role gave up.
+// Waits for the phase of `bar` with the given parity, max_wait_ns at most, or until another role gave up.
 // Without a suspend-time hint: the waits here are short and many, and a hinted one was seen to resume late.
-constexpr uint64_t kMaxWaitNs = 2000000000ull;
+constexpr uint64_t kMaxWaitNs = 2000000000ull;  // unless a test asks for less
 __device__ __forceinline__ uint64_t now_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
@@ -96,7 +97,7 @@ __device__ __forceinline__ bool wait_long(Barriers& s, uint64_t* bar, uint32_t p
   const uint64_t from = now_ns();
   while (!try_once(bar, parity)) {
     if (*static_cast<volatile int*>(&s.quit)) return false;
-    if (now_ns() - from > kMaxWaitNs) {
+    if (now_ns() - from > s.max_wait_ns) {
       *static_cast<volatile int*>(&s.quit) = 1;
       record_status(LKV_DEV_WAIT_TIMEOUT);
       return false;
@@ -310,6 +311,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       mbar_init(&s.raw_empty[i], 4);
     }
     for (int i = 0; i < kInfo; ++i) mbar_init(&s.info[i], INT8 ? 8 : 1);
+    s.max_wait_ns = p.max_wait_ns;
     s.quit = 0;
     fence_mbar_init();
   }
@@ -341,7 +343,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       const float back = stage_query<D, INT8>(src, q_tiles + (two ? u * T::kBytes : 0), r, two || u == 0, sign < 0.0f ? 0x80008000u : 0u);
       if (INT8) s.back[u][r] = back;
       fence_async();
-      warp_arrive(&s.q_full, lane);
+      if (p.stall != 1 || warp != 0) warp_arrive(&s.q_full, lane);
     }
     float scale[4];
 #pragma unroll
@@ -486,7 +488,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
         st_wait();
       }
       tc_before();
-      warp_arrive(&s.p_full[u], lane);
+      if (p.stall != 2 || warp != 0) warp_arrive(&s.p_full[u], lane);
     }
     // ---- the rows' partials -------------------------------------------------------------------------
     const bool any_job = n_done > 0;
@@ -613,10 +615,9 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       pv(i);
       if (i + 2 < n_jobs) qk(i + 2);
     }
-    if (!ok) {  // nothing is freed under a product in flight
-      commit(&s.drain, mine);
-      mbar_wait(&s.drain, 0);
-    }
+    // Nothing is freed under a product in flight, whoever gave up and when.
+    commit(&s.drain, mine);
+    mbar_wait(&s.drain, 0);
     __syncwarp();
   } else if (warp == 9) {
     // ---- copies: the pages of one operand tile at a time, keys then values ----------------------------
@@ -684,10 +685,9 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
         filled = n + 1;
       }
     }
-    if (!ok) {  // no copy may land after the CTA has gone
-      const int kSlots = INT8 ? T::kRaw : n_stages;
-      for (int n = max(0, filled - kSlots); n < filled; ++n) mbar_wait(INT8 ? &s.raw_full[n % kSlots] : &s.full[n % kSlots], (n / kSlots) & 1);
-    }
+    // No copy may land after the CTA has gone, also where the others gave up behind this warp's last copy.
+    const int kSlots = INT8 ? T::kRaw : n_stages;
+    for (int n = max(0, filled - kSlots); n < filled; ++n) mbar_wait(INT8 ? &s.raw_full[n % kSlots] : &s.full[n % kSlots], (n / kSlots) & 1);
     __syncwarp();
   } else if (warp >= 12) {
     if constexpr (INT8) {
@@ -796,8 +796,26 @@ int tile_splits(int rows, int h, int64_t prefix_len) {
   return (int)((tiles + chunk - 1) / chunk);
 }
 
-int run_tiles(const Params& p, int d, bool int8, cudaStream_t st) {
+// Test hooks (lkv_debug_set): the bound of the waits, and what warp 0 of every CTA of the next call withholds.
+static uint64_t g_max_wait_ns = kMaxWaitNs;
+static int g_stall_next = 0;
+
+int set_tile_wait(int64_t ns) {
+  if (ns < 1 || ns > (int64_t)kMaxWaitNs) return fail(LKV_ERR_ARG, "lkv_debug_set: prefix wait bound %lld ns outside [1, %llu]", (long long)ns, (unsigned long long)kMaxWaitNs);
+  g_max_wait_ns = (uint64_t)ns;
+  return LKV_OK;
+}
+int set_tile_stall(int64_t which) {
+  if (which < 0 || which > 2) return fail(LKV_ERR_ARG, "lkv_debug_set: no stall %lld of the prefix tiles (0, 1 or 2)", (long long)which);
+  g_stall_next = (int)which;
+  return LKV_OK;
+}
+
+int run_tiles(Params p, int d, bool int8, cudaStream_t st) {
   static const char* who = "lkv_prefix_attention";
+  p.max_wait_ns = g_max_wait_ns;
+  p.stall = g_stall_next;
+  g_stall_next = 0;
   const int tiles = (p.prefix_len + kTile - 1) / kTile, chunk = (tiles + p.n_splits - 1) / p.n_splits;
   if ((p.rows + 2 * kTile - 1) / (2 * kTile) > 65535) return fail(LKV_ERR_ARG, "%s: too many rows", who);
   CUtensorMap map = {};

@@ -1183,6 +1183,10 @@ int lkv_debug_set(int key, int64_t value) {
       return LKV_OK;
     case LKV_DEBUG_EXCHANGE_WAIT_ITERS:
       return exchange_set_wait_iters(value);
+    case LKV_DEBUG_PREFIX_WAIT_NS:
+      return prefix::set_tile_wait(value);
+    case LKV_DEBUG_PREFIX_STALL_NEXT:
+      return prefix::set_tile_stall(value);
     default:
       return fail(LKV_ERR_ARG, "lkv_debug_set: unknown key %d", key);
   }
