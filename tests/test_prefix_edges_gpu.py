@@ -63,18 +63,21 @@ def attend(query: torch.Tensor, pages: torch.Tensor, scales: torch.Tensor | None
     return out.view(b, t, hq, d), lse.view(b, t, hq), mass.view(b, t, hq, d), reach.view(b, t, hq), top.view(b, t, hq)
 
 
-def near(cache: Cache, query: torch.Tensor, tables, lens, prefix_table, prefix: int, scale: float, out: torch.Tensor, lse: torch.Tensor,
-         queries: slice = slice(None)) -> None:
+def near(cache: Cache, *rest) -> None:  # noqa: ANN002
+    near_pages(cache.pages.cuda(), None if cache.scales is None else cache.scales.cuda(), *rest)
+
+
+def near_pages(pages: torch.Tensor, scales: torch.Tensor | None, query: torch.Tensor, tables, lens, prefix_table, prefix: int, scale: float,
+               out: torch.Tensor, lse: torch.Tensor, queries: slice = slice(None)) -> None:
     """out (float32) and lse, of some of a step's queries, against `attend`. A score is a float32 sum of d products (two more roundings for the scales):
     off by at most delta = (d + 4) 2^-24 reach, which moves a weight by a factor within e^(+-delta); exp2 is off by 2^-22 and
     the sums over n keys by n 2^-24 at most. bf16 pages: a weight is rounded to bfloat16, 2^-8 of it. int8 pages: a weight
     times its value's scale is rounded to f16, 2^-11 of it or 2^-25 of a unit of which the row's largest such product has
     2^6 at least; codes go up to 127, so n keys make that n 2^-31 top at most; four more float32 roundings."""
-    pages, scales = cache.pages.cuda(), None if cache.scales is None else cache.scales.cuda()
     want, wlse, mass, reach, top = attend(query, pages, scales, tables, lens, prefix_table, prefix, scale)
-    n = prefix + max(len(x) for x in tables) * cache.bs
+    n = prefix + max(len(x) for x in tables) * pages.shape[3]
     sums = (query.shape[-1] + 4) * 2.0**-24 * reach + 2.0**-22 + n * 2.0**-24
-    if cache.int8:
+    if scales is not None:
         bound = (2.0**-11 + 2 * sums[..., None] + 4 * 2.0**-24) * mass + n * 2.0**-31 * top[..., None] + 2.0**-23 * want.abs()
     else:
         bound = (2.0**-8 + 2 * sums[..., None]) * mass + 2.0**-23 * want.abs()
@@ -207,3 +210,63 @@ def test_a_value_that_is_not_finite_counts_under_any_weight(b: int, prefix: int,
     assert not bool(out[..., 3].isfinite().any()) and bool(lse.isfinite().all())
     if not int8:  # (int8: one scale for the whole row)
         assert bool(out[..., :3].isfinite().all()) and bool(out[..., 4:].isfinite().all())
+
+
+def random_pages(gen: torch.Generator, n: int, h: int, bs: int, d: int, int8: bool) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """A cache on the GPU, every row of it filled."""
+    if not int8:
+        return torch.randn((n, h, 2, bs, d), generator=gen, device="cuda").bfloat16(), None
+    pages = torch.randint(-127, 128, (n, h, 2, bs, d), generator=gen, device="cuda", dtype=torch.int8)
+    return pages, (0.5 + torch.rand((n, h, 2, bs), generator=gen, device="cuda")) / 64
+
+
+@pytest.mark.parametrize("b,h,g,t", [(20, 148, 1, 1), (35, 148, 4, 1), (50, 74, 2, 3)], ids=["one row tile", "two row tiles", "several CTAs of rows"])
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_tiles_of_the_prefix_in_one_cta(d: int, int8: bool, b: int, h: int, g: int, t: int) -> None:
+    """A CTA of rows per SM: each takes the whole prefix, 22 tiles, past two turns of every ring it has. Scores grow and
+    fall from tile to tile, so references move and outputs are rescaled; some pages are missing, two tiles have none at
+    all, and the last tile is not full."""
+    from lazykv_b200 import kernels as K
+
+    gen = torch.Generator(device="cuda").manual_seed(b + d)
+    bs, prefix = 64, 21 * 128 + 37
+    cols = -(-prefix // bs)
+    pages, scales = random_pages(gen, cols + b + 2, h, bs, d, int8)
+    order = torch.randperm(cols + b + 2, generator=gen, device="cuda").tolist()
+    prefix_table, tables = order[:cols], [[x] for x in order[cols : cols + b]]
+    for col in range(cols):  # (the first tile's scores are small)
+        by = (0.25, 0.5, 4.0, 1.0, 8.0, 0.125, 16.0)[(col // 2) % 7]
+        (pages if scales is None else scales)[prefix_table[col], :, 0] *= by
+    for col in (5, 14, 15, 16, 17, 30):
+        prefix_table[col] = -1 if col % 2 else len(pages) + col
+    lens = [(7 * i) % 64 for i in range(b)]
+    query = (1.5 * torch.randn((b, t, h * g, d), generator=gen, device="cuda")).bfloat16()
+    out, lse = K.prefix_attention(query, pages, torch.tensor(tables, dtype=torch.int32, device="cuda"), torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                                  torch.tensor(prefix_table, dtype=torch.int32, device="cuda"), prefix, d**-0.5, scales=scales, out_dtype=torch.float32)
+    near_pages(pages, scales, query, tables, lens, prefix_table, prefix, d**-0.5, out, lse)
+    assert K.device_status() == 0
+
+
+@pytest.mark.parametrize("prefix", [0, 700])
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_more_stages_of_the_stream_than_its_warps_hold(d: int, int8: bool, prefix: int) -> None:
+    """Own tokens of 64 sequences, up to 2,000 and 4,000, some none: every warp that the GPU holds takes some thirty
+    stages or more, past many turns of its ring, over several sequences; scores grow and fall along a list."""
+    from lazykv_b200 import kernels as K
+
+    gen = torch.Generator(device="cuda").manual_seed(prefix + d)
+    b, h, g, t, bs, most = 64, 8, 2, 2, 32, 2000 if d == 128 else 4000
+    cols, pcols = -(-most // bs), -(-prefix // bs)
+    pages, scales = random_pages(gen, b * cols + pcols, h, bs, d, int8)
+    order = torch.randperm(b * cols + pcols, generator=gen, device="cuda")
+    for turn in range(5):
+        (pages if scales is None else scales)[turn::7, :, 0] *= 2.0 ** (turn - 2)
+    table, ptab = order[: b * cols].view(b, cols).int(), order[b * cols :].int()
+    lens = [most - (977 * i + 5) % 500 if i % 9 else 0 for i in range(b)]
+    query = (1.5 * torch.randn((b, t, h * g, d), generator=gen, device="cuda")).bfloat16()
+    out, lse = K.prefix_attention(query, pages, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), ptab, prefix, d**-0.5, scales=scales,
+                                  out_dtype=torch.float32)
+    near_pages(pages, scales, query, table.tolist(), lens, ptab.tolist(), prefix, d**-0.5, out, lse)
+    assert K.device_status() == 0
