@@ -629,6 +629,11 @@ int lkv_paged_read(const lkv_paged_args* args, void* stream);
  * The prefix is read once for up to 256 query rows per KV head (batch * tokens * hq / h). Partials go to the workspace (any contents,
  * lkv_prefix_attention_workspace bytes with own_reach = table_cols * bs, 16-byte aligned) and are merged
  * by the last of two or three launches. Calls that may overlap on the GPU need a workspace each.
+ * Roundings: scores, references and sums are float32. bf16 pages: a weight enters the product with the
+ * values as two bf16 terms (2^-15 of it is lost); with a bf16 output and a prefix for more than 16 rows per
+ * KV head, there as one (2^-8). int8 pages: codes are exact, a weight times its value's scale is rounded to
+ * f16 (2^-11 of it, and 2^-31 of the row's largest such product times 127), and a query's elements lose
+ * what is below 2^-25 of the row's largest.
  */
 typedef struct {
   const void* q;

@@ -20,8 +20,8 @@
 // contiguous bytes of a row (a dot product does not mind, and the output's permutation ends in contiguous
 // runs again).
 //
-// bf16 pages: probabilities are rounded to bf16 for the second product (2^-8 relative at most, unbiased
-// over the keys). int8 pages: codes and queries are f16 (prefix_tile.cu tells how exactly), a key's scale
+// bf16 pages: a probability goes into the second product as two bf16 terms, itself rounded and the rest (2^-16 of
+// it is lost): twice the products at 0 to 3% of the time, since copies bound it. int8 pages: codes and queries are f16 (prefix_tile.cu tells how exactly), a key's scale
 // multiplies its column of scores in float32, and a value's scale its column of weights, before they are
 // rounded to f16, the only rounding of the second product's operands (prefix.cuh, weight_room: 2^-11 relative,
 // and an absolute 2^-31 of the largest weight times scale).
@@ -209,7 +209,7 @@ __device__ __forceinline__ void fold_values_singly(State<D>& st, const char* val
     const int c2 = (t & 7) >> 1, owner = (lane & ~3) | c2;  // the lane that holds this token's weights of rows r, r + 8
     const float x0 = t < 8 ? (t & 1 ? s[0][1] : s[0][0]) : (t & 1 ? s[1][1] : s[1][0]);
     const float x1 = t < 8 ? (t & 1 ? s[0][3] : s[0][2]) : (t & 1 ? s[1][3] : s[1][2]);
-    const float p0 = bf16_round(__shfl_sync(0xffffffffu, x0, owner)), p1 = bf16_round(__shfl_sync(0xffffffffu, x1, owner));
+    const float p0 = __shfl_sync(0xffffffffu, x0, owner), p1 = __shfl_sync(0xffffffffu, x1, owner);
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) {
       // Column n of output tile i is in what lane (n, c2) copied: load t % 2 + 2 (t / 8), and i / kVCh of it.
@@ -353,6 +353,12 @@ __device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D 
     auto packed = [](float x, float y) { return INT8 ? pack_f16(x, y) : pack_bf16(x, y); };
     const uint32_t a[4] = {packed(s[2 * g][0], s[2 * g][1]), packed(s[2 * g][2], s[2 * g][3]), packed(s[2 * g + 1][0], s[2 * g + 1][1]),
                            packed(s[2 * g + 1][2], s[2 * g + 1][3])};
+    [[maybe_unused]] uint32_t low[4];  // what the rounding left
+    if constexpr (!INT8) {
+      auto left = [](uint32_t hi, float x, float y) { return pack_bf16(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u)); };
+      low[0] = left(a[0], s[2 * g][0], s[2 * g][1]), low[1] = left(a[1], s[2 * g][2], s[2 * g][3]);
+      low[2] = left(a[2], s[2 * g + 1][0], s[2 * g + 1][1]), low[3] = left(a[3], s[2 * g + 1][2], s[2 * g + 1][3]);
+    }
 #pragma unroll
     for (int y = 0; y < S::kVLoads; ++y)
 #pragma unroll
@@ -368,8 +374,12 @@ __device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D 
           mma16816<true>(o[2], a, hi01.x, hi23.x);
           mma16816<true>(o[3], a, hi01.y, hi23.y);
         } else {
-          mma16816<false>(st.o[S::kVCh * y + 2 * i], a, __byte_perm(v[0][i], v[1][i], 0x5410), __byte_perm(v[2][i], v[3][i], 0x5410));
-          mma16816<false>(st.o[S::kVCh * y + 2 * i + 1], a, __byte_perm(v[0][i], v[1][i], 0x7632), __byte_perm(v[2][i], v[3][i], 0x7632));
+          const uint32_t even[2] = {__byte_perm(v[0][i], v[1][i], 0x5410), __byte_perm(v[2][i], v[3][i], 0x5410)};
+          const uint32_t odd[2] = {__byte_perm(v[0][i], v[1][i], 0x7632), __byte_perm(v[2][i], v[3][i], 0x7632)};
+          mma16816<false>(st.o[S::kVCh * y + 2 * i], a, even[0], even[1]);
+          mma16816<false>(st.o[S::kVCh * y + 2 * i + 1], a, odd[0], odd[1]);
+          mma16816<false>(st.o[S::kVCh * y + 2 * i], low, even[0], even[1]);
+          mma16816<false>(st.o[S::kVCh * y + 2 * i + 1], low, odd[0], odd[1]);
         }
       }
   }

@@ -595,6 +595,9 @@ def prefix_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tens
     bfloat16 by default, lse [batch, T, hq] float32); a row that attends nothing (no prefix, no own token,
     all pages missing) gets out = 0 and lse = -inf. lens and both tables are read on the device, so a
     captured graph follows them as they change; prefix_len and the shapes are fixed at capture.
+    Scores, references and sums are float32. Weights enter the product with the values rounded: int8 pages 2^-11 of
+    each (and 2^-31 of the row's largest weight times value); bfloat16 pages 2^-15 for a float32 output and up to 2^-8
+    for a bfloat16 one, whose prefix of more than 16 rows per KV head is then a quarter faster.
     The partials' workspace comes from torch's allocator call by call, so calls on several streams and
     several captured graphs do not share it.
     """

@@ -69,18 +69,21 @@ def near(cache: Cache, *rest) -> None:  # noqa: ANN002
 
 def near_pages(pages: torch.Tensor, scales: torch.Tensor | None, query: torch.Tensor, tables, lens, prefix_table, prefix: int, scale: float,
                out: torch.Tensor, lse: torch.Tensor, queries: slice = slice(None)) -> None:
-    """out (float32) and lse, of some of a step's queries, against `attend`. A score is a float32 sum of d products (two more roundings for the scales):
+    """out and lse, of some of a step's queries, against `attend`. A score is a float32 sum of d products (two more roundings for the scales):
     off by at most delta = (d + 4) 2^-24 reach, which moves a weight by a factor within e^(+-delta); exp2 is off by 2^-22 and
-    the sums over n keys by n 2^-24 at most. bf16 pages: a weight is rounded to bfloat16, 2^-8 of it. int8 pages: a weight
+    the sums over n keys by n 2^-24 at most. bf16 pages: a weight is rounded to bfloat16, 2^-8 of it, or, for a float32 output, has a second
+    term for what is left: 2^-7 of it at most, less 2^-8 of that. int8 pages: a weight
     times its value's scale is rounded to f16, 2^-11 of it or 2^-25 of a unit of which the row's largest such product has
-    2^6 at least; codes go up to 127, so n keys make that n 2^-31 top at most; four more float32 roundings."""
+    2^6 at least; codes go up to 127, so n keys make that n 2^-31 top at most; four more float32 roundings. A bfloat16 output is rounded once more, 2^-8 of it."""
     want, wlse, mass, reach, top = attend(query, pages, scales, tables, lens, prefix_table, prefix, scale)
     n = prefix + max(len(x) for x in tables) * pages.shape[3]
     sums = (query.shape[-1] + 4) * 2.0**-24 * reach + 2.0**-22 + n * 2.0**-24
+    fine = out.dtype == torch.float32
     if scales is not None:
-        bound = (2.0**-11 + 2 * sums[..., None] + 4 * 2.0**-24) * mass + n * 2.0**-31 * top[..., None] + 2.0**-23 * want.abs()
+        bound = (2.0**-11 + 2 * sums[..., None] + 4 * 2.0**-24) * mass + n * 2.0**-31 * top[..., None]
     else:
-        bound = (2.0**-8 + 2 * sums[..., None]) * mass + 2.0**-23 * want.abs()
+        bound = ((2.0**-15 if fine else 2.0**-8) + 2 * sums[..., None]) * mass
+    bound = bound + (2.0**-23 if fine else 2.0**-8 * (1 + 2.0**-7)) * want.abs() + (0 if fine else 2.0**-8 * bound)
     want, wlse, bound, sums, out, lse = (x[:, queries] for x in (want, wlse, bound, sums, out, lse))
     empty = wlse == -math.inf
     err, lerr = (out.double() - want).abs(), (lse.double() - wlse).abs()
@@ -222,8 +225,9 @@ def random_pages(gen: torch.Generator, n: int, h: int, bs: int, d: int, int8: bo
 
 @pytest.mark.parametrize("b,h,g,t", [(20, 148, 1, 1), (35, 148, 4, 1), (50, 74, 2, 3)], ids=["one row tile", "two row tiles", "several CTAs of rows"])
 @pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["to f32", "to bf16"])
 @pytest.mark.parametrize("d", [64, 128])
-def test_many_tiles_of_the_prefix_in_one_cta(d: int, int8: bool, b: int, h: int, g: int, t: int) -> None:
+def test_many_tiles_of_the_prefix_in_one_cta(d: int, dtype: torch.dtype, int8: bool, b: int, h: int, g: int, t: int) -> None:
     """A CTA of rows per SM: each takes the whole prefix, 22 tiles, past two turns of every ring it has. Scores grow and
     fall from tile to tile, so references move and outputs are rescaled; some pages are missing, two tiles have none at
     all, and the last tile is not full."""
@@ -243,7 +247,8 @@ def test_many_tiles_of_the_prefix_in_one_cta(d: int, int8: bool, b: int, h: int,
     lens = [(7 * i) % 64 for i in range(b)]
     query = (1.5 * torch.randn((b, t, h * g, d), generator=gen, device="cuda")).bfloat16()
     out, lse = K.prefix_attention(query, pages, torch.tensor(tables, dtype=torch.int32, device="cuda"), torch.tensor(lens, dtype=torch.int32, device="cuda"),
-                                  torch.tensor(prefix_table, dtype=torch.int32, device="cuda"), prefix, d**-0.5, scales=scales, out_dtype=torch.float32)
+                                  torch.tensor(prefix_table, dtype=torch.int32, device="cuda"), prefix, d**-0.5, scales=scales, out_dtype=dtype)
+    assert out.dtype == dtype
     near_pages(pages, scales, query, tables, lens, prefix_table, prefix, d**-0.5, out, lse)
     assert K.device_status() == 0
 
@@ -270,3 +275,20 @@ def test_more_stages_of_the_stream_than_its_warps_hold(d: int, int8: bool, prefi
                                   out_dtype=torch.float32)
     near_pages(pages, scales, query, table.tolist(), lens, ptab.tolist(), prefix, d**-0.5, out, lse)
     assert K.device_status() == 0
+
+
+@pytest.mark.parametrize("b,prefix", [(2, 1000), (40, 1000), (5, 0)], ids=["streamed", "tiled", "own tokens"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_float32_output_of_bf16_pages_has_the_bits_of_one(d: int, b: int, prefix: int) -> None:
+    """All values of a channel are alike, so that a weight's rounding shows in the output as it is and no mean over keys
+    hides it: 2^-15 of it and the float32 sums, where one bfloat16 term would leave up to 2^-8."""
+    from lazykv_b200 import kernels as K
+
+    gen = torch.Generator().manual_seed(d + b)
+    lens = [30 + i for i in range(b)]
+    cache, prefix_table, tables = build(gen, 2, d, 16, False, prefix, lens, fill=0.0)
+    cache.pages[:, :, 1] = torch.linspace(-3, 5, d).bfloat16()
+    pages, scales, ptab, table, n = on_gpu(cache, prefix_table, tables, lens)
+    query = (2 * torch.randn((b, 1, 4, d), generator=gen)).bfloat16()
+    out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, prefix, d**-0.5, out_dtype=torch.float32)
+    near(cache, query, tables, lens, prefix_table, prefix, d**-0.5, out, lse)

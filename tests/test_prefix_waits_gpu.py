@@ -15,9 +15,9 @@ pytestmark = pytest.mark.gpu
 
 @pytest.mark.parametrize("stall", [1, 2], ids=["queries", "weights"])
 @pytest.mark.parametrize("b,h,prefix", [(40, 2, 200), (150, 2, 700), (20, 150, 1500)], ids=["one row tile", "two row tiles", "many tiles a CTA"])
-@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("int8,dtype", [(False, torch.bfloat16), (False, torch.float32), (True, torch.bfloat16)], ids=["bf16", "bf16 to f32", "int8"])
 @pytest.mark.parametrize("d", [64, 128])
-def test_a_wait_that_runs_out_is_reported_and_poisons_only_that_call(d: int, int8: bool, b: int, h: int, prefix: int, stall: int) -> None:
+def test_a_wait_that_runs_out_is_reported_and_poisons_only_that_call(d: int, int8: bool, dtype: torch.dtype, b: int, h: int, prefix: int, stall: int) -> None:
     from lazykv_b200 import _lib
     from lazykv_b200 import kernels as K
 
@@ -29,7 +29,7 @@ def test_a_wait_that_runs_out_is_reported_and_poisons_only_that_call(d: int, int
     query = torch.randn((b, 1, 2 * h, d), generator=gen).bfloat16().cuda()
 
     def call() -> tuple[torch.Tensor, torch.Tensor]:
-        done = K.prefix_attention(query, pages, table, n, ptab, prefix, d**-0.5, scales=scales)
+        done = K.prefix_attention(query, pages, table, n, ptab, prefix, d**-0.5, scales=scales, out_dtype=dtype)
         torch.cuda.synchronize()
         return done
 
