@@ -153,6 +153,8 @@ def speculative_decode(model: PreTrainedModel, cache: Cache, draft_model: PreTra
             raise ValueError(f"speculative decoding takes rejected tokens back: {name} ({type(c).__name__}) has no truncate()")
     if n_draft < 1 or n_tokens < 0 or temperature <= 0:
         raise ValueError(f"n_draft {n_draft} is at least 1, n_tokens {n_tokens} at least 0, temperature {temperature} above 0")
+    if cache is draft_cache:
+        raise ValueError("the target and the draft need a cache each")
     if cache.get_seq_length() != draft_cache.get_seq_length():
         raise ValueError(f"the caches hold {cache.get_seq_length()} and {draft_cache.get_seq_length()} tokens")
     sizes = [m.get_input_embeddings().num_embeddings for m in (model, draft_model)] + [m.config.vocab_size for m in (model, draft_model)]

@@ -22,3 +22,13 @@ def test_tokens_that_one_of_the_models_does_not_know(target: int, draft: int, fi
     with pytest.raises(ValueError, match=message):
         speculative_decode(_model(target), caches[0], _model(draft), caches[1], first, 4, 2)
     assert all(c.get_seq_length() == 0 for c in caches)
+
+
+def test_one_cache_for_both_models() -> None:
+    from lazykv_b200.cache import FullGPUCache
+    from lazykv_b200.generate import speculative_decode
+
+    cache, model = FullGPUCache(1, 16), _model(32)
+    with pytest.raises(ValueError, match="a cache each"):
+        speculative_decode(model, cache, model, cache, 1, 4, 2)
+    assert cache.get_seq_length() == 0
