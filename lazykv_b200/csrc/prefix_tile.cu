@@ -354,9 +354,10 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       if (p.stall != 1 || warp != 0) warp_arrive(&s.q_full, lane);
     }
     float scale[4];
-#pragma unroll
     // (At least a number: a score of -infinity stays one under a softmax scale of zero.)
-    for (int i = 0; i < 4; ++i) scale[i] = (p.scale_log2 == 0.0f ? FLT_MIN : p.scale_log2 * sign) * (INT8 ? s.back[u][(warp % 4) * 32 + g + 8 * i] : 1.0f);  // this warp's own rows
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      scale[i] = p.scale_log2 == 0.0f ? FLT_MIN : p.scale_log2 * sign * (INT8 ? s.back[u][(warp % 4) * 32 + g + 8 * i] : 1.0f);  // this warp's own rows
     const uint32_t lanes = (uint32_t)(warp % 4) << 21;  // lane 32 (warp % 4) of tensor memory
     const uint32_t ts = tmem + lanes + u * kTile, to = tmem + lanes + 2 * kTile + u * D;
     const bool any_live = base - g < n_rows;  // does this warp hold a row at all

@@ -292,3 +292,17 @@ def test_a_float32_output_of_bf16_pages_has_the_bits_of_one(d: int, b: int, pref
     query = (2 * torch.randn((b, 1, 4, d), generator=gen)).bfloat16()
     out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, prefix, d**-0.5, out_dtype=torch.float32)
     near(cache, query, tables, lens, prefix_table, prefix, d**-0.5, out, lse)
+
+
+@pytest.mark.parametrize("b", [2, 40])
+def test_a_softmax_scale_of_zero_makes_any_queries_alike(b: int) -> None:
+    """int8 pages, queries of 2^120 and more: every seen key has the same weight."""
+    from lazykv_b200 import kernels as K
+
+    gen = torch.Generator().manual_seed(b)
+    lens = [5] * b
+    cache, prefix_table, tables = build(gen, 1, 64, 16, True, 200, lens)
+    pages, scales, ptab, table, n = on_gpu(cache, prefix_table, tables, lens)
+    query = (torch.randn((b, 1, 4, 64), generator=gen) * 2.0**122).bfloat16()
+    out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, 200, 0.0, scales=scales, out_dtype=torch.float32)
+    near(cache, query, tables, lens, prefix_table, 200, 0.0, out, lse)
