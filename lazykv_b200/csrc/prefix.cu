@@ -258,10 +258,13 @@ __device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D 
         const char* sp = slot + g * S::kGranBytes + (S::kKBytes + S::kVAll) * 32 + nt * 256 + lane * 8;
         const float2 ks = *reinterpret_cast<const float2*>(sp);
         vs[2 * g + nt] = *reinterpret_cast<const float2*>(sp + 512);
-        x[0] *= ks.x, x[1] *= ks.y, x[2] *= ks.x, x[3] *= ks.y;
-      }
+        // The scales' product first: a key's and a query row's may be as far apart as float32 goes.
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] *= scale[e >> 1];
+        for (int e = 0; e < 4; ++e) x[e] *= (e & 1 ? ks.y : ks.x) * scale[e >> 1];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] *= scale[e >> 1];
+      }
     }
   }
   if constexpr (MASKED) {

@@ -96,11 +96,12 @@ __device__ __forceinline__ uint2 biased_to_f16(uint32_t u) {
 __device__ __forceinline__ uint2 codes_to_f16(uint32_t w) { return biased_to_f16(w ^ 0x80808080u); }
 
 // For queries against int8 pages: the power of two 2^-e that brings a row's largest magnitude (its bf16
-// bits) to [1, 2), and 2^e, which its scores have to be multiplied with. Both are normal numbers; an
-// infinity or a NaN is what it is at any scale.
+// bits) to [1, 2), or below 2^16 where that is above 2^113, and 2^e, which its scores have to be multiplied
+// with. Both are normal numbers, times a power of two of the factors beside them too; an infinity or a NaN is
+// what it is at any scale.
 __device__ __forceinline__ float2 row_scales(uint32_t top_bits) {
   int e = (int)(top_bits >> 7) - 127;
-  e = e > 126 ? 126 : e < -126 ? -126 : e;
+  e = e > 112 ? 112 : e < -126 ? -126 : e;
   return make_float2(__int_as_float((127 - e) << 23), __int_as_float((127 + e) << 23));
 }
 

@@ -53,6 +53,10 @@ constexpr float kMostBf16 = 1048576.0f;  // 2^20
 // int8: a weight times its value's scale has to stay below 2^kMostF16. That is asked of the sum and the tile's
 // largest scale: where a token of little weight has that scale, references are looked up for nothing.
 constexpr int kMostF16 = 15;
+// int8: sums of codes times a query's f16 are below 2^15, and a key's scale may be 2^121: it is kept 2^9 smaller, and
+// the row's factor that much larger, so that no product passes float32's end. (A scale below 2^-117 loses bits: fourteen
+// are left at the least. The product of the two factors first would cost 3% of the time.)
+constexpr float kKeyDown = 1.0f / 512.0f, kKeyUp = 512.0f;
 
 template <int D, bool INT8>
 struct Tiles {
@@ -289,7 +293,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   char* q_tiles = smem;
   char* raws = q_tiles + (2 + T::kStages) * T::kBytes;
-  float* scale_ring = reinterpret_cast<float*>(raws + T::kRaw * T::kRawBytes);  // [kInfo][2][kTile]: keys', values' x kScaleDown
+  float* scale_ring = reinterpret_cast<float*>(raws + T::kRaw * T::kRawBytes);  // [kInfo][2][kTile]: keys' x kKeyDown, values' x kScaleDown
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int split = blockIdx.x, j = blockIdx.y, row0 = blockIdx.z * 2 * kTile;
   const int n_rows = min(2 * kTile, p.rows - row0);
@@ -349,15 +353,14 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
         src = p.q + (int64_t)(bt / p.tokens) * p.q_sb + (int64_t)(bt % p.tokens) * p.q_st + (int64_t)(j * p.group + gr) * p.q_sh;
       }
       const float back = stage_query<D, INT8>(src, q_tiles + (two ? u * T::kBytes : 0), r, two || u == 0, sign < 0.0f ? 0x80008000u : 0u);
-      if (INT8) s.back[u][r] = back;
+      if (INT8) s.back[u][r] = (p.scale_log2 == 0.0f ? 1.0f : back) * kKeyUp;
       fence_async();
       if (p.stall != 1 || warp != 0) warp_arrive(&s.q_full, lane);
     }
     float scale[4];
     // (At least a number: a score of -infinity stays one under a softmax scale of zero.)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      scale[i] = p.scale_log2 == 0.0f ? FLT_MIN : p.scale_log2 * sign * (INT8 ? s.back[u][(warp % 4) * 32 + g + 8 * i] : 1.0f);  // this warp's own rows
+    for (int i = 0; i < 4; ++i) scale[i] = (p.scale_log2 == 0.0f ? FLT_MIN : p.scale_log2 * sign) * (INT8 ? s.back[u][(warp % 4) * 32 + g + 8 * i] : 1.0f);  // its own warp's rows
     const uint32_t lanes = (uint32_t)(warp % 4) << 21;  // lane 32 (warp % 4) of tensor memory
     const uint32_t ts = tmem + lanes + u * kTile, to = tmem + lanes + 2 * kTile + u * D;
     const bool any_live = base - g < n_rows;  // does this warp hold a row at all
@@ -750,7 +753,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
         const int n = 2 * t + kv, raw = n % T::kRaw, slot = n % n_stages, info = t % kInfo;
         // The ring entry's last reader is more than two tiles behind (see the copies): it is free.
         float* ring = scale_ring + (info * 2 + kv) * kTile;
-        ring[i] = kv == 1 ? scale * kScaleDown : scale;
+        ring[i] = scale * (kv == 1 ? kScaleDown : kKeyDown);
         if (kv == 1) {
           const int top = __reduce_max_sync(0xffffffffu, scaled_top(scale * kScaleDown));
           if (lane == 0) s.top[info][warp - 16] = top;

@@ -306,3 +306,21 @@ def test_a_softmax_scale_of_zero_makes_any_queries_alike(b: int) -> None:
     query = (torch.randn((b, 1, 4, 64), generator=gen) * 2.0**122).bfloat16()
     out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, 200, 0.0, scales=scales, out_dtype=torch.float32)
     near(cache, query, tables, lens, prefix_table, 200, 0.0, out, lse)
+
+
+@pytest.mark.parametrize("up,queries", [(126, -126), (-108, 108), (-108, 122), (108, 4)])
+@pytest.mark.parametrize("b", [2, 40])
+def test_int8_keys_and_queries_far_apart(b: int, up: int, queries: int) -> None:
+    """Key scales times 2^up and queries times 2^queries under a softmax scale that makes ordinary scores of them: no
+    product of two of the three, nor with the codes, passes float32's end on the way."""
+    from lazykv_b200 import kernels as K
+
+    gen = torch.Generator().manual_seed(b)
+    lens = [5 + i % 7 for i in range(b)]
+    cache, prefix_table, tables = build(gen, 1, 64, 16, True, 200, lens, fill=0.0)
+    cache.scales[:, :, 0] = (cache.scales[:, :, 0].double() * 2.0**up).float()
+    pages, scales, ptab, table, n = on_gpu(cache, prefix_table, tables, lens)
+    query = (torch.randn((b, 1, 4, 64), generator=gen).double() * 2.0**queries).bfloat16()
+    scale = 0.125 * 2.0 ** -(up + queries)
+    out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, 200, scale, scales=scales, out_dtype=torch.float32)
+    near(cache, query, tables, lens, prefix_table, 200, scale, out, lse)
