@@ -14,12 +14,15 @@
 // int8 pages warps 12-15 turn codes of keys into f16 operands and warps 16-19 those of values. All of it is
 // joined by mbarriers, every wait bounded.
 //
-// Measured at 512 rows of a KV head on 32,768 tokens, d 128: int8 100 us, the tensor cores busy 33% of the time
-// and the exponentials' unit 40%; bf16 78 us, 43% and 50%. 128 sequences of 8 KV heads with 4 query heads each
-// on 131,072 int8 tokens, with their own tokens: 391 us, 0.71 PFLOP/s. What bounds it is the chain of one tile
+// Measured at 512 rows of each of 8 KV heads on 32,768 tokens, d 128: int8 105 us, the tensor cores busy 32% of the
+// time and the exponentials' unit 38%; bf16 78 us, 43% and 51%. 128 sequences of 8 KV heads with 4 query heads each
+// on 131,072 int8 tokens: 332 us, 0.83 PFLOP/s, and 402 to 413 us with up to 2,000 own tokens each, which the stream
+// takes behind the tiles (no CTA of it fits beside one of these). What bounds it is the chain of one tile
 // of rows, scores -> weights -> products -> next scores: S and P share 128 columns of tensor memory (two tiles
 // of S and O of d 128 fill it), so a tile's next scores wait for its present product, and two tiles do not
 // fill each other's gaps. Short prefixes add a start of 5 to 8 us (tensor memory, queries, the first pages).
+// Registers: the int8 forms store 72 bytes of a thread's to local memory and the two-term ones 172; the bf16
+// forms 4.
 //
 // bf16 pages: P and V are bf16; the pages come by tensor-map TMA straight into the swizzled operand layout (a
 // page that is missing as a row past the tensor's end, that is as zeros). For a float32 output P has two terms,
@@ -811,7 +814,8 @@ cudaError_t launch_tile(const Params& p, const CUtensorMap& map, int chunk, cuda
 }  // namespace
 
 // One CTA per SM: the number of splits whose waves of CTAs take the least time, a CTA's start and end
-// counted as two tiles of the prefix.
+// counted as two tiles of the prefix. (One or four in its place: the same times within 0.5% at 20 to 512 rows of 8
+// heads on 8,191 to 131,072 tokens.)
 int tile_splits(int rows, int h, int64_t prefix_len) {
   const int64_t tiles = (prefix_len + kTile - 1) / kTile, units = (int64_t)h * ((rows + 2 * kTile - 1) / (2 * kTile));
   int64_t best = 0, best_cost = 0;
