@@ -157,11 +157,12 @@ def speculative_decode(model: PreTrainedModel, cache: Cache, draft_model: PreTra
         raise ValueError("the target and the draft need a cache each")
     if cache.get_seq_length() != draft_cache.get_seq_length():
         raise ValueError(f"the caches hold {cache.get_seq_length()} and {draft_cache.get_seq_length()} tokens")
-    sizes = [m.get_input_embeddings().num_embeddings for m in (model, draft_model)] + [m.config.vocab_size for m in (model, draft_model)]
-    if len(set(sizes)) != 1:  # a token of one model has to be an index into the other's embedding
-        raise ValueError(f"the models' vocabularies differ: embeddings of {sizes[0]} and {sizes[1]}, logits of {sizes[2]} and {sizes[3]} tokens")
-    if not 0 <= first_token < sizes[0]:
-        raise ValueError(f"first_token {first_token} is outside the vocabulary of {sizes[0]}")
+    known = [m.get_input_embeddings().num_embeddings for m in (model, draft_model)]
+    drawn = [m.config.get_text_config().vocab_size for m in (model, draft_model)]
+    if drawn[0] != drawn[1] or min(known) < drawn[0]:  # a token of one model has to be an index into the other's embedding
+        raise ValueError(f"the models' vocabularies differ: embeddings of {known[0]} and {known[1]}, logits of {drawn[0]} and {drawn[1]} tokens")
+    if not 0 <= first_token < min(known):
+        raise ValueError(f"first_token {first_token} is outside the vocabulary of {min(known)}")
     from lazykv_b200 import kernels
 
     def probabilities(m: PreTrainedModel, c: Cache, tokens: torch.Tensor, keep: int) -> torch.Tensor:
