@@ -20,8 +20,8 @@
 // for the page's id and that for the table's row.
 //
 // Measured (8 heads, d 128, bf16 tokens, int8 pages): 12 x up to 16,000 tokens read back at 6.0 TB/s, 0.94 of a
-// plain copy (989 MB, 163 us): memory bounds it. 65,536 tokens of a prompt written at 3.7 TB/s, 0.57 of a copy
-// (407 MB, 110 us): quantising bounds it, 74% of the issue slots. A token of each of 64 sequences written and
+// plain copy (989 MB, 163 us): memory bounds it. 65,536 tokens of a prompt written at 4.0 TB/s, 0.61 of a copy
+// (407 MB, 103 us): quantising bounds it, 74% of the issue slots (model-type pages: 6.6 TB/s). A token of each of 64 sequences written and
 // read back: 5.9 us, two launches of three dependent loads each.
 #include <float.h>
 
