@@ -633,7 +633,8 @@ int lkv_paged_read(const lkv_paged_args* args, void* stream);
  * values as two bf16 terms (2^-15 of it is lost); with a bf16 output and a prefix for more than 16 rows per
  * KV head, there as one (2^-8). int8 pages: codes are exact, a weight times its value's scale is rounded to
  * f16 (2^-11 of it, and 2^-31 of the row's largest such product times 127), and a query's elements lose
- * what is below 2^-25 of the row's largest.
+ * what is below 2^-25 of the row's largest. Sums of weights times values are float32 before they are divided,
+ * with weights of up to 2^20: bf16 values above 2^107 / keys may pass its end; int8 pages of any scale do not.
  */
 typedef struct {
   const void* q;

@@ -20,10 +20,10 @@
 // contiguous bytes of a row (a dot product does not mind, and the output's permutation ends in contiguous
 // runs again).
 //
-// bf16 pages: a probability goes into the second product as two bf16 terms, itself rounded and the rest (2^-16 of
-// it is lost): twice the products at 0 to 3% of the time, since copies bound it. int8 pages: codes and queries are f16 (prefix_tile.cu tells how exactly), a key's scale
-// multiplies its column of scores in float32, and a value's scale its column of weights, before they are
-// rounded to f16, the only rounding of the second product's operands (prefix.cuh, weight_room: 2^-11 relative,
+// bf16 pages: a weight goes into the second product as two bf16 terms (prefix.cuh, rest_of: 2^-15 of it is
+// lost): twice the products at 0 to 3% of the time, since copies bound it. int8 pages: codes and queries are f16
+// (prefix_tile.cu tells how exactly), a key's scale multiplies its column of scores in float32, and a value's scale
+// its column of weights, before they are rounded to f16, the only rounding of the second product's operands (prefix.cuh, weight_room: 2^-11 relative,
 // and an absolute 2^-31 of the largest weight times scale).
 //
 // Measured: 6 sequences on 32,768 bf16 tokens, 16 KV heads, d 128: 276 MB in 63 us, 4.4 TB/s; each further
@@ -354,14 +354,14 @@ __device__ __forceinline__ void fold_stage(State<D>& st, const uint32_t (&qf)[D 
         continue;
       }
     }
-    auto packed = [](float x, float y) { return INT8 ? pack_f16(x, y) : pack_bf16(x, y); };
+    auto packed = [](float x, float y) { return INT8 ? pack_f16(x, y) : upper_halves(x, y); };
     const uint32_t a[4] = {packed(s[2 * g][0], s[2 * g][1]), packed(s[2 * g][2], s[2 * g][3]), packed(s[2 * g + 1][0], s[2 * g + 1][1]),
                            packed(s[2 * g + 1][2], s[2 * g + 1][3])};
-    [[maybe_unused]] uint32_t low[4];  // what the rounding left
+    [[maybe_unused]] uint32_t low[4];  // the second terms
     if constexpr (!INT8) {
-      auto left = [](uint32_t hi, float x, float y) { return pack_bf16(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u)); };
-      low[0] = left(a[0], s[2 * g][0], s[2 * g][1]), low[1] = left(a[1], s[2 * g][2], s[2 * g][3]);
-      low[2] = left(a[2], s[2 * g + 1][0], s[2 * g + 1][1]), low[3] = left(a[3], s[2 * g + 1][2], s[2 * g + 1][3]);
+      auto rest = [](float x, float y) { return pack_bf16(rest_of(x), rest_of(y)); };
+      low[0] = rest(s[2 * g][0], s[2 * g][1]), low[1] = rest(s[2 * g][2], s[2 * g][3]);
+      low[2] = rest(s[2 * g + 1][0], s[2 * g + 1][1]), low[3] = rest(s[2 * g + 1][2], s[2 * g + 1][3]);
     }
 #pragma unroll
     for (int y = 0; y < S::kVLoads; ++y)

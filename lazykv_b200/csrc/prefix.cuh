@@ -80,6 +80,13 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&b);
 }
+// A weight of bf16 pages in two bf16 terms: its upper half, and the rest and 2^-20 of it more, so that a weight's
+// second term is never zero either (0 x infinity would make a NaN of an infinite value). Less than 2^-7 of the
+// weight is left to the second term, whose rounding loses 2^-8 of that. Here for two weights at a time.
+constexpr float kAndMore = 1.0f + 1.0f / 1048576.0f;
+__device__ __forceinline__ uint32_t upper_halves(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
+__device__ __forceinline__ float rest_of(float x) { return fmaf(x, kAndMore, -__uint_as_float(__float_as_uint(x) & 0xffff0000u)); }
+
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 b = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&b);

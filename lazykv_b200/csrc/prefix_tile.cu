@@ -25,8 +25,8 @@
 // forms 4.
 //
 // bf16 pages: P and V are bf16; the pages come by tensor-map TMA straight into the swizzled operand layout (a
-// page that is missing as a row past the tensor's end, that is as zeros). For a float32 output P has two terms,
-// the weight's upper half and the rest (2^-15 of it is lost), each multiplied by V. For a bfloat16 output, which
+// page that is missing as a row past the tensor's end, that is as zeros). For a float32 output P has two terms
+// (prefix.cuh, rest_of: 2^-15 of a weight is lost), each multiplied by V. For a bfloat16 output, which
 // is rounded itself, it has one (2^-8 at most): the second costs a third of the time (512 rows of each of 8 heads
 // on 32,768 tokens, d 128: 85 and 111 us), and without it such an output's mean error is 1.4 times the rounding's.
 // int8 pages: codes are exact in f16, and so is a query row after a power of two that brings its largest
@@ -487,9 +487,9 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
                 uint32_t& to = w[n][r / 2][2 * k + (r & 1)];
                 if constexpr (!FINE) {
                   to = INT8 ? pack_f16(first_of(z), second_of(z)) : pack_bf16(first_of(z), second_of(z));
-                } else {  // the upper halves of both, and what is left of them
-                  to = __byte_perm((uint32_t)z, (uint32_t)(z >> 32), 0x7632);
-                  z = add2(z, (z & 0xffff0000ffff0000ull) ^ 0x8000000080000000ull);
+                } else {  // as upper_halves and rest_of
+                  to = upper_halves(first_of(z), second_of(z));
+                  z = fma2(z, pair(kAndMore, kAndMore), (z & 0xffff0000ffff0000ull) ^ 0x8000000080000000ull);
                   low[n][r / 2][2 * k + (r & 1)] = pack_bf16(first_of(z), second_of(z));
                 }
               }

@@ -324,3 +324,31 @@ def test_int8_keys_and_queries_far_apart(b: int, up: int, queries: int) -> None:
     scale = 0.125 * 2.0 ** -(up + queries)
     out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, 200, scale, scales=scales, out_dtype=torch.float32)
     near(cache, query, tables, lens, prefix_table, 200, scale, out, lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["to f32", "to bf16"])
+@pytest.mark.parametrize("b,prefix,at", [(2, 0, 5), (2, 0, 70), (2, 1000, 17), (2, 1000, 999), (40, 1000, 17), (40, 1000, 999), (150, 300, 40)])
+def test_an_infinite_value_that_is_seen_makes_an_infinite_output(b: int, prefix: int, at: int, dtype: torch.dtype) -> None:
+    """bf16 pages, one value infinite, of an ordinary weight: its channel is infinite with its sign, as in the definition,
+    and the other channels are what they are without it. Values with few bits and equal scores make terms of zero likely."""
+    from lazykv_b200 import kernels as K
+
+    d, bs, n_own = 64, 16, 80
+    gen = torch.Generator().manual_seed(at)
+    cache, prefix_table, tables = build(gen, 1, d, bs, False, prefix, [n_own] * b)
+    cache.pages[:, :, 0] = 0.0  # every score is zero, every weight the same power of two
+    for table in [prefix_table] if prefix else tables:
+        cache.pages[table[at // bs], 0, 1, at % bs, 3] = math.inf
+        cache.pages[table[at // bs], 0, 1, at % bs, 40] = -math.inf
+    query = torch.randn((b, 1, 4, d), generator=gen).bfloat16()
+    for spread in (0.0, 0.3):
+        if spread:
+            cache.pages[:, :, 0] = (spread * torch.randn(cache.pages[:, :, 0].shape, generator=gen)).bfloat16()
+        pages, scales, ptab, table, n = on_gpu(cache, prefix_table, tables, [n_own] * b)
+        out, lse = K.prefix_attention(query.cuda(), pages, table, n, ptab, prefix, d**-0.5, out_dtype=dtype)
+        assert bool((out[..., 3] == math.inf).all()) and bool((out[..., 40] == -math.inf).all())
+        plain = Cache(1, 1, bs, d, False)
+        plain.pages = cache.pages.clone()
+        plain.pages[:, :, 1, :, [3, 40]] = 0.0
+        out[..., [3, 40]] = 0.0
+        near(plain, query, tables, [n_own] * b, prefix_table, prefix, d**-0.5, out, lse)
