@@ -619,6 +619,81 @@ int lkv_paged_write(const lkv_paged_args* args, void* stream);
 int lkv_paged_read(const lkv_paged_args* args, void* stream);
 
 /*
+ * A step's new tokens from the projections into the pages (no reference counterpart: the reference's models
+ * rotate in the host framework). The tokens come packed: rows [rows, heads, d] (element strides of token and
+ * head, channels contiguous, dtype float32 or bfloat16), sequence b's at offsets[b] .. offsets[b + 1] - 1 (int32,
+ * ascending), the last of its lens[b] tokens: row r goes to position lens[b] - offsets[b + 1] + r of its pages. A
+ * head's row x of q and of keys becomes weight x / sqrt(mean(x^2) + eps) where a weight [d] (dtype) is given, and
+ * then its pair i < pairs of channels, (i, i + pairs) or, interleaved, (2 i, 2 i + 1), turns by positions[r] x
+ * frequencies[i] radians. q goes to out (any strides; it may be q itself), keys and values to the pages as
+ * lkv_paged_write puts them. A row of no sequence is left alone; one without a page has its q only.
+ * bfloat16 rows are computed in float32, float32 rows in float64, angles in float64; each element of out and of
+ * model-dtype pages is rounded once, codes are made of the float32 values. d 64 or 128, pairs a multiple of 4.
+ */
+typedef struct {
+  const void* q;
+  const void* keys;
+  const void* values;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  void* out;
+  int64_t o_st, o_sh;
+  int dtype, rows, hq, h, d;
+  const int32_t* positions;
+  const float* frequencies;
+  int pairs, interleaved;
+  const void* q_weight;
+  const void* k_weight;
+  float eps;
+  void* pages;
+  int kind;
+  float* scales;
+  int64_t n_pages;
+  int bs;
+  const int32_t* table;
+  int64_t table_ld;
+  int table_cols;
+  const int32_t* lens;
+  const int32_t* offsets;
+  int batch;
+} lkv_rotate_args;
+int lkv_paged_write_rotated(const lkv_rotate_args* args, void* stream);
+
+/*
+ * A budget for the sequences' own tokens (no reference counterpart: the reference's tiers move blocks, and
+ * drop none). Of each sequence's lens[b] tokens (slots of its pages) every KV head keeps `keep`: those whose
+ * positions are below `sinks` or at or above since[b] (optional) before all others, then those of the highest
+ * sums (NaN last), ties to the lowest slot. Kept tokens in slots below `keep` stay; the i-th one behind them
+ * moves to the i-th such slot whose token is not kept, with its scales, sum and position. sums (float32) and
+ * positions (int32) are [batch, h, cap], cap at least what lens says; out_sums and out_positions get their new
+ * contents (0 and -1 in the slots behind) and may be sums and positions themselves; out_lens [batch] gets
+ * min(lens[b], keep). Sequences of up to `keep` tokens keep them all. dtype is that of model-dtype pages.
+ * Workspace: lkv_paged_evict_workspace bytes, 8-byte aligned, any contents.
+ */
+typedef struct {
+  void* pages;
+  int kind, dtype;
+  float* scales;
+  int64_t n_pages;
+  int h, bs, d, batch;
+  const int32_t* table;
+  int64_t table_ld;
+  int table_cols;
+  const int32_t* lens;
+  const float* sums;
+  const int32_t* positions;
+  int cap;
+  float* out_sums;
+  int32_t* out_positions;
+  int32_t* out_lens;
+  int keep, sinks;
+  const int32_t* since;
+  void* workspace;
+  size_t workspace_bytes;
+} lkv_evict_args;
+size_t lkv_paged_evict_workspace(int batch, int h, int cap, int keep);
+int lkv_paged_evict(const lkv_evict_args* args, void* stream);
+
+/*
  * Attention of a batch whose sequences share a prefix (no reference counterpart). Query t of sequence b
  * (q [batch, tokens, hq, d] bfloat16, element strides, 16-byte aligned rows) attends the prefix's
  * prefix_len tokens, whose pages prefix_table lists, and the first lens[b] - tokens + t + 1 of its

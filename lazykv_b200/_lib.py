@@ -88,6 +88,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lkv_prefix_attention_workspace": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int64, c_int, c_int64]),
     "lkv_prefix_attention": (c_int, [c_void_p, c_void_p]),
     "lkv_verify_drafts": (c_int, [c_void_p, c_void_p]),
+    "lkv_paged_write_rotated": (c_int, [c_void_p, c_void_p]),
+    "lkv_paged_evict_workspace": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "lkv_paged_evict": (c_int, [c_void_p, c_void_p]),
     "lkv_ragged_stage_records": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p,
                                          c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
 }
@@ -125,6 +128,8 @@ class SplitStepArgs(ctypes.Structure):
 # same order), packed in native alignment: a third of the time of a ctypes.Structure or of as many arguments.
 PAGED_ARGS = struct.Struct("@PPqqqqqqiiiiiPiPqiPqiPPPP")
 PREFIX_ARGS = struct.Struct("@PiqqqPiPqiiiiiiPqiPPiqfPiPPN")
+ROTATE_ARGS = struct.Struct("@PPPqqqqqqPqqiiiiiPPiiPPfPiPqiPqiPPi")
+EVICT_ARGS = struct.Struct("@PiiPqiiiiPqiPPPiPPPiiPPN")
 VERIFY_ARGS = struct.Struct("@PqqPqqPqPqiiiPP")
 
 

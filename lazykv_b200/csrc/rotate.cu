@@ -1,0 +1,339 @@
+// A step's queries and keys, normalised per head and rotated to their positions, and the keys and values
+// written into their pages, in one pass over the projections' outputs.
+//
+// A head's row x of d channels becomes y = w x / sqrt(mean(x^2) + eps) where weights are given, and pair p
+// of its channels (a, b), for p < pairs, turns by the angle t = position x frequencies[p]:
+//   a cos t - b sin t,  b cos t + a sin t.
+// Pairs are (p, p + pairs) or, interleaved, (2 p, 2 p + 1); channels from 2 pairs on do not turn. Queries are
+// rounded once, to the model's type; keys and values go to model-dtype pages rounded once, or to int8
+// codes as paged.cu quantises them, from the float32 values.
+//
+// What is rounded where: bfloat16 rows are computed in float32, float32 rows in float64, since a code is
+// decided by the side of a border that its value lies on. The angle is a float64 product, brought below half
+// a turn in float64 before its sine and cosine are taken: at position 10^6 a float32 angle is off by 0.03.
+//
+// Bytes bound it: each row is read once and written once. A group of d / 8 lanes carries a row, a lane four
+// channels of the first elements of pairs and the four of their second ones, so that a rotation needs no other
+// lane. A CTA computes the angles of its tokens once for all heads.
+#include "paged.cuh"
+
+namespace lkv {
+namespace {
+
+using namespace paged;
+
+constexpr int kThreads = 256;
+constexpr int kMostTokens = 4;  // tokens of a CTA of a long call
+
+struct RotateParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  void* out;
+  int64_t o_st, o_sh;
+  int rows, hq, h;
+  const int32_t* positions;
+  const float* frequencies;
+  int pairs, interleaved;
+  const void* q_weight;
+  const void* k_weight;
+  float eps;
+  void* pages;
+  float* scales;
+  int64_t n_pages;
+  int page_shift;
+  const int32_t* table;
+  int64_t table_ld;
+  int table_cols;
+  const int32_t* lens;
+  const int32_t* offsets;
+  int batch;
+  int token_shift;  // log2 of the tokens per CTA
+};
+
+template <typename T>
+struct Wide {
+  using type = float;
+};
+template <>
+struct Wide<float> {
+  using type = double;
+};
+
+// Four consecutive elements.
+template <typename T>
+struct Four;
+template <>
+struct Four<__nv_bfloat16> {
+  uint2 w;
+};
+template <>
+struct Four<float> {
+  float4 w;
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ Four<T> load4(const T* p) {
+  Four<T> f;
+  if constexpr (VEC) {
+    f.w = *reinterpret_cast<const decltype(f.w)*>(p);
+  } else if constexpr (sizeof(T) == 2) {
+    const uint16_t* b = reinterpret_cast<const uint16_t*>(p);
+    f.w = make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
+  } else {
+    f.w = make_float4(p[0], p[1], p[2], p[3]);
+  }
+  return f;
+}
+template <typename W>
+__device__ __forceinline__ void widen(const Four<__nv_bfloat16>& f, W* x) {
+  x[0] = __uint_as_float(f.w.x << 16), x[1] = __uint_as_float(f.w.x & 0xffff0000u);
+  x[2] = __uint_as_float(f.w.y << 16), x[3] = __uint_as_float(f.w.y & 0xffff0000u);
+}
+template <typename W>
+__device__ __forceinline__ void widen(const Four<float>& f, W* x) {
+  x[0] = f.w.x, x[1] = f.w.y, x[2] = f.w.z, x[3] = f.w.w;
+}
+template <bool VEC>
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float* x) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+  if constexpr (VEC) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  } else {
+    p[0] = a.x, p[1] = a.y, p[2] = b.x, p[3] = b.y;
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void store4(float* p, const float* x) {
+  if constexpr (VEC) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = x[i];
+  }
+}
+
+// Cosine and sine of position x frequency. 2 pi in two parts: the whole turns' product is exact enough in two
+// fused steps for any int32 position.
+__device__ __forceinline__ void turn_of(int position, float frequency, float* c, float* s) {
+  const double a = (double)position * (double)frequency, n = rint(a * 0.15915494309189535);
+  double r = fma(-n, 6.283185307179586, a);
+  r = fma(-n, 2.4492935982947064e-16, r);
+  sincospif((float)(r * 0.3183098861837907), s, c);
+}
+__device__ __forceinline__ void turn_of(int position, float frequency, double* c, double* s) {
+  const double a = (double)position * (double)frequency, n = rint(a * 0.15915494309189535);
+  double r = fma(-n, 6.283185307179586, a);
+  r = fma(-n, 2.4492935982947064e-16, r);
+  sincospi(r * 0.3183098861837907, s, c);
+}
+__device__ __forceinline__ float inverse_root(float x) { return 1.0f / sqrtf(x); }
+__device__ __forceinline__ double inverse_root(double x) { return 1.0 / sqrt(x); }
+
+template <typename T, int D, bool INT8, bool VEC>
+__global__ void __launch_bounds__(kThreads) rotate_kernel(const RotateParams p) {
+  using W = typename Wide<T>::type;
+  constexpr int L = D / 8, kGroups = kThreads / L, U = sizeof(T) == 2 ? 4 : 2;  // rows that a group has in flight
+  __shared__ W turns[2][kMostTokens][D / 2];  // cosines, sines
+  __shared__ int64_t where[kMostTokens];      // row 0 of the token's place in its page; -1: no page; -2: no sequence's token
+  pdl_wait();
+  pdl_release();
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, tokens = 1 << p.token_shift, row0 = blockIdx.x << p.token_shift;
+  const int bs = 1 << p.page_shift;
+
+  // A group's token, its heads, and a lane's pairs: 4 l .. 4 l + 3, at channels c0 .. and c1 ..
+  const int per = kGroups >> p.token_shift, group = tid / L, l = tid % L, t = group / per, sub = group % per, row = row0 + t;
+  const uint32_t mask = L == 32 ? 0xffffffffu : ((1u << L) - 1) << (lane / L * L);
+  int c0 = 8 * l, c1 = c0 + 4;
+  if (!p.interleaved) {
+    const int pr = 4 * l;
+    c0 = pr < p.pairs ? pr : pr + p.pairs;
+    c1 = pr < p.pairs ? pr + p.pairs : pr + D / 2;
+  }
+  Four<T> lo[U], hi[U];
+  const T* q = static_cast<const T*>(p.q) + (int64_t)row * p.q_st;
+  auto fetch = [&](int j0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * per;
+      if (row < p.rows && j < p.hq) lo[u] = load4<T, VEC>(q + j * p.q_sh + c0), hi[u] = load4<T, VEC>(q + j * p.q_sh + c1);
+    }
+  };
+  fetch(sub);
+
+  if (warp >= 8 - tokens) {  // the last warps find the tokens' places
+    const int mine = 7 - warp, r = row0 + mine;
+    int b = 0;
+    for (int i = lane; i < p.batch; i += 32) b += r < p.rows && p.offsets[i + 1] <= r;
+    b = __reduce_add_sync(0xffffffffu, b);
+    if (lane == 0) {
+      int64_t at = -2;
+      if (r < p.rows && b < p.batch) {
+        const int from = p.offsets[b], end = p.offsets[b + 1];
+        if (from <= r && r < end) {
+          at = -1;
+          const int64_t pos = (int64_t)p.lens[b] - end + r, col = pos >> p.page_shift;
+          if (pos >= 0 && col < p.table_cols) {
+            const int64_t page = p.table[(int64_t)b * p.table_ld + col];
+            if (page >= 0 && page < p.n_pages) at = page * p.h * 2 * bs + (pos & (bs - 1));
+          }
+        }
+      }
+      where[mine] = at;
+    }
+  }
+  for (int i = tid; i < tokens * (D / 2); i += kThreads) {
+    const int tt = i / (D / 2), pr = i % (D / 2);
+    W c = 1, s = 0;
+    if (row0 + tt < p.rows && pr < p.pairs) turn_of(p.positions[row0 + tt], p.frequencies[pr], &c, &s);
+    turns[0][tt][pr] = c, turns[1][tt][pr] = s;
+  }
+  __syncthreads();
+  const int64_t place = where[t];
+  if (place == -2) return;
+  W cs[4], sn[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) cs[i] = turns[0][t][4 * l + i], sn[i] = turns[1][t][4 * l + i];
+
+  // x: a lane's channels c0 .. and c1 .., normalised (weights w) and turned.
+  auto turn = [&](W* x, const W* w, bool norm) {
+    if (norm) {
+      W sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
+      const W inv = inverse_root(sum * (W)(1.0 / D) + (W)p.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= inv * w[i];
+    }
+    if (4 * l >= p.pairs) return;  // (a turn by nothing would still make a NaN of an infinite neighbour)
+    if (p.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const W a = x[2 * i], b = x[2 * i + 1];
+        x[2 * i] = a * cs[i] - b * sn[i], x[2 * i + 1] = b * cs[i] + a * sn[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const W a = x[i], b = x[4 + i];
+        x[i] = a * cs[i] - b * sn[i], x[4 + i] = b * cs[i] + a * sn[i];
+      }
+    }
+  };
+  auto weights = [&](const void* from, W* w) {
+    if (from == nullptr) return;
+    widen(load4<T, VEC>(static_cast<const T*>(from) + c0), w);
+    widen(load4<T, VEC>(static_cast<const T*>(from) + c1), w + 4);
+  };
+
+  W w[8];
+  weights(p.q_weight, w);
+  T* out = static_cast<T*>(p.out) + (int64_t)row * p.o_st;
+  for (int j0 = sub; j0 < p.hq; j0 += U * per) {
+    if (j0 != sub) fetch(j0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * per;
+      if (j >= p.hq) break;
+      W x[8];
+      widen(lo[u], x), widen(hi[u], x + 4);
+      turn(x, w, p.q_weight != nullptr);
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = (float)x[i];
+      store4<VEC>(out + j * p.o_sh + c0, y);
+      store4<VEC>(out + j * p.o_sh + c1, y + 4);
+    }
+  }
+  if (place < 0) return;
+
+  weights(p.k_weight, w);
+  const T* k = static_cast<const T*>(p.k) + (int64_t)row * p.k_st;
+  const T* v = static_cast<const T*>(p.v) + (int64_t)row * p.v_st;
+  for (int j = sub; j < 2 * p.h; j += per) {  // the keys of all heads, then their values
+    const int kv = j >= p.h, head = j - kv * p.h;
+    const T* src = kv ? v + head * p.v_sh : k + head * p.k_sh;
+    W x[8];
+    widen(load4<T, VEC>(src + c0), x), widen(load4<T, VEC>(src + c1), x + 4);
+    if (!kv) turn(x, w, p.k_weight != nullptr);
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = (float)x[i];
+    const int64_t to = place + ((int64_t)head * 2 + kv) * bs;
+    if constexpr (INT8) {
+      uint32_t top = 0, codes[2];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+      const float s = scale_of(top);
+      quantise<8>(y, s, codes);
+      int8_t* dst = static_cast<int8_t*>(p.pages) + to * D;
+      *reinterpret_cast<uint32_t*>(dst + c0) = codes[0];
+      *reinterpret_cast<uint32_t*>(dst + c1) = codes[1];
+      if (l == 0) p.scales[to] = s;
+    } else {
+      T* dst = static_cast<T*>(p.pages) + to * D;
+      store4<true>(dst + c0, y);
+      store4<true>(dst + c1, y + 4);
+    }
+  }
+}
+
+template <typename T, int D>
+cudaError_t launch(const RotateParams& p, bool int8, bool vec, cudaStream_t st) {
+  const unsigned grid = (unsigned)(((int64_t)p.rows + (1 << p.token_shift) - 1) >> p.token_shift);
+  if (int8) return vec ? launch_pdl(rotate_kernel<T, D, true, true>, dim3(grid), dim3(kThreads), 0, st, 0, p)
+                       : launch_pdl(rotate_kernel<T, D, true, false>, dim3(grid), dim3(kThreads), 0, st, 0, p);
+  return vec ? launch_pdl(rotate_kernel<T, D, false, true>, dim3(grid), dim3(kThreads), 0, st, 0, p)
+             : launch_pdl(rotate_kernel<T, D, false, false>, dim3(grid), dim3(kThreads), 0, st, 0, p);
+}
+
+}  // namespace
+}  // namespace lkv
+
+using namespace lkv;
+
+extern "C" int lkv_paged_write_rotated(const lkv_rotate_args* a, void* stream) {
+  static const char* who = "lkv_paged_write_rotated";
+  if (a == nullptr) return fail(LKV_ERR_PTR, "%s: null arguments", who);
+  if (int rc = check_cache(who, a->kind, a->dtype, a->h, a->bs, a->d, a->n_pages, a->pages, a->scales)) return rc;
+  if (a->rows < 0 || a->rows > (1 << 30) || a->hq < 0 || a->batch < 0 || a->table_cols < 0 || (a->batch > 1 && a->table_ld < a->table_cols) || a->hq > 65536 || a->h > 65536)
+    return fail(LKV_ERR_ARG, "%s: bad shape (rows %d, heads %d and %d, batch %d, table of %d columns)", who, a->rows, a->hq, a->h, a->batch, a->table_cols);
+  if (a->pairs < 0 || a->pairs > a->d / 2 || a->pairs % 4 != 0) return fail(LKV_ERR_ARG, "%s: %d rotated pairs of head_dim %d (a multiple of 4)", who, a->pairs, a->d);
+  if (!(a->eps >= 0.0f)) return fail(LKV_ERR_ARG, "%s: eps %g", who, (double)a->eps);
+  if (a->rows == 0 || a->batch == 0) return LKV_OK;
+  if (a->keys == nullptr || a->values == nullptr || a->lens == nullptr || a->offsets == nullptr || (a->table == nullptr && a->table_cols > 0) ||
+      (a->hq > 0 && (a->q == nullptr || a->out == nullptr)) || (a->pairs > 0 && (a->positions == nullptr || a->frequencies == nullptr)))
+    return fail(LKV_ERR_PTR, "%s: null pointer", who);
+  const int size = (int)dtype_size(a->dtype);
+  const void* all[6] = {a->q, a->keys, a->values, a->out, a->q_weight, a->k_weight};
+  bool vec = ((a->q_st | a->q_sh | a->k_st | a->k_sh | a->v_st | a->v_sh | a->o_st | a->o_sh) & 3) == 0;
+  for (const void* x : all) {
+    if (!aligned(x, size)) return fail(LKV_ERR_PTR, "%s: misaligned rows or weights", who);
+    vec = vec && aligned(x, 4 * size);
+  }
+  RotateParams p = {};
+  p.q = a->q, p.k = a->keys, p.v = a->values;
+  p.q_st = a->q_st, p.q_sh = a->q_sh, p.k_st = a->k_st, p.k_sh = a->k_sh, p.v_st = a->v_st, p.v_sh = a->v_sh;
+  p.out = a->out, p.o_st = a->o_st, p.o_sh = a->o_sh;
+  p.rows = a->rows, p.hq = a->hq, p.h = a->h;
+  p.positions = a->positions, p.frequencies = a->frequencies, p.pairs = a->pairs, p.interleaved = a->interleaved != 0;
+  p.q_weight = a->q_weight, p.k_weight = a->k_weight, p.eps = a->eps;
+  p.pages = a->pages, p.scales = a->scales, p.n_pages = a->n_pages, p.page_shift = shift_of(a->bs);
+  p.table = a->table, p.table_ld = a->table_ld, p.table_cols = a->table_cols, p.lens = a->lens, p.offsets = a->offsets, p.batch = a->batch;
+  // One token to a CTA until every SM has four CTAs.
+  p.token_shift = a->rows <= 4 * kNumSMs ? 0 : 2;
+  const bool int8 = a->kind == LKV_CACHE_INT8;
+  cudaStream_t st = as_stream(stream);
+  cudaError_t e;
+  if (a->dtype == LKV_BF16)
+    e = a->d == 64 ? launch<__nv_bfloat16, 64>(p, int8, vec, st) : launch<__nv_bfloat16, 128>(p, int8, vec, st);
+  else
+    e = a->d == 64 ? launch<float, 64>(p, int8, vec, st) : launch<float, 128>(p, int8, vec, st);
+  if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+  return LKV_OK;
+}

@@ -577,6 +577,102 @@ def paged_read(pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, n
     return out
 
 
+def _packed(who: str, name: str, t: torch.Tensor, rows: int, d: int, dtype: torch.dtype) -> tuple[int, int, int]:
+    """(heads, token stride, head stride) of packed rows [rows, heads, d] with contiguous channels."""
+    if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != d or t.dtype is not dtype or t.stride(2) != 1:
+        raise ValueError(f"{who}: {name} must be {dtype} [{rows}, heads, {d}] with contiguous channels, got {t.dtype} {tuple(t.shape)}")
+    return t.shape[1], t.stride(0), t.stride(1)
+
+
+def paged_write_rotated(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, pages: torch.Tensor,
+                        table: torch.Tensor, lens: torch.Tensor, offsets: torch.Tensor, scales: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
+                        k_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """New tokens from a layer's projections into the cache, one launch (lkv_paged_write_rotated): query [rows, hq, d]
+    and keys [rows, h, d] are normalised per head (where q_weight / k_weight [d] are given: weight x / rms) and
+    rotated to positions [rows] (int32), keys and values [rows, h, d] written into the pages as paged_write does.
+    Returns the rotated query (in `out`, which may be `query` itself).
+
+    Tokens are packed: sequence b's are rows offsets[b] .. offsets[b + 1] - 1 (offsets int32 [batch + 1]) and go to the
+    last places of its lens[b] (int32 [batch]). Rows of no sequence are left alone (in a new `out`: not set), so a batch
+    may be padded. Pair i of the len(frequencies) (float32, a multiple of 4, at most d / 2) turns by position x
+    frequencies[i]: channels (i, i + len) or, interleaved, (2 i, 2 i + 1); the others do not turn. positions are the
+    rotation's only, not the place in the pages.
+    """
+    who = "paged_write_rotated"
+    index = _one_device(who, query, keys, values, positions, frequencies, pages, table, lens, offsets, scales, q_weight, k_weight, out)
+    n, h, bs, d, kind, at, batch, ld, cols = _cache_geometry(who, pages, scales, table)
+    dtype, rows = keys.dtype, keys.shape[0]
+    code = 1 if dtype is _BF16 else dtype_code(dtype)
+    kh, k_st, k_sh = _packed(who, "keys", keys, rows, d, dtype)
+    vh, v_st, v_sh = _packed(who, "values", values, rows, d, dtype)
+    hq, q_st, q_sh = _packed(who, "query", query, rows, d, dtype)
+    if kh != h or vh != h or (kind == 0 and pages.dtype is not dtype):
+        raise ValueError(f"{who}: {dtype} keys of {kh} heads and values of {vh} do not fit pages {tuple(pages.shape)} {pages.dtype}")
+    if positions.dtype is not _I32 or positions.shape != (rows,) or not positions.is_contiguous():
+        raise ValueError(f"{who}: positions must be a contiguous int32 [{rows}]")
+    pairs = frequencies.numel()
+    if frequencies.dtype is not _F32 or frequencies.dim() != 1 or not frequencies.is_contiguous() or pairs % 4 or 2 * pairs > d:
+        raise ValueError(f"{who}: frequencies must be a contiguous float32 [n], n a multiple of 4 and at most {d // 2}, got {frequencies.dtype} {tuple(frequencies.shape)}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.dtype is not dtype or w.shape != (d,) or not w.is_contiguous()):
+            raise ValueError(f"{who}: {name} must be a contiguous {dtype} [{d}], got {w.dtype} {tuple(w.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"{who}: eps {eps}")
+    _per_sequence(who, "lens", lens, batch)
+    _per_sequence(who, "offsets", offsets, batch + 1)
+    if out is None:
+        out = query.new_empty((rows, hq, d))
+    oh, o_st, o_sh = _packed(who, "out", out, rows, d, dtype)
+    if oh != hq:
+        raise ValueError(f"{who}: out of {oh} heads for a query of {hq}")
+    _run("lkv_paged_write_rotated", L.ROTATE_ARGS.pack(
+        query.data_ptr(), keys.data_ptr(), values.data_ptr(), q_st, q_sh, k_st, k_sh, v_st, v_sh, out.data_ptr(), o_st, o_sh, code, rows, hq, h, d,
+        positions.data_ptr(), frequencies.data_ptr(), pairs, int(interleaved), 0 if q_weight is None else q_weight.data_ptr(),
+        0 if k_weight is None else k_weight.data_ptr(), eps, pages.data_ptr(), kind, at, n, bs, table.data_ptr(), ld, cols, lens.data_ptr(), offsets.data_ptr(), batch), index)
+    return out
+
+
+def paged_evict(pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, sums: torch.Tensor, positions: torch.Tensor, keep: int,
+                since: torch.Tensor | None = None, sinks: int = 0, scales: torch.Tensor | None = None,
+                out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Cuts each sequence's own tokens down to `keep` per KV head, one launch (lkv_paged_evict): the tokens at positions
+    below `sinks` or from since[b] (int32 [batch]) on first, then those of the highest sums, ties to the lowest slot.
+
+    lens [batch] counts the tokens in the pages' slots, sums [batch, h, cap] float32 are their weights (attention_sums) and
+    positions [batch, h, cap] int32 what they were rotated to: heads keep different tokens. Kept tokens behind slot
+    keep - 1 move into the slots of dropped ones, in place, with their scales, so slots are no longer in the order of
+    the positions; attention does not need one, as long as new tokens follow in slots of their own. Returns (min(lens,
+    keep), sums, positions): the last two new, or in `out`, which may be sums and positions themselves; 0 and -1 stand in
+    slots without a token. A token without a page is ranked like the others and not moved.
+    """
+    who = "paged_evict"
+    index = _one_device(who, pages, table, lens, sums, positions, since, scales)
+    n, h, bs, d, kind, at, batch, ld, cols = _cache_geometry(who, pages, scales, table)
+    _per_sequence(who, "lens", lens, batch)
+    if since is not None:
+        _per_sequence(who, "since", since, batch)
+    if sums.dtype is not _F32 or sums.dim() != 3 or sums.shape[:2] != (batch, h) or not sums.is_contiguous():
+        raise ValueError(f"{who}: sums must be a contiguous float32 [{batch}, {h}, slots], got {sums.dtype} {tuple(sums.shape)}")
+    if positions.dtype is not _I32 or positions.shape != sums.shape or not positions.is_contiguous():
+        raise ValueError(f"{who}: positions must be a contiguous int32 {tuple(sums.shape)}, got {positions.dtype} {tuple(positions.shape)}")
+    cap = sums.shape[2]
+    if keep < 1:
+        raise ValueError(f"{who}: a budget of {keep} tokens")
+    code = 0 if kind == 1 else dtype_code(pages.dtype)
+    if out is None:
+        out = torch.empty_like(sums), torch.empty_like(positions)
+    for o, like in zip(out, (sums, positions)):
+        if o.dtype is not like.dtype or o.shape != like.shape or not o.is_contiguous() or o.get_device() != index:
+            raise ValueError(f"{who}: out must be like sums and positions, {tuple(sums.shape)} on cuda:{index}")
+    left = torch.empty_like(lens)
+    nbytes = batch * h * min(keep, cap - keep) * 8 if cap > keep else 0
+    ws = lens.new_empty(nbytes // 4) if nbytes else None
+    _run("lkv_paged_evict", L.EVICT_ARGS.pack(
+        pages.data_ptr(), kind, code, at, n, h, bs, d, batch, table.data_ptr(), ld, cols, lens.data_ptr(), sums.data_ptr(), positions.data_ptr(), cap,
+        out[0].data_ptr(), out[1].data_ptr(), left.data_ptr(), keep, sinks, 0 if since is None else since.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes), index)
+    return left, out[0], out[1]
+
+
 @functools.lru_cache(maxsize=4096)
 def _prefix_workspace(batch: int, tokens: int, hq: int, h: int, d: int, prefix_len: int, kind: int, reach: int) -> int:
     return int(L.lib().lkv_prefix_attention_workspace(batch, tokens, hq, h, d, prefix_len, kind, reach))
