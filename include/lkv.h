@@ -517,14 +517,17 @@ int lkv_status_poll(int* status, int clear);
  * its peers. LKV_DEBUG_PREFIX_WAIT_NS sets the bound (nanoseconds, 1 .. 2 x 10^9) of the waits of
  * lkv_prefix_attention's tiled prefix; LKV_DEBUG_PREFIX_STALL_NEXT makes a warp of every CTA of the next
  * call with a tiled prefix withhold its arrival for the queries (1) or for the weights (2), so that the
- * waits run out: status 1, and NaN in every row. Not for production use; not thread-safe.
+ * waits run out: status 1, and NaN in every row. LKV_DEBUG_CHUNK_WAIT_NS and LKV_DEBUG_CHUNK_STALL_NEXT do the same for
+ * lkv_chunk_attention. Not for production use; not thread-safe.
  */
 enum {
   LKV_DEBUG_SELECT_WAIT_ITERS = 1,
   LKV_DEBUG_SELECT_STALL_NEXT = 2,
   LKV_DEBUG_EXCHANGE_WAIT_ITERS = 3,
   LKV_DEBUG_PREFIX_WAIT_NS = 4,
-  LKV_DEBUG_PREFIX_STALL_NEXT = 5
+  LKV_DEBUG_PREFIX_STALL_NEXT = 5,
+  LKV_DEBUG_CHUNK_WAIT_NS = 6,
+  LKV_DEBUG_CHUNK_STALL_NEXT = 7
 };
 int lkv_debug_set(int key, int64_t value);
 
@@ -737,6 +740,50 @@ typedef struct {
 } lkv_prefix_args;
 size_t lkv_prefix_attention_workspace(int batch, int tokens, int hq, int h, int d, int64_t prefix_len, int kind, int64_t own_reach);
 int lkv_prefix_attention(const lkv_prefix_args* args, void* stream);
+
+/*
+ * Attention of chunks of new tokens (no reference counterpart: the reference prefills through the host framework's
+ * attention, one sequence at a time). The queries come packed as lkv_paged_write_rotated's rows: q [rows, hq, d]
+ * bfloat16 (element strides, 16-byte aligned rows), sequence b's n at offsets[b] .. offsets[b + 1] - 1, the last of its
+ * lens[b] own tokens, in the pages already. Query i attends the prefix's prefix_len tokens, whose pages prefix_table
+ * lists, and the first lens[b] - n + i + 1 own tokens, in any order of the slots before the chunk; a token without a page
+ * is not attended. Scores are scale q k or, with cap > 0, cap tanh(scale q k / cap). out [rows, hq, d] bfloat16 and lse
+ * [rows, hq] float32, both contiguous; a row that attends nothing gets out = 0, lse = -inf; rows of no sequence are
+ * left alone. lens, offsets and the tables are read on the device. Two launches; the workspace
+ * (lkv_chunk_attention_workspace bytes with own_reach = table_cols * bs, 16-byte aligned, any contents) belongs to
+ * one call at a time. batch <= 8192, rows * hq / h <= 2^30, n_pages * 2 * h * bs < 2^31.
+ * Roundings: scores, references and sums are float32; a weight, times its value's scale of int8 pages, is rounded to
+ * bf16 (2^-8). Sums of weights times values are float32 before they are divided, with weights of up to 2^20: values above
+ * 2^107 / keys may pass its end. An infinite value that is seen makes an infinite output (NaN where the weight is 0 in float32).
+ * The kernels' waits are bounded (lkv_device_status 1: rows hold NaN or were not written).
+ */
+typedef struct {
+  const void* q;
+  int64_t q_st, q_sh;
+  int dtype; /* of q and of model-dtype pages: LKV_BF16 */
+  int rows, hq, h, d;
+  void* pages;
+  int kind;
+  const float* scales;
+  int64_t n_pages;
+  int bs;
+  const int32_t* table;
+  int64_t table_ld;
+  int table_cols;
+  const int32_t* lens;
+  const int32_t* offsets;
+  int batch;
+  const int32_t* prefix_table;
+  int prefix_cols;
+  int64_t prefix_len;
+  float scale, cap;
+  void* out;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+} lkv_chunk_args;
+size_t lkv_chunk_attention_workspace(int rows, int batch, int hq, int h, int d, int64_t prefix_len, int64_t own_reach);
+int lkv_chunk_attention(const lkv_chunk_args* args, void* stream);
 
 /*
  * Verification of k drafted tokens per sequence (no reference counterpart; the reference decodes one

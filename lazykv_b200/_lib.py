@@ -22,6 +22,7 @@ LKV_ORDER_BOUND, LKV_ORDER_BLOCK = 0, 1
 LKV_CACHE_MODEL, LKV_CACHE_INT8 = 0, 1
 LKV_DEBUG_SELECT_WAIT_ITERS, LKV_DEBUG_SELECT_STALL_NEXT, LKV_DEBUG_EXCHANGE_WAIT_ITERS = 1, 2, 3
 LKV_DEBUG_PREFIX_WAIT_NS, LKV_DEBUG_PREFIX_STALL_NEXT = 4, 5
+LKV_DEBUG_CHUNK_WAIT_NS, LKV_DEBUG_CHUNK_STALL_NEXT = 6, 7
 LKV_DEV_WAIT_TIMEOUT, LKV_DEV_LIST_OVERFLOW = 1, 2
 
 _lib: ctypes.CDLL | None = None
@@ -89,6 +90,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lkv_prefix_attention": (c_int, [c_void_p, c_void_p]),
     "lkv_verify_drafts": (c_int, [c_void_p, c_void_p]),
     "lkv_paged_write_rotated": (c_int, [c_void_p, c_void_p]),
+    "lkv_chunk_attention_workspace": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int64, c_int64]),
+    "lkv_chunk_attention": (c_int, [c_void_p, c_void_p]),
     "lkv_paged_evict_workspace": (c_size_t, [c_int, c_int, c_int, c_int]),
     "lkv_paged_evict": (c_int, [c_void_p, c_void_p]),
     "lkv_ragged_stage_records": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p,
@@ -129,6 +132,7 @@ class SplitStepArgs(ctypes.Structure):
 PAGED_ARGS = struct.Struct("@PPqqqqqqiiiiiPiPqiPqiPPPP")
 PREFIX_ARGS = struct.Struct("@PiqqqPiPqiiiiiiPqiPPiqfPiPPN")
 ROTATE_ARGS = struct.Struct("@PPPqqqqqqPqqiiiiiPPiiPPfPiPqiPqiPPi")
+CHUNK_ARGS = struct.Struct("@PqqiiiiiPiPqiPqiPPiPiqffPPPN")
 EVICT_ARGS = struct.Struct("@PiiPqiiiiPqiPPPiPPPiiPPN")
 VERIFY_ARGS = struct.Struct("@PqqPqqPqPqiiiPP")
 

@@ -37,6 +37,11 @@ namespace prefix {
 int set_tile_wait(int64_t ns);
 int set_tile_stall(int64_t which);
 }
+// The same of chunk.cu's kernels.
+cudaError_t chunk_device_status(int* status, int clear);
+cudaError_t chunk_status_attach(int* mirror);
+int chunk_set_wait(int64_t ns);
+int chunk_set_stall(int64_t which);
 // The exchange's status word (exchange.cu), its host mirror, and the bound of its wait.
 cudaError_t exchange_device_status(int* status, int clear);
 cudaError_t exchange_status_attach(int* mirror);

@@ -1187,6 +1187,10 @@ int lkv_debug_set(int key, int64_t value) {
       return prefix::set_tile_wait(value);
     case LKV_DEBUG_PREFIX_STALL_NEXT:
       return prefix::set_tile_stall(value);
+    case LKV_DEBUG_CHUNK_WAIT_NS:
+      return chunk_set_wait(value);
+    case LKV_DEBUG_CHUNK_STALL_NEXT:
+      return chunk_set_stall(value);
     default:
       return fail(LKV_ERR_ARG, "lkv_debug_set: unknown key %d", key);
   }

@@ -736,6 +736,63 @@ def prefix_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tens
     return out, lse
 
 
+@functools.lru_cache(maxsize=4096)
+def _chunk_workspace(rows: int, batch: int, hq: int, h: int, d: int, prefix_len: int, reach: int) -> int:
+    return int(L.lib().lkv_chunk_attention_workspace(rows, batch, hq, h, d, prefix_len, reach))
+
+
+def chunk_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, offsets: torch.Tensor, scale: float,
+                    scales: torch.Tensor | None = None, prefix_table: torch.Tensor | None = None, prefix_len: int = 0, cap: float = 0.0,
+                    out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention of chunks of new tokens, of any length per sequence, over the paged cache (lkv_chunk_attention, two
+    launches): query [rows, hq, d] bfloat16 is packed, sequence b's at rows offsets[b] .. offsets[b + 1] - 1 (int32
+    [batch + 1]), the last of its lens[b] own tokens, which are in the pages already (paged_write_rotated). Each query
+    attends the prefix_len tokens of the pages that prefix_table lists, and its sequence's own tokens up to itself; scores
+    are scale q k or, with a cap, cap tanh(scale q k / cap).
+
+    pages are bfloat16 or int8 with scales. Returns (out [rows, hq, d] bfloat16, lse [rows, hq] float32). A row that attends
+    nothing gets out = 0 and lse = -inf; rows of no sequence are left alone (in new tensors: not set), so a batch may be
+    padded, and sequences may have no new tokens. lens, offsets and the tables are read on the device, so a captured graph
+    follows them as they change; the shapes and prefix_len are fixed at capture. Scores and sums are float32, weights are
+    rounded to bfloat16 (2^-8) where they multiply the values. The workspace comes from torch's allocator call by call.
+    """
+    who = "chunk_attention"
+    index = _one_device(who, query, pages, table, lens, offsets, scales, prefix_table, out, lse)
+    n, h, bs, d, kind, at, batch, ld, cols = _cache_geometry(who, pages, scales, table)
+    if query.dim() != 3 or query.dtype is not _BF16 or query.shape[2] != d or query.shape[1] < 1 or query.shape[1] % h or (kind == 0 and pages.dtype is not _BF16):
+        raise ValueError(f"{who}: query must be bfloat16 [rows, heads, {d}], heads a multiple of {h}, over bfloat16 or int8 pages; got {query.dtype} "
+                         f"{tuple(query.shape)}, {pages.dtype} pages {tuple(pages.shape)}")
+    rows, hq, _ = query.shape
+    _per_sequence(who, "lens", lens, batch)
+    _per_sequence(who, "offsets", offsets, batch + 1)
+    pcols = 0
+    if prefix_table is not None:
+        pcols = prefix_table.numel()
+        if prefix_table.dtype is not _I32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous():
+            raise ValueError(f"{who}: prefix_table must be a contiguous int32 [columns]")
+    if not 0 <= prefix_len <= pcols * bs:
+        raise ValueError(f"{who}: prefix_table of {pcols} pages of {bs} cannot hold {prefix_len} tokens")
+    if not 0 <= cap < math.inf:
+        raise ValueError(f"{who}: cap {cap}")
+    st, sh, sc = query.stride()
+    if sc != 1 or (st | sh) & 7 or query.data_ptr() & 15:
+        query = query.clone(memory_format=torch.contiguous_format)
+        st, sh, _ = query.stride()
+    for name, o, shape, dtype in (("out", out, (rows, hq, d), _BF16), ("lse", lse, (rows, hq), _F32)):
+        if o is not None and (o.shape != shape or o.dtype is not dtype or not o.is_contiguous()):
+            raise ValueError(f"{who}: {name} must be a contiguous {dtype} {shape}, got {o.dtype} {tuple(o.shape)}")
+    if out is None:
+        out = query.new_empty((rows, hq, d))
+    if lse is None:
+        lse = query.new_empty((rows, hq), dtype=_F32)
+    nbytes = _chunk_workspace(rows, batch, hq, h, d, prefix_len, cols * bs)
+    ws = query.new_empty((nbytes + 1) // 2) if nbytes else None
+    _run("lkv_chunk_attention", L.CHUNK_ARGS.pack(
+        query.data_ptr(), st, sh, 1, rows, hq, h, d, pages.data_ptr(), kind, at, n, bs, table.data_ptr(), ld, cols, lens.data_ptr(), offsets.data_ptr(), batch,
+        0 if prefix_table is None else prefix_table.data_ptr(), pcols, prefix_len, scale, cap, out.data_ptr(), lse.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes), index)
+    return out, lse
+
+
 def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torch.Tensor, uniforms: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Which of k drafted tokens per sequence are kept, and the token that follows them (one launch,
     lkv_verify_drafts). target [batch, k + 1, vocab] and draft [batch, k, vocab] are float32
