@@ -786,6 +786,40 @@ size_t lkv_chunk_attention_workspace(int rows, int batch, int hq, int h, int d, 
 int lkv_chunk_attention(const lkv_chunk_args* args, void* stream);
 
 /*
+ * The weight that each own token of the sequences got from the queries of their new chunks (no reference
+ * counterpart): out[b, j, s] = sums[b, j, s] + the sum over the last `last` query tokens i of sequence b's chunk and the
+ * query heads g of KV head j, as far as they see token s, of exp(score - lse[row, g]). q, offsets, lens, the pages, scale
+ * and cap_scores (the scores' cap) are as lkv_chunk_attention's and lse [rows, hq] what it returned, a prefix's part in
+ * it included. sums (float32 [batch, h, cap], optional: zeros; it may be out) holds for the tokens in front of the chunk;
+ * those of the chunk start from 0, slots without a token get 0, a token whose page is missing keeps its sum. A row with
+ * lse = -inf has no weights. One launch, no workspace, no atomics: the same sums every time. Limits and bounded waits as
+ * lkv_chunk_attention's (a token whose wait ran out gets NaN).
+ */
+typedef struct {
+  const void* q;
+  int64_t q_st, q_sh;
+  int dtype; /* of q and of model-dtype pages: LKV_BF16 */
+  int rows, hq, h, d;
+  const float* lse;
+  void* pages;
+  int kind;
+  const float* scales;
+  int64_t n_pages;
+  int bs;
+  const int32_t* table;
+  int64_t table_ld;
+  int table_cols;
+  const int32_t* lens;
+  const int32_t* offsets;
+  int batch, last;
+  const float* sums;
+  float* out;
+  int cap;
+  float scale, cap_scores;
+} lkv_sums_args;
+int lkv_attention_sums(const lkv_sums_args* args, void* stream);
+
+/*
  * Verification of k drafted tokens per sequence (no reference counterpart; the reference decodes one
  * token at a time, lazykv/generate.py:134-154). target [batch, k + 1, vocab] and draft [batch, k,
  * vocab] float32 probabilities (element strides, rows contiguous; draft null: the drafted token was

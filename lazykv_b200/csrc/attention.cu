@@ -2293,14 +2293,16 @@ int lkv_ragged_exact_attention(const void* q, int rows, int g, int d, int bs, in
 
 int lkv_device_status(int* status, int clear) {
   if (status == nullptr) return fail(LKV_ERR_PTR, "lkv_device_status: null pointer");
-  int a = 0, b = 0, c = 0, f = 0, g = 0;
-  cudaError_t e = tu_device_status(&a, clear);
-  if (e == cudaSuccess) e = select_device_status(&b, clear);
-  if (e == cudaSuccess) e = exchange_device_status(&c, clear);
-  if (e == cudaSuccess) e = prefix_device_status(&f, clear);
-  if (e == cudaSuccess) e = chunk_device_status(&g, clear);
+  // Every translation unit with waits has a word of its own; the first that is set counts.
+  int found = 0;
+  cudaError_t e = cudaSuccess;
+  for (auto read : {tu_device_status, select_device_status, exchange_device_status, prefix_device_status, chunk_device_status, sums_device_status}) {
+    int one = 0;
+    if (e == cudaSuccess) e = read(&one, clear);
+    if (found == 0) found = one;
+  }
   if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "lkv_device_status: %s", cudaGetErrorString(e));
-  *status = a != 0 ? a : (b != 0 ? b : (c != 0 ? c : (f != 0 ? f : g)));
+  *status = found;
   return LKV_OK;
 }
 
@@ -2324,6 +2326,7 @@ int lkv_status_attach(void) {
   if (e == cudaSuccess) e = exchange_status_attach(dev_word);
   if (e == cudaSuccess) e = prefix_status_attach(dev_word);
   if (e == cudaSuccess) e = chunk_status_attach(dev_word);
+  if (e == cudaSuccess) e = sums_status_attach(dev_word);
   if (e != cudaSuccess) return fail(LKV_ERR_CUDA, "lkv_status_attach: %s", cudaGetErrorString(e));
   return LKV_OK;
 }

@@ -37,7 +37,9 @@ namespace prefix {
 int set_tile_wait(int64_t ns);
 int set_tile_stall(int64_t which);
 }
-// The same of chunk.cu's kernels.
+// The same of sums.cu's and chunk.cu's kernels.
+cudaError_t sums_device_status(int* status, int clear);
+cudaError_t sums_status_attach(int* mirror);
 cudaError_t chunk_device_status(int* status, int clear);
 cudaError_t chunk_status_attach(int* mirror);
 int chunk_set_wait(int64_t ns);

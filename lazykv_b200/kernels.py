@@ -793,6 +793,49 @@ def chunk_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tenso
     return out, lse
 
 
+def attention_sums(query: torch.Tensor, lse: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, offsets: torch.Tensor, scale: float,
+                   sums: torch.Tensor | None = None, last: int | None = None, cap: float = 0.0, scales: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """The attention weight that every own token got from the queries of the chunks, added to `sums` (lkv_attention_sums, one
+    launch): [batch, h, slots] float32, slots = columns * block size without sums or out. query, offsets, lens, scale and cap
+    are those of chunk_attention, lse [rows, hq] what it (or prefix_attention) returned. With `last`, only the last so many
+    query tokens of each chunk count. What paged_evict ranks tokens by.
+
+    sums [batch, h, slots] are those of earlier steps (None: zeros) for the tokens in front of the chunk; the chunk's own
+    start from 0, and slots without a token are 0. The result is new or in `out`, which may be sums itself. Sums are
+    float32 in the order of the queries, the same every time.
+    """
+    who = "attention_sums"
+    index = _one_device(who, query, lse, pages, table, lens, offsets, sums, scales, out)
+    n, h, bs, d, kind, at, batch, ld, cols = _cache_geometry(who, pages, scales, table)
+    if query.dim() != 3 or query.dtype is not _BF16 or query.shape[2] != d or query.shape[1] < 1 or query.shape[1] % h or (kind == 0 and pages.dtype is not _BF16):
+        raise ValueError(f"{who}: query must be bfloat16 [rows, heads, {d}], heads a multiple of {h}, over bfloat16 or int8 pages; got {query.dtype} "
+                         f"{tuple(query.shape)}, {pages.dtype} pages {tuple(pages.shape)}")
+    rows, hq, _ = query.shape
+    if lse.dtype is not _F32 or lse.shape != (rows, hq) or not lse.is_contiguous():
+        raise ValueError(f"{who}: lse must be a contiguous float32 [{rows}, {hq}], got {lse.dtype} {tuple(lse.shape)}")
+    _per_sequence(who, "lens", lens, batch)
+    _per_sequence(who, "offsets", offsets, batch + 1)
+    slots = cols * bs if sums is None and out is None else (out if sums is None else sums).shape[-1]
+    for name, t in (("sums", sums), ("out", out)):
+        if t is not None and (t.dtype is not _F32 or t.shape != (batch, h, slots) or not t.is_contiguous()):
+            raise ValueError(f"{who}: {name} must be a contiguous float32 [{batch}, {h}, {slots}], got {t.dtype} {tuple(t.shape)}")
+    if last is not None and last < 1:
+        raise ValueError(f"{who}: the last {last} tokens of a chunk")
+    if not 0 <= cap < math.inf:
+        raise ValueError(f"{who}: cap {cap}")
+    st, sh, sc = query.stride()
+    if sc != 1 or (st | sh) & 7 or query.data_ptr() & 15:
+        query = query.clone(memory_format=torch.contiguous_format)
+        st, sh, _ = query.stride()
+    if out is None:
+        out = query.new_empty((batch, h, slots), dtype=_F32)
+    _run("lkv_attention_sums", L.SUMS_ARGS.pack(
+        query.data_ptr(), st, sh, 1, rows, hq, h, d, lse.data_ptr(), pages.data_ptr(), kind, at, n, bs, table.data_ptr(), ld, cols, lens.data_ptr(), offsets.data_ptr(), batch,
+        2**31 - 1 if last is None else min(last, 2**31 - 1), 0 if sums is None else sums.data_ptr(), out.data_ptr(), slots, scale, cap), index)
+    return out
+
+
 def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torch.Tensor, uniforms: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Which of k drafted tokens per sequence are kept, and the token that follows them (one launch,
     lkv_verify_drafts). target [batch, k + 1, vocab] and draft [batch, k, vocab] are float32
