@@ -50,7 +50,7 @@ using prefix::pack_bf16;
 constexpr int kBlock = 2 * kTile;  // rows of a unit
 constexpr int kInfo = 8;           // tiles whose scales and page bits are kept (see the copies)
 constexpr int kRing = 4;           // units that are handed out ahead
-constexpr int kClean = 4;          // cleaned tiles ahead of their product
+constexpr int kClean = 8;          // tiles to be cleaned or cleaned ahead of their product: more than the stages hold
 constexpr int kPad = 1;            // a unit's start and end count as this many tiles more on the line
 constexpr int kMinShare = 2;       // tiles of the line that a CTA takes at least
 constexpr int kMostBatch = 8192;
@@ -83,6 +83,16 @@ struct ChunkParams {
   int stall;  // test hook: warp 0 withholds an arrival
 };
 
+// A place in a ring of n entries, with the parity of its present round.
+struct Cursor {
+  int slot;
+  uint32_t phase;
+  __device__ __forceinline__ void step(int by, int n) {
+    slot += by;
+    if (slot >= n) slot -= n, phase ^= 1;
+  }
+};
+
 // A piece of a unit.
 struct Unit {
   int b, j;          // sequence, KV head; b < 0: the end
@@ -109,12 +119,12 @@ struct Tiles {
   static constexpr int kScaleBytes = INT8 ? kInfo * 2 * kTile * 4 : 0;
   static constexpr int kSmem = 2 * kBytes + kStages * kBytes + kRaw * kRawBytes + kScaleBytes + 1024;
   static constexpr int kReaders = INT8 ? 18 : 11;       // warps that read a unit: weights, products, copies, and cleaning or converters
-  static_assert(kStages * kBytes >= kMostBatch * 12, "the plan fits the stages");
+  static_assert((2 + kStages) * kBytes >= kMostBatch * 12, "the plan fits the tiles");
 };
 
 struct Barriers {
   uint64_t q_full, o_full[2], s_full[2], p_full[2], drain, other_full, other_empty;
-  uint64_t full[8], empty[8], raw_full[3], raw_empty[3], info[kInfo], dirty[kClean], clean[kClean], unit_full[kRing], unit_empty[kRing];
+  uint64_t full[9], empty[9], raw_full[3], raw_empty[3], info[kInfo], dirty[kClean], clean[kClean], unit_full[kRing], unit_empty[kRing];
   uint32_t have[kInfo][4];  // together, bit g: tokens 16 g .. 16 g + 15 of the tile have a page
   Unit unit[kRing];
   int bad[kRing];           // values that are not finite were taken out of a tile of this unit
@@ -184,13 +194,11 @@ __device__ __forceinline__ bool not_finite(uint32_t two) {
 template <int D, bool INT8, bool CAP>
 __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(const ChunkParams p, const __grid_constant__ CUtensorMap pages_map) {
   using T = Tiles<D, INT8>;
-  constexpr int kStages = T::kStages;
   extern __shared__ char raw_smem[];
   __shared__ Barriers s;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   char* q_tiles = smem;
-  char* stages = q_tiles + 2 * T::kBytes;
-  char* raws = stages + kStages * T::kBytes;
+  char* raws = q_tiles + (2 + T::kStages) * T::kBytes;
   float* scale_ring = reinterpret_cast<float*>(raws + T::kRaw * T::kRawBytes);  // [kInfo][2][kTile]: keys', values'
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int n_prefix = prefix_tiles(p), bs = 1 << p.page_shift;
@@ -204,7 +212,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.p_full[i], 4);
     }
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i <= T::kStages; ++i) {
       mbar_init(&s.full[i], INT8 ? 4 : 1);
       mbar_init(&s.empty[i], 1);
     }
@@ -237,12 +245,14 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
   pdl_wait();
   pdl_release();
 
-  // Every sequence's length on the line, per KV head, into the stages (no copy is under way yet): short chunks by
-  // a thread, long ones by all.
-  int64_t* lengths = reinterpret_cast<int64_t*>(stages);
+  // Every sequence's length on the line, per KV head, into shared memory that nothing else uses yet: short chunks
+  // by a thread, long ones by all.
+  int64_t* lengths = reinterpret_cast<int64_t*>(smem);
+  int two_tiles = 0;  // has some unit two tiles of rows
   int* longs = reinterpret_cast<int*>(lengths + kMostBatch);
   for (int b = tid; b < p.batch; b += T::kThreads) {
     const Sequence q = sequence_of(p, b);
+    two_tiles |= (int64_t)q.n * p.group > kTile;
     int64_t sum = 0;
     if (q.blocks <= 8) {
       for (int i = 0; i < q.blocks; ++i) sum += tiles_of(p, i, q.n, q.base, q.reach) + kPad;
@@ -251,7 +261,10 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
     }
     lengths[b] = sum;
   }
-  __syncthreads();
+  two_tiles = __syncthreads_or(two_tiles);
+  // The second tile of queries is one stage more where no unit has one.
+  const int n_stages = T::kStages + (two_tiles ? 0 : 1);
+  char* stages = q_tiles + (two_tiles ? 2 : 1) * T::kBytes;
   for (int k = 0; k < s.n_long; ++k) {
     const int b = longs[k];
     const Sequence q = sequence_of(p, b);
@@ -569,7 +582,8 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
     // ---- matrix products: issued by one lane, in order -----------------------------------------------
     constexpr uint32_t kQk = instruction<false>(kTile, false), kPv = instruction<false>(D, true);
     const uint32_t q_u = smem_u32(q_tiles), st_u = smem_u32(stages), mine = elect(), tm = __shfl_sync(0xffffffffu, tmem, 0);
-    int tiles = 0, jobs[2] = {0, 0}, cleaned = 0;
+    int jobs[2] = {0, 0}, cleaned = 0;
+    Cursor keys = {0, 0}, values = {1, 0};  // stages of the next tile's
     bool ok = true;
     for (;; unit_done()) {
       const Unit un = next_unit(ok);
@@ -577,14 +591,11 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
       const bool two = un.n_rows > kTile;
       const int n_jobs = two ? 2 * un.n_tiles : un.n_tiles, first = first_limit(p, un);
       // Keys of job i's tile, or its values, are in place (asked once per tile).
-      auto wait_keys = [&](int i) {
-        const int n = 2 * (tiles + (two ? i >> 1 : i));
-        return i >= n_jobs || (two && (i & 1) != 0) || wait_for(s, &s.full[n % kStages], (n / kStages) & 1);
-      };
+      auto wait_keys = [&](int i) { return i >= n_jobs || (two && (i & 1) != 0) || wait_for(s, &s.full[keys.slot], keys.phase); };
       auto wait_values = [&](int i) {
-        const int t = two ? i >> 1 : i, n = 2 * (tiles + t) + 1;
+        const int t = two ? i >> 1 : i;
         if (two && (i & 1) != 0) return true;
-        if (!wait_for(s, &s.full[n % kStages], (n / kStages) & 1)) return false;
+        if (!wait_for(s, &s.full[values.slot], values.phase)) return false;
         if (!INT8 && partly_seen(p, un.t0 + t, n_prefix, first)) {
           if (!wait_for(s, &s.clean[cleaned % kClean], (cleaned / kClean) & 1)) return false;
           ++cleaned;
@@ -592,7 +603,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
         return true;
       };
       auto qk = [&](int i) {
-        const int t = two ? i >> 1 : i, u = i & 1, slot = 2 * (tiles + t) % kStages;
+        const int u = i & 1, slot = keys.slot;
         const uint64_t a = desc_of(q_u + (two ? u * T::kBytes : 0), 16), b = desc_of(st_u + slot * T::kBytes, 16);
 #pragma unroll
         for (int x = 0; x < D / 16; ++x) {  // 16 channels further: 32 bytes, in units of 16
@@ -600,19 +611,24 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
           mma_ss(tm + u * kTile, a + step, b + step, kQk, x > 0, mine);
         }
         commit(&s.s_full[u], mine);
-        if (!two || u == 1) commit(&s.empty[slot], mine);
+        if (!two || u == 1) {
+          commit(&s.empty[slot], mine);
+          keys.step(2, n_stages);
+        }
       };
       auto pv = [&](int i) {
-        const int t = two ? i >> 1 : i, u = i & 1, slot = (2 * (tiles + t) + 1) % kStages;
+        const int u = i & 1, slot = values.slot;
         const uint64_t b = desc_of(st_u + slot * T::kBytes, T::kHalfBytes);
 #pragma unroll
         for (int x = 0; x < kTile / 16; ++x)  // 16 tokens further: 2 KB of V, 8 columns of weights
           mma_ts(tm + 2 * kTile + u * D, tm + u * kTile + 8 * x, b + x * (2048 / 16), kPv, x > 0 || i > 1, mine);
-        if (!two || u == 1) commit(&s.empty[slot], mine);
+        if (!two || u == 1) {
+          commit(&s.empty[slot], mine);
+          values.step(2, n_stages);
+        }
         if (two && i + 2 >= n_jobs) commit(&s.o_full[u], mine);
       };
-      // The scores of job i + 2 follow the output of job i at once (the weights wait for both): their
-      // operands are asked for before the weights are.
+      // The scores of job i + 2 follow the output of job i at once (the weights wait for both).
       ok = wait_for(s, &s.q_full, unit_count & 1);
       for (int i = 0; ok && i < 2 && i < n_jobs; ++i) {
         ok = wait_keys(i);
@@ -620,19 +636,20 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
         if (ok) qk(i);
       }
       for (int i = 0; ok && i < n_jobs; ++i) {
-        ok = wait_values(i) && wait_keys(i + 2) && wait_for(s, &s.p_full[i & 1], jobs[i & 1] & 1);
+        ok = wait_values(i) && wait_for(s, &s.p_full[i & 1], jobs[i & 1] & 1);
         if (!ok) break;
         tc_after();
         pv(i);
         ++jobs[i & 1];
-        if (i + 2 < n_jobs) qk(i + 2);
+        // (Behind the product: three stages may hold the keys of job i + 2 only once its values' has left them.)
+        ok = wait_keys(i + 2);
+        if (ok && i + 2 < n_jobs) qk(i + 2);
       }
       if (!ok) break;
       if (!two) {
         commit(&s.o_full[0], mine);
         commit(&s.o_full[1], mine);
       }
-      tiles += un.n_tiles;
     }
     // Nothing is freed under a product in flight, whoever gave up and when.
     commit(&s.drain, mine);
@@ -641,10 +658,11 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
   } else if (warp == 9) {
     // ---- copies: the pages of one operand tile at a time, keys then values ----------------------------
     // An entry of the info ring is written again kInfo = 8 tiles later. That tile's keys, or the tile's before
-    // it, have a stage that a tile's at most (kStages + 1) / 2 = 4 before has left, and its products follow the
+    // it, have a stage that a tile's at most (n_stages + 1) / 2 = 5 before has left, and its products follow the
     // weights of all but the two jobs before them: the entry's last reader is done.
     const int per = kTile >> p.page_shift;  // pages per tile
     int tiles = 0, filled = 0;
+    Cursor at = {0, 0};
     [[maybe_unused]] int dirty = 0;
     bool ok = true;
     for (;; unit_done()) {
@@ -666,14 +684,13 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
       };
       look_up(0);
       for (int n = 0; ok && n < 2 * un.n_tiles; ++n) {
-        const int t = n >> 1, kv = n & 1, at = 2 * tiles + n, info = (tiles + t) % kInfo;
+        const int t = n >> 1, kv = n & 1, info = (tiles + t) % kInfo, slot = at.slot;
         if (kv == 0) {
           page = next < p.n_pages ? next : -1;
           look_up(t + 1);
         }
         if constexpr (!INT8) {
-          const int slot = at % kStages;
-          if (at >= kStages) ok = wait_for(s, &s.empty[slot], (at / kStages - 1) & 1);
+          ok = wait_for(s, &s.empty[slot], at.phase ^ 1);  // (of the first round: at once)
           if (!ok) break;
           const uint32_t granules = lane < per && page >= 0 ? ((1u << (bs / 16)) - 1) << (lane * (bs / 16)) : 0u;
           const uint32_t have = __reduce_or_sync(0xffffffffu, granules);
@@ -686,7 +703,8 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
 #pragma unroll
             for (int h2 = 0; h2 < T::kHalves; ++h2) tma_2d(dst + h2 * T::kHalfBytes, &pages_map, 64 * h2, y, &s.full[slot]);
           }
-          filled = at + 1;
+          ++filled;
+          at.step(1, n_stages);
           // To be cleaned: said behind the copies, so that the cleaner never waits for a filling before the last one.
           if (kv == 1 && partly_seen(p, un.t0 + t, n_prefix, first)) warp_arrive(&s.dirty[dirty++ % kClean], lane);
           if (lane == 0 && kv == 0) {
@@ -695,8 +713,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
             mbar_arrive(&s.info[info]);
           }
         } else {
-          const int slot = at % T::kRaw;
-          if (at >= T::kRaw) ok = wait_for(s, &s.raw_empty[slot], (at / T::kRaw - 1) & 1);
+          ok = wait_for(s, &s.raw_empty[slot], at.phase ^ 1);
           if (!ok) break;
           const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, page >= 0));
           if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[slot], n_copies * bs * D);
@@ -704,14 +721,15 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
           if (page >= 0)
             tma_load_1d(raws + slot * T::kRawBytes + lane * bs * D,
                         static_cast<const char*>(p.pages) + (((int64_t)page * p.h + un.j) * 2 + kv) * ((int64_t)bs * D), bs * D, &s.raw_full[slot]);
-          filled = at + 1;
+          ++filled;
+          at.step(1, T::kRaw);
         }
       }
       if (!ok) break;
       tiles += un.n_tiles;
     }
     // No copy may land after the CTA has gone, also where the others gave up behind this warp's last copy.
-    const int slots = INT8 ? T::kRaw : kStages;
+    const int slots = INT8 ? T::kRaw : n_stages;
     for (int n = max(0, filled - slots); n < filled; ++n) mbar_wait(INT8 ? &s.raw_full[n % slots] : &s.full[n % slots], (n / slots) & 1);
     __syncwarp();
   } else if (warp == 10) {
@@ -766,7 +784,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
       }
       pos = (int)at;
     }
-    fence_async();  // the plan is read: copies may have the stages
+    fence_async();  // the plan is read: queries and copies may have its place
     int count = 0;
     auto hand_out = [&](const Unit& un) {
       const int slot = count % kRing;
@@ -817,16 +835,17 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
   } else if (warp == 11) {
     if constexpr (!INT8) {
       // ---- values that are not finite are taken out of tiles that some row does not see whole --------------
-      int tiles = 0, cleaned = 0;
+      int cleaned = 0;
+      Cursor values = {1, 0};
       bool ok = true;
       for (;; unit_done()) {
         const Unit un = next_unit(ok);
         if (un.b < 0) break;
         const int first = first_limit(p, un);
-        for (int t = 0; ok && t < un.n_tiles; ++t) {
+        for (int t = 0; ok && t < un.n_tiles; ++t, values.step(2, n_stages)) {
           if (!partly_seen(p, un.t0 + t, n_prefix, first)) continue;
-          const int n = 2 * (tiles + t) + 1, slot = n % kStages;
-          ok = wait_for(s, &s.dirty[cleaned % kClean], (cleaned / kClean) & 1) && wait_for(s, &s.full[slot], (n / kStages) & 1);
+          const int slot = values.slot;
+          ok = wait_for(s, &s.dirty[cleaned % kClean], (cleaned / kClean) & 1) && wait_for(s, &s.full[slot], values.phase);
           if (!ok) break;
           uint4* v = reinterpret_cast<uint4*>(stages + slot * T::kBytes);
           bool found = false;
@@ -849,7 +868,6 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
           ++cleaned;
         }
         if (!ok) break;
-        tiles += un.n_tiles;
       }
     }
   } else {
@@ -865,6 +883,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
       const int from = (tok0 * kPer + c) * 16, row = (c / 4) * T::kHalfBytes + tok0 * 128, at = (c % 4) * 2;
       const int to0 = row + ((at ^ (tok0 & 7)) << 4), to1 = row + (((at + 1) ^ (tok0 & 7)) << 4);
       int tiles = 0;
+      Cursor to = {kv, 0}, raw = {kv, 0};
       bool ok = true;
       for (;; unit_done()) {
         const Unit un = next_unit(ok);
@@ -896,7 +915,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
         page_of(0);
         scales_of(0);
         for (int t = 0; t < un.n_tiles; ++t) {
-          const int n = 2 * (tiles + t) + kv, raw = n % T::kRaw, slot = n % kStages, info = (tiles + t) % kInfo;
+          const int info = (tiles + t) % kInfo;
           // The ring entry's last reader is more than two tiles behind (see the copies): it is free.
           scale_ring[(info * 2 + kv) * kTile + i] = scale;
           if (kv == 0) {
@@ -905,11 +924,10 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
           }
           warp_arrive(&s.info[info], lane);
           scales_of(t + 1);
-          ok = ok && wait_for(s, &s.raw_full[raw], (n / T::kRaw) & 1);
-          if (ok && n >= kStages) ok = wait_for(s, &s.empty[slot], (n / kStages - 1) & 1);
+          ok = ok && wait_for(s, &s.raw_full[raw.slot], raw.phase) && wait_for(s, &s.empty[to.slot], to.phase ^ 1);
           if (!ok) break;
-          const char* src = raws + raw * T::kRawBytes + from;
-          char* dst = stages + slot * T::kBytes;
+          const char* src = raws + raw.slot * T::kRawBytes + from;
+          char* dst = stages + to.slot * T::kBytes;
 #pragma unroll
           for (int x0 = 0; x0 < kPer; x0 += 4) {
             uint4 w[4];
@@ -917,7 +935,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
             for (int x = 0; x < 4; ++x) w[x] = *reinterpret_cast<const uint4*>(src + (x0 + x) * (kStep * kPer * 16));
             if (x0 + 4 >= kPer) {
               __syncwarp();
-              if (lane == 0) mbar_arrive(&s.raw_empty[raw]);
+              if (lane == 0) mbar_arrive(&s.raw_empty[raw.slot]);
             }
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
@@ -927,7 +945,9 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
             }
           }
           fence_async();
-          warp_arrive(&s.full[slot], lane);
+          warp_arrive(&s.full[to.slot], lane);
+          to.step(2, n_stages);
+          raw.step(2, T::kRaw);
         }
         if (!ok) break;
         tiles += un.n_tiles;

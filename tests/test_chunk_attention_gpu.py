@@ -65,6 +65,8 @@ CASES = [
     (1, 4, 64, 3000, [33] * 12, [33 + 50 * i for i in range(12)]),
     (1, 40, 16, 17, [5, 2], [5, 900]),          # 40 query heads a KV head
     (4, 2, 16, 0, [1] * 300, [1 + (7 * i) % 190 for i in range(300)]),  # more units than CTAs
+    (8, 1, 16, 0, [1] * 40, [1000 + 9 * i for i in range(40)]),                       # many tiles a CTA, all of few rows
+    (8, 1, 16, 40, [1] * 30 + [140], [1000 + 9 * i for i in range(30)] + [1400]),  # and one unit of two row tiles among them
     (1, 1, 16, 0, [2, 3], [1, 0]),              # chunks longer than what their sequences hold: rows that see nothing
 ]
 
