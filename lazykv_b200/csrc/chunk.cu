@@ -19,7 +19,8 @@
 //
 // Roundings: scores, references, sums are float32; a weight (times its value's scale, of int8 pages) is rounded to
 // bf16 once, 2^-9 of it on average half, and the output to bf16. Codes, and bf16 queries, keys and values, are
-// exact operands. Capped scores are c tanh(x / c) = c (1 - 2 / (1 + 2^(2 x log2(e) / c))).
+// exact operands. Capped scores are c tanh(x / c), by a polynomial while a warp's scores of a tile stay within the cap,
+// and otherwise by exponentials (scores.cuh).
 //
 // Masks: a row sees a token if its page exists and the token is in front of the row's limit. Weights of others are
 // zero, but 0 x infinity is a NaN, and a tile's values multiply all of its rows: in tiles that some row does not see
@@ -35,6 +36,7 @@
 
 #include "paged.cuh"
 #include "prefix.cuh"
+#include "scores.cuh"
 #include "tensor.cuh"
 
 namespace lkv {
@@ -70,7 +72,7 @@ struct ChunkParams {
   const int32_t* offsets;
   const int32_t* prefix_table;
   int prefix_cols, prefix_len;
-  float scale;     // scores x this are in the log2 domain (capped: 2 / cap of it); not negative
+  float scale;     // scores x this are in the log2 domain (capped: scores divided by the cap); not negative
   uint32_t flip;   // the queries' sign bits to turn (a negative softmax scale)
   float cap_log2;  // cap x log2(e)
   __nv_bfloat16* out;  // [rows, hq, d]
@@ -166,25 +168,6 @@ __device__ __forceinline__ Sequence sequence_of(const ChunkParams& p, int b) {
 __device__ __forceinline__ int first_limit(const ChunkParams& p, const Unit& u) { return min(max(0, u.base + u.row0 / p.group + 1), u.seen); }
 __device__ __forceinline__ bool partly_seen(const ChunkParams& p, int tile, int n_prefix, int first) {
   return tile < n_prefix ? tile == n_prefix - 1 && p.prefix_len % kTile != 0 : (tile - n_prefix + 1) * kTile > first;
-}
-
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// c tanh(x / c), where x is given as 2 x log2(e) / c.
-__device__ __forceinline__ float capped(float x, float c) { return fmaf(-2.0f * c, rcp(1.0f + ex2(x)), c); }
-
-// Four int8 codes as bf16, exactly: 0x4300 | b is 128 + b for b < 128, and 0x4380 is 256.
-__device__ __forceinline__ uint2 codes_to_bf16(uint32_t w) {
-  const uint32_t a = __byte_perm(w, 0x43434343u, 0x4140), b = __byte_perm(w, 0x43434343u, 0x4342);
-  auto code = [](uint32_t x) {
-    const uint32_t hi = x & 0xff7fff7fu, lo = x & 0xff80ff80u;
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&hi), *reinterpret_cast<const __nv_bfloat162*>(&lo));
-    return *reinterpret_cast<const uint32_t*>(&d);
-  };
-  return make_uint2(code(a), code(b));
 }
 
 __device__ __forceinline__ bool not_finite(uint32_t two) {
@@ -337,6 +320,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
 #pragma unroll
       for (int i = 0; i < 4; ++i) from[i] = -INFINITY, l[i] = 0.0f;
       bool unset = true;  // has some row no reference yet
+      [[maybe_unused]] bool wide_unit = false;  // had a tile scores above their cap's size
       const int n_jobs = two ? 2 * un.n_tiles : un.n_tiles;  // job i: rows i % 2, tile two ? i / 2 : i
       int n_done = 0;
       for (int i = u; i < n_jobs; i += 2, ++n_done) {
@@ -352,19 +336,24 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
         if (!ok) break;
         tc_after();
         if (any_live) {
-          auto weigh = [&](auto mask) {
+          // WIDE: a score may be above its cap's size; false where one is and WIDE is not (nothing is written then).
+          auto weigh = [&](auto mask, [[maybe_unused]] auto any_size) {
             constexpr bool MASK = decltype(mask)::value;
+            [[maybe_unused]] constexpr bool WIDE = decltype(any_size)::value;
+            [[maybe_unused]] float most = 0.0f;  // of the squares of scores divided by their cap
             constexpr int N = kTile / 16;
             [[maybe_unused]] int upto[4];  // columns of the tile that a row sees
             if constexpr (MASK) {
 #pragma unroll
               for (int r = 0; r < 4; ++r) upto[r] = tile < n_prefix ? p.prefix_len - tile * kTile : limit[r] - start;
             }
-            // The scores of column pair k of fragment n, row r, up to their factor (capped: in the log2 domain).
-            auto score = [&](const Frag& a, int n, int k, int r, [[maybe_unused]] uint64_t kk) {
-              uint64_t z = pair(__uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1)]), __uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1) + 1]));
-              if constexpr (INT8) z = mul2(z, kk);
-              if constexpr (CAP) z = pair(capped(first_of(z) * scale, p.cap_log2), capped(second_of(z) * scale, p.cap_log2));
+            // The scores of column pair k of fragment n, row r, up to their factor.
+            auto raw_score = [&](const Frag& a, int k, int r, [[maybe_unused]] uint64_t kk) {
+              const uint64_t z = pair(__uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1)]), __uint_as_float(a.v[r / 2][4 * k + 2 * (r & 1) + 1]));
+              return INT8 ? mul2(z, kk) : z;
+            };
+            auto wide = [&](uint64_t z) { return pair(capped(first_of(z) * (2.0f * kLog2e * scale), p.cap_log2), capped(second_of(z) * (2.0f * kLog2e * scale), p.cap_log2)); };
+            auto seen = [&](uint64_t z, int n, int k, int r) {  // minus infinity where a row does not see a column
               if constexpr (MASK) {
                 const int col = 16 * n + 8 * k + c2, to_col = (have >> n) & 1 ? upto[r] : 0;
                 z = pair(col < to_col ? first_of(z) : -INFINITY, col + 1 < to_col ? second_of(z) : -INFINITY);
@@ -388,7 +377,9 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
                     if constexpr (INT8) kk = ks[4 * (2 * n + k)];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                      const uint64_t z = score(f[0], n, k, r, kk);
+                      uint64_t z = raw_score(f[0], k, r, kk);
+                      if constexpr (CAP) z = wide(z);
+                      z = seen(z, n, k, r);
                       top[r] = fmaxf(fmaxf(top[r], first_of(z)), second_of(z));
                     }
                   }
@@ -439,8 +430,17 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
                   if constexpr (INT8) kk = ks[4 * (2 * n + k)], vv = vs[4 * (2 * n + k)];
 #pragma unroll
                   for (int r = 0; r < 4; ++r) {
-                    uint64_t z = score(f[n & 1], n, k, r, kk);
-                    z = CAP ? add2(z, ref[r]) : fma2(z, scale2, ref[r]);
+                    uint64_t z = raw_score(f[n & 1], k, r, kk);
+                    if constexpr (CAP && WIDE) {
+                      z = add2(wide(z), ref[r]);
+                    } else if constexpr (CAP) {
+                      uint64_t square;
+                      z = capped2(mul2(z, scale2), p.cap_log2, ref[r], &square);
+                      most = fmaxf(fmaxf(most, first_of(square)), second_of(square));
+                    } else {
+                      z = fma2(z, scale2, ref[r]);
+                    }
+                    z = seen(z, n, k, r);
                     z = pair(ex2(first_of(z)), ex2(second_of(z)));
                     sum[r] = add2(sum[r], z);
                     if constexpr (INT8) {
@@ -454,6 +454,9 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
                 }
                 if (n + 1 < N) ld_wait(f[(n + 1) & 1]);
               }
+              if constexpr (CAP && !WIDE) {
+                if (__any_sync(0xffffffffu, most > 1.0f)) return false;
+              }
               // No weight is above the sum that it is part of.
               bool over = false;
 #pragma unroll
@@ -464,11 +467,19 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
               for (int n = 0; n < N; ++n) st_packed(ts + 8 * n, w[n]);  // over the scores
 #pragma unroll
               for (int r = 0; r < 4; ++r) l[r] += first_of(sum[r]) + second_of(sum[r]);
-              break;
+              return true;
             }
           };
-          if (masked) weigh(std::true_type());
-          else weigh(std::false_type());
+          const std::true_type yes;
+          const std::false_type no;
+          if (CAP && wide_unit) {
+            if (masked) weigh(yes, yes);
+            else weigh(no, yes);
+          } else if (!(masked ? weigh(yes, no) : weigh(no, no))) {
+            wide_unit = true;  // large scores come together
+            if (masked) weigh(yes, yes);
+            else weigh(no, yes);
+          }
           st_wait();
         }
         tc_before();
@@ -1082,7 +1093,7 @@ int lkv_chunk_attention(const lkv_chunk_args* a, void* stream) {
   const bool cap = a->cap > 0.0f;
   // (At least a number: a score of -infinity stays one under a softmax scale of zero.)
   const float size = fabsf(a->scale) * kLog2e;
-  p.scale = cap ? 2.0f * size / a->cap : size == 0.0f ? FLT_MIN : size;
+  p.scale = cap ? fabsf(a->scale) / a->cap : size == 0.0f ? FLT_MIN : size;
   p.flip = a->scale < 0.0f ? 0x80008000u : 0u;
   p.cap_log2 = a->cap * kLog2e;
   p.out = static_cast<__nv_bfloat16*>(a->out), p.lse = a->lse;

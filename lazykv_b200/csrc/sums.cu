@@ -21,6 +21,7 @@
 
 #include "paged.cuh"
 #include "prefix.cuh"
+#include "scores.cuh"
 #include "tensor.cuh"
 
 namespace lkv {
@@ -34,6 +35,9 @@ using prefix::kLog2e;
 constexpr int kPair = 2 * kTile;  // tokens of a step
 constexpr int kMostBatch = 8192;
 constexpr int kQStages = 2;
+// Tiles whose scales and page bits are kept. A tile's copies begin when the keys at most three tiles before it have been
+// multiplied, and those are not before the scores two steps (four tiles) back are read.
+constexpr int kInfo = 16;
 
 struct SumsParams {
   const __nv_bfloat16* q;
@@ -52,7 +56,7 @@ struct SumsParams {
   const float* sums;  // [batch, h, cap], or null: zeros
   float* out;
   int cap;
-  float scale, cap_log2;  // scores x scale are in the log2 domain (capped: 2 / cap of it)
+  float scale, cap_log2;  // scores x scale are in the log2 domain (capped: divided by the cap)
   uint64_t max_wait_ns;
 };
 
@@ -62,14 +66,18 @@ struct Geometry {
   static constexpr int kStages = INT8 ? 3 : 4;  // tiles of keys
   static constexpr int kRawBytes = INT8 ? kTile * D : 0, kRaw = INT8 ? 3 : 0;
   static constexpr int kThreads = INT8 ? 768 : 512;
-  static constexpr int kSmemTiles = (kStages + kQStages) * kBytes + kRaw * kRawBytes;
+  // Registers per thread: the warpgroups that sum take what the others leave of the launch's.
+  static constexpr int kMany = INT8 ? 128 : 168, kFew = INT8 ? 56 : 80;
+  static_assert(256 * kMany + (kThreads - 256) * kFew <= kThreads * (INT8 ? 80 : 128), "the register split is the launch's own");
+  static constexpr int kSmemTiles = (kStages + kQStages) * kBytes + kRaw * kRawBytes + (INT8 ? kInfo * kTile * 4 : 0);
   static constexpr int kSmem = (kSmemTiles > kMostBatch * 8 ? kSmemTiles : kMostBatch * 8) + 1024;
 };
 
 struct Barriers {
-  uint64_t k_full[4], k_empty[4], raw_full[3], raw_empty[3], q_full[kQStages], q_empty[kQStages], s_full[2][2], s_empty[2][2], drain;
+  uint64_t k_full[4], k_empty[4], raw_full[3], raw_empty[3], q_full[kQStages], q_empty[kQStages], s_full[2][2], s_empty[2][2], info[kInfo], drain;
   alignas(16) float minus[kQStages][kTile];  // (read four at a time) -lse in the log2 domain; minus infinity: the row does not count
   alignas(16) int limit[kQStages][kTile];    // tokens that the row sees
+  uint32_t have[kInfo];          // bit g: tokens 16 g .. 16 g + 15 of the tile have a page
   int64_t pos, end;              // this CTA's piece of the line: where its first step begins, and where it ends
   int b, k;                      // that step
   uint64_t max_wait_ns;
@@ -133,13 +141,6 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float capped(float x, float c) { return fmaf(-2.0f * c, rcp(1.0f + ex2(x)), c); }
-
 // 16 columns of a thread's own lane of tensor memory.
 struct Lane {
   uint32_t v[16];
@@ -155,17 +156,6 @@ __device__ __forceinline__ void ld_wait(Lane& f) {
   for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(f.v[i]));
 }
 
-// Four int8 codes as bf16 (as chunk.cu).
-__device__ __forceinline__ uint2 codes_to_bf16(uint32_t w) {
-  const uint32_t a = __byte_perm(w, 0x43434343u, 0x4140), b = __byte_perm(w, 0x43434343u, 0x4342);
-  auto code = [](uint32_t x) {
-    const uint32_t hi = x & 0xff7fff7fu, lo = x & 0xff80ff80u;
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&hi), *reinterpret_cast<const __nv_bfloat162*>(&lo));
-    return *reinterpret_cast<const uint32_t*>(&d);
-  };
-  return make_uint2(code(a), code(b));
-}
-
 template <int D, bool INT8, bool CAP>
 __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(const SumsParams p, const __grid_constant__ CUtensorMap pages_map) {
   using G = Geometry<D, INT8>;
@@ -176,6 +166,7 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
   char* q_stages = smem;
   char* stages = q_stages + kQStages * G::kBytes;
   char* raws = stages + kStages * G::kBytes;
+  float* scale_ring = reinterpret_cast<float*>(raws + G::kRaw * G::kRawBytes);  // [kInfo][kTile]: the keys'
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, bs = 1 << p.page_shift;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -194,6 +185,7 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
       mbar_init(&s.s_full[i / 2][i % 2], 1);
       mbar_init(&s.s_empty[i / 2][i % 2], 4);
     }
+    for (int i = 0; i < kInfo; ++i) mbar_init(&s.info[i], 1);
     mbar_init(&s.drain, 1);
     s.max_wait_ns = p.max_wait_ns;
     s.quit = 0;
@@ -258,24 +250,26 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
   fence_async();
   __syncthreads();
 
+  if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::kMany));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kFew));
   if (warp < 8) {
     // ---- sums: a thread has a token -------------------------------------------------------------------
     const int u = warp / 4, i = tid % kTile;
     const uint32_t ts = tmem + ((uint32_t)(warp % 4) << 21) + u * 2 * kTile;
-    int q_count = 0, job = 0;
+    int q_count = 0, job = 0, tile = u;
     bool ok = true;
-    for (Walk w(p, s); w.more() && ok; w.next(p)) {
-      const int token = w.step * kPair + u * kTile + i;
+    for (Walk w(p, s); w.more() && ok; w.next(p), tile += 2) {
+      const int token = w.step * kPair + u * kTile + i, info = tile % kInfo;
       const int64_t at = ((int64_t)w.b * p.h + w.j) * p.cap + token;
-      float old = 0.0f, factor = p.scale;
-      bool there = false;
-      if (token < w.q.seen) {
-        const int id = p.table[w.b * p.table_ld + (token >> p.page_shift)];
-        there = id >= 0 && id < p.n_pages;
-        if (INT8 && there) factor *= p.scales[(((int64_t)id * p.h + w.j) * 2) * bs + (token & (bs - 1))];
-        if (p.sums != nullptr && token < w.q.old) old = p.sums[at];
-      }
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      float old = 0.0f;
+      if (p.sums != nullptr && token < min(w.q.old, w.q.seen)) old = p.sums[at];
+      ok = wait_for(s, &s.info[info], (tile / kInfo) & 1);
+      if (!ok) break;
+      const bool there = token < w.q.seen && (s.have[info] >> (i / 16) & 1);
+      const float factor = INT8 && there ? p.scale * scale_ring[info * kTile + i] : p.scale;
+      const uint64_t factor2 = pair(factor, factor);
+      uint64_t sum[2] = {0, 0};
+      bool wide_step = false;  // capped scores above their cap's size
       for (int c = w.from; c < w.q.chunks; ++c, ++job) {
         const int buf = job & 1, stage = q_count % kQStages;
         ok = wait_for(s, &s.q_full[stage], (q_count / kQStages) & 1) && wait_for(s, &s.s_full[u][buf], (job >> 1) & 1);
@@ -285,26 +279,38 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
         const bool masked = n_cols % 16 != 0 || s.limit[stage][0] < w.step * kPair + u * kTile + kTile;
         const float4* minus = reinterpret_cast<const float4*>(s.minus[stage]);
         const int4* limit = reinterpret_cast<const int4*>(s.limit[stage]);
-        auto add = [&](const Lane& f, int n, auto mask) {
+        // MASK: some row does not see the tile whole. WIDE: scores may be above their cap's size; false where one is and WIDE
+        // is not.
+        auto all = [&](auto mask, [[maybe_unused]] auto any_size) {
+          constexpr bool MASK = decltype(mask)::value, WIDE = decltype(any_size)::value;
+          uint64_t more[2] = {sum[0], sum[1]};
+          float most = 0.0f;
+          auto add = [&](const Lane& f, int n) {
 #pragma unroll
-          for (int x = 0; x < 16; x += 4) {
-            const float4 m = minus[(16 * n + x) / 4];
-            const float by[4] = {m.x, m.y, m.z, m.w};
-            int upto[4] = {};
-            if constexpr (decltype(mask)::value) {
-              const int4 y = limit[(16 * n + x) / 4];
-              upto[0] = y.x, upto[1] = y.y, upto[2] = y.z, upto[3] = y.w;
-            }
+            for (int x = 0; x < 16; x += 4) {
+              const float4 m = minus[(16 * n + x) / 4];
+              [[maybe_unused]] int4 upto;
+              if constexpr (MASK) upto = limit[(16 * n + x) / 4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float z = __uint_as_float(f.v[x + e]);
-              float y = ex2(CAP ? capped(z * factor, p.cap_log2) + by[e] : fmaf(z, factor, by[e]));
-              if constexpr (decltype(mask)::value) y = token < upto[e] ? y : 0.0f;
-              sum[e] += y;
+              for (int e = 0; e < 2; ++e) {
+                uint64_t z = pair(__uint_as_float(f.v[x + 2 * e]), __uint_as_float(f.v[x + 2 * e + 1]));
+                const uint64_t by = e == 0 ? pair(m.x, m.y) : pair(m.z, m.w);
+                if constexpr (!CAP) {
+                  z = fma2(z, factor2, by);
+                } else if constexpr (WIDE) {
+                  z = mul2(z, pair(2.0f * kLog2e * factor, 2.0f * kLog2e * factor));
+                  z = add2(pair(capped(first_of(z), p.cap_log2), capped(second_of(z), p.cap_log2)), by);
+                } else {
+                  uint64_t square;
+                  z = capped2(mul2(z, factor2), p.cap_log2, by, &square);
+                  most = fmaxf(fmaxf(most, first_of(square)), second_of(square));
+                }
+                z = pair(ex2(first_of(z)), ex2(second_of(z)));
+                if constexpr (MASK) z = pair(token < (e == 0 ? upto.x : upto.z) ? first_of(z) : 0.0f, token < (e == 0 ? upto.y : upto.w) ? second_of(z) : 0.0f);
+                more[e] = add2(more[e], z);
+              }
             }
-          }
-        };
-        auto all = [&](auto mask) {
+          };
           Lane f[2];
           const int n = (n_cols + 15) / 16;
           ld(f[0], ts + buf * kTile);
@@ -312,15 +318,28 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
 #pragma unroll 1
           for (int x = 0; x < n; x += 2) {
             if (x + 1 < n) ld(f[1], ts + buf * kTile + 16 * (x + 1));
-            add(f[0], x, mask);
+            add(f[0], x);
             if (x + 1 < n) ld_wait(f[1]);
             if (x + 2 < n) ld(f[0], ts + buf * kTile + 16 * (x + 2));
-            if (x + 1 < n) add(f[1], x + 1, mask);
+            if (x + 1 < n) add(f[1], x + 1);
             if (x + 2 < n) ld_wait(f[0]);
           }
+          if constexpr (CAP && !WIDE) {
+            if (__any_sync(0xffffffffu, most > 1.0f)) return false;
+          }
+          sum[0] = more[0], sum[1] = more[1];
+          return true;
         };
-        if (masked) all(std::true_type());
-        else all(std::false_type());
+        const std::true_type yes;
+        const std::false_type no;
+        if (CAP && wide_step) {
+          if (masked) all(yes, yes);
+          else all(no, yes);
+        } else if (!(masked ? all(yes, no) : all(no, no))) {
+          wide_step = true;
+          if (masked) all(yes, yes);
+          else all(no, yes);
+        }
         tc_before();
         warp_arrive(&s.s_empty[u][buf], lane);
         // (One chunk a sequence and head stays for all of its steps.)
@@ -329,8 +348,8 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
           ++q_count;
         }
       }
-      if (!ok) sum[0] = __uint_as_float(0x7fc00000u);
-      if (token < p.cap) p.out[at] = old + (there ? (sum[0] + sum[1]) + (sum[2] + sum[3]) : 0.0f);
+      const float got = (first_of(sum[0]) + second_of(sum[0])) + (first_of(sum[1]) + second_of(sum[1]));
+      if (token < p.cap) p.out[at] = old + (!ok ? __uint_as_float(0x7fc00000u) : there ? got : 0.0f);
     }
   } else if (warp == 8) {
     // ---- matrix products ------------------------------------------------------------------------------
@@ -374,20 +393,36 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
     int filled = 0;
     bool ok = true;
     constexpr int kSlots = INT8 ? G::kRaw : kStages;
-    for (Walk w(p, s); w.more() && ok; w.next(p)) {
-      int pages[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {  // lane i has page i of each tile
-        const int token = w.step * kPair + u * kTile + lane * bs;
-        pages[u] = lane < per && token < w.q.seen ? p.table[w.b * p.table_ld + (token >> p.page_shift)] : -1;
-        if (pages[u] >= p.n_pages) pages[u] = -1;
-      }
+    // Lane i has page i of each tile, looked up a step ahead (their ids, checked where they are used).
+    int ahead[2] = {-1, -1};
+    auto look_up = [&](const Walk& w) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int slot = filled % kSlots, page = pages[u];
+        const int token = w.step * kPair + u * kTile + lane * bs;
+        ahead[u] = w.more() && lane < per && token < w.q.seen ? p.table[w.b * p.table_ld + (token >> p.page_shift)] : -1;
+      }
+    };
+    Walk next(p, s);
+    look_up(next);
+    while (next.more() && ok) {
+      const Walk w = next;
+      const int pages[2] = {ahead[0], ahead[1]};
+      next.next(p);
+      look_up(next);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int slot = filled % kSlots, page = pages[u] < p.n_pages ? pages[u] : -1;
         uint64_t* full = INT8 ? &s.raw_full[slot % 3] : &s.k_full[slot];
         if (filled >= kSlots) ok = ok && wait_for(s, INT8 ? &s.raw_empty[slot % 3] : &s.k_empty[slot], (filled / kSlots - 1) & 1);
         if (!ok) break;
+        const int info = filled % kInfo;
+        const uint32_t granules = page >= 0 ? ((1u << (bs / 16)) - 1) << (lane * (bs / 16)) : 0u;
+        const uint32_t have = __reduce_or_sync(0xffffffffu, granules);
+        if (lane == 0) {
+          s.have[info] = have;
+          if (INT8) mbar_arrive_expect_tx(&s.info[info], __popc(have) * 64);  // 16 scales of each 16 tokens
+          else mbar_arrive(&s.info[info]);
+        }
         if constexpr (!INT8) {
           if (lane == 0) mbar_arrive_expect_tx(full, G::kBytes);
           __syncwarp();
@@ -402,12 +437,15 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
           const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, page >= 0));
           if (lane == 0) mbar_arrive_expect_tx(full, n_copies * bs * D);
           __syncwarp();
-          if (page >= 0)
+          if (page >= 0) {
+            tma_load_1d(scale_ring + info * kTile + lane * bs, p.scales + ((int64_t)page * p.h + w.j) * 2 * bs, bs * 4, &s.info[info]);
             tma_load_1d(raws + slot * G::kRawBytes + lane * bs * D, static_cast<const char*>(p.pages) + (((int64_t)page * p.h + w.j) * 2) * ((int64_t)bs * D), bs * D, full);
+          }
         }
         ++filled;
       }
     }
+    for (int n = max(0, filled - kInfo); n < filled; ++n) mbar_wait(&s.info[n % kInfo], (n / kInfo) & 1);
     for (int n = max(0, filled - kSlots); n < filled; ++n) mbar_wait(INT8 ? &s.raw_full[n % 3] : &s.k_full[n % kSlots], (n / kSlots) & 1);
     __syncwarp();
   } else if (warp < 12) {
@@ -539,8 +577,7 @@ extern "C" int lkv_attention_sums(const lkv_sums_args* a, void* stream) {
   p.table = a->table, p.table_ld = a->table_ld, p.table_cols = a->table_cols, p.lens = a->lens, p.offsets = a->offsets;
   p.last = a->last, p.sums = a->sums, p.out = a->out, p.cap = a->cap;
   const bool cap = a->cap_scores > 0.0f;
-  const float size = a->scale * kLog2e;
-  p.scale = cap ? 2.0f * size / a->cap_scores : size;
+  p.scale = cap ? a->scale / a->cap_scores : a->scale * kLog2e;
   p.cap_log2 = a->cap_scores * kLog2e;
   p.max_wait_ns = kMaxTensorWaitNs;
   const bool int8 = a->kind == LKV_CACHE_INT8;
