@@ -792,8 +792,9 @@ int lkv_chunk_attention(const lkv_chunk_args* args, void* stream);
  * and cap_scores (the scores' cap) are as lkv_chunk_attention's and lse [rows, hq] what it returned, a prefix's part in
  * it included. sums (float32 [batch, h, cap], optional: zeros; it may be out) holds for the tokens in front of the chunk;
  * those of the chunk start from 0, slots without a token get 0, a token whose page is missing keeps its sum. A row with
- * lse = -inf has no weights. One launch, no workspace, no atomics: the same sums every time. Limits and bounded waits as
- * lkv_chunk_attention's (a token whose wait ran out gets NaN).
+ * lse = -inf has no weights. One or two launches, no atomics: the same sums every time. The workspace
+ * (lkv_attention_sums_workspace bytes, 16-byte aligned, any contents) belongs to one call at a time. Limits and bounded
+ * waits as lkv_chunk_attention's (a token whose wait ran out gets NaN).
  */
 typedef struct {
   const void* q;
@@ -816,7 +817,10 @@ typedef struct {
   float* out;
   int cap;
   float scale, cap_scores;
+  void* workspace;
+  size_t workspace_bytes;
 } lkv_sums_args;
+size_t lkv_attention_sums_workspace(int batch, int h, int cap);
 int lkv_attention_sums(const lkv_sums_args* args, void* stream);
 
 /*

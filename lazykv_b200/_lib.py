@@ -92,6 +92,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lkv_paged_write_rotated": (c_int, [c_void_p, c_void_p]),
     "lkv_chunk_attention_workspace": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int64, c_int64]),
     "lkv_chunk_attention": (c_int, [c_void_p, c_void_p]),
+    "lkv_attention_sums_workspace": (c_size_t, [c_int, c_int, c_int]),
     "lkv_attention_sums": (c_int, [c_void_p, c_void_p]),
     "lkv_paged_evict_workspace": (c_size_t, [c_int, c_int, c_int, c_int]),
     "lkv_paged_evict": (c_int, [c_void_p, c_void_p]),
@@ -134,7 +135,7 @@ PAGED_ARGS = struct.Struct("@PPqqqqqqiiiiiPiPqiPqiPPPP")
 PREFIX_ARGS = struct.Struct("@PiqqqPiPqiiiiiiPqiPPiqfPiPPN")
 ROTATE_ARGS = struct.Struct("@PPPqqqqqqPqqiiiiiPPiiPPfPiPqiPqiPPi")
 CHUNK_ARGS = struct.Struct("@PqqiiiiiPiPqiPqiPPiPiqffPPPN")
-SUMS_ARGS = struct.Struct("@PqqiiiiiPPiPqiPqiPPiiPPiff")
+SUMS_ARGS = struct.Struct("@PqqiiiiiPPiPqiPqiPPiiPPiffPN")
 EVICT_ARGS = struct.Struct("@PiiPqiiiiPqiPPPiPPPiiPPN")
 VERIFY_ARGS = struct.Struct("@PqqPqqPqPqiiiPP")
 

@@ -360,30 +360,38 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
               }
               return z;
             };
-            Frag f[2];
+            // The tile's scores 16 columns at a time, the next under way.
+            auto sweep = [&](auto&& use) {
+              Frag f[2];
+              ld(f[0], ts);
+              ld_wait(f[0]);
+#pragma unroll
+              for (int n = 0; n < N; ++n) {
+                if (n + 1 < N) ld(f[(n + 1) & 1], ts + 16 * (n + 1));
+                use(f[n & 1], n);
+                if (n + 1 < N) ld_wait(f[(n + 1) & 1]);
+              }
+            };
             // One pass, from the references as they are; where there are none yet or a score has outgrown them, they
             // are set from the tile's maxima first.
 #pragma unroll 1
             for (bool set = unset, again = false;; again = true) {
               if (set) {
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-                for (int n = 0; n < N; ++n) {
-                  ld(f[0], ts + 16 * n);
-                  ld_wait(f[0]);
+                sweep([&](const Frag& f, int n) {
 #pragma unroll
                   for (int k = 0; k < 2; ++k) {
                     [[maybe_unused]] uint64_t kk = 0;
                     if constexpr (INT8) kk = ks[4 * (2 * n + k)];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                      uint64_t z = raw_score(f[0], k, r, kk);
+                      uint64_t z = raw_score(f, k, r, kk);
                       if constexpr (CAP) z = wide(z);
                       z = seen(z, n, k, r);
                       top[r] = fmaxf(fmaxf(top[r], first_of(z)), second_of(z));
                     }
                   }
-                }
+                });
                 float by[4];
                 bool none = false;
 #pragma unroll
@@ -398,16 +406,17 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
                 }
                 unset = __any_sync(0xffffffffu, none);
                 if (n_done > 0) {  // the products of this row tile's last job are done: its scores came after them
+                  Frag f;
 #pragma unroll 1
                   for (int n = 0; n < D / 16; ++n) {
-                    ld(f[0], to + 16 * n);
-                    ld_wait(f[0]);
+                    ld(f, to + 16 * n);
+                    ld_wait(f);
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
-                      uint32_t& w = f[0].v[x / 8][x % 8];
+                      uint32_t& w = f.v[x / 8][x % 8];
                       w = __float_as_uint(__uint_as_float(w) * by[2 * (x / 8) + (x % 4) / 2]);
                     }
-                    st(to + 16 * n, f[0]);
+                    st(to + 16 * n, f);
                   }
                 }
               }
@@ -419,41 +428,43 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
                 ref[r] = pair(x, x);
               }
               uint32_t w[N][2][4];
-              ld(f[0], ts);
-              ld_wait(f[0]);
-#pragma unroll
-              for (int n = 0; n < N; ++n) {
-                if (n + 1 < N) ld(f[(n + 1) & 1], ts + 16 * (n + 1));
+              sweep([&](const Frag& f, int n) {
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                   [[maybe_unused]] uint64_t kk = 0, vv = 0;
                   if constexpr (INT8) kk = ks[4 * (2 * n + k)], vv = vs[4 * (2 * n + k)];
+                  // (Capped scores step by step for four rows: their longer chains of results do not wait for one another.)
+                  constexpr int R = CAP ? 4 : 1;
 #pragma unroll
-                  for (int r = 0; r < 4; ++r) {
-                    uint64_t z = raw_score(f[n & 1], k, r, kk);
+                  for (int r0 = 0; r0 < 4; r0 += R) {
+                    uint64_t z[R];
+#pragma unroll
+                    for (int r = 0; r < R; ++r) z[r] = raw_score(f, k, r0 + r, kk);
                     if constexpr (CAP && WIDE) {
-                      z = add2(wide(z), ref[r]);
+#pragma unroll
+                      for (int r = 0; r < R; ++r) z[r] = add2(wide(z[r]), ref[r0 + r]);
                     } else if constexpr (CAP) {
-                      uint64_t square;
-                      z = capped2(mul2(z, scale2), p.cap_log2, ref[r], &square);
-                      most = fmaxf(fmaxf(most, first_of(square)), second_of(square));
+#pragma unroll
+                      for (int r = 0; r < R; ++r) z[r] = mul2(z[r], scale2);
+                      capped2(z, p.cap_log2, ref, most);
                     } else {
-                      z = fma2(z, scale2, ref[r]);
+                      z[0] = fma2(z[0], scale2, ref[r0]);
                     }
-                    z = seen(z, n, k, r);
-                    z = pair(ex2(first_of(z)), ex2(second_of(z)));
-                    sum[r] = add2(sum[r], z);
-                    if constexpr (INT8) {
-                      uint64_t x = mul2(z, vv);
-                      // A scale of a token that the row does not see may be anything.
-                      if constexpr (MASK) x = pair(first_of(z) == 0.0f ? 0.0f : first_of(x), second_of(z) == 0.0f ? 0.0f : second_of(x));
-                      z = x;
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                      z[r] = seen(z[r], n, k, r0 + r);
+                      z[r] = pair(ex2(first_of(z[r])), ex2(second_of(z[r])));
+                      sum[r0 + r] = add2(sum[r0 + r], z[r]);
+                      if constexpr (INT8) {
+                        const uint64_t x = mul2(z[r], vv);
+                        // A scale of a token that the row does not see may be anything.
+                        z[r] = MASK ? pair(first_of(z[r]) == 0.0f ? 0.0f : first_of(x), second_of(z[r]) == 0.0f ? 0.0f : second_of(x)) : x;
+                      }
+                      w[n][(r0 + r) / 2][2 * k + ((r0 + r) & 1)] = pack_bf16(first_of(z[r]), second_of(z[r]));
                     }
-                    w[n][r / 2][2 * k + (r & 1)] = pack_bf16(first_of(z), second_of(z));
                   }
                 }
-                if (n + 1 < N) ld_wait(f[(n + 1) & 1]);
-              }
+              });
               if constexpr (CAP && !WIDE) {
                 if (__any_sync(0xffffffffu, most > 1.0f)) return false;
               }

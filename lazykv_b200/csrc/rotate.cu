@@ -16,6 +16,7 @@
 // channels of the first elements of pairs and the four of their second ones, so that a rotation needs no other
 // lane. A CTA computes the angles of its tokens once for all heads.
 #include "paged.cuh"
+#include "tensor.cuh"
 
 namespace lkv {
 namespace {
@@ -23,7 +24,7 @@ namespace {
 using namespace paged;
 
 constexpr int kThreads = 256;
-constexpr int kMostTokens = 4;  // tokens of a CTA of a long call
+constexpr int kMostTokens = 8;  // tokens of a CTA of a long call
 
 struct RotateParams {
   const void* q;
@@ -128,13 +129,58 @@ __device__ __forceinline__ void turn_of(int position, float frequency, double* c
   r = fma(-n, 2.4492935982947064e-16, r);
   sincospi(r * 0.3183098861837907, s, c);
 }
-__device__ __forceinline__ float inverse_root(float x) { return 1.0f / sqrtf(x); }
+__device__ __forceinline__ float inverse_root(float x) { return rsqrtf(x); }
 __device__ __forceinline__ double inverse_root(double x) { return 1.0 / sqrt(x); }
 
-template <typename T, int D, bool INT8, bool VEC>
-__global__ void __launch_bounds__(kThreads) rotate_kernel(const RotateParams p) {
+// What a lane does to its pairs (a, b) of every row of one kind: weights and turn as four factors a pair, so that a
+// normalised row is (a ca + b sb, b cb + a sa) / rms.
+template <typename W>
+struct Turn {
+  W ca[4], sa[4], cb[4], sb[4];
+  bool norm, turns;
+};
+__device__ __forceinline__ void apply(const Turn<double>& t, double (&a)[4], double (&b)[4], double inv) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const double x = t.turns ? a[i] * t.ca[i] + b[i] * t.sb[i] : a[i] * t.ca[i], y = t.turns ? b[i] * t.cb[i] + a[i] * t.sa[i] : b[i] * t.cb[i];
+    a[i] = x * inv, b[i] = y * inv;
+  }
+}
+__device__ __forceinline__ void apply(const Turn<float>& t, float (&a)[4], float (&b)[4], float inv) {
+  using namespace tc;
+  const uint64_t by = pair(inv, inv);
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const uint64_t x = pair(a[i], a[i + 1]), y = pair(b[i], b[i + 1]);
+    uint64_t u = mul2(x, pair(t.ca[i], t.ca[i + 1])), v = mul2(y, pair(t.cb[i], t.cb[i + 1]));
+    if (t.turns) {  // (a turn by nothing would still make a NaN of an infinite neighbour)
+      u = fma2(y, pair(t.sb[i], t.sb[i + 1]), u);
+      v = fma2(x, pair(t.sa[i], t.sa[i + 1]), v);
+    }
+    if (t.norm) u = mul2(u, by), v = mul2(v, by);
+    a[i] = first_of(u), a[i + 1] = second_of(u), b[i] = first_of(v), b[i + 1] = second_of(v);
+  }
+}
+__device__ __forceinline__ float squares(const float (&a)[4], const float (&b)[4]) {
+  using namespace tc;
+  uint64_t s = mul2(pair(a[0], a[1]), pair(a[0], a[1]));
+  s = fma2(pair(a[2], a[3]), pair(a[2], a[3]), s);
+  s = fma2(pair(b[0], b[1]), pair(b[0], b[1]), s);
+  s = fma2(pair(b[2], b[3]), pair(b[2], b[3]), s);
+  return first_of(s) + second_of(s);
+}
+__device__ __forceinline__ double squares(const double (&a)[4], const double (&b)[4]) {
+  double s = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s += a[i] * a[i] + b[i] * b[i];
+  return s;
+}
+
+// INTER: pairs of neighbours. Grid: p.token_shift tokens a CTA.
+template <typename T, int D, bool INT8, bool VEC, bool INTER>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2) rotate_kernel(const RotateParams p) {
   using W = typename Wide<T>::type;
-  constexpr int L = D / 8, kGroups = kThreads / L, U = sizeof(T) == 2 ? 4 : 2;  // rows that a group has in flight
+  constexpr int L = D / 8, kGroups = kThreads / L, U = 2;  // rows that a group asks for at once
   __shared__ W turns[2][kMostTokens][D / 2];  // cosines, sines
   __shared__ int64_t where[kMostTokens];      // row 0 of the token's place in its page; -1: no page; -2: no sequence's token
   pdl_wait();
@@ -142,25 +188,28 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const RotateParams p) 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, tokens = 1 << p.token_shift, row0 = blockIdx.x << p.token_shift;
   const int bs = 1 << p.page_shift;
 
-  // A group's token, its heads, and a lane's pairs: 4 l .. 4 l + 3, at channels c0 .. and c1 ..
+  // A group's token, its heads sub, sub + per, .., and a lane's pairs: 4 l .. 4 l + 3, at channels c0 .. and c1 ..
   const int per = kGroups >> p.token_shift, group = tid / L, l = tid % L, t = group / per, sub = group % per, row = row0 + t;
   const uint32_t mask = L == 32 ? 0xffffffffu : ((1u << L) - 1) << (lane / L * L);
   int c0 = 8 * l, c1 = c0 + 4;
-  if (!p.interleaved) {
+  if (!INTER) {
     const int pr = 4 * l;
     c0 = pr < p.pairs ? pr : pr + p.pairs;
     c1 = pr < p.pairs ? pr + p.pairs : pr + D / 2;
   }
+  // A group's rows of one kind: sub, sub + per, ..; U of them are asked for at once.
   Four<T> lo[U], hi[U];
-  const T* q = static_cast<const T*>(p.q) + (int64_t)row * p.q_st;
-  auto fetch = [&](int j0) {
+  auto fetch = [&](const T* src, int64_t s_head, int j0, int n) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = j0 + u * per;
-      if (row < p.rows && j < p.hq) lo[u] = load4<T, VEC>(q + j * p.q_sh + c0), hi[u] = load4<T, VEC>(q + j * p.q_sh + c1);
+      if (row < p.rows && j < n) lo[u] = load4<T, VEC>(src + j * s_head + c0), hi[u] = load4<T, VEC>(src + j * s_head + c1);
     }
   };
-  fetch(sub);
+  const T* q = static_cast<const T*>(p.q) + (int64_t)row * p.q_st;
+  const T* k = static_cast<const T*>(p.k) + (int64_t)row * p.k_st;
+  const T* v = static_cast<const T*>(p.v) + (int64_t)row * p.v_st;
+  fetch(q, p.q_sh, sub, p.hq);
 
   if (warp >= 8 - tokens) {  // the last warps find the tokens' places
     const int mine = 7 - warp, r = row0 + mine;
@@ -192,104 +241,122 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(const RotateParams p) 
   __syncthreads();
   const int64_t place = where[t];
   if (place == -2) return;
-  W cs[4], sn[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) cs[i] = turns[0][t][4 * l + i], sn[i] = turns[1][t][4 * l + i];
 
-  // x: a lane's channels c0 .. and c1 .., normalised (weights w) and turned.
-  auto turn = [&](W* x, const W* w, bool norm) {
-    if (norm) {
-      W sum = 0;
+  auto of = [](const Four<T>& x, const Four<T>& y, W (&a)[4], W (&b)[4]) {  // a lane's channels as its pairs
+    W w[8];
+    widen(x, w), widen(y, w + 4);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
+    for (int i = 0; i < 4; ++i) a[i] = INTER ? w[2 * i] : w[i], b[i] = INTER ? w[2 * i + 1] : w[4 + i];
+  };
+  auto turn_with = [&](const void* weight) {
+    Turn<W> f;
+    f.norm = weight != nullptr, f.turns = 4 * l < p.pairs;
+    W a[4] = {1, 1, 1, 1}, b[4] = {1, 1, 1, 1};
+    if (f.norm) of(load4<T, VEC>(static_cast<const T*>(weight) + c0), load4<T, VEC>(static_cast<const T*>(weight) + c1), a, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const W c = turns[0][t][4 * l + i], s = turns[1][t][4 * l + i];
+      f.ca[i] = a[i] * c, f.sa[i] = a[i] * s, f.cb[i] = b[i] * c, f.sb[i] = -b[i] * s;
+    }
+    return f;
+  };
+  auto turned = [&](const Turn<W>& f, W (&a)[4], W (&b)[4]) {
+    W inv = 1;
+    if (f.norm) {
+      W sum = squares(a, b);
 #pragma unroll
       for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
-      const W inv = inverse_root(sum * (W)(1.0 / D) + (W)p.eps);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= inv * w[i];
+      inv = inverse_root(sum * (W)(1.0 / D) + (W)p.eps);
     }
-    if (4 * l >= p.pairs) return;  // (a turn by nothing would still make a NaN of an infinite neighbour)
-    if (p.interleaved) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const W a = x[2 * i], b = x[2 * i + 1];
-        x[2 * i] = a * cs[i] - b * sn[i], x[2 * i + 1] = b * cs[i] + a * sn[i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const W a = x[i], b = x[4 + i];
-        x[i] = a * cs[i] - b * sn[i], x[4 + i] = b * cs[i] + a * sn[i];
-      }
-    }
+    apply(f, a, b, inv);
   };
-  auto weights = [&](const void* from, W* w) {
-    if (from == nullptr) return;
-    widen(load4<T, VEC>(static_cast<const T*>(from) + c0), w);
-    widen(load4<T, VEC>(static_cast<const T*>(from) + c1), w + 4);
+  auto in_order = [](const W (&a)[4], const W (&b)[4], float (&z)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[INTER ? 2 * i : i] = (float)a[i], z[INTER ? 2 * i + 1 : 4 + i] = (float)b[i];
   };
-
-  W w[8];
-  weights(p.q_weight, w);
-  T* out = static_cast<T*>(p.out) + (int64_t)row * p.o_st;
-  for (int j0 = sub; j0 < p.hq; j0 += U * per) {
-    if (j0 != sub) fetch(j0);
+  {
+    const Turn<W> f = turn_with(p.q_weight);
+    T* out = static_cast<T*>(p.out) + (int64_t)row * p.o_st;
+    for (int j0 = sub; j0 < p.hq; j0 += U * per) {
+      if (j0 != sub) fetch(q, p.q_sh, j0, p.hq);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = j0 + u * per;
-      if (j >= p.hq) break;
-      W x[8];
-      widen(lo[u], x), widen(hi[u], x + 4);
-      turn(x, w, p.q_weight != nullptr);
-      float y[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = (float)x[i];
-      store4<VEC>(out + j * p.o_sh + c0, y);
-      store4<VEC>(out + j * p.o_sh + c1, y + 4);
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * per;
+        if (j >= p.hq) break;
+        W a[4], b[4];
+        of(lo[u], hi[u], a, b);
+        turned(f, a, b);
+        float z[8];
+        in_order(a, b, z);
+        store4<VEC>(out + j * p.o_sh + c0, z);
+        store4<VEC>(out + j * p.o_sh + c1, z + 4);
+      }
     }
   }
   if (place < 0) return;
-
-  weights(p.k_weight, w);
-  const T* k = static_cast<const T*>(p.k) + (int64_t)row * p.k_st;
-  const T* v = static_cast<const T*>(p.v) + (int64_t)row * p.v_st;
-  for (int j = sub; j < 2 * p.h; j += per) {  // the keys of all heads, then their values
-    const int kv = j >= p.h, head = j - kv * p.h;
-    const T* src = kv ? v + head * p.v_sh : k + head * p.k_sh;
-    W x[8];
-    widen(load4<T, VEC>(src + c0), x), widen(load4<T, VEC>(src + c1), x + 4);
-    if (!kv) turn(x, w, p.k_weight != nullptr);
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = (float)x[i];
-    const int64_t to = place + ((int64_t)head * 2 + kv) * bs;
+  auto put = [&](const float (&z)[8], int j, int kv) {
+    const int64_t to = place + ((int64_t)j * 2 + kv) * bs;
     if constexpr (INT8) {
       uint32_t top = 0, codes[2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
+      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(z[i]) & 0x7fffffffu);
 #pragma unroll
       for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
       const float s = scale_of(top);
-      quantise<8>(y, s, codes);
+      quantise<8>(z, s, codes);
       int8_t* dst = static_cast<int8_t*>(p.pages) + to * D;
       *reinterpret_cast<uint32_t*>(dst + c0) = codes[0];
       *reinterpret_cast<uint32_t*>(dst + c1) = codes[1];
       if (l == 0) p.scales[to] = s;
     } else {
       T* dst = static_cast<T*>(p.pages) + to * D;
-      store4<true>(dst + c0, y);
-      store4<true>(dst + c1, y + 4);
+      store4<true>(dst + c0, z);
+      store4<true>(dst + c1, z + 4);
+    }
+  };
+  {
+    const Turn<W> f = turn_with(p.k_weight);
+    for (int j0 = sub; j0 < p.h; j0 += U * per) {
+      fetch(k, p.k_sh, j0, p.h);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * per;
+        if (j >= p.h) break;
+        W a[4], b[4];
+        of(lo[u], hi[u], a, b);
+        turned(f, a, b);
+        float z[8];
+        in_order(a, b, z);
+        put(z, j, 0);
+      }
+    }
+  }
+  for (int j0 = sub; j0 < p.h; j0 += U * per) {
+    fetch(v, p.v_sh, j0, p.h);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * per;
+      if (j >= p.h) break;
+      W w[8];
+      widen(lo[u], w), widen(hi[u], w + 4);
+      float z[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] = (float)w[i];
+      put(z, j, 1);
     }
   }
 }
 
+template <typename T, int D, bool INT8, bool VEC>
+cudaError_t launch_as(const RotateParams& p, unsigned grid, cudaStream_t st) {
+  return p.interleaved ? launch_pdl(rotate_kernel<T, D, INT8, VEC, true>, dim3(grid), dim3(kThreads), 0, st, 0, p)
+                       : launch_pdl(rotate_kernel<T, D, INT8, VEC, false>, dim3(grid), dim3(kThreads), 0, st, 0, p);
+}
 template <typename T, int D>
 cudaError_t launch(const RotateParams& p, bool int8, bool vec, cudaStream_t st) {
   const unsigned grid = (unsigned)(((int64_t)p.rows + (1 << p.token_shift) - 1) >> p.token_shift);
-  if (int8) return vec ? launch_pdl(rotate_kernel<T, D, true, true>, dim3(grid), dim3(kThreads), 0, st, 0, p)
-                       : launch_pdl(rotate_kernel<T, D, true, false>, dim3(grid), dim3(kThreads), 0, st, 0, p);
-  return vec ? launch_pdl(rotate_kernel<T, D, false, true>, dim3(grid), dim3(kThreads), 0, st, 0, p)
-             : launch_pdl(rotate_kernel<T, D, false, false>, dim3(grid), dim3(kThreads), 0, st, 0, p);
+  if (int8) return vec ? launch_as<T, D, true, true>(p, grid, st) : launch_as<T, D, true, false>(p, grid, st);
+  return vec ? launch_as<T, D, false, true>(p, grid, st) : launch_as<T, D, false, false>(p, grid, st);
 }
 
 }  // namespace
@@ -325,8 +392,9 @@ extern "C" int lkv_paged_write_rotated(const lkv_rotate_args* a, void* stream) {
   p.q_weight = a->q_weight, p.k_weight = a->k_weight, p.eps = a->eps;
   p.pages = a->pages, p.scales = a->scales, p.n_pages = a->n_pages, p.page_shift = shift_of(a->bs);
   p.table = a->table, p.table_ld = a->table_ld, p.table_cols = a->table_cols, p.lens = a->lens, p.offsets = a->offsets, p.batch = a->batch;
-  // One token to a CTA until every SM has four CTAs.
-  p.token_shift = a->rows <= 4 * kNumSMs ? 0 : 2;
+  // As many tokens to a CTA, up to eight, as leave every SM two CTAs (their angles, places and waits are shared: a prompt of
+  // 32,768 tokens, 32 and 8 heads, d 128, to int8 in 186 us with eight, 189 with four).
+  while (p.token_shift < 3 && a->rows >> (p.token_shift + 1) >= 2 * kNumSMs) ++p.token_shift;
   const bool int8 = a->kind == LKV_CACHE_INT8;
   cudaStream_t st = as_stream(stream);
   cudaError_t e;

@@ -13,18 +13,57 @@ __device__ __forceinline__ float capped(float x, float c) {  // x: 2 s log2(e) /
   return fmaf(-2.0f * c, r, c);
 }
 
-// The same of two scores of up to the cap's size, without that unit, which the weights themselves keep busy: tanh(y) is
+// The same of N pairs of scores of up to the cap's size, without that unit, which the weights themselves keep busy: tanh(y) is
 // y times a polynomial of degree 6 in y^2, fitted on [0, 1] to least relative error (5 x 10^-8; 2^-22.6 in
-// float32). y: s / c; returns its squares (above 1: not good) and c tanh(y) + add.
-__device__ __forceinline__ uint64_t capped2(uint64_t y, float c, uint64_t add, uint64_t* square) {
+// float32). y: s / c; replaced by c tanh(y) + add, and `most` by the largest square where that is larger (above 1: not
+// good). Step by step for all pairs: one after the other they would wait for their own results.
+template <int N>
+__device__ __forceinline__ void capped2(uint64_t (&y)[N], float c, const uint64_t (&add)[N], float& most) {
   using namespace tc;
   constexpr float k[7] = {0.9999999403953552f, -0.33332839608192444f, 0.13325203955173492f, -0.05345702916383743f, 0.020289981737732887f, -0.006203379016369581f, 0.0010410224786028266f};
-  const uint64_t u = mul2(y, y);
-  uint64_t t = pair(k[6], k[6]);
+  uint64_t u[N], t[N];
 #pragma unroll
-  for (int i = 5; i >= 0; --i) t = fma2(t, u, pair(k[i], k[i]));
-  *square = u;
-  return fma2(mul2(y, pair(c, c)), t, add);
+  for (int n = 0; n < N; ++n) u[n] = mul2(y[n], y[n]);
+#pragma unroll
+  for (int n = 0; n < N; ++n) most = fmaxf(fmaxf(most, first_of(u[n])), second_of(u[n]));
+#pragma unroll
+  for (int n = 0; n < N; ++n) t[n] = fma2(pair(k[6], k[6]), u[n], pair(k[5], k[5]));
+#pragma unroll
+  for (int i = 4; i >= 0; --i) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) t[n] = fma2(t[n], u[n], pair(k[i], k[i]));
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) y[n] = mul2(y[n], pair(c, c));
+#pragma unroll
+  for (int n = 0; n < N; ++n) y[n] = fma2(y[n], t[n], add[n]);
+}
+
+#define LKV_R16(v, i) LKV_R8(v, i), LKV_R8(v, i + 8)
+#define LKV_R32(v, i) LKV_R16(v, i), LKV_R16(v, i + 16)
+
+// N columns of a thread's own lane of tensor memory (32 rows to a warp).
+template <int N>
+struct Lane {
+  uint32_t v[N];
+};
+__device__ __forceinline__ void ld(Lane<32>& f, uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : LKV_R32(f.v, 0)
+      : "r"(addr));
+}
+__device__ __forceinline__ void ld(Lane<16>& f, uint32_t addr) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : LKV_R16(f.v, 0)
+               : "r"(addr));
+}
+template <int N>
+__device__ __forceinline__ void ld_wait(Lane<N>& f) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(f.v[i]));
 }
 
 // Four int8 codes as bf16, exactly: 0x4300 | b is 128 + b for b < 128, and 0x4380 is 256.

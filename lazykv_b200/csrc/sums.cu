@@ -56,6 +56,8 @@ struct SumsParams {
   const float* sums;  // [batch, h, cap], or null: zeros
   float* out;
   int cap;
+  float* part;            // [2 CTAs][kPair]: sums of a tile's first and last chunks in the CTA's piece
+  int4* part_of;          // (1: a part, 3: the tile's last; sequence, head, step)
   float scale, cap_log2;  // scores x scale are in the log2 domain (capped: divided by the cap)
   uint64_t max_wait_ns;
 };
@@ -64,22 +66,24 @@ template <int D, bool INT8>
 struct Geometry {
   static constexpr int kHalves = D / 64, kHalfBytes = kTile * 128, kBytes = kHalves * kHalfBytes;
   static constexpr int kStages = INT8 ? 3 : 4;  // tiles of keys
-  static constexpr int kRawBytes = INT8 ? kTile * D : 0, kRaw = INT8 ? 3 : 0;
+  static constexpr int kRawBytes = INT8 ? kTile * D : 0, kRaw = INT8 ? 5 : 0;
+  // Query rows of a chunk: with int8 pages half as many, so that five tiles of codes may be under way.
+  static constexpr int kRows = INT8 ? 64 : 128, kQBytes = kHalves * kRows * 128;
   static constexpr int kThreads = INT8 ? 768 : 512;
   // Registers per thread: the warpgroups that sum take what the others leave of the launch's.
   static constexpr int kMany = INT8 ? 128 : 168, kFew = INT8 ? 56 : 80;
   static_assert(256 * kMany + (kThreads - 256) * kFew <= kThreads * (INT8 ? 80 : 128), "the register split is the launch's own");
-  static constexpr int kSmemTiles = (kStages + kQStages) * kBytes + kRaw * kRawBytes + (INT8 ? kInfo * kTile * 4 : 0);
+  static constexpr int kSmemTiles = kStages * kBytes + kQStages * kQBytes + kRaw * kRawBytes + (INT8 ? kInfo * kTile * 4 : 0);
   static constexpr int kSmem = (kSmemTiles > kMostBatch * 8 ? kSmemTiles : kMostBatch * 8) + 1024;
 };
 
 struct Barriers {
-  uint64_t k_full[4], k_empty[4], raw_full[3], raw_empty[3], q_full[kQStages], q_empty[kQStages], s_full[2][2], s_empty[2][2], info[kInfo], drain;
+  uint64_t k_full[4], k_empty[4], raw_full[5], raw_empty[5], q_full[kQStages], q_empty[kQStages], s_full[2][2], s_empty[2][2], info[kInfo], drain;
   alignas(16) float minus[kQStages][kTile];  // (read four at a time) -lse in the log2 domain; minus infinity: the row does not count
   alignas(16) int limit[kQStages][kTile];    // tokens that the row sees
   uint32_t have[kInfo];          // bit g: tokens 16 g .. 16 g + 15 of the tile have a page
-  int64_t pos, end;              // this CTA's piece of the line: where its first step begins, and where it ends
-  int b, k;                      // that step
+  int64_t jobs;                  // of this CTA's piece of the line
+  int b, j, step, chunk;         // its first
   uint64_t max_wait_ns;
   uint32_t tmem;
   int quit;
@@ -93,6 +97,7 @@ struct Sequence {
   int steps;        // of kPair tokens, per KV head
   int chunks;       // of query rows
 };
+template <int kRows>
 __device__ __forceinline__ Sequence sequence_of(const SumsParams& p, int b) {
   Sequence s;
   const int from = max(0, p.offsets[b]), end = min(p.rows, p.offsets[b + 1]), n = max(0, end - from), used = min(n, p.last);
@@ -103,58 +108,64 @@ __device__ __forceinline__ Sequence sequence_of(const SumsParams& p, int b) {
   s.limit = (int)max((int64_t)INT32_MIN / 2, min((int64_t)len - used + 1, (int64_t)INT32_MAX / 2));
   s.seen = (int)max((int64_t)0, min(min((int64_t)len, (int64_t)p.cap), (int64_t)p.table_cols << p.page_shift));
   s.steps = s.n_rows > 0 ? (s.seen + kPair - 1) / kPair : 0;
-  s.chunks = (s.n_rows + kTile - 1) / kTile;
+  s.chunks = (s.n_rows + kRows - 1) / kRows;
   return s;
 }
 
-// The steps of this CTA, in order; every role walks along.
+// The first chunk with a row that sees a token of the step (row r sees tokens up to limit + r / group).
+template <int kRows>
+__device__ __forceinline__ int first_chunk(const SumsParams& p, const Sequence& q, int step) {
+  const int64_t row = (int64_t)(step * kPair - q.limit + 1) * p.group;
+  return row < kRows ? 0 : (int)min((int64_t)(q.chunks - 1), row / kRows);
+}
+// Jobs of a sequence, per KV head.
+template <int kRows>
+__device__ __forceinline__ int64_t jobs_of(const SumsParams& p, const Sequence& q) {
+  int64_t n = (int64_t)q.steps * q.chunks;
+  for (int step = q.steps - 1; step >= 0; --step) {  // only steps among the chunk's own tokens have fewer
+    const int from = first_chunk<kRows>(p, q, step);
+    if (from == 0) break;
+    n -= from;
+  }
+  return n;
+}
+
+// The tiles of this CTA's piece, in order, each with the chunks that are the CTA's; every role walks along.
+template <int kRows>
 struct Walk {
   Sequence q;
-  int64_t pos, end;
-  int b, k, j, step, from;  // from: the first chunk with a row that sees a token of the step
-  bool first, last;         // of the CTA's steps of this sequence and head
-  __device__ __forceinline__ Walk(const SumsParams& p, const Barriers& s) : pos(s.pos), end(s.end), b(s.b), k(s.k), first(true) {
-    if (pos < end) q = sequence_of(p, b), place(p);
+  int64_t left;  // jobs from this tile on
+  int b, j, step;
+  int from, to;      // its chunks
+  bool begun, last;  // an earlier CTA has chunks of the tile; the CTA's last tile of this sequence and head
+  __device__ __forceinline__ Walk(const SumsParams& p, const Barriers& s) : left(s.jobs), b(s.b), j(s.j), step(s.step) {
+    if (left > 0) q = sequence_of<kRows>(p, b), place(s.chunk), begun = from > first_chunk<kRows>(p, q, step);
   }
-  __device__ __forceinline__ bool more() const { return pos < end; }
-  __device__ __forceinline__ void place(const SumsParams& p) {
-    j = k / q.steps, step = k - j * q.steps;
-    last = step == q.steps - 1 || pos + q.chunks >= end;
-    // Row r sees tokens up to limit + r / group: the chunk's last row decides.
-    const int64_t row = (int64_t)(step * kPair - q.limit + 1) * p.group;  // the first row that sees the step's first token
-    from = row <= 0 ? 0 : (int)min((int64_t)(q.chunks - 1), row / kTile);
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  __device__ __forceinline__ bool whole() const { return !begun && to == q.chunks; }
+  __device__ __forceinline__ void place(int chunk) {
+    from = chunk, to = (int)min((int64_t)q.chunks, chunk + left), begun = false;
+    last = step == q.steps - 1 || left <= to - from;
   }
   __device__ __forceinline__ void next(const SumsParams& p) {
-    pos += q.chunks;
-    first = last;
+    left -= to - from;
     if (!more()) return;
-    if (++k == p.h * q.steps) {
-      k = 0;
-      do q = sequence_of(p, ++b);
-      while (q.steps == 0 && b + 1 < p.batch);
-      if (q.steps == 0) {
-        pos = end;
-        return;
+    if (++step == q.steps) {
+      step = 0;
+      if (++j == p.h) {
+        j = 0;
+        do {
+          if (++b == p.batch) {
+            left = 0;
+            return;
+          }
+          q = sequence_of<kRows>(p, b);
+        } while (q.steps == 0);
       }
     }
-    place(p);
+    place(first_chunk<kRows>(p, q, step));
   }
 };
-
-// 16 columns of a thread's own lane of tensor memory.
-struct Lane {
-  uint32_t v[16];
-};
-__device__ __forceinline__ void ld(Lane& f, uint32_t addr) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-               : LKV_R8(f.v, 0), LKV_R8(f.v, 8)
-               : "r"(addr));
-}
-__device__ __forceinline__ void ld_wait(Lane& f) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(f.v[i]));
-}
 
 template <int D, bool INT8, bool CAP>
 __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(const SumsParams p, const __grid_constant__ CUtensorMap pages_map) {
@@ -164,7 +175,7 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
   __shared__ Barriers s;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   char* q_stages = smem;
-  char* stages = q_stages + kQStages * G::kBytes;
+  char* stages = q_stages + kQStages * G::kQBytes;
   char* raws = stages + kStages * G::kBytes;
   float* scale_ring = reinterpret_cast<float*>(raws + G::kRaw * G::kRawBytes);  // [kInfo][kTile]: the keys'
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, bs = 1 << p.page_shift;
@@ -205,8 +216,7 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
   // Every sequence's length on the line, into shared memory that no copy uses yet; then this CTA's piece.
   int64_t* lengths = reinterpret_cast<int64_t*>(smem);
   for (int b = tid; b < p.batch; b += G::kThreads) {
-    const Sequence q = sequence_of(p, b);
-    lengths[b] = (int64_t)q.steps * q.chunks * p.h;
+    lengths[b] = jobs_of<G::kRows>(p, sequence_of<G::kRows>(p, b)) * p.h;
   }
   __syncthreads();
   if (warp == 0) {
@@ -215,37 +225,45 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
     for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
     const int64_t n = gridDim.x, c = blockIdx.x;
     const int64_t lo = all / n * c + all % n * c / n, hi = all / n * (c + 1) + all % n * (c + 1) / n;
-    // The first step that begins at or behind lo.
-    int64_t before = 0;
-    int found = -1;
-    int64_t k = 0, pos = hi;
-    for (int b0 = 0; b0 < p.batch && found < 0 && lo < hi; b0 += 32) {
-      const int b = b0 + lane;
-      int64_t upto = b < p.batch ? lengths[b] : 0;
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
+    int64_t at = lo;
+    int b = 0, j = 0, step = 0;
+    if (lo < hi) {
+      for (;; b += 32) {  // the sequence, 32 at a time
+        int64_t upto = b + lane < p.batch ? lengths[b + lane] : 0;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += x;
+        }
+        const uint32_t behind = __ballot_sync(0xffffffffu, upto > at);
+        if (behind != 0) {
+          const int first = __ffs(behind) - 1;
+          if (first > 0) at -= __shfl_sync(0xffffffffu, upto, first - 1);
+          b += first;
+          break;
+        }
+        at -= __shfl_sync(0xffffffffu, upto, 31);
       }
-      const uint32_t behind = __ballot_sync(0xffffffffu, before + upto > lo);
-      if (behind != 0) {
-        const int l = __ffs(behind) - 1;
-        if (l > 0) before += __shfl_sync(0xffffffffu, upto, l - 1);
-        found = b0 + l;
-      } else {
-        before += __shfl_sync(0xffffffffu, upto, 31);
+      const Sequence q = sequence_of<G::kRows>(p, b);
+      const int64_t per_head = lengths[b] / p.h;
+      j = (int)(at / per_head);
+      at -= j * per_head;
+      step = (int)min(at / q.chunks, (int64_t)(q.steps - 1));
+      // (Steps among the chunk's own tokens have fewer jobs: the quotient is too low there.)
+      int64_t before = (int64_t)step * q.chunks;
+      for (int x = step - 1; x >= 0; --x) {
+        const int from = first_chunk<G::kRows>(p, q, x);
+        if (from == 0) break;
+        before -= from;
       }
+      for (;; ++step) {
+        const int n = q.chunks - first_chunk<G::kRows>(p, q, step);
+        if (at < before + n) break;
+        before += n;
+      }
+      at += first_chunk<G::kRows>(p, q, step) - before;
     }
-    if (found >= 0) {
-      const Sequence q = sequence_of(p, found);
-      k = (max(lo - before, (int64_t)0) + q.chunks - 1) / q.chunks;
-      pos = before + k * q.chunks;
-      while (pos < hi && k >= (int64_t)sequence_of(p, found).steps * p.h) {  // behind this sequence's last step: the next one's first
-        do ++found;
-        while (found + 1 < p.batch && lengths[found] == 0);
-        k = 0;
-      }
-    }
-    if (lane == 0) s.pos = pos, s.end = hi, s.b = max(found, 0), s.k = (int)k;
+    if (lane == 0) s.jobs = hi - lo, s.b = b, s.j = j, s.step = step, s.chunk = (int)at;
+    if (lane < 2) p.part_of[2 * blockIdx.x + lane] = make_int4(0, 0, 0, 0);
   }
   fence_async();
   __syncthreads();
@@ -258,11 +276,11 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
     const uint32_t ts = tmem + ((uint32_t)(warp % 4) << 21) + u * 2 * kTile;
     int q_count = 0, job = 0, tile = u;
     bool ok = true;
-    for (Walk w(p, s); w.more() && ok; w.next(p), tile += 2) {
+    for (Walk<G::kRows> w(p, s); w.more() && ok; w.next(p), tile += 2) {
       const int token = w.step * kPair + u * kTile + i, info = tile % kInfo;
       const int64_t at = ((int64_t)w.b * p.h + w.j) * p.cap + token;
       float old = 0.0f;
-      if (p.sums != nullptr && token < min(w.q.old, w.q.seen)) old = p.sums[at];
+      if (w.whole() && p.sums != nullptr && token < min(w.q.old, w.q.seen)) old = p.sums[at];
       ok = wait_for(s, &s.info[info], (tile / kInfo) & 1);
       if (!ok) break;
       const bool there = token < w.q.seen && (s.have[info] >> (i / 16) & 1);
@@ -270,13 +288,13 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
       const uint64_t factor2 = pair(factor, factor);
       uint64_t sum[2] = {0, 0};
       bool wide_step = false;  // capped scores above their cap's size
-      for (int c = w.from; c < w.q.chunks; ++c, ++job) {
+      for (int c = w.from; c < w.to; ++c, ++job) {
         const int buf = job & 1, stage = q_count % kQStages;
         ok = wait_for(s, &s.q_full[stage], (q_count / kQStages) & 1) && wait_for(s, &s.s_full[u][buf], (job >> 1) & 1);
         if (!ok) break;
         tc_after();
-        const int n_cols = min(kTile, w.q.n_rows - c * kTile);
-        const bool masked = n_cols % 16 != 0 || s.limit[stage][0] < w.step * kPair + u * kTile + kTile;
+        const int n_cols = min(G::kRows, w.q.n_rows - c * G::kRows);
+        const bool masked = n_cols % 32 != 0 || s.limit[stage][0] < w.step * kPair + u * kTile + kTile;
         const float4* minus = reinterpret_cast<const float4*>(s.minus[stage]);
         const int4* limit = reinterpret_cast<const int4*>(s.limit[stage]);
         // MASK: some row does not see the tile whole. WIDE: scores may be above their cap's size; false where one is and WIDE
@@ -285,44 +303,66 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
           constexpr bool MASK = decltype(mask)::value, WIDE = decltype(any_size)::value;
           uint64_t more[2] = {sum[0], sum[1]};
           float most = 0.0f;
-          auto add = [&](const Lane& f, int n) {
+          auto add = [&](const auto& f, int first) {  // columns from `first` on
+            constexpr int N = sizeof(f.v) / 4;
 #pragma unroll
-            for (int x = 0; x < 16; x += 4) {
-              const float4 m = minus[(16 * n + x) / 4];
-              [[maybe_unused]] int4 upto;
-              if constexpr (MASK) upto = limit[(16 * n + x) / 4];
+            for (int x = 0; x < N; x += 16) {  // step by step for eight pairs: their chains of results do not wait for one another
+              uint64_t z[8], by[8];
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                uint64_t z = pair(__uint_as_float(f.v[x + 2 * e]), __uint_as_float(f.v[x + 2 * e + 1]));
-                const uint64_t by = e == 0 ? pair(m.x, m.y) : pair(m.z, m.w);
-                if constexpr (!CAP) {
-                  z = fma2(z, factor2, by);
-                } else if constexpr (WIDE) {
-                  z = mul2(z, pair(2.0f * kLog2e * factor, 2.0f * kLog2e * factor));
-                  z = add2(pair(capped(first_of(z), p.cap_log2), capped(second_of(z), p.cap_log2)), by);
-                } else {
-                  uint64_t square;
-                  z = capped2(mul2(z, factor2), p.cap_log2, by, &square);
-                  most = fmaxf(fmaxf(most, first_of(square)), second_of(square));
-                }
-                z = pair(ex2(first_of(z)), ex2(second_of(z)));
-                if constexpr (MASK) z = pair(token < (e == 0 ? upto.x : upto.z) ? first_of(z) : 0.0f, token < (e == 0 ? upto.y : upto.w) ? second_of(z) : 0.0f);
-                more[e] = add2(more[e], z);
+              for (int e = 0; e < 8; e += 2) {
+                const float4 m = minus[(first + x) / 4 + e / 2];
+                by[e] = pair(m.x, m.y), by[e + 1] = pair(m.z, m.w);
               }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) z[e] = pair(__uint_as_float(f.v[x + 2 * e]), __uint_as_float(f.v[x + 2 * e + 1]));
+              if constexpr (!CAP) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = fma2(z[e], factor2, by[e]);
+              } else if constexpr (WIDE) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  z[e] = mul2(z[e], pair(2.0f * kLog2e * factor, 2.0f * kLog2e * factor));
+                  z[e] = add2(pair(capped(first_of(z[e]), p.cap_log2), capped(second_of(z[e]), p.cap_log2)), by[e]);
+                }
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = mul2(z[e], factor2);
+                capped2(z, p.cap_log2, by, most);
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) z[e] = pair(ex2(first_of(z[e])), ex2(second_of(z[e])));
+              if constexpr (MASK) {
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                  const int4 upto = limit[(first + x) / 4 + e / 2];
+                  z[e] = pair(token < upto.x ? first_of(z[e]) : 0.0f, token < upto.y ? second_of(z[e]) : 0.0f);
+                  z[e + 1] = pair(token < upto.z ? first_of(z[e + 1]) : 0.0f, token < upto.w ? second_of(z[e + 1]) : 0.0f);
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) more[e & 1] = add2(more[e & 1], z[e]);
             }
           };
-          Lane f[2];
-          const int n = (n_cols + 15) / 16;
-          ld(f[0], ts + buf * kTile);
-          ld_wait(f[0]);
+          const uint32_t from = ts + buf * kTile;
+          if (n_cols <= 16) {
+            Lane<16> f;
+            ld(f, from);
+            ld_wait(f);
+            add(f, 0);
+          } else {  // (columns past the last are masked)
+            constexpr int N = CAP ? 16 : 32;  // capped scores take longer, and more registers
+            Lane<N> f[2];
+            ld(f[0], from);
+            ld_wait(f[0]);
 #pragma unroll 1
-          for (int x = 0; x < n; x += 2) {
-            if (x + 1 < n) ld(f[1], ts + buf * kTile + 16 * (x + 1));
-            add(f[0], x);
-            if (x + 1 < n) ld_wait(f[1]);
-            if (x + 2 < n) ld(f[0], ts + buf * kTile + 16 * (x + 2));
-            if (x + 1 < n) add(f[1], x + 1);
-            if (x + 2 < n) ld_wait(f[0]);
+            for (int x = 0; x < n_cols; x += 2 * N) {
+              if (x + N < n_cols) ld(f[1], from + x + N);
+              add(f[0], x);
+              if (x + N < n_cols) ld_wait(f[1]);
+              if (x + 2 * N < n_cols) ld(f[0], from + x + 2 * N);
+              if (x + N < n_cols) add(f[1], x + N);
+              if (x + 2 * N < n_cols) ld_wait(f[0]);
+            }
           }
           if constexpr (CAP && !WIDE) {
             if (__any_sync(0xffffffffu, most > 1.0f)) return false;
@@ -349,32 +389,39 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
         }
       }
       const float got = (first_of(sum[0]) + second_of(sum[0])) + (first_of(sum[1]) + second_of(sum[1]));
-      if (token < p.cap) p.out[at] = old + (!ok ? __uint_as_float(0x7fc00000u) : there ? got : 0.0f);
+      const float mine = !ok ? __uint_as_float(0x7fc00000u) : there ? got : 0.0f;
+      if (w.whole()) {
+        if (token < p.cap) p.out[at] = old + mine;
+      } else {
+        const int slot = 2 * blockIdx.x + (w.begun ? 0 : 1);
+        p.part[(int64_t)slot * kPair + u * kTile + i] = mine;
+        if (warp == 0 && lane == 0) p.part_of[slot] = make_int4(w.to == w.q.chunks ? 3 : 1, w.b, w.j, w.step);
+      }
     }
   } else if (warp == 8) {
     // ---- matrix products ------------------------------------------------------------------------------
     const uint32_t q_u = smem_u32(q_stages), k_u = smem_u32(stages), mine = elect(), tm = __shfl_sync(0xffffffffu, tmem, 0);
     int q_count = 0, job = 0, tiles = 0;
     bool ok = true;
-    for (Walk w(p, s); w.more() && ok; w.next(p), tiles += 2) {
-      for (int c = w.from; ok && c < w.q.chunks; ++c, ++job) {
+    for (Walk<G::kRows> w(p, s); w.more() && ok; w.next(p), tiles += 2) {
+      for (int c = w.from; ok && c < w.to; ++c, ++job) {
         const int buf = job & 1, stage = q_count % kQStages;
         ok = wait_for(s, &s.q_full[stage], (q_count / kQStages) & 1);
-        const uint32_t inst = instruction<false>((min(kTile, w.q.n_rows - c * kTile) + 15) / 16 * 16, false);
+        const uint32_t inst = instruction<false>((min(G::kRows, w.q.n_rows - c * G::kRows) + 15) / 16 * 16, false);
         for (int u = 0; ok && u < 2; ++u) {
           const int slot = (tiles + u) % kStages;
           if (c == w.from) ok = wait_for(s, &s.k_full[slot], ((tiles + u) / kStages) & 1);
           if (ok && job >= 2) ok = wait_for(s, &s.s_empty[u][buf], ((job >> 1) - 1) & 1);
           if (!ok) break;
           tc_after();
-          const uint64_t a = desc_of(k_u + slot * G::kBytes, 16), b = desc_of(q_u + stage * G::kBytes, 16);
+          const uint64_t a = desc_of(k_u + slot * G::kBytes, 16), b = desc_of(q_u + stage * G::kQBytes, 16);
 #pragma unroll
           for (int x = 0; x < D / 16; ++x) {
-            const uint64_t off = ((x / 4) * G::kHalfBytes + (x % 4) * 32) / 16;
-            mma_ss(tm + u * 2 * kTile + buf * kTile, a + off, b + off, inst, x > 0, mine);
+            const uint32_t off = (x % 4) * 32;  // 16 channels further, or the next 64
+            mma_ss(tm + u * 2 * kTile + buf * kTile, a + ((x / 4) * G::kHalfBytes + off) / 16, b + ((x / 4) * (G::kRows * 128) + off) / 16, inst, x > 0, mine);
           }
           commit(&s.s_full[u][buf], mine);
-          if (c == w.q.chunks - 1) commit(&s.k_empty[slot], mine);
+          if (c == w.to - 1) commit(&s.k_empty[slot], mine);
         }
         if (!ok) break;
         if (w.q.chunks > 1 || w.last) {
@@ -395,25 +442,25 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
     constexpr int kSlots = INT8 ? G::kRaw : kStages;
     // Lane i has page i of each tile, looked up a step ahead (their ids, checked where they are used).
     int ahead[2] = {-1, -1};
-    auto look_up = [&](const Walk& w) {
+    auto look_up = [&](const Walk<G::kRows>& w) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int token = w.step * kPair + u * kTile + lane * bs;
         ahead[u] = w.more() && lane < per && token < w.q.seen ? p.table[w.b * p.table_ld + (token >> p.page_shift)] : -1;
       }
     };
-    Walk next(p, s);
+    Walk<G::kRows> next(p, s);
     look_up(next);
     while (next.more() && ok) {
-      const Walk w = next;
+      const Walk<G::kRows> w = next;
       const int pages[2] = {ahead[0], ahead[1]};
       next.next(p);
       look_up(next);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int slot = filled % kSlots, page = pages[u] < p.n_pages ? pages[u] : -1;
-        uint64_t* full = INT8 ? &s.raw_full[slot % 3] : &s.k_full[slot];
-        if (filled >= kSlots) ok = ok && wait_for(s, INT8 ? &s.raw_empty[slot % 3] : &s.k_empty[slot], (filled / kSlots - 1) & 1);
+        uint64_t* full = INT8 ? &s.raw_full[slot % 5] : &s.k_full[slot];
+        if (filled >= kSlots) ok = ok && wait_for(s, INT8 ? &s.raw_empty[slot % 5] : &s.k_empty[slot], (filled / kSlots - 1) & 1);
         if (!ok) break;
         const int info = filled % kInfo;
         const uint32_t granules = page >= 0 ? ((1u << (bs / 16)) - 1) << (lane * (bs / 16)) : 0u;
@@ -446,13 +493,13 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
       }
     }
     for (int n = max(0, filled - kInfo); n < filled; ++n) mbar_wait(&s.info[n % kInfo], (n / kInfo) & 1);
-    for (int n = max(0, filled - kSlots); n < filled; ++n) mbar_wait(INT8 ? &s.raw_full[n % 3] : &s.k_full[n % kSlots], (n / kSlots) & 1);
+    for (int n = max(0, filled - kSlots); n < filled; ++n) mbar_wait(INT8 ? &s.raw_full[n % 5] : &s.k_full[n % kSlots], (n / kSlots) & 1);
     __syncwarp();
   } else if (warp < 12) {
     // ---- slots that no step covers: what was there goes on, new and missing tokens have nothing -----------
     const int64_t n = (int64_t)p.batch * p.h;
     for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
-      const Sequence q = sequence_of(p, (int)(row / p.h));
+      const Sequence q = sequence_of<G::kRows>(p, (int)(row / p.h));
       const int go_on = min(q.old, q.seen);
       for (int64_t i = (int64_t)q.steps * kPair + tid - 10 * 32; i < p.cap; i += 64) {
         p.out[row * p.cap + i] = p.sums != nullptr && i < go_on ? p.sums[row * p.cap + i] : 0.0f;
@@ -462,21 +509,23 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
     // ---- queries: a thread has a row of the chunk ------------------------------------------------------
     const int r = tid % kTile;
     int q_count = 0;
-    bool ok = true;
-    for (Walk w(p, s); w.more() && ok; w.next(p)) {
-      if (w.q.chunks == 1 && !w.first) continue;
-      for (int c = w.from; c < w.q.chunks; ++c, ++q_count) {
-        const int stage = q_count % kQStages, row = c * kTile + r;
+    bool ok = true, here = false;  // here: the tile before had this sequence and head too
+    for (Walk<G::kRows> w(p, s); w.more() && ok; w.next(p)) {
+      const bool again = here;
+      here = !w.last;
+      if (w.q.chunks == 1 && again) continue;
+      for (int c = w.from; c < w.to; ++c, ++q_count) {
+        const int stage = q_count % kQStages, row = c * G::kRows + r;
         if (q_count >= kQStages) ok = wait_for(s, &s.q_empty[stage], (q_count / kQStages - 1) & 1);
         if (!ok) break;
-        const bool live = row < w.q.n_rows;
+        const bool live = r < G::kRows && row < w.q.n_rows;
         const int t = live ? row / p.group : 0, head = live ? w.j * p.group + row - t * p.group : 0;
         const __nv_bfloat16* src = p.q + (int64_t)(w.q.q0 + t) * p.q_st + (int64_t)head * p.q_sh;
-        char* dst = q_stages + stage * G::kBytes + r * 128;
-        if (row < w.q.n_rows + 16) {  // (rows of the product past the last one: zeros)
+        char* dst = q_stages + stage * G::kQBytes + r * 128;
+        if (r < G::kRows && row < w.q.n_rows + 16) {  // (rows of the product past the last one: zeros)
 #pragma unroll
           for (int i = 0; i < D / 8; ++i)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + (i / 8) * (kTile * 128) + (((i % 8) ^ (r & 7)) << 4))), "l"(src + 8 * i),
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + (i / 8) * (G::kRows * 128) + (((i % 8) ^ (r & 7)) << 4))), "l"(src + 8 * i),
                          "r"(live ? 16 : 0)
                          : "memory");
         }
@@ -499,7 +548,7 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
     const int to0 = row + ((at ^ (tok0 & 7)) << 4), to1 = row + (((at + 1) ^ (tok0 & 7)) << 4);
     bool ok = true;
     int n = u;
-    for (Walk w(p, s); w.more() && ok; w.next(p), n += 2) {
+    for (Walk<G::kRows> w(p, s); w.more() && ok; w.next(p), n += 2) {
       const int raw = n % G::kRaw, slot = n % kStages;
       ok = wait_for(s, &s.raw_full[raw], (n / G::kRaw) & 1);
       if (ok && n >= kStages) ok = wait_for(s, &s.k_empty[slot], (n / kStages - 1) & 1);
@@ -533,14 +582,43 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
   }
 }
 
+// Tiles whose chunks more than one CTA had: CTA c of the line began one and did not end it, the following ones have the
+// others.
+template <int kRows>
+__global__ void __launch_bounds__(kPair) sums_merge_kernel(const SumsParams p) {
+  pdl_wait();
+  pdl_release();
+  const int c = blockIdx.x;
+  const int4 of = p.part_of[2 * c + 1];
+  if (of.x == 0) return;
+  const Sequence q = sequence_of<kRows>(p, of.y);
+  const int token = of.w * kPair + threadIdx.x;
+  const int64_t at = ((int64_t)of.y * p.h + of.z) * p.cap + token;
+  float sum = p.part[(int64_t)(2 * c + 1) * kPair + threadIdx.x];
+  for (int k = c + 1; k < (int)gridDim.x; ++k) {
+    const int state = p.part_of[2 * k].x;
+    if (state == 0) continue;  // (fewer jobs than CTAs: that one had none)
+    sum += p.part[(int64_t)2 * k * kPair + threadIdx.x];
+    if (state == 3) break;
+  }
+  if (token < p.cap) p.out[at] = (p.sums != nullptr && token < min(q.old, q.seen) ? p.sums[at] : 0.0f) + sum;
+}
+
 template <int D, bool INT8, bool CAP>
 cudaError_t launch(const SumsParams& p, const CUtensorMap& map, int grid, cudaStream_t st) {
   using G = Geometry<D, INT8>;
   auto k = sums_kernel<D, INT8, CAP>;
   static std::atomic<uint64_t> done{0};
-  const cudaError_t e = prefix::allow_smem(k, G::kSmem, done);
-  return e != cudaSuccess ? e : launch_pdl(k, dim3(grid), dim3(G::kThreads), G::kSmem, st, 0, p, map);
+  cudaError_t e = prefix::allow_smem(k, G::kSmem, done);
+  if (e == cudaSuccess) e = launch_pdl(k, dim3(grid), dim3(G::kThreads), G::kSmem, st, 0, p, map);
+  // (Where all rows of the call are one chunk no tile is cut.)
+  if (e == cudaSuccess && (int64_t)p.rows * p.group > G::kRows) e = launch_pdl(sums_merge_kernel<G::kRows>, dim3(grid), dim3(kPair), 0, st, 0, p);
+  return e;
 }
+
+// One CTA per SM, or one per 256 slots (they write the slots that no job covers, too).
+int grid_of(int cap, int batch, int h) { return (int)std::min<int64_t>(kNumSMs, ((int64_t)cap + kPair - 1) / kPair * h * batch); }
+constexpr size_t kPartBytes = 2 * (kPair * sizeof(float) + sizeof(int4));  // of a CTA
 
 }  // namespace
 
@@ -550,6 +628,10 @@ cudaError_t sums_status_attach(int* mirror) { return tu_status_attach(mirror); }
 }  // namespace lkv
 
 using namespace lkv;
+
+extern "C" size_t lkv_attention_sums_workspace(int batch, int h, int cap) {
+  return batch <= 0 || h <= 0 || cap <= 0 ? 0 : grid_of(cap, batch, h) * kPartBytes;
+}
 
 extern "C" int lkv_attention_sums(const lkv_sums_args* a, void* stream) {
   static const char* who = "lkv_attention_sums";
@@ -590,9 +672,11 @@ extern "C" int lkv_attention_sums(const lkv_sums_args* a, void* stream) {
                                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(LKV_ERR_CUDA, "%s: the pages' tensor map was refused (%d)", who, (int)r);
   }
-  // One CTA per SM, or one per step that the call can have at most (some all the same: they write the other slots).
-  const int64_t steps = ((int64_t)a->cap + kPair - 1) / kPair * a->h * a->batch;
-  const int grid = (int)std::min<int64_t>(kNumSMs, steps);
+  const int grid = grid_of(a->cap, a->batch, a->h);
+  if (a->workspace == nullptr || a->workspace_bytes < grid * kPartBytes) return fail(LKV_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, a->workspace_bytes, grid * kPartBytes);
+  if (!aligned(a->workspace, 16)) return fail(LKV_ERR_PTR, "%s: workspace must be 16-byte aligned", who);
+  p.part_of = static_cast<int4*>(a->workspace);
+  p.part = reinterpret_cast<float*>(p.part_of + 2 * grid);
   cudaStream_t st = as_stream(stream);
   auto go = [&](auto dim) {
     constexpr int D = decltype(dim)::value;

@@ -577,13 +577,6 @@ def paged_read(pages: torch.Tensor, table: torch.Tensor, starts: torch.Tensor, n
     return out
 
 
-def _packed(who: str, name: str, t: torch.Tensor, rows: int, d: int, dtype: torch.dtype) -> tuple[int, int, int]:
-    """(heads, token stride, head stride) of packed rows [rows, heads, d] with contiguous channels."""
-    if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != d or t.dtype is not dtype or t.stride(2) != 1:
-        raise ValueError(f"{who}: {name} must be {dtype} [{rows}, heads, {d}] with contiguous channels, got {t.dtype} {tuple(t.shape)}")
-    return t.shape[1], t.stride(0), t.stride(1)
-
-
 def paged_write_rotated(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, pages: torch.Tensor,
                         table: torch.Tensor, lens: torch.Tensor, offsets: torch.Tensor, scales: torch.Tensor | None = None, q_weight: torch.Tensor | None = None,
                         k_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -599,36 +592,46 @@ def paged_write_rotated(query: torch.Tensor, keys: torch.Tensor, values: torch.T
     rotation's only, not the place in the pages.
     """
     who = "paged_write_rotated"
-    index = _one_device(who, query, keys, values, positions, frequencies, pages, table, lens, offsets, scales, q_weight, k_weight, out)
+    index = keys.get_device()
+    if index < 0 or not (query.get_device() == values.get_device() == positions.get_device() == frequencies.get_device() == pages.get_device() == table.get_device()
+                         == lens.get_device() == offsets.get_device() == index):
+        _one_device(who, query, keys, values, positions, frequencies, pages, table, lens, offsets)
     n, h, bs, d, kind, at, batch, ld, cols = _cache_geometry(who, pages, scales, table)
-    dtype, rows = keys.dtype, keys.shape[0]
-    code = 1 if dtype is _BF16 else dtype_code(dtype)
-    kh, k_st, k_sh = _packed(who, "keys", keys, rows, d, dtype)
-    vh, v_st, v_sh = _packed(who, "values", values, rows, d, dtype)
-    hq, q_st, q_sh = _packed(who, "query", query, rows, d, dtype)
-    if kh != h or vh != h or (kind == 0 and pages.dtype is not dtype):
-        raise ValueError(f"{who}: {dtype} keys of {kh} heads and values of {vh} do not fit pages {tuple(pages.shape)} {pages.dtype}")
+    dtype, shape, q_shape = keys.dtype, keys.shape, query.shape
+    if len(q_shape) != 3 or len(shape) != 3 or shape[1:] != (h, d) or q_shape[::2] != shape[::2] or values.shape != shape or not (query.dtype is values.dtype is dtype) or (
+            kind == 0 and pages.dtype is not dtype):
+        raise ValueError(f"{who}: query [rows, hq, d], keys and values [rows, h, d] of one type must fit pages {tuple(pages.shape)} {pages.dtype}; got {query.dtype} "
+                         f"{tuple(q_shape)}, {dtype} {tuple(shape)} and {values.dtype} {tuple(values.shape)}")
+    rows, hq = shape[0], q_shape[1]
+    (k_st, k_sh, kc), (v_st, v_sh, vc), (q_st, q_sh, qc) = keys.stride(), values.stride(), query.stride()
+    if kc != 1 or vc != 1 or qc != 1:
+        raise ValueError(f"{who}: channels must be contiguous")
     if positions.dtype is not _I32 or positions.shape != (rows,) or not positions.is_contiguous():
         raise ValueError(f"{who}: positions must be a contiguous int32 [{rows}]")
     pairs = frequencies.numel()
-    if frequencies.dtype is not _F32 or frequencies.dim() != 1 or not frequencies.is_contiguous() or pairs % 4 or 2 * pairs > d:
+    if frequencies.dtype is not _F32 or frequencies.dim() != 1 or not frequencies.is_contiguous() or pairs & 3 or 2 * pairs > d:
         raise ValueError(f"{who}: frequencies must be a contiguous float32 [n], n a multiple of 4 and at most {d // 2}, got {frequencies.dtype} {tuple(frequencies.shape)}")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.dtype is not dtype or w.shape != (d,) or not w.is_contiguous()):
-            raise ValueError(f"{who}: {name} must be a contiguous {dtype} [{d}], got {w.dtype} {tuple(w.shape)}")
+    weights = [0, 0]
+    for i, w in enumerate((q_weight, k_weight)):
+        if w is not None:
+            if w.dtype is not dtype or w.shape != (d,) or not w.is_contiguous() or w.get_device() != index:
+                raise ValueError(f"{who}: {'qk'[i]}_weight must be a contiguous {dtype} [{d}] on cuda:{index}, got {w.dtype} {tuple(w.shape)}")
+            weights[i] = w.data_ptr()
     if not eps >= 0:
         raise ValueError(f"{who}: eps {eps}")
     _per_sequence(who, "lens", lens, batch)
     _per_sequence(who, "offsets", offsets, batch + 1)
     if out is None:
-        out = query.new_empty((rows, hq, d))
-    oh, o_st, o_sh = _packed(who, "out", out, rows, d, dtype)
-    if oh != hq:
-        raise ValueError(f"{who}: out of {oh} heads for a query of {hq}")
+        out = query.new_empty(q_shape)
+    elif out.shape != q_shape or out.dtype is not dtype or out.stride(2) != 1 or out.get_device() != index:
+        raise ValueError(f"{who}: out must be {dtype} {tuple(q_shape)} with contiguous channels on cuda:{index}")
+    o_st, o_sh, _ = out.stride()
+    if scales is not None and scales.get_device() != index:
+        _one_device(who, pages, scales)
     _run("lkv_paged_write_rotated", L.ROTATE_ARGS.pack(
-        query.data_ptr(), keys.data_ptr(), values.data_ptr(), q_st, q_sh, k_st, k_sh, v_st, v_sh, out.data_ptr(), o_st, o_sh, code, rows, hq, h, d,
-        positions.data_ptr(), frequencies.data_ptr(), pairs, int(interleaved), 0 if q_weight is None else q_weight.data_ptr(),
-        0 if k_weight is None else k_weight.data_ptr(), eps, pages.data_ptr(), kind, at, n, bs, table.data_ptr(), ld, cols, lens.data_ptr(), offsets.data_ptr(), batch), index)
+        query.data_ptr(), keys.data_ptr(), values.data_ptr(), q_st, q_sh, k_st, k_sh, v_st, v_sh, out.data_ptr(), o_st, o_sh, 1 if dtype is _BF16 else dtype_code(dtype), rows, hq, h,
+        d, positions.data_ptr(), frequencies.data_ptr(), pairs, interleaved, weights[0], weights[1], eps, pages.data_ptr(), kind, at, n, bs, table.data_ptr(), ld, cols,
+        lens.data_ptr(), offsets.data_ptr(), batch), index)
     return out
 
 
@@ -646,24 +649,29 @@ def paged_evict(pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, su
     slots without a token. A token without a page is ranked like the others and not moved.
     """
     who = "paged_evict"
-    index = _one_device(who, pages, table, lens, sums, positions, since, scales)
+    index = pages.get_device()
+    if index < 0 or not (table.get_device() == lens.get_device() == sums.get_device() == positions.get_device() == index) or (since is not None and since.get_device() != index) or (
+            scales is not None and scales.get_device() != index):
+        _one_device(who, pages, table, lens, sums, positions, since, scales)
     n, h, bs, d, kind, at, batch, ld, cols = _cache_geometry(who, pages, scales, table)
     _per_sequence(who, "lens", lens, batch)
     if since is not None:
         _per_sequence(who, "since", since, batch)
-    if sums.dtype is not _F32 or sums.dim() != 3 or sums.shape[:2] != (batch, h) or not sums.is_contiguous():
-        raise ValueError(f"{who}: sums must be a contiguous float32 [{batch}, {h}, slots], got {sums.dtype} {tuple(sums.shape)}")
-    if positions.dtype is not _I32 or positions.shape != sums.shape or not positions.is_contiguous():
-        raise ValueError(f"{who}: positions must be a contiguous int32 {tuple(sums.shape)}, got {positions.dtype} {tuple(positions.shape)}")
-    cap = sums.shape[2]
+    shape = sums.shape
+    if sums.dtype is not _F32 or len(shape) != 3 or shape[:2] != (batch, h) or not sums.is_contiguous():
+        raise ValueError(f"{who}: sums must be a contiguous float32 [{batch}, {h}, slots], got {sums.dtype} {tuple(shape)}")
+    if positions.dtype is not _I32 or positions.shape != shape or not positions.is_contiguous():
+        raise ValueError(f"{who}: positions must be a contiguous int32 {tuple(shape)}, got {positions.dtype} {tuple(positions.shape)}")
+    cap = shape[2]
     if keep < 1:
         raise ValueError(f"{who}: a budget of {keep} tokens")
     code = 0 if kind == 1 else dtype_code(pages.dtype)
     if out is None:
         out = torch.empty_like(sums), torch.empty_like(positions)
-    for o, like in zip(out, (sums, positions)):
-        if o.dtype is not like.dtype or o.shape != like.shape or not o.is_contiguous() or o.get_device() != index:
-            raise ValueError(f"{who}: out must be like sums and positions, {tuple(sums.shape)} on cuda:{index}")
+    else:
+        for o, like in zip(out, (sums, positions)):
+            if o.dtype is not like.dtype or o.shape != shape or not o.is_contiguous() or o.get_device() != index:
+                raise ValueError(f"{who}: out must be like sums and positions, {tuple(shape)} on cuda:{index}")
     left = torch.empty_like(lens)
     nbytes = batch * h * min(keep, cap - keep) * 8 if cap > keep else 0
     ws = lens.new_empty(nbytes // 4) if nbytes else None
@@ -757,7 +765,9 @@ def chunk_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tenso
     rounded to bfloat16 (2^-8) where they multiply the values. The workspace comes from torch's allocator call by call.
     """
     who = "chunk_attention"
-    index = _one_device(who, query, pages, table, lens, offsets, scales, prefix_table, out, lse)
+    index = query.get_device()
+    if index < 0 or not (pages.get_device() == table.get_device() == lens.get_device() == offsets.get_device() == index):
+        _one_device(who, query, pages, table, lens, offsets)
     n, h, bs, d, kind, at, batch, ld, cols = _cache_geometry(who, pages, scales, table)
     if query.dim() != 3 or query.dtype is not _BF16 or query.shape[2] != d or query.shape[1] < 1 or query.shape[1] % h or (kind == 0 and pages.dtype is not _BF16):
         raise ValueError(f"{who}: query must be bfloat16 [rows, heads, {d}], heads a multiple of {h}, over bfloat16 or int8 pages; got {query.dtype} "
@@ -768,8 +778,8 @@ def chunk_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tenso
     pcols = 0
     if prefix_table is not None:
         pcols = prefix_table.numel()
-        if prefix_table.dtype is not _I32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous():
-            raise ValueError(f"{who}: prefix_table must be a contiguous int32 [columns]")
+        if prefix_table.dtype is not _I32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous() or prefix_table.get_device() != index:
+            raise ValueError(f"{who}: prefix_table must be a contiguous int32 [columns] on cuda:{index}")
     if not 0 <= prefix_len <= pcols * bs:
         raise ValueError(f"{who}: prefix_table of {pcols} pages of {bs} cannot hold {prefix_len} tokens")
     if not 0 <= cap < math.inf:
@@ -778,13 +788,16 @@ def chunk_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tenso
     if sc != 1 or (st | sh) & 7 or query.data_ptr() & 15:
         query = query.clone(memory_format=torch.contiguous_format)
         st, sh, _ = query.stride()
-    for name, o, shape, dtype in (("out", out, (rows, hq, d), _BF16), ("lse", lse, (rows, hq), _F32)):
-        if o is not None and (o.shape != shape or o.dtype is not dtype or not o.is_contiguous()):
-            raise ValueError(f"{who}: {name} must be a contiguous {dtype} {shape}, got {o.dtype} {tuple(o.shape)}")
     if out is None:
         out = query.new_empty((rows, hq, d))
+    elif out.shape != (rows, hq, d) or out.dtype is not _BF16 or not out.is_contiguous() or out.get_device() != index:
+        raise ValueError(f"{who}: out must be a contiguous bfloat16 {(rows, hq, d)} on cuda:{index}")
     if lse is None:
         lse = query.new_empty((rows, hq), dtype=_F32)
+    elif lse.shape != (rows, hq) or lse.dtype is not _F32 or not lse.is_contiguous() or lse.get_device() != index:
+        raise ValueError(f"{who}: lse must be a contiguous float32 {(rows, hq)} on cuda:{index}")
+    if scales is not None and scales.get_device() != index:
+        _one_device(who, query, scales)
     nbytes = _chunk_workspace(rows, batch, hq, h, d, prefix_len, cols * bs)
     ws = query.new_empty((nbytes + 1) // 2) if nbytes else None
     _run("lkv_chunk_attention", L.CHUNK_ARGS.pack(
@@ -793,11 +806,16 @@ def chunk_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tenso
     return out, lse
 
 
+@functools.lru_cache(maxsize=4096)
+def _sums_workspace(batch: int, h: int, slots: int) -> int:
+    return int(L.lib().lkv_attention_sums_workspace(batch, h, slots))
+
+
 def attention_sums(query: torch.Tensor, lse: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, offsets: torch.Tensor, scale: float,
                    sums: torch.Tensor | None = None, last: int | None = None, cap: float = 0.0, scales: torch.Tensor | None = None,
                    out: torch.Tensor | None = None) -> torch.Tensor:
     """The attention weight that every own token got from the queries of the chunks, added to `sums` (lkv_attention_sums, one
-    launch): [batch, h, slots] float32, slots = columns * block size without sums or out. query, offsets, lens, scale and cap
+    or two launches): [batch, h, slots] float32, slots = columns * block size without sums or out. query, offsets, lens, scale and cap
     are those of chunk_attention, lse [rows, hq] what it (or prefix_attention) returned. With `last`, only the last so many
     query tokens of each chunk count. What paged_evict ranks tokens by.
 
@@ -806,7 +824,10 @@ def attention_sums(query: torch.Tensor, lse: torch.Tensor, pages: torch.Tensor, 
     float32 in the order of the queries, the same every time.
     """
     who = "attention_sums"
-    index = _one_device(who, query, lse, pages, table, lens, offsets, sums, scales, out)
+    index = query.get_device()
+    if index < 0 or not (lse.get_device() == pages.get_device() == table.get_device() == lens.get_device() == offsets.get_device() == index) or (
+            scales is not None and scales.get_device() != index):
+        _one_device(who, query, lse, pages, table, lens, offsets, scales)
     n, h, bs, d, kind, at, batch, ld, cols = _cache_geometry(who, pages, scales, table)
     if query.dim() != 3 or query.dtype is not _BF16 or query.shape[2] != d or query.shape[1] < 1 or query.shape[1] % h or (kind == 0 and pages.dtype is not _BF16):
         raise ValueError(f"{who}: query must be bfloat16 [rows, heads, {d}], heads a multiple of {h}, over bfloat16 or int8 pages; got {query.dtype} "
@@ -818,8 +839,8 @@ def attention_sums(query: torch.Tensor, lse: torch.Tensor, pages: torch.Tensor, 
     _per_sequence(who, "offsets", offsets, batch + 1)
     slots = cols * bs if sums is None and out is None else (out if sums is None else sums).shape[-1]
     for name, t in (("sums", sums), ("out", out)):
-        if t is not None and (t.dtype is not _F32 or t.shape != (batch, h, slots) or not t.is_contiguous()):
-            raise ValueError(f"{who}: {name} must be a contiguous float32 [{batch}, {h}, {slots}], got {t.dtype} {tuple(t.shape)}")
+        if t is not None and (t.dtype is not _F32 or t.shape != (batch, h, slots) or not t.is_contiguous() or t.get_device() != index):
+            raise ValueError(f"{who}: {name} must be a contiguous float32 [{batch}, {h}, {slots}] on cuda:{index}, got {t.dtype} {tuple(t.shape)}")
     if last is not None and last < 1:
         raise ValueError(f"{who}: the last {last} tokens of a chunk")
     if not 0 <= cap < math.inf:
@@ -830,9 +851,12 @@ def attention_sums(query: torch.Tensor, lse: torch.Tensor, pages: torch.Tensor, 
         st, sh, _ = query.stride()
     if out is None:
         out = query.new_empty((batch, h, slots), dtype=_F32)
+    nbytes = _sums_workspace(batch, h, slots)
+    ws = query.new_empty((nbytes + 1) // 2) if nbytes else None
     _run("lkv_attention_sums", L.SUMS_ARGS.pack(
         query.data_ptr(), st, sh, 1, rows, hq, h, d, lse.data_ptr(), pages.data_ptr(), kind, at, n, bs, table.data_ptr(), ld, cols, lens.data_ptr(), offsets.data_ptr(), batch,
-        2**31 - 1 if last is None else min(last, 2**31 - 1), 0 if sums is None else sums.data_ptr(), out.data_ptr(), slots, scale, cap), index)
+        2**31 - 1 if last is None else min(last, 2**31 - 1), 0 if sums is None else sums.data_ptr(), out.data_ptr(), slots, scale, cap,
+        0 if ws is None else ws.data_ptr(), nbytes), index)
     return out
 
 
