@@ -378,7 +378,11 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
             for (bool set = unset, again = false;; again = true) {
               if (set) {
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                sweep([&](const Frag& f, int n) {
+#pragma unroll 1
+                for (int n = 0; n < N; ++n) {
+                  Frag f;
+                  ld(f, ts + 16 * n);
+                  ld_wait(f);
 #pragma unroll
                   for (int k = 0; k < 2; ++k) {
                     [[maybe_unused]] uint64_t kk = 0;
@@ -391,7 +395,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
                       top[r] = fmaxf(fmaxf(top[r], first_of(z)), second_of(z));
                     }
                   }
-                });
+                }
                 float by[4];
                 bool none = false;
 #pragma unroll
@@ -483,10 +487,10 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
           };
           const std::true_type yes;
           const std::false_type no;
-          if (CAP && wide_unit) {
-            if (masked) weigh(yes, yes);
-            else weigh(no, yes);
-          } else if (!(masked ? weigh(yes, no) : weigh(no, no))) {
+          if constexpr (!CAP) {
+            if (masked) weigh(yes, no);
+            else weigh(no, no);
+          } else if (wide_unit || !(masked ? weigh(yes, no) : weigh(no, no))) {
             wide_unit = true;  // large scores come together
             if (masked) weigh(yes, yes);
             else weigh(no, yes);

@@ -74,6 +74,10 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p) {
   pdl_release();
   const cg::cluster_group cluster = cg::this_cluster();
   const int rank = cluster.block_rank(), n_ranks = cluster.num_blocks();
+  auto sync = [&] {
+    if (n_ranks == 1) __syncthreads();
+    else cluster.sync();
+  };
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int row = blockIdx.x / n_ranks, b = row / p.h, j = row % p.h;
   const int n = (int)max((int64_t)0, min((int64_t)p.lens[b], min((int64_t)p.cap, (int64_t)p.table_cols << p.page_shift)));
@@ -119,7 +123,7 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p) {
       const uint32_t k = key(i);
       if (pass == 0 || (k >> above) == found) atomicAdd(&s.hist[pass][(k >> shift) & (pass == 2 ? 1023u : 2047u)], 1u);
     }
-    cluster.sync();
+    sync();
     // Thread t has the four bins 2047 - 4 t and below.
     uint32_t count[4] = {0, 0, 0, 0};
     for (int r = 0; r < n_ranks; ++r) {
@@ -157,7 +161,7 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p) {
     for (int w = 0; w < kWarps; ++w) sum += s.ties[w];
     s.all_ties = sum;
   }
-  cluster.sync();
+  sync();
   uint32_t tie_base = 0;
   for (int r = 0; r < rank; ++r) tie_base += *cluster.map_shared_rank(&s.all_ties, r);
   for (int w = 0; w < warp; ++w) tie_base += s.ties[w];
@@ -184,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p) {
     for (int w = 0; w < kWarps; ++w) sum.x += s.moving[w].x, sum.y += s.moving[w].y;
     s.all_moving = sum;
   }
-  cluster.sync();
+  sync();
   uint2 base = make_uint2(0, 0);
   uint32_t n_moves = 0;
   for (int r = 0; r < n_ranks; ++r) {
@@ -200,7 +204,7 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p) {
     base.x += __popc(lose), base.y += __popc(move);
     if (kept && i < p.keep) out_sums[i] = sums[i], out_positions[i] = positions[i];
   });
-  cluster.sync();
+  sync();
 
   constexpr int kChunks = RB / 16, kPer = 2 * kChunks;  // 16-byte pieces of a row, of a token's key and value
   const int bs = 1 << p.page_shift;
@@ -232,7 +236,7 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p) {
       if (r >= 0) *reinterpret_cast<uint4*>(pages + (r + (c / kChunks) * bs) * RB + (c % kChunks) * 16) = x[i];
     }
   }
-  cluster.sync();  // (in place, the tail's sums are read by the moves)
+  sync();  // (in place, the tail's sums are read by the moves)
   clear();
 }
 

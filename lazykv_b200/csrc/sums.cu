@@ -35,8 +35,9 @@ using prefix::kLog2e;
 constexpr int kPair = 2 * kTile;  // tokens of a step
 constexpr int kMostBatch = 8192;
 constexpr int kQStages = 2;
-// Tiles whose scales and page bits are kept. A tile's copies begin when the keys at most three tiles before it have been
-// multiplied, and those are not before the scores two steps (four tiles) back are read.
+// Tiles whose scales and page bits are kept. A tile's copies begin when the codes at most six tiles before it have been turned
+// into operands, that when the keys four tiles before have been multiplied, and that when the scores two steps (four tiles) back
+// are read: fourteen tiles.
 constexpr int kInfo = 16;
 
 struct SumsParams {
@@ -65,9 +66,9 @@ struct SumsParams {
 template <int D, bool INT8>
 struct Geometry {
   static constexpr int kHalves = D / 64, kHalfBytes = kTile * 128, kBytes = kHalves * kHalfBytes;
-  static constexpr int kStages = INT8 ? 3 : 4;  // tiles of keys
-  static constexpr int kRawBytes = INT8 ? kTile * D : 0, kRaw = INT8 ? 5 : 0;
-  // Query rows of a chunk: with int8 pages half as many, so that five tiles of codes may be under way.
+  static constexpr int kStages = 4;  // tiles of keys: two steps
+  static constexpr int kRawBytes = INT8 ? kTile * D : 0, kRaw = INT8 ? (D == 128 ? 3 : 6) : 0;
+  // Query rows of a chunk: with int8 pages fewer, which leaves room for codes under way.
   static constexpr int kRows = INT8 ? 64 : 128, kQBytes = kHalves * kRows * 128;
   static constexpr int kThreads = INT8 ? 768 : 512;
   // Registers per thread: the warpgroups that sum take what the others leave of the launch's.
@@ -78,7 +79,7 @@ struct Geometry {
 };
 
 struct Barriers {
-  uint64_t k_full[4], k_empty[4], raw_full[5], raw_empty[5], q_full[kQStages], q_empty[kQStages], s_full[2][2], s_empty[2][2], info[kInfo], drain;
+  uint64_t k_full[4], k_empty[4], raw_full[6], raw_empty[6], q_full[kQStages], q_empty[kQStages], s_full[2][2], s_empty[2][2], info[kInfo], drain;
   alignas(16) float minus[kQStages][kTile];  // (read four at a time) -lse in the log2 domain; minus infinity: the row does not count
   alignas(16) int limit[kQStages][kTile];    // tokens that the row sees
   uint32_t have[kInfo];          // bit g: tokens 16 g .. 16 g + 15 of the tile have a page
@@ -372,10 +373,10 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
         };
         const std::true_type yes;
         const std::false_type no;
-        if (CAP && wide_step) {
-          if (masked) all(yes, yes);
-          else all(no, yes);
-        } else if (!(masked ? all(yes, no) : all(no, no))) {
+        if constexpr (!CAP) {
+          if (masked) all(yes, no);
+          else all(no, no);
+        } else if (wide_step || !(masked ? all(yes, no) : all(no, no))) {
           wide_step = true;
           if (masked) all(yes, yes);
           else all(no, yes);
@@ -459,8 +460,8 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int slot = filled % kSlots, page = pages[u] < p.n_pages ? pages[u] : -1;
-        uint64_t* full = INT8 ? &s.raw_full[slot % 5] : &s.k_full[slot];
-        if (filled >= kSlots) ok = ok && wait_for(s, INT8 ? &s.raw_empty[slot % 5] : &s.k_empty[slot], (filled / kSlots - 1) & 1);
+        uint64_t* full = INT8 ? &s.raw_full[slot % 6] : &s.k_full[slot];
+        if (filled >= kSlots) ok = ok && wait_for(s, INT8 ? &s.raw_empty[slot % 6] : &s.k_empty[slot], (filled / kSlots - 1) & 1);
         if (!ok) break;
         const int info = filled % kInfo;
         const uint32_t granules = page >= 0 ? ((1u << (bs / 16)) - 1) << (lane * (bs / 16)) : 0u;
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
       }
     }
     for (int n = max(0, filled - kInfo); n < filled; ++n) mbar_wait(&s.info[n % kInfo], (n / kInfo) & 1);
-    for (int n = max(0, filled - kSlots); n < filled; ++n) mbar_wait(INT8 ? &s.raw_full[n % 5] : &s.k_full[n % kSlots], (n / kSlots) & 1);
+    for (int n = max(0, filled - kSlots); n < filled; ++n) mbar_wait(INT8 ? &s.raw_full[n % kSlots % 6] : &s.k_full[n % kSlots], (n / kSlots) & 1);
     __syncwarp();
   } else if (warp < 12) {
     // ---- slots that no step covers: what was there goes on, new and missing tokens have nothing -----------
@@ -652,7 +653,12 @@ extern "C" int lkv_attention_sums(const lkv_sums_args* a, void* stream) {
   if (a->lens == nullptr || a->offsets == nullptr || a->out == nullptr || (a->table == nullptr && a->table_cols > 0) || (a->rows > 0 && (a->q == nullptr || a->lse == nullptr)))
     return fail(LKV_ERR_PTR, "%s: null pointer", who);
   if (!aligned(a->q, 16) || (a->q_st & 7) != 0 || (a->q_sh & 7) != 0) return fail(LKV_ERR_PTR, "%s: query rows must be 16-byte aligned", who);
+  const int grid = grid_of(a->cap, a->batch, a->h);
+  if (a->workspace == nullptr || a->workspace_bytes < grid * kPartBytes) return fail(LKV_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, a->workspace_bytes, grid * kPartBytes);
+  if (!aligned(a->workspace, 16)) return fail(LKV_ERR_PTR, "%s: workspace must be 16-byte aligned", who);
   SumsParams p = {};
+  p.part_of = static_cast<int4*>(a->workspace);
+  p.part = reinterpret_cast<float*>(p.part_of + 2 * grid);
   p.q = static_cast<const __nv_bfloat16*>(a->q), p.q_st = a->q_st, p.q_sh = a->q_sh, p.lse = a->lse;
   p.pages = a->pages, p.scales = a->scales, p.n_pages = (int)a->n_pages, p.page_shift = shift_of(a->bs);
   p.rows = a->rows, p.batch = a->batch, p.h = a->h, p.group = group;
@@ -672,11 +678,6 @@ extern "C" int lkv_attention_sums(const lkv_sums_args* a, void* stream) {
                                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(LKV_ERR_CUDA, "%s: the pages' tensor map was refused (%d)", who, (int)r);
   }
-  const int grid = grid_of(a->cap, a->batch, a->h);
-  if (a->workspace == nullptr || a->workspace_bytes < grid * kPartBytes) return fail(LKV_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, a->workspace_bytes, grid * kPartBytes);
-  if (!aligned(a->workspace, 16)) return fail(LKV_ERR_PTR, "%s: workspace must be 16-byte aligned", who);
-  p.part_of = static_cast<int4*>(a->workspace);
-  p.part = reinterpret_cast<float*>(p.part_of + 2 * grid);
   cudaStream_t st = as_stream(stream);
   auto go = [&](auto dim) {
     constexpr int D = decltype(dim)::value;

@@ -6,12 +6,21 @@ nothing in common. Here every sequence is a fork of one prefix (a system prompt,
 samples of one request). A step takes T new tokens of every sequence (one, or a token and those
 drafted after it), writes their keys and values into the sequences' pages (kernels.paged_write),
 attends their queries to the prefix and to their own tokens (kernels.prefix_attention), and, where
-tokens were drafted, keeps those that the verification accepted (kernels.verify_drafts).
+tokens were drafted, keeps those that the verification accepted (kernels.verify_drafts). A chunk takes any
+number of new tokens of each sequence at once (a user's turn, a prompt of its own), straight from the
+projections: normalised and rotated into the pages (kernels.paged_write_rotated) and attended
+(kernels.chunk_attention).
+
+A batch with track=True keeps to a budget: every step and chunk adds up the weight that each own token
+gets from its queries (kernels.attention_sums), and evict() keeps the tokens of most weight of each head
+(kernels.paged_evict) and frees the pages behind them.
 
 Layout (one layer): pages [n_pages, h, 2, page, d] in the model dtype, or int8 codes with scales
 [n_pages, h, 2, page] float32, one per token, head and key or value; page tables int32, -1 past a
 sequence's own pages. The prefix's tokens are positions 0 .. prefix_len - 1 of its own page list and a
-sequence's own tokens positions 0 .. of its; rotary positions are the caller's (prefix_len + position).
+sequence's own tokens positions 0 .. of its; rotary positions are the caller's (prefix_len + position), or
+chunk()'s own. After evict() a sequence's slots are in no order and differ by head; `positions` says which
+token is where.
 """
 
 from __future__ import annotations
@@ -26,11 +35,12 @@ class PagedBatch:
     """One layer's KV for up to `max_seqs` sequences of up to `max_tokens` own tokens behind one prefix.
 
     `n_pages` pages of `page` tokens hold the prefix and every sequence's own tokens; `quant` is "int8"
-    or None (the model dtype).
+    or None (the model dtype). `track` keeps the sums and positions that evict() needs: `sums` [max_seqs,
+    heads, slots] float32 and `positions` int32 alike, by sequence id.
     """
 
     def __init__(self, heads: int, group: int, head_dim: int, max_seqs: int, max_tokens: int, n_pages: int, page: int = 16, quant: str | None = "int8",
-                 device: torch.device | str = "cuda", dtype: torch.dtype = torch.bfloat16) -> None:
+                 device: torch.device | str = "cuda", dtype: torch.dtype = torch.bfloat16, track: bool = False) -> None:
         if dtype != torch.bfloat16 or head_dim not in (64, 128) or page not in (16, 32, 64, 128):
             raise ValueError("a paged batch is bfloat16 with head_dim 64 or 128 and pages of 16, 32, 64 or 128 tokens")
         if quant not in (None, "int8"):
@@ -49,11 +59,15 @@ class PagedBatch:
         self.table = torch.full((max_seqs, self.cols), -1, dtype=torch.int32, device=self.dev)
         self.prefix_table = torch.empty(0, dtype=torch.int32, device=self.dev)
         self.prefix_len = 0
+        self.sums = torch.zeros((max_seqs, heads, self.cols * page), device=self.dev) if track else None
+        self.positions = torch.full((max_seqs, heads, self.cols * page), -1, dtype=torch.int32, device=self.dev) if track else None
         K.status_attach(self.pages.device)
         self._prefix_pages: list[int] = []
         self._free_pages = list(range(n_pages - 1, -1, -1))
         self._free_seqs = list(range(max_seqs - 1, -1, -1))
         self.lengths: dict[int, int] = {}  # own tokens of each live sequence
+        self._dropped: dict[int, int] = {}  # tokens that evict() has dropped of it
+        self._settled: dict[int, int] = {}  # its tokens that evict() may have moved
         self._pages_of: dict[int, list[int]] = {}
 
     # -- the prefix and the sequences -------------------------------------------------------------------
@@ -97,20 +111,20 @@ class PagedBatch:
         if not self._free_seqs:
             raise RuntimeError(f"all {self.max_seqs} sequences are taken")
         s = self._free_seqs.pop()
-        self.lengths[s], self._pages_of[s] = 0, []
+        self.lengths[s], self._pages_of[s], self._dropped[s], self._settled[s] = 0, [], 0, 0
         return s
 
     def drop(self, s: int) -> None:
         """Retire sequence `s`: its pages and its id are free again."""
-        del self.lengths[s]
+        del self.lengths[s], self._dropped[s], self._settled[s]
         self._free_pages.extend(reversed(self._pages_of.pop(s)))
         self.table[s].fill_(-1)
         self._free_seqs.append(s)
 
-    def _reserve(self, seq_ids: list[int], t: int) -> None:
-        """Pages for t more tokens of every sequence, or of none where they do not suffice."""
+    def _reserve(self, seq_ids: list[int], counts: list[int]) -> None:
+        """Pages for counts[i] more tokens of every sequence, or of none where they do not suffice."""
         rows, cols, new = [], [], []
-        for s in seq_ids:
+        for s, t in zip(seq_ids, counts):
             if self.lengths[s] + t > self.max_tokens:
                 raise RuntimeError(f"sequence {s} is at {self.lengths[s]} of its {self.max_tokens} tokens: no room for {t}")
             for c in range(len(self._pages_of[s]), -(-(self.lengths[s] + t) // self.page)):
@@ -144,26 +158,108 @@ class PagedBatch:
         if query.shape != (n, t, self.h * self.g, self.d):
             raise ValueError(f"expected query [{n}, {t}, {self.h * self.g}, {self.d}], got {tuple(query.shape)}")
         require_cuda(query, keys, values)
-        self._reserve(seq_ids, t)
+        self._reserve(seq_ids, [t] * n)
         lens = [self.lengths[s] for s in seq_ids]
-        ints = self._to_device(torch.tensor([seq_ids, lens, [x + t for x in lens]], dtype=torch.int32, pin_memory=True))
+        first = [self._next(s) for s in seq_ids]
+        ints = self._to_device(torch.tensor([seq_ids, lens, [x + t for x in lens], first], dtype=torch.int32, pin_memory=True))
         table = self.table.index_select(0, ints[0])
         K.paged_write(keys, values, self.pages, table, ints[1], scales=self.scales)
         done = K.prefix_attention(query, self.pages, table, ints[2], self.prefix_table, self.prefix_len, scale, scales=self.scales, out_dtype=out_dtype)
+        if self.sums is not None and n * t:
+            offsets = torch.arange(0, n * t + 1, t, dtype=torch.int32, device=self.dev)
+            place = torch.arange(t, dtype=torch.int32, device=self.dev).repeat(n)
+            self._track(ints[0], place, ints[1].repeat_interleave(t), ints[3].repeat_interleave(t), t, query.reshape(n * t, -1, self.d), done[1].view(n * t, -1), table, ints[2],
+                        offsets, scale, 0.0)
         for s in seq_ids:  # behind the calls: a refused step leaves the sequences as they were
             self.lengths[s] += t
         return done
 
+    def _next(self, s: int) -> int:
+        """The rotary position of sequence `s`'s next token."""
+        return self.prefix_len + self._dropped[s] + self.lengths[s]
+
+    def _track(self, ids: torch.Tensor, place: torch.Tensor, held: torch.Tensor, first: torch.Tensor, counts: int | torch.Tensor, query: torch.Tensor, lse: torch.Tensor,
+               table: torch.Tensor, lens: torch.Tensor, offsets: torch.Tensor, scale: float, cap: float) -> None:
+        """Adds the weights of packed queries to the sums, and notes the new tokens' positions (row i is token place[i] of a
+        chunk behind held[i] others, at position first[i] + place[i])."""
+        owner = ids.repeat_interleave(counts, output_size=place.numel())
+        self.positions[owner.long(), :, (held + place).long()] = (first + place)[:, None]
+        sums = self.sums.index_select(0, ids)
+        K.attention_sums(query, lse, self.pages, table, lens, offsets, scale, sums=sums, cap=cap, scales=self.scales, out=sums)
+        self.sums.index_copy_(0, ids.long(), sums)
+
+    def chunk(self, seq_ids: list[int], counts: list[int], query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, scale: float,
+              frequencies: torch.Tensor | None = None, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+              interleaved: bool = False, cap: float = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
+        """counts[i] new tokens (0 too) of sequence seq_ids[i], packed in this order: query [rows, h * g, d], keys and values
+        [rows, h, d] as the projections leave them. Queries and keys are normalised (where weights are given) and rotated
+        by `frequencies` (none: not at all) to the sequences' next positions behind the prefix, keys and values written, and
+        the queries attend the prefix and their sequences' tokens up to themselves. Returns (out [rows, h * g, d] bfloat16,
+        lse [rows, h * g] float32)."""
+        K.raise_on_status("PagedBatch.chunk")  # an earlier call's wait that ran out (not synchronised)
+        n, rows = len(seq_ids), sum(counts)
+        if len(set(seq_ids)) != n or len(counts) != n or min(counts, default=0) < 0:
+            raise ValueError(f"expected a count of new tokens for each of the sequences {seq_ids}, each named once; got {counts}")
+        if keys.shape != (rows, self.h, self.d) or values.shape != keys.shape or keys.dtype != self.dtype or query.shape != (rows, self.h * self.g, self.d):
+            raise ValueError(f"expected query [{rows}, {self.h * self.g}, {self.d}], keys and values [{rows}, {self.h}, {self.d}] {self.dtype}")
+        require_cuda(query, keys, values)
+        self._reserve(seq_ids, counts)
+        held = [self.lengths[s] for s in seq_ids]
+        first = [self._next(s) for s in seq_ids]
+        ends = [sum(counts[:i]) for i in range(n + 1)]
+        ints = self._to_device(torch.tensor([seq_ids + [0], held + [0], [x + t for x, t in zip(held, counts)] + [0], first + [0], counts + [0], ends], dtype=torch.int32, pin_memory=True))
+        ids, lens, offsets = ints[0, :n], ints[2, :n], ints[5]
+        table = self.table.index_select(0, ids)
+        place = torch.arange(rows, dtype=torch.int32, device=self.dev) - offsets[:n].repeat_interleave(ints[4, :n], output_size=rows)
+        start = ints[3, :n].repeat_interleave(ints[4, :n], output_size=rows)
+        if frequencies is None:
+            frequencies = torch.empty(0, device=self.dev)
+        query = K.paged_write_rotated(query, keys, values, start + place, frequencies, self.pages, table, lens, offsets, scales=self.scales, q_weight=q_weight,
+                                      k_weight=k_weight, eps=eps, interleaved=interleaved)
+        done = K.chunk_attention(query, self.pages, table, lens, offsets, scale, scales=self.scales, prefix_table=self.prefix_table, prefix_len=self.prefix_len, cap=cap)
+        if self.sums is not None and rows:
+            before = ints[1, :n].repeat_interleave(ints[4, :n], output_size=rows)
+            self._track(ids, place, before, start, ints[4, :n], query, done[1], table, lens, offsets, scale, cap)
+        for s, t in zip(seq_ids, counts):  # behind the calls: a refused chunk leaves the sequences as they were
+            self.lengths[s] += t
+        return done
+
+    def evict(self, seq_ids: list[int], keep: int, recent: int = 0, sinks: int = 0) -> None:
+        """Cuts the own tokens of these sequences down to `keep` a head: the first `sinks` and the last `recent` of the sequence
+        (by position) and then those of most weight so far. Pages behind them are free again; shorter sequences stay as they
+        are. Needs track=True."""
+        if self.sums is None:
+            raise RuntimeError("evict() ranks tokens by their weights: the batch was made without track=True")
+        if len(set(seq_ids)) != len(seq_ids) or keep < 1 or min(recent, sinks) < 0 or recent + sinks > keep:
+            raise ValueError(f"expected sequences named once and a budget that holds the {sinks} first and {recent} last tokens, got {seq_ids} and {keep}")
+        long = [s for s in seq_ids if self.lengths[s] > keep]
+        if not long:
+            return
+        ints = self._to_device(torch.tensor([long, [self.lengths[s] for s in long], [self._next(s) - recent for s in long]], dtype=torch.int32, pin_memory=True))
+        sums, positions = self.sums.index_select(0, ints[0]), self.positions.index_select(0, ints[0])
+        K.paged_evict(self.pages, self.table.index_select(0, ints[0]), ints[1], sums, positions, keep, since=ints[2], sinks=self.prefix_len + sinks, scales=self.scales,
+                      out=(sums, positions))
+        at = ints[0].long()
+        self.sums.index_copy_(0, at, sums)
+        self.positions.index_copy_(0, at, positions)
+        cols = -(-keep // self.page)
+        self.table[:, cols:].index_fill_(0, at, -1)
+        for s in long:
+            self._free_pages.extend(reversed(self._pages_of[s][cols:]))
+            del self._pages_of[s][cols:]
+            self._dropped[s] += self.lengths[s] - keep
+            self.lengths[s] = self._settled[s] = keep
+
     def take_back(self, s: int, tokens: int) -> None:
         """Forget the last `tokens` own tokens of sequence `s` (drafted ones that were rejected); their pages stay
-        the sequence's and are written again."""
-        if not 0 <= tokens <= self.lengths[s]:
-            raise ValueError(f"sequence {s} has {self.lengths[s]} tokens, not {tokens} to take back")
+        the sequence's and are written again. What evict() has moved cannot be taken back."""
+        if not 0 <= tokens <= self.lengths[s] - self._settled[s]:
+            raise ValueError(f"sequence {s} has {self.lengths[s] - self._settled[s]} tokens to take back, not {tokens}")
         self.lengths[s] -= tokens
 
     def read(self, s: int, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """The whole sequence, prefix and own tokens, as (keys, values) [h, L, d] in the model dtype (or `dtype`,
-        of int8 pages): what a step attends, say for RaggedTier.add."""
+        of int8 pages): what a step attends, say for RaggedTier.add (in the slots' order)."""
         dtype = dtype or self.dtype
         zero = torch.zeros(1, dtype=torch.int32, device=self.dev)
         parts = []

@@ -75,7 +75,7 @@ def scores(cache, query: torch.Tensor, b: int, tables: list[list[int]], lens: li
         z = cap * torch.tanh(z / cap)
     at = torch.arange(prefix + own) - prefix
     limit = lens[b] - n + 1 + torch.arange(n)
-    seen = there & (at < limit[:, None])
+    seen = there & ((at < 0) | (at < limit[:, None]))  # the prefix is in front of every row
     z = torch.where(seen[:, None], z, -torch.inf)
     return z, torch.where(seen[:, None], size, 0.0), v, seen
 
