@@ -70,7 +70,12 @@ struct Tiles {
   static constexpr int kBytes = kHalves * kHalfBytes;    // one operand tile
   static constexpr int kStages = INT8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8);
   static constexpr int kRawBytes = INT8 ? kTile * D : 0; // one tile of codes
-  static constexpr int kRaw = INT8 ? 3 : 0;
+  // Codes under way: a ring for keys and one for values. (One ring for both would give a place to the two warpgroups that turn
+  // codes into operands by turns; each waits for its own tiles only, and could take the other's last round for its own.)
+  static constexpr int kRawKeys = INT8 ? (D == 128 ? 2 : 3) : 0, kRawValues = INT8 ? (D == 128 ? 1 : 3) : 0, kRaw = kRawKeys + kRawValues;
+  // The place of tile t's keys or values in them, and how often it was filled before.
+  __device__ static __forceinline__ int raw_place(int t, int kv) { return kv == 0 ? t % max(kRawKeys, 1) : kRawKeys + t % max(kRawValues, 1); }
+  __device__ static __forceinline__ int raw_round(int t, int kv) { return t / max(kv == 0 ? kRawKeys : kRawValues, 1); }
   static constexpr int kThreads = INT8 ? 640 : 384;      // five warpgroups, or three
   // Registers per thread: the warpgroups that compute weights take what the others leave of the launch's
   // 96 (or 168) per thread. The split's sum stays within the launch's.
@@ -82,7 +87,7 @@ struct Tiles {
 
 struct Barriers {
   uint64_t q_full, o_full[2], s_full[2], p_full[2], tail, drain;
-  uint64_t full[9], empty[9], raw_full[3], raw_empty[3], info[kInfo];
+  uint64_t full[9], empty[9], raw_full[6], raw_empty[6], info[kInfo];
   uint32_t have[kInfo][4];   // together, bit g: tokens 16 g .. 16 g + 15 of the tile have a page
   int32_t top[kInfo][4];     // int8: 2^top is above every finite value scale x kScaleDown, per warp of converters
   float back[2][kTile];      // int8: what a row's scores are multiplied with (stage_query)
@@ -554,8 +559,8 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
           warp_arrive(&s.tail, lane);
         }
       } else {
-        const int slot = n % T::kRaw;
-        if (n >= T::kRaw) ok = wait_for(s, &s.raw_empty[slot], (n / T::kRaw - 1) & 1);
+        const int slot = T::raw_place(t, kv), round = T::raw_round(t, kv);
+        if (round > 0) ok = wait_for(s, &s.raw_empty[slot], (round - 1) & 1);
         if (!ok) break;
         const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, page >= 0));
         if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[slot], n_copies * bs * D);
@@ -567,8 +572,14 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       }
     }
     // No copy may land after the CTA has gone, also where the others gave up behind this warp's last copy.
-    const int kSlots = INT8 ? T::kRaw : n_stages;
-    for (int n = max(0, filled - kSlots); n < filled; ++n) mbar_wait(INT8 ? &s.raw_full[n % kSlots] : &s.full[n % kSlots], (n / kSlots) & 1);
+    for (int n = max(0, filled - (INT8 ? 2 * T::kRaw : n_stages)); n < filled; ++n) {
+      if constexpr (INT8) {
+        const int t = n >> 1, kv = n & 1, size = kv == 0 ? T::kRawKeys : T::kRawValues;
+        if (t + size > (filled - 1 - kv) / 2) mbar_wait(&s.raw_full[T::raw_place(t, kv)], T::raw_round(t, kv) & 1);  // its place's last filling
+      } else {
+        mbar_wait(&s.full[n % n_stages], (n / n_stages) & 1);
+      }
+    }
     __syncwarp();
   } else if (warp >= 12) {
     if constexpr (INT8) {
@@ -604,7 +615,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
       const int from = (tok0 * kPer + c) * 16, row = (c / 4) * T::kHalfBytes + tok0 * 128, at = (c % 4) * 2;
       const int to0 = row + ((at ^ (tok0 & 7)) << 4), to1 = row + (((at + 1) ^ (tok0 & 7)) << 4);
       for (int t = 0; t < n_tiles; ++t) {
-        const int n = 2 * t + kv, raw = n % T::kRaw, slot = n % n_stages, info = t % kInfo;
+        const int n = 2 * t + kv, raw = T::raw_place(t, kv), slot = n % n_stages, info = t % kInfo;
         // The ring entry's last reader is more than two tiles behind (see the copies): it is free.
         float* ring = scale_ring + (info * 2 + kv) * kTile;
         ring[i] = scale * (kv == 1 ? kScaleDown : kKeyDown);
@@ -617,7 +628,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
         }
         warp_arrive(&s.info[info], lane);
         scales_of(t + 1);
-        ok = ok && wait_for(s, &s.raw_full[raw], (n / T::kRaw) & 1);
+        ok = ok && wait_for(s, &s.raw_full[raw], T::raw_round(t, kv) & 1);
         if (ok && n >= n_stages) ok = wait_for(s, &s.empty[slot], (n / n_stages - 1) & 1);
         if (!ok) break;
         const char* src = raws + raw * T::kRawBytes + from;
