@@ -85,13 +85,13 @@ struct ChunkParams {
   int stall;  // test hook: warp 0 withholds an arrival
 };
 
-// A place in a ring of n entries, with the parity of its present round.
+// A place in a ring of n entries, and how often it was filled before.
 struct Cursor {
-  int slot;
-  uint32_t phase;
+  int slot, round;
+  __device__ __forceinline__ uint32_t phase() const { return round & 1; }
   __device__ __forceinline__ void step(int by, int n) {
     slot += by;
-    if (slot >= n) slot -= n, phase ^= 1;
+    if (slot >= n) slot -= n, ++round;
   }
 };
 
@@ -113,7 +113,9 @@ struct Tiles {
   static constexpr int kBytes = kHalves * kHalfBytes;   // one operand tile
   static constexpr int kStages = INT8 ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 8);
   static constexpr int kRawBytes = INT8 ? kTile * D : 0;
-  static constexpr int kRaw = INT8 ? 3 : 0;
+  // Codes under way: a ring for keys and one for values. (One ring for both would give a place to the two warpgroups that turn
+  // codes into operands by turns; each waits for its own tiles only, and could take the other's last round for its own.)
+  static constexpr int kRawKeys = INT8 ? (D == 128 ? 2 : 3) : 0, kRawValues = INT8 ? (D == 128 ? 1 : 3) : 0, kRaw = kRawKeys + kRawValues;
   static constexpr int kThreads = INT8 ? 640 : 384;     // five warpgroups, or three
   // Registers per thread: the warpgroups that compute weights take what the others leave of the launch's.
   static constexpr int kMany = INT8 ? 160 : 208, kFew = INT8 ? 48 : 88;
@@ -126,7 +128,7 @@ struct Tiles {
 
 struct Barriers {
   uint64_t q_full, o_full[2], s_full[2], p_full[2], drain, other_full, other_empty;
-  uint64_t full[9], empty[9], raw_full[3], raw_empty[3], info[kInfo], dirty[kClean], clean[kClean], unit_full[kRing], unit_empty[kRing];
+  uint64_t full[9], empty[2][9], raw_full[6], raw_empty[6], info[kInfo], dirty[kClean], clean[kClean], unit_full[kRing], unit_empty[kRing];
   uint32_t have[kInfo][4];  // together, bit g: tokens 16 g .. 16 g + 15 of the tile have a page
   Unit unit[kRing];
   int bad[kRing];           // values that are not finite were taken out of a tile of this unit
@@ -197,7 +199,8 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
     }
     for (int i = 0; i <= T::kStages; ++i) {
       mbar_init(&s.full[i], INT8 ? 4 : 1);
-      mbar_init(&s.empty[i], 1);
+      mbar_init(&s.empty[0][i], 1);
+      mbar_init(&s.empty[1][i], 1);
     }
     for (int i = 0; i < T::kRaw; ++i) {
       mbar_init(&s.raw_full[i], 1);
@@ -258,6 +261,16 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
   }
   fence_async();
   __syncthreads();
+
+  // A stage is free to be filled: what was in it has been multiplied. Keys and values take an odd number of stages by turns;
+  // each kind's products have barriers of their own, so that whoever fills a stage has waited for every phase of the barrier
+  // that it waits on (keys' and values' codes are turned into operands by different warps).
+  auto wait_empty = [&](const Cursor& c) {
+    if (c.round == 0) return true;
+    const int before = c.round - 1;
+    const bool both = n_stages % 2 != 0;
+    return wait_for(s, &s.empty[(both ? c.slot + before : c.slot) & 1][c.slot], (both ? before >> 1 : before) & 1);
+  };
 
   // The next unit of the line, for a whole warp: a copy of it, or b < 0 at the end (or where a wait ran out).
   int unit_count = 0;
@@ -607,22 +620,25 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
   } else if (warp == 8) {
     // ---- matrix products: issued by one lane, in order -----------------------------------------------
     constexpr uint32_t kQk = instruction<false>(kTile, false), kPv = instruction<false>(D, true);
-    const uint32_t q_u = smem_u32(q_tiles), st_u = smem_u32(stages), mine = elect(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t q_u = smem_u32(q_tiles), st_u = smem_u32(stages), mine = elect(), tm = __reduce_max_sync(0xffffffffu, tmem);
     int jobs[2] = {0, 0}, cleaned = 0;
     Cursor keys = {0, 0}, values = {1, 0};  // stages of the next tile's
     bool ok = true;
     for (;; unit_done()) {
       const Unit un = next_unit(ok);
       if (un.b < 0) break;
-      const bool two = un.n_rows > kTile;
-      const int n_jobs = two ? 2 * un.n_tiles : un.n_tiles, first = first_limit(p, un);
+      // What a vote or a reduction gives is known to be the whole warp's: the loop and the operands' addresses stay in uniform
+      // registers, and a product issues in a few cycles.
+      const bool two = __any_sync(0xffffffffu, un.n_rows > kTile);
+      const int n_tiles = __reduce_max_sync(0xffffffffu, un.n_tiles), t0 = __reduce_max_sync(0xffffffffu, un.t0);
+      const int n_jobs = two ? 2 * n_tiles : n_tiles, first = __reduce_max_sync(0xffffffffu, first_limit(p, un));
       // Keys of job i's tile, or its values, are in place (asked once per tile).
-      auto wait_keys = [&](int i) { return i >= n_jobs || (two && (i & 1) != 0) || wait_for(s, &s.full[keys.slot], keys.phase); };
+      auto wait_keys = [&](int i) { return i >= n_jobs || (two && (i & 1) != 0) || wait_for(s, &s.full[keys.slot], keys.phase()); };
       auto wait_values = [&](int i) {
         const int t = two ? i >> 1 : i;
         if (two && (i & 1) != 0) return true;
-        if (!wait_for(s, &s.full[values.slot], values.phase)) return false;
-        if (!INT8 && partly_seen(p, un.t0 + t, n_prefix, first)) {
+        if (!wait_for(s, &s.full[values.slot], values.phase())) return false;
+        if (!INT8 && partly_seen(p, t0 + t, n_prefix, first)) {
           if (!wait_for(s, &s.clean[cleaned % kClean], (cleaned / kClean) & 1)) return false;
           ++cleaned;
         }
@@ -638,7 +654,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
         }
         commit(&s.s_full[u], mine);
         if (!two || u == 1) {
-          commit(&s.empty[slot], mine);
+          commit(&s.empty[0][slot], mine);
           keys.step(2, n_stages);
         }
       };
@@ -649,7 +665,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
         for (int x = 0; x < kTile / 16; ++x)  // 16 tokens further: 2 KB of V, 8 columns of weights
           mma_ts(tm + 2 * kTile + u * D, tm + u * kTile + 8 * x, b + x * (2048 / 16), kPv, x > 0 || i > 1, mine);
         if (!two || u == 1) {
-          commit(&s.empty[slot], mine);
+          commit(&s.empty[1][slot], mine);
           values.step(2, n_stages);
         }
         if (two && i + 2 >= n_jobs) commit(&s.o_full[u], mine);
@@ -688,7 +704,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
     // weights of all but the two jobs before them: the entry's last reader is done.
     const int per = kTile >> p.page_shift;  // pages per tile
     int tiles = 0, filled = 0;
-    Cursor at = {0, 0};
+    Cursor at = {0, 0}, raw[2] = {{0, 0}, {T::kRawKeys, 0}};
     [[maybe_unused]] int dirty = 0;
     bool ok = true;
     for (;; unit_done()) {
@@ -710,13 +726,14 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
       };
       look_up(0);
       for (int n = 0; ok && n < 2 * un.n_tiles; ++n) {
-        const int t = n >> 1, kv = n & 1, info = (tiles + t) % kInfo, slot = at.slot;
+        const int t = n >> 1, kv = n & 1, info = (tiles + t) % kInfo;
         if (kv == 0) {
           page = next < p.n_pages ? next : -1;
           look_up(t + 1);
         }
         if constexpr (!INT8) {
-          ok = wait_for(s, &s.empty[slot], at.phase ^ 1);  // (of the first round: at once)
+          const int slot = at.slot;
+          ok = wait_empty(at);
           if (!ok) break;
           const uint32_t granules = lane < per && page >= 0 ? ((1u << (bs / 16)) - 1) << (lane * (bs / 16)) : 0u;
           const uint32_t have = __reduce_or_sync(0xffffffffu, granules);
@@ -739,7 +756,8 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
             mbar_arrive(&s.info[info]);
           }
         } else {
-          ok = wait_for(s, &s.raw_empty[slot], at.phase ^ 1);
+          const int slot = raw[kv].slot;
+          ok = wait_for(s, &s.raw_empty[slot], raw[kv].phase() ^ 1);  // (of the first round: at once)
           if (!ok) break;
           const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, page >= 0));
           if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[slot], n_copies * bs * D);
@@ -748,15 +766,23 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
             tma_load_1d(raws + slot * T::kRawBytes + lane * bs * D,
                         static_cast<const char*>(p.pages) + (((int64_t)page * p.h + un.j) * 2 + kv) * ((int64_t)bs * D), bs * D, &s.raw_full[slot]);
           ++filled;
-          at.step(1, T::kRaw);
+          if (++raw[kv].slot == (kv == 0 ? T::kRawKeys : T::kRaw)) raw[kv].slot = kv == 0 ? 0 : T::kRawKeys, ++raw[kv].round;
         }
       }
       if (!ok) break;
       tiles += un.n_tiles;
     }
     // No copy may land after the CTA has gone, also where the others gave up behind this warp's last copy.
-    const int slots = INT8 ? T::kRaw : n_stages;
-    for (int n = max(0, filled - slots); n < filled; ++n) mbar_wait(INT8 ? &s.raw_full[n % slots] : &s.full[n % slots], (n / slots) & 1);
+    if constexpr (INT8) {
+      // The last round of each ring: keys are every other copy, the first one theirs.
+      const int n_of[2] = {(filled + 1) / 2, filled / 2};
+      for (int kv = 0; kv < 2; ++kv) {
+        const int size = kv == 0 ? T::kRawKeys : T::kRawValues;
+        for (int n = max(0, n_of[kv] - size); n < n_of[kv]; ++n) mbar_wait(&s.raw_full[kv * T::kRawKeys + n % size], (n / size) & 1);
+      }
+    } else {
+      for (int n = max(0, filled - n_stages); n < filled; ++n) mbar_wait(&s.full[n % n_stages], (n / n_stages) & 1);
+    }
     __syncwarp();
   } else if (warp == 10) {
     // ---- the walk along the line -----------------------------------------------------------------------
@@ -871,7 +897,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
         for (int t = 0; ok && t < un.n_tiles; ++t, values.step(2, n_stages)) {
           if (!partly_seen(p, un.t0 + t, n_prefix, first)) continue;
           const int slot = values.slot;
-          ok = wait_for(s, &s.dirty[cleaned % kClean], (cleaned / kClean) & 1) && wait_for(s, &s.full[slot], values.phase);
+          ok = wait_for(s, &s.dirty[cleaned % kClean], (cleaned / kClean) & 1) && wait_for(s, &s.full[slot], values.phase());
           if (!ok) break;
           uint4* v = reinterpret_cast<uint4*>(stages + slot * T::kBytes);
           bool found = false;
@@ -909,7 +935,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
       const int from = (tok0 * kPer + c) * 16, row = (c / 4) * T::kHalfBytes + tok0 * 128, at = (c % 4) * 2;
       const int to0 = row + ((at ^ (tok0 & 7)) << 4), to1 = row + (((at + 1) ^ (tok0 & 7)) << 4);
       int tiles = 0;
-      Cursor to = {kv, 0}, raw = {kv, 0};
+      Cursor to = {kv, 0}, raw = {kv * T::kRawKeys, 0};
       bool ok = true;
       for (;; unit_done()) {
         const Unit un = next_unit(ok);
@@ -950,7 +976,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
           }
           warp_arrive(&s.info[info], lane);
           scales_of(t + 1);
-          ok = ok && wait_for(s, &s.raw_full[raw.slot], raw.phase) && wait_for(s, &s.empty[to.slot], to.phase ^ 1);
+          ok = ok && wait_for(s, &s.raw_full[raw.slot], raw.phase()) && wait_empty(to);
           if (!ok) break;
           const char* src = raws + raw.slot * T::kRawBytes + from;
           char* dst = stages + to.slot * T::kBytes;
@@ -973,7 +999,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
           fence_async();
           warp_arrive(&s.full[to.slot], lane);
           to.step(2, n_stages);
-          raw.step(2, T::kRaw);
+          if (++raw.slot == (kv == 0 ? T::kRawKeys : T::kRaw)) raw.slot = kv * T::kRawKeys, ++raw.round;
         }
         if (!ok) break;
         tiles += un.n_tiles;

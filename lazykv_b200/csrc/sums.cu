@@ -67,9 +67,12 @@ template <int D, bool INT8>
 struct Geometry {
   static constexpr int kHalves = D / 64, kHalfBytes = kTile * 128, kBytes = kHalves * kHalfBytes;
   static constexpr int kStages = 4;  // tiles of keys: two steps
-  static constexpr int kRawBytes = INT8 ? kTile * D : 0, kRaw = INT8 ? (D == 128 ? 3 : 6) : 0;
+  static constexpr int kRawBytes = INT8 ? kTile * D : 0, kRaw = INT8 ? (D == 128 ? 4 : 6) : 0;
+  // Two warpgroups turn codes of the two tiles of a step into operands, and each waits for its own tiles only: a place in a
+  // ring has to be the same one's every time, or it could take the other's last round for its own.
+  static_assert(kStages % 2 == 0 && kRaw % 2 == 0, "every place belongs to one warpgroup");
   // Query rows of a chunk: with int8 pages fewer, which leaves room for codes under way.
-  static constexpr int kRows = INT8 ? 64 : 128, kQBytes = kHalves * kRows * 128;
+  static constexpr int kRows = INT8 ? 32 : 128, kQBytes = kHalves * kRows * 128;
   static constexpr int kThreads = INT8 ? 768 : 512;
   // Registers per thread: the warpgroups that sum take what the others leave of the launch's.
   static constexpr int kMany = INT8 ? 128 : 168, kFew = INT8 ? 56 : 80;
@@ -653,6 +656,7 @@ extern "C" int lkv_attention_sums(const lkv_sums_args* a, void* stream) {
   if (a->lens == nullptr || a->offsets == nullptr || a->out == nullptr || (a->table == nullptr && a->table_cols > 0) || (a->rows > 0 && (a->q == nullptr || a->lse == nullptr)))
     return fail(LKV_ERR_PTR, "%s: null pointer", who);
   if (!aligned(a->q, 16) || (a->q_st & 7) != 0 || (a->q_sh & 7) != 0) return fail(LKV_ERR_PTR, "%s: query rows must be 16-byte aligned", who);
+  if (!aligned(a->scales, 16)) return fail(LKV_ERR_PTR, "%s: scales must be 16-byte aligned", who);
   const int grid = grid_of(a->cap, a->batch, a->h);
   if (a->workspace == nullptr || a->workspace_bytes < grid * kPartBytes) return fail(LKV_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, a->workspace_bytes, grid * kPartBytes);
   if (!aligned(a->workspace, 16)) return fail(LKV_ERR_PTR, "%s: workspace must be 16-byte aligned", who);
