@@ -27,6 +27,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kMostKeys = 16384;  // keys of a CTA's slots that shared memory holds; of longer slices they are computed again
 constexpr int kMovesAtOnce = 8;   // of a warp
+constexpr int kMostRanks = 8;     // CTAs of a cluster
 
 struct EvictParams {
   void* pages;
@@ -126,10 +127,13 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p) {
     sync();
     // Thread t has the four bins 2047 - 4 t and below.
     uint32_t count[4] = {0, 0, 0, 0};
-    for (int r = 0; r < n_ranks; ++r) {
-      const uint4 x = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&s.hist[pass][kBins - 4 - 4 * tid], r));
-      count[0] += x.w, count[1] += x.z, count[2] += x.y, count[3] += x.x;
-    }
+    uint4 of[kMostRanks];  // (asked for together: another CTA's shared memory is a microsecond away)
+#pragma unroll
+    for (int r = 0; r < kMostRanks; ++r)
+      if (r < n_ranks) of[r] = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&s.hist[pass][kBins - 4 - 4 * tid], r));
+#pragma unroll
+    for (int r = 0; r < kMostRanks; ++r)
+      if (r < n_ranks) count[0] += of[r].w, count[1] += of[r].z, count[2] += of[r].y, count[3] += of[r].x;
     const uint32_t mine = count[0] + count[1] + count[2] + count[3];
     uint32_t upto = mine;
 #pragma unroll
@@ -140,7 +144,8 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p) {
     if (lane == 31) s.scan[warp] = upto;
     __syncthreads();
     uint32_t before = upto - mine;
-    for (int w = 0; w < warp; ++w) before += s.scan[w];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) before += w < warp ? s.scan[w] : 0u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (before < want && want <= before + count[i]) s.digit = kBins - 1 - 4 * tid - i, s.left = want - before;
@@ -163,8 +168,10 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p) {
   }
   sync();
   uint32_t tie_base = 0;
-  for (int r = 0; r < rank; ++r) tie_base += *cluster.map_shared_rank(&s.all_ties, r);
-  for (int w = 0; w < warp; ++w) tie_base += s.ties[w];
+#pragma unroll
+  for (int r = 0; r < kMostRanks; ++r) tie_base += r < rank ? *cluster.map_shared_rank(&s.all_ties, r) : 0u;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) tie_base += w < warp ? s.ties[w] : 0u;
 
   // Which slots in front of `keep` lose their token and which tokens behind it stay, in slot order; `use` gets
   // each slot with its token's fate.
@@ -191,12 +198,15 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p) {
   sync();
   uint2 base = make_uint2(0, 0);
   uint32_t n_moves = 0;
-  for (int r = 0; r < n_ranks; ++r) {
-    const uint2 x = *cluster.map_shared_rank(&s.all_moving, r);
+#pragma unroll
+  for (int r = 0; r < kMostRanks; ++r) {
+    const uint2 x = r < n_ranks ? *cluster.map_shared_rank(&s.all_moving, r) : make_uint2(0, 0);
     if (r < rank) base.x += x.x, base.y += x.y;
     n_moves += x.x;
   }
-  for (int w = 0; w < warp; ++w) base.x += s.moving[w].x, base.y += s.moving[w].y;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w)
+    if (w < warp) base.x += s.moving[w].x, base.y += s.moving[w].y;
   int2* moves = p.moves + (int64_t)row * p.max_moves;
   walk([&](int i, bool kept, uint32_t lose, uint32_t move) {
     if (lose >> lane & 1) moves[base.x + __popc(lose & below)].y = i;
@@ -297,7 +307,7 @@ int lkv_paged_evict(const lkv_evict_args* a, void* stream) {
   // CTAs of a cluster: as many as leave each some 2,048 slots, while the GPU has room for them.
   const int rows = a->batch * a->h;
   int n_ranks = 1;
-  while (n_ranks < 8 && a->cap / n_ranks > 2048 && (int64_t)rows * n_ranks < 2 * kNumSMs) n_ranks *= 2;
+  while (n_ranks < kMostRanks && a->cap / n_ranks > 2048 && (int64_t)rows * n_ranks < 2 * kNumSMs) n_ranks *= 2;
   const int span = (int)(((int64_t)a->cap + n_ranks - 1) / n_ranks + 31) / 32 * 32;
   p.cached = span <= kMostKeys ? span : 0;
   const int rb = a->d * (a->kind == LKV_CACHE_INT8 ? 1 : (int)dtype_size(a->dtype));

@@ -58,7 +58,7 @@ BASE = {"q": FAKE, "k": FAKE, "v": FAKE, "q_st": 512, "q_sh": 64, "k_st": 128, "
         ({"workspace_bytes": 100}, 4, "needed"), ({"prefix_table": 0}, 2, "null"), ({"n_pages": 2**30}, 1, "rows of pages")]),
     ("lkv_attention_sums", L.SUMS_ARGS, SUMS, {}, [
         ({"last": 0}, 1, "last"), ({"hq": 5}, 1, "query heads"), ({"cap_scores": -2.0}, 1, "cap"), ({"lse": 0}, 2, "null"), ({"out": 0}, 2, "null"), ({"workspace_bytes": 0}, 4, "needed"),
-        ({"cap": 2**30 + 1}, 1, "bad shape"), ({"q_sh": 60}, 2, "16-byte")]),
+        ({"cap": 2**30 + 1}, 1, "bad shape"), ({"q_sh": 60}, 2, "16-byte"), ({"kind": 1, "scales": FAKE + 4}, 2, "scales must be 16-byte")]),
 ])
 def test_entries_refuse(lib, entry, layout, names, more, bad) -> None:  # noqa: ANN001
     make = _fields(layout, {**BASE, **more}, names)
