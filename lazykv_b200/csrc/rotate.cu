@@ -12,9 +12,12 @@
 // decided by the side of a border that its value lies on. The angle is a float64 product, brought below half
 // a turn in float64 before its sine and cosine are taken: at position 10^6 a float32 angle is off by 0.03.
 //
-// Bytes bound it: each row is read once and written once. A group of d / 8 lanes carries a row, a lane four
-// channels of the first elements of pairs and the four of their second ones, so that a rotation needs no other
-// lane. A CTA computes the angles of its tokens once for all heads.
+// Each row is read once and written once. A group of d / 8 lanes carries a row, a lane four channels of the first
+// elements of pairs and the four of their second ones, so that a rotation needs no other lane. A CTA computes the angles
+// of its tokens once for all heads.
+//
+// Measured: 32,768 tokens, 32 query and 8 KV heads, d 128, norms, to int8 pages 181 us (738 MB: 0.62 of a plain copy), the
+// issue slots busy for the larger part; 64 tokens 4.8 us, three dependent loads and the angles.
 #include "paged.cuh"
 #include "tensor.cuh"
 

@@ -126,7 +126,7 @@ __device__ __forceinline__ Sequence sequence_of(const SumsParams& p, int b) {
 // The first chunk with a row that sees a token of the step (row r sees tokens up to limit + r / group).
 template <int kRows>
 __device__ __forceinline__ int first_chunk(const SumsParams& p, const Sequence& q, int step) {
-  const int64_t row = (int64_t)(step * kPair - q.limit + 1) * p.group;
+  const int64_t row = ((int64_t)step * kPair - q.limit + 1) * p.group;
   return row < kRows ? 0 : (int)min((int64_t)(q.chunks - 1), row / kRows);
 }
 // Jobs of a sequence, per KV head.
