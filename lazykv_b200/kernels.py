@@ -663,8 +663,8 @@ def paged_evict(pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, su
     if positions.dtype is not _I32 or positions.shape != shape or not positions.is_contiguous():
         raise ValueError(f"{who}: positions must be a contiguous int32 {tuple(shape)}, got {positions.dtype} {tuple(positions.shape)}")
     cap = shape[2]
-    if keep < 1:
-        raise ValueError(f"{who}: a budget of {keep} tokens")
+    if not (1 <= keep < 2**31 and 0 <= sinks < 2**31):
+        raise ValueError(f"{who}: a budget of {keep} tokens, the first {sinks} of them kept")
     code = 0 if kind == 1 else dtype_code(pages.dtype)
     if out is None:
         out = torch.empty_like(sums), torch.empty_like(positions)

@@ -217,3 +217,23 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(int8: bool,
     again = call()
     assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
     assert K.device_status(clear=True) == 0 and K.status_poll(clear=True) == 0
+
+
+def test_refusals() -> None:
+    K = _kernels()
+    pages, table = torch.zeros(4, 2, 2, 16, 64, dtype=torch.bfloat16, device="cuda"), _i32([[0, 1], [2, 3]])
+    q, lens, where = torch.zeros(5, 4, 64, dtype=torch.bfloat16, device="cuda"), _i32([5, 9]), _i32([0, 2, 5])
+    base = {"query": q, "pages": pages, "table": table, "lens": lens, "offsets": where, "scale": 0.1}
+    lse = torch.zeros(5, 4, device="cuda")
+    for change in ({"query": q.float()}, {"query": q[:, :3]}, {"query": q[..., :32]}, {"pages": pages.float()}, {"lens": lens[:1]}, {"offsets": where[:2]}, {"cap": -1.0}, {"cap": math.inf},
+                   {"table": table.long()}):
+        with pytest.raises(ValueError):
+            K.chunk_attention(**{**base, **change})
+        with pytest.raises(ValueError):
+            K.attention_sums(**{**base, **change}, lse=lse)
+    for change in ({"prefix_len": 1}, {"prefix_len": 40, "prefix_table": _i32([1, 2])}, {"out": q.float()}, {"lse": lse[:4]}, {"prefix_table": _i32([[1, 2]])}):
+        with pytest.raises(ValueError):
+            K.chunk_attention(**{**base, **change})
+    for change in ({"lse": lse[:4]}, {"last": 0}, {"sums": torch.zeros(2, 2, 30)}, {"sums": torch.zeros(2, 1, 32, device="cuda")}, {"out": torch.zeros(2, 2, 32, dtype=torch.float64, device="cuda")}):
+        with pytest.raises(ValueError):
+            K.attention_sums(**{**base, "lse": lse, **change})

@@ -124,3 +124,15 @@ def test_captured_and_replayed_with_other_lengths() -> None:
         want_len, want_s, want_p, moves = P.evict(lens, sums, positions, 100, None, 0)
         assert left.tolist() == want_len and torch.equal(got_p.cpu(), want_p) and torch.equal(got_s.cpu(), want_s)
         assert torch.equal(dpages.cpu(), _moved(pages, table, moves, 16))
+
+
+def test_refusals() -> None:
+    K = _kernels()
+    table, pages, _ = _cache(2, 1, 32, 16, 64, "bf16", seed=7)
+    lens, sums, positions = _i32([32, 32]).cuda(), torch.zeros(2, 1, 32, device="cuda"), torch.zeros(2, 1, 32, dtype=torch.int32, device="cuda")
+    pages, table = pages.cuda(), table.cuda()
+    for change in ({"keep": 0}, {"keep": 2**31}, {"sinks": -1}, {"sums": sums[:, :, ::2]}, {"sums": sums.double()}, {"positions": positions.long()}, {"lens": lens[:1]},
+                   {"since": lens[:1]}, {"out": (sums[:1], positions)}, {"pages": pages[0]}, {"scales": sums}):
+        args = {"pages": pages, "table": table, "lens": lens, "sums": sums, "positions": positions, "keep": 4, **change}
+        with pytest.raises(ValueError):
+            K.paged_evict(**args)

@@ -156,3 +156,16 @@ def test_missing_pages_long_tables_and_odd_offsets() -> None:
     got = pages.cpu().double()
     assert (got[1, 0, 0, 0] - y[3, 0]).abs().max() < 0.05 and (got[0, 0, 0, :2] - y[5:7, 0]).abs().max() < 0.05
     assert torch.count_nonzero(got[1, :, :, 1:]) == 0 and torch.count_nonzero(got[0, :, :, 2:]) == 0
+
+
+def test_refusals() -> None:
+    K = _kernels()
+    q, k, v, table, pages, _, lens, offsets = _case(torch.bfloat16, 64, 2, 2, [5], [0], 16, False)
+    base = {"query": q, "keys": k, "values": v, "positions": _i32(range(5)), "frequencies": torch.ones(8, device="cuda"), "pages": pages.cuda(), "table": table.cuda(),
+            "lens": _i32(lens), "offsets": _i32(offsets)}
+    for change in ({"query": q[:4]}, {"keys": k[:, :1]}, {"values": v.float()}, {"positions": _i32(range(4))}, {"positions": torch.zeros(5, device="cuda")},
+                   {"frequencies": torch.ones(6, device="cuda")}, {"frequencies": torch.ones(36, device="cuda")}, {"lens": _i32([5, 5])}, {"offsets": _i32([0])}, {"eps": -1.0},
+                   {"q_weight": torch.ones(64, device="cuda")}, {"k_weight": torch.ones(32, dtype=torch.bfloat16, device="cuda")}, {"out": q[:, :1]},
+                   {"keys": k.transpose(1, 2).contiguous().transpose(1, 2)}, {"scales": torch.ones(1, device="cuda")}):
+        with pytest.raises(ValueError):
+            K.paged_write_rotated(**{**base, **change})
