@@ -16,7 +16,7 @@
 // elements of pairs and the four of their second ones, so that a rotation needs no other lane. A CTA computes the angles
 // of its tokens once for all heads.
 //
-// Measured: 32,768 tokens, 32 query and 8 KV heads, d 128, norms, to int8 pages 181 us (738 MB: 0.62 of a plain copy), the
+// Measured: 32,768 tokens, 32 query and 8 KV heads, d 128, norms, to int8 pages 174 us (738 MB: 0.65 of a plain copy), the
 // issue slots busy for the larger part; 64 tokens 4.8 us, three dependent loads and the angles.
 #include "paged.cuh"
 #include "tensor.cuh"
@@ -200,19 +200,18 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2) rotate_kerne
     c0 = pr < p.pairs ? pr : pr + p.pairs;
     c1 = pr < p.pairs ? pr + p.pairs : pr + D / 2;
   }
-  // A group's rows of one kind: sub, sub + per, ..; U of them are asked for at once.
+  // A group's rows of one kind: sub, sub + per, ..; U of them are asked for at once. Addresses go on by a step a row.
   Four<T> lo[U], hi[U];
-  auto fetch = [&](const T* src, int64_t s_head, int j0, int n) {
+  const int to_c1 = c1 - c0;
+  auto fetch = [&](const T* at, int64_t step, int j0, int n) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = j0 + u * per;
-      if (row < p.rows && j < n) lo[u] = load4<T, VEC>(src + j * s_head + c0), hi[u] = load4<T, VEC>(src + j * s_head + c1);
-    }
+    for (int u = 0; u < U; ++u)
+      if (row < p.rows && j0 + u * per < n) lo[u] = load4<T, VEC>(at + u * step), hi[u] = load4<T, VEC>(at + u * step + to_c1);
   };
-  const T* q = static_cast<const T*>(p.q) + (int64_t)row * p.q_st;
-  const T* k = static_cast<const T*>(p.k) + (int64_t)row * p.k_st;
-  const T* v = static_cast<const T*>(p.v) + (int64_t)row * p.v_st;
-  fetch(q, p.q_sh, sub, p.hq);
+  auto first_of_kind = [&](const void* rows, int64_t s_token, int64_t s_head) { return static_cast<const T*>(rows) + (int64_t)row * s_token + sub * s_head + c0; };
+  const T* q = first_of_kind(p.q, p.q_st, p.q_sh);
+  const int64_t q_step = per * p.q_sh;
+  fetch(q, q_step, sub, p.hq);
 
   if (warp >= 8 - tokens) {  // the last warps find the tokens' places
     const int mine = 7 - warp, r = row0 + mine;
@@ -279,9 +278,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2) rotate_kerne
   };
   {
     const Turn<W> f = turn_with(p.q_weight);
-    T* out = static_cast<T*>(p.out) + (int64_t)row * p.o_st;
+    T* out = static_cast<T*>(p.out) + (int64_t)row * p.o_st + sub * p.o_sh + c0;
+    const int64_t o_step = per * p.o_sh;
     for (int j0 = sub; j0 < p.hq; j0 += U * per) {
-      if (j0 != sub) fetch(q, p.q_sh, j0, p.hq);
+      if (j0 != sub) fetch(q, q_step, j0, p.hq);
+      q += U * q_step;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int j = j0 + u * per;
@@ -291,14 +292,15 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2) rotate_kerne
         turned(f, a, b);
         float z[8];
         in_order(a, b, z);
-        store4<VEC>(out + j * p.o_sh + c0, z);
-        store4<VEC>(out + j * p.o_sh + c1, z + 4);
+        store4<VEC>(out, z);
+        store4<VEC>(out + to_c1, z + 4);
+        out += o_step;
       }
     }
   }
   if (place < 0) return;
-  auto put = [&](const float (&z)[8], int j, int kv) {
-    const int64_t to = place + ((int64_t)j * 2 + kv) * bs;
+  const int64_t row_step = (int64_t)per * 2 * bs;
+  auto put = [&](const float (&z)[8], int64_t to) {  // to: the row of the pages
     if constexpr (INT8) {
       uint32_t top = 0, codes[2];
 #pragma unroll
@@ -319,8 +321,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2) rotate_kerne
   };
   {
     const Turn<W> f = turn_with(p.k_weight);
-    for (int j0 = sub; j0 < p.h; j0 += U * per) {
-      fetch(k, p.k_sh, j0, p.h);
+    const T* k = first_of_kind(p.k, p.k_st, p.k_sh);
+    const int64_t k_step = per * p.k_sh;
+    int64_t to = place + (int64_t)sub * 2 * bs;
+    for (int j0 = sub; j0 < p.h; j0 += U * per, k += U * k_step) {
+      fetch(k, k_step, j0, p.h);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int j = j0 + u * per;
@@ -330,12 +335,16 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2) rotate_kerne
         turned(f, a, b);
         float z[8];
         in_order(a, b, z);
-        put(z, j, 0);
+        put(z, to);
+        to += row_step;
       }
     }
   }
-  for (int j0 = sub; j0 < p.h; j0 += U * per) {
-    fetch(v, p.v_sh, j0, p.h);
+  const T* v = first_of_kind(p.v, p.v_st, p.v_sh);
+  const int64_t v_step = per * p.v_sh;
+  int64_t to = place + ((int64_t)sub * 2 + 1) * bs;
+  for (int j0 = sub; j0 < p.h; j0 += U * per, v += U * v_step) {
+    fetch(v, v_step, j0, p.h);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = j0 + u * per;
@@ -345,7 +354,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2) rotate_kerne
       float z[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) z[i] = (float)w[i];
-      put(z, j, 1);
+      put(z, to);
+      to += row_step;
     }
   }
 }
@@ -395,8 +405,8 @@ extern "C" int lkv_paged_write_rotated(const lkv_rotate_args* a, void* stream) {
   p.q_weight = a->q_weight, p.k_weight = a->k_weight, p.eps = a->eps;
   p.pages = a->pages, p.scales = a->scales, p.n_pages = a->n_pages, p.page_shift = shift_of(a->bs);
   p.table = a->table, p.table_ld = a->table_ld, p.table_cols = a->table_cols, p.lens = a->lens, p.offsets = a->offsets, p.batch = a->batch;
-  // As many tokens to a CTA, up to eight, as leave every SM two CTAs (their angles, places and waits are shared: a prompt of
-  // 32,768 tokens, 32 and 8 heads, d 128, to int8 in 186 us with eight, 189 with four).
+  // As many tokens to a CTA, up to eight, as leave every SM two CTAs (their angles, places and waits are shared: 2%
+  // less time with eight than with four for a prompt of 32,768 tokens, 32 and 8 heads, d 128, to int8 pages).
   while (p.token_shift < 3 && a->rows >> (p.token_shift + 1) >= 2 * kNumSMs) ++p.token_shift;
   const bool int8 = a->kind == LKV_CACHE_INT8;
   cudaStream_t st = as_stream(stream);
