@@ -518,7 +518,9 @@ int lkv_status_poll(int* status, int clear);
  * lkv_prefix_attention's tiled prefix; LKV_DEBUG_PREFIX_STALL_NEXT makes a warp of every CTA of the next
  * call with a tiled prefix withhold its arrival for the queries (1) or for the weights (2), so that the
  * waits run out: status 1, and NaN in every row. LKV_DEBUG_CHUNK_WAIT_NS and LKV_DEBUG_CHUNK_STALL_NEXT do the same for
- * lkv_chunk_attention. Not for production use; not thread-safe.
+ * lkv_chunk_attention, LKV_DEBUG_SUMS_WAIT_NS and LKV_DEBUG_SUMS_STALL_NEXT for lkv_attention_sums (the arrival withheld is
+ * for the queries, 1, or for the room of scores that were read, 2); LKV_DEBUG_SUMS_STALL_CTA names the one CTA
+ * that does so (-1, as at the start: every CTA). Not for production use; not thread-safe.
  */
 enum {
   LKV_DEBUG_SELECT_WAIT_ITERS = 1,
@@ -527,7 +529,10 @@ enum {
   LKV_DEBUG_PREFIX_WAIT_NS = 4,
   LKV_DEBUG_PREFIX_STALL_NEXT = 5,
   LKV_DEBUG_CHUNK_WAIT_NS = 6,
-  LKV_DEBUG_CHUNK_STALL_NEXT = 7
+  LKV_DEBUG_CHUNK_STALL_NEXT = 7,
+  LKV_DEBUG_SUMS_WAIT_NS = 8,
+  LKV_DEBUG_SUMS_STALL_NEXT = 9,
+  LKV_DEBUG_SUMS_STALL_CTA = 10
 };
 int lkv_debug_set(int key, int64_t value);
 
@@ -794,7 +799,8 @@ int lkv_chunk_attention(const lkv_chunk_args* args, void* stream);
  * those of the chunk start from 0, slots without a token get 0, a token whose page is missing keeps its sum. A row with
  * lse = -inf has no weights. One or two launches, no atomics: the same sums every time. The workspace
  * (lkv_attention_sums_workspace bytes, 16-byte aligned, any contents) belongs to one call at a time. Limits and bounded
- * waits as lkv_chunk_attention's (a token whose wait ran out gets NaN).
+ * waits as lkv_chunk_attention's: where one ran out (lkv_device_status 1), every token that lost weights to it gets NaN, the
+ * others what they should.
  */
 typedef struct {
   const void* q;

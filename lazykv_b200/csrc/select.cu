@@ -1191,6 +1191,12 @@ int lkv_debug_set(int key, int64_t value) {
       return chunk_set_wait(value);
     case LKV_DEBUG_CHUNK_STALL_NEXT:
       return chunk_set_stall(value);
+    case LKV_DEBUG_SUMS_WAIT_NS:
+      return sums_set_wait(value);
+    case LKV_DEBUG_SUMS_STALL_NEXT:
+      return sums_set_stall(value);
+    case LKV_DEBUG_SUMS_STALL_CTA:
+      return sums_set_stall_cta(value);
     default:
       return fail(LKV_ERR_ARG, "lkv_debug_set: unknown key %d", key);
   }

@@ -68,6 +68,7 @@ struct SumsParams {
   int4* part_of;          // (1: a part, 3: the tile's last; sequence, head, step)
   float scale, cap_log2;  // scores x scale are in the log2 domain (capped: divided by the cap)
   uint64_t max_wait_ns;
+  int stall, stall_cta;  // test hook: a warp of this CTA (-1: of every CTA) withholds an arrival
 };
 
 template <int D, bool INT8>
@@ -190,6 +191,7 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
   char* raws = stages + kStages * G::kBytes;
   float* scale_ring = reinterpret_cast<float*>(raws + G::kRaw * G::kRawBytes);  // [kInfo][kTile]: the keys'
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, bs = 1 << p.page_shift;
+  auto stalls = [&](int which) { return p.stall == which && (p.stall_cta < 0 || p.stall_cta == (int)blockIdx.x); };
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s.k_full[i], INT8 ? 4 : 1);
@@ -283,23 +285,24 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
   else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kFew));
   if (warp < 8) {
     // ---- sums: a thread has a token -------------------------------------------------------------------
+    // (Where a wait ran out these warps go on to the end of the CTA's piece, without waiting: every tile that is left,
+    // or its part, is NaN, and every part is there for the merge.)
     const int u = warp / 4, i = tid % kTile;
     const uint32_t ts = tmem + ((uint32_t)(warp % 4) << 21) + u * 2 * kTile;
     int q_count = 0, job = 0, tile = u;
     bool ok = true;
-    for (Walk<G::kRows> w(p, s); w.more() && ok; w.next(p), tile += 2) {
+    for (Walk<G::kRows> w(p, s); w.more(); w.next(p), tile += 2) {
       const int token = w.step * kPair + u * kTile + i, info = tile % kInfo;
       const int64_t at = ((int64_t)w.b * p.h + w.j) * p.cap + token;
       float old = 0.0f;
       if (w.whole() && p.sums != nullptr && token < min(w.q.old, w.q.seen)) old = p.sums[at];
-      ok = wait_for(s, &s.info[info], (tile / kInfo) & 1);
-      if (!ok) break;
+      ok = ok && wait_for(s, &s.info[info], (tile / kInfo) & 1);
       const bool there = token < w.q.seen && (s.have[info] >> (i / 16) & 1);
       const float factor = INT8 && there ? p.scale * scale_ring[info * kTile + i] : p.scale;
       const uint64_t factor2 = pair(factor, factor);
       uint64_t sum[2] = {0, 0};
       bool wide_step = false;  // capped scores above their cap's size
-      for (int c = w.from; c < w.to; ++c, ++job) {
+      for (int c = w.from; ok && c < w.to; ++c, ++job) {
         const int buf = job & 1, stage = q_count % kQStages;
         ok = wait_for(s, &s.q_full[stage], (q_count / kQStages) & 1) && wait_for(s, &s.s_full[u][buf], (job >> 1) & 1);
         if (!ok) break;
@@ -392,7 +395,7 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
           else all(no, yes);
         }
         tc_before();
-        warp_arrive(&s.s_empty[u][buf], lane);
+        if (!stalls(2) || warp != 0) warp_arrive(&s.s_empty[u][buf], lane);
         // (One chunk a sequence and head stays for all of its steps.)
         if (w.q.chunks > 1 || w.last) {
           warp_arrive(&s.q_empty[stage], lane);
@@ -400,7 +403,7 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
         }
       }
       const float got = (first_of(sum[0]) + second_of(sum[0])) + (first_of(sum[1]) + second_of(sum[1]));
-      const float mine = !ok ? __uint_as_float(0x7fc00000u) : there ? got : 0.0f;
+      const float mine = token >= w.q.seen ? 0.0f : !ok ? __uint_as_float(0x7fc00000u) : there ? got : 0.0f;
       if (w.whole()) {
         if (token < p.cap) p.out[at] = old + mine;
       } else {
@@ -545,7 +548,7 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
         s.limit[stage][r] = live && lse != -INFINITY ? w.q.limit + t : 0;
         asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
         fence_async();
-        warp_arrive(&s.q_full[stage], lane);
+        if (!stalls(1) || warp != 12) warp_arrive(&s.q_full[stage], lane);
       }
     }
   } else if constexpr (INT8) {
@@ -631,7 +634,26 @@ cudaError_t launch(const SumsParams& p, const CUtensorMap& map, int grid, cudaSt
 int grid_of(int cap, int batch, int h) { return (int)std::min<int64_t>(kNumSMs, ((int64_t)cap + kPair - 1) / kPair * h * batch); }
 constexpr size_t kPartBytes = 2 * (kPair * sizeof(float) + sizeof(int4));  // of a CTA
 
+uint64_t g_sums_wait_ns = kMaxTensorWaitNs;
+int g_sums_stall_next = 0, g_sums_stall_cta = -1;
+
 }  // namespace
+
+int sums_set_wait(int64_t ns) {
+  if (ns < 1 || ns > (int64_t)kMaxTensorWaitNs) return fail(LKV_ERR_ARG, "lkv_debug_set: sums wait bound %lld ns outside [1, %llu]", (long long)ns, (unsigned long long)kMaxTensorWaitNs);
+  g_sums_wait_ns = (uint64_t)ns;
+  return LKV_OK;
+}
+int sums_set_stall(int64_t which) {
+  if (which < 0 || which > 2) return fail(LKV_ERR_ARG, "lkv_debug_set: no stall %lld of the attention sums (0, 1 or 2)", (long long)which);
+  g_sums_stall_next = (int)which;
+  return LKV_OK;
+}
+int sums_set_stall_cta(int64_t cta) {
+  if (cta < -1 || cta > INT32_MAX) return fail(LKV_ERR_ARG, "lkv_debug_set: no CTA %lld of the attention sums (-1: all)", (long long)cta);
+  g_sums_stall_cta = (int)cta;
+  return LKV_OK;
+}
 
 cudaError_t sums_device_status(int* status, int clear) { return tu_device_status(status, clear); }
 cudaError_t sums_status_attach(int* mirror) { return tu_status_attach(mirror); }
@@ -678,7 +700,9 @@ extern "C" int lkv_attention_sums(const lkv_sums_args* a, void* stream) {
   const bool cap = a->cap_scores > 0.0f;
   p.scale = cap ? a->scale / a->cap_scores : a->scale * kLog2e;
   p.cap_log2 = a->cap_scores * kLog2e;
-  p.max_wait_ns = kMaxTensorWaitNs;
+  p.max_wait_ns = g_sums_wait_ns;
+  p.stall = g_sums_stall_next, p.stall_cta = g_sums_stall_cta;
+  g_sums_stall_next = 0;
   const bool int8 = a->kind == LKV_CACHE_INT8;
   CUtensorMap map = {};
   if (!int8) {
