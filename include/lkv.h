@@ -519,8 +519,8 @@ int lkv_status_poll(int* status, int clear);
  * call with a tiled prefix withhold its arrival for the queries (1) or for the weights (2), so that the
  * waits run out: status 1, and NaN in every row. LKV_DEBUG_CHUNK_WAIT_NS and LKV_DEBUG_CHUNK_STALL_NEXT do the same for
  * lkv_chunk_attention, LKV_DEBUG_SUMS_WAIT_NS and LKV_DEBUG_SUMS_STALL_NEXT for lkv_attention_sums (the arrival withheld is
- * for the queries, 1, or for the room of scores that were read, 2); LKV_DEBUG_SUMS_STALL_CTA names the one CTA
- * that does so (-1, as at the start: every CTA). Not for production use; not thread-safe.
+ * for the queries, 1, or for the room of scores that were read, 2); LKV_DEBUG_SUMS_STALL_CTA and
+ * LKV_DEBUG_CHUNK_STALL_CTA name the one CTA that does so (-1, as at the start: every CTA). Not for production use; not thread-safe.
  */
 enum {
   LKV_DEBUG_SELECT_WAIT_ITERS = 1,
@@ -532,7 +532,8 @@ enum {
   LKV_DEBUG_CHUNK_STALL_NEXT = 7,
   LKV_DEBUG_SUMS_WAIT_NS = 8,
   LKV_DEBUG_SUMS_STALL_NEXT = 9,
-  LKV_DEBUG_SUMS_STALL_CTA = 10
+  LKV_DEBUG_SUMS_STALL_CTA = 10,
+  LKV_DEBUG_CHUNK_STALL_CTA = 11
 };
 int lkv_debug_set(int key, int64_t value);
 
@@ -760,7 +761,7 @@ int lkv_prefix_attention(const lkv_prefix_args* args, void* stream);
  * Roundings: scores, references and sums are float32; a weight, times its value's scale of int8 pages, is rounded to
  * bf16 (2^-8). Sums of weights times values are float32 before they are divided, with weights of up to 2^20: values above
  * 2^107 / keys may pass its end. An infinite value that is seen makes an infinite output (NaN where the weight is 0 in float32).
- * The kernels' waits are bounded (lkv_device_status 1: rows hold NaN or were not written).
+ * The kernels' waits are bounded (lkv_device_status 1): where one ran out, rows are right, hold NaN, or were not written.
  */
 typedef struct {
   const void* q;

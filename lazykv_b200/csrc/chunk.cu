@@ -61,6 +61,7 @@ constexpr int kClean = 8;          // tiles to be cleaned or cleaned ahead of th
 constexpr int kPad = 1;            // a unit's start and end count as this many tiles more on the line
 constexpr int kMinShare = 2;       // tiles of the line that a CTA takes at least
 constexpr int kMostBatch = 8192;
+constexpr int kLost = 4;           // of a part: its CTA gave up a wait, it may hold anything
 constexpr float kMostWeight = 1048576.0f;  // 2^20: what the sum of a thread's weights may grow to before its references are set again
 
 struct ChunkParams {
@@ -85,9 +86,9 @@ struct ChunkParams {
   // Parts of units, two slots a CTA: 2 c the unit it begins in the middle of, 2 c + 1 the one it does not end.
   float* part_o;    // [slots][kBlock][d], not divided by the sum
   float2* part_ml;  // [slots][kBlock]: (reference in the log2 domain, sum)
-  int4* part_of;    // [slots]: (1: a part, 3: the unit's last), sequence, head, first row
+  int4* part_of;    // [slots]: (1: a part, 3: the unit's last, + kLost: not to be used), sequence, head, first row
   uint64_t max_wait_ns;
-  int stall;  // test hook: warp 0 withholds an arrival
+  int stall, stall_cta;  // test hook: warp 0 of this CTA (-1: of every CTA) withholds an arrival
 };
 
 // A place in a ring of n entries, and how often it was filled before.
@@ -142,6 +143,7 @@ struct Barriers {
   uint32_t tmem;
   int quit;
   int n_long;
+  int4 of[2];               // the parts that the walk handed out
 };
 
 // Tiles of row block i of a chunk of n tokens behind `base` others (a block that sees nothing has one all the same).
@@ -192,6 +194,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
   float* scale_ring = reinterpret_cast<float*>(raws + T::kRaw * T::kRawBytes);  // [kInfo][2][kTile]: keys', values'
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int n_prefix = prefix_tiles(p), bs = 1 << p.page_shift;
+  auto stalls = [&](int which) { return p.stall == which && (p.stall_cta < 0 || p.stall_cta == (int)blockIdx.x); };
   if (tid == 0) {
     mbar_init(&s.q_full, 8);
     mbar_init(&s.drain, 1);
@@ -325,7 +328,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
           }
         }
         fence_async();
-        if (p.stall != 1 || warp != 0) warp_arrive(&s.q_full, lane);
+        if (!stalls(1) || warp != 0) warp_arrive(&s.q_full, lane);
       }
       int limit[4];  // own tokens that a row sees
 #pragma unroll
@@ -516,7 +519,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
           st_wait();
         }
         tc_before();
-        if (p.stall != 2 || warp != 0) warp_arrive(&s.p_full[u], lane);
+        if (!stalls(2) || warp != 0) warp_arrive(&s.p_full[u], lane);
       }
       jobs += n_done;
       // ---- the rows' results ------------------------------------------------------------------------
@@ -887,7 +890,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
       un.b = -1;
       hand_out(un);
     }
-    if (lane < 2) p.part_of[2 * c + lane] = of[lane];
+    if (lane < 2) s.of[lane] = of[lane];
     __syncwarp();
   } else if (warp == 11) {
     if constexpr (!INT8) {
@@ -1013,6 +1016,12 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
     }
   }
   __syncthreads();
+  // Units are handed out ahead: a part that is named here need not have been written where a wait ran out.
+  if (tid < 2) {
+    int4 of = s.of[tid];
+    if (of.x != 0 && *static_cast<volatile int*>(&s.quit) != 0) of.x |= kLost;
+    p.part_of[2 * blockIdx.x + tid] = of;
+  }
   if (warp == 8) {
     tc_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -1028,15 +1037,16 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const ChunkParams p) {
   const int c = blockIdx.x, lane = threadIdx.x % 32;
   const int4 of = p.part_of[2 * c + 1];
   if (of.x == 0) return;
-  int last = c + 1;
-  while (last + 1 < (int)gridDim.x && p.part_of[2 * last].x == 1) ++last;
+  int last = c + 1, found = of.x | p.part_of[2 * last].x;
+  while (last + 1 < (int)gridDim.x && (p.part_of[2 * last].x & 3) == 1) found |= p.part_of[2 * ++last].x;
+  const bool lost = (found & kLost) != 0;
   const Sequence q = sequence_of(p, of.y);
   const int n_rows = (int)min((int64_t)kBlock, (int64_t)q.n * p.group - of.w);
   for (int row = blockIdx.y * 8 + threadIdx.x / 32; row < n_rows; row += gridDim.y * 8) {
     float m = -INFINITY;
     for (int k = c; k <= last; ++k) m = fmaxf(m, p.part_ml[(int64_t)(k == c ? 2 * c + 1 : 2 * k) * kBlock + row].x);
     const float ref = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, o[D / 32] = {};
+    float l = lost ? __uint_as_float(0x7fc00000u) : 0.0f, o[D / 32] = {};
     for (int k = c; k <= last; ++k) {
       const int64_t at = (int64_t)(k == c ? 2 * c + 1 : 2 * k) * kBlock + row;
       const float2 ml = p.part_ml[at];
@@ -1078,7 +1088,7 @@ int grid_of(int rows, int batch, int h, int group, int64_t prefix_len, int64_t o
 size_t slot_bytes(int d) { return (size_t)kBlock * d * 4 + (size_t)kBlock * 8 + 16; }
 
 uint64_t g_chunk_wait_ns = kMaxTensorWaitNs;
-int g_chunk_stall_next = 0;
+int g_chunk_stall_next = 0, g_chunk_stall_cta = -1;
 
 }  // namespace
 
@@ -1090,6 +1100,11 @@ int chunk_set_wait(int64_t ns) {
 int chunk_set_stall(int64_t which) {
   if (which < 0 || which > 2) return fail(LKV_ERR_ARG, "lkv_debug_set: no stall %lld of the chunk attention (0, 1 or 2)", (long long)which);
   g_chunk_stall_next = (int)which;
+  return LKV_OK;
+}
+int chunk_set_stall_cta(int64_t cta) {
+  if (cta < -1 || cta > INT32_MAX) return fail(LKV_ERR_ARG, "lkv_debug_set: no CTA %lld of the chunk attention (-1: all)", (long long)cta);
+  g_chunk_stall_cta = (int)cta;
   return LKV_OK;
 }
 cudaError_t chunk_device_status(int* status, int clear) { return tu_device_status(status, clear); }
@@ -1148,7 +1163,7 @@ int lkv_chunk_attention(const lkv_chunk_args* a, void* stream) {
   p.part_ml = reinterpret_cast<float2*>(p.part_of + 2 * grid);
   p.part_o = reinterpret_cast<float*>(p.part_ml + (size_t)2 * grid * kBlock);
   p.max_wait_ns = g_chunk_wait_ns;
-  p.stall = g_chunk_stall_next;
+  p.stall = g_chunk_stall_next, p.stall_cta = g_chunk_stall_cta;
   g_chunk_stall_next = 0;
   const bool int8 = a->kind == LKV_CACHE_INT8;
   CUtensorMap map = {};

@@ -44,6 +44,7 @@ cudaError_t chunk_device_status(int* status, int clear);
 cudaError_t chunk_status_attach(int* mirror);
 int chunk_set_wait(int64_t ns);
 int chunk_set_stall(int64_t which);
+int chunk_set_stall_cta(int64_t cta);
 int sums_set_wait(int64_t ns);
 int sums_set_stall(int64_t which);
 int sums_set_stall_cta(int64_t cta);

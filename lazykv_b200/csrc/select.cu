@@ -1191,6 +1191,8 @@ int lkv_debug_set(int key, int64_t value) {
       return chunk_set_wait(value);
     case LKV_DEBUG_CHUNK_STALL_NEXT:
       return chunk_set_stall(value);
+    case LKV_DEBUG_CHUNK_STALL_CTA:
+      return chunk_set_stall_cta(value);
     case LKV_DEBUG_SUMS_WAIT_NS:
       return sums_set_wait(value);
     case LKV_DEBUG_SUMS_STALL_NEXT:

@@ -13,6 +13,7 @@ from lazykv_b200 import _lib as L
     (L.LKV_DEBUG_SUMS_WAIT_NS, (0, -1, 2_000_000_001), "sums wait bound"),
     (L.LKV_DEBUG_SUMS_STALL_NEXT, (-1, 3), "of the attention sums"),
     (L.LKV_DEBUG_SUMS_STALL_CTA, (-2, 2**31), "of the attention sums"),
+    (L.LKV_DEBUG_CHUNK_STALL_CTA, (-2, 2**31), "of the chunk attention"),
 ])
 def test_hooks_are_bounded(key: int, values: tuple[int, ...], says: str) -> None:
     if not L.LIB_PATH.exists():
