@@ -25,10 +25,24 @@ token is where.
 
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
 from lazykv_b200 import kernels as K
 from lazykv_b200._lib import require_cuda
+
+
+@dataclass
+class _LastCall:
+    """What a sequence's last step or chunk added to its sums, as take_back() needs it."""
+
+    held: int  # own tokens in front of the call's
+    sums: torch.Tensor  # [heads, slots] before it
+    query: torch.Tensor | None  # the call's rows and their lse, where some of them may stay
+    lse: torch.Tensor | None
+    scale: float
+    cap: float
 
 
 class PagedBatch:
@@ -36,8 +50,11 @@ class PagedBatch:
 
     `n_pages` pages of `page` tokens hold the prefix and every sequence's own tokens; `quant` is "int8"
     or None (the model dtype). `track` keeps the sums and positions that evict() needs: `sums` [max_seqs,
-    heads, slots] float32 and `positions` int32 alike, by sequence id.
+    heads, slots] float32 and `positions` int32 alike, by sequence id. For take_back(), a tracked batch also holds
+    each sequence's sums as they were before its last call, and that call's queries where they are up to MOST_DRAFTED.
     """
+
+    MOST_DRAFTED = 64  # new tokens of a tracked call of which take_back() can take back a part
 
     def __init__(self, heads: int, group: int, head_dim: int, max_seqs: int, max_tokens: int, n_pages: int, page: int = 16, quant: str | None = "int8",
                  device: torch.device | str = "cuda", dtype: torch.dtype = torch.bfloat16, track: bool = False) -> None:
@@ -69,6 +86,7 @@ class PagedBatch:
         self._dropped: dict[int, int] = {}  # tokens that evict() has dropped of it
         self._settled: dict[int, int] = {}  # its tokens that evict() may have moved
         self._pages_of: dict[int, list[int]] = {}
+        self._last: dict[int, _LastCall] = {}  # of a tracked batch
 
     # -- the prefix and the sequences -------------------------------------------------------------------
 
@@ -117,6 +135,7 @@ class PagedBatch:
     def drop(self, s: int) -> None:
         """Retire sequence `s`: its pages and its id are free again."""
         del self.lengths[s], self._dropped[s], self._settled[s]
+        self._last.pop(s, None)
         self._free_pages.extend(reversed(self._pages_of.pop(s)))
         self.table[s].fill_(-1)
         self._free_seqs.append(s)
@@ -168,8 +187,11 @@ class PagedBatch:
         if self.sums is not None and n * t:
             offsets = torch.arange(0, n * t + 1, t, dtype=torch.int32, device=self.dev)
             place = torch.arange(t, dtype=torch.int32, device=self.dev).repeat(n)
-            self._track(ints[0], place, ints[1].repeat_interleave(t), ints[3].repeat_interleave(t), t, query.reshape(n * t, -1, self.d), done[1].view(n * t, -1), table, ints[2],
-                        offsets, scale, 0.0)
+            rows = query.reshape(n * t, -1, self.d)
+            last = self._track(ints[0], place, ints[1].repeat_interleave(t), ints[3].repeat_interleave(t), t, rows, done[1].view(n * t, -1), table, ints[2], offsets, scale, 0.0)
+            if 1 < t <= self.MOST_DRAFTED:  # (the caller's tensor may change)
+                rows = rows.clone()
+            self._note(seq_ids, [t] * n, last, rows, done[1].view(n * t, -1), scale, 0.0)
         for s in seq_ids:  # behind the calls: a refused step leaves the sequences as they were
             self.lengths[s] += t
         return done
@@ -179,14 +201,26 @@ class PagedBatch:
         return self.prefix_len + self._dropped[s] + self.lengths[s]
 
     def _track(self, ids: torch.Tensor, place: torch.Tensor, held: torch.Tensor, first: torch.Tensor, counts: int | torch.Tensor, query: torch.Tensor, lse: torch.Tensor,
-               table: torch.Tensor, lens: torch.Tensor, offsets: torch.Tensor, scale: float, cap: float) -> None:
+               table: torch.Tensor, lens: torch.Tensor, offsets: torch.Tensor, scale: float, cap: float) -> torch.Tensor:
         """Adds the weights of packed queries to the sums, and notes the new tokens' positions (row i is token place[i] of a
-        chunk behind held[i] others, at position first[i] + place[i])."""
+        chunk behind held[i] others, at position first[i] + place[i]). Returns the sums [n, heads, slots] as they were."""
         owner = ids.repeat_interleave(counts, output_size=place.numel())
         self.positions[owner.long(), :, (held + place).long()] = (first + place)[:, None]
-        sums = self.sums.index_select(0, ids)
-        K.attention_sums(query, lse, self.pages, table, lens, offsets, scale, sums=sums, cap=cap, scales=self.scales, out=sums)
-        self.sums.index_copy_(0, ids.long(), sums)
+        before = self.sums.index_select(0, ids)
+        self.sums.index_copy_(0, ids.long(), K.attention_sums(query, lse, self.pages, table, lens, offsets, scale, sums=before, cap=cap, scales=self.scales))
+        return before
+
+    def _note(self, seq_ids: list[int], counts: list[int], before: torch.Tensor, query: torch.Tensor, lse: torch.Tensor, scale: float, cap: float) -> None:
+        """Keeps what take_back() needs of a call's packed rows (before the lengths grow)."""
+        if any(1 < t <= self.MOST_DRAFTED for t in counts):
+            lse = lse.clone()  # (the caller has it too)
+        at = 0
+        for i, (s, t) in enumerate(zip(seq_ids, counts)):
+            if t:
+                rows = slice(at, at + t)
+                part = 1 < t <= self.MOST_DRAFTED
+                self._last[s] = _LastCall(self.lengths[s], before[i], query[rows] if part else None, lse[rows] if part else None, scale, cap)
+            at += t
 
     def chunk(self, seq_ids: list[int], counts: list[int], query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, scale: float,
               frequencies: torch.Tensor | None = None, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
@@ -219,7 +253,8 @@ class PagedBatch:
         done = K.chunk_attention(query, self.pages, table, lens, offsets, scale, scales=self.scales, prefix_table=self.prefix_table, prefix_len=self.prefix_len, cap=cap)
         if self.sums is not None and rows:
             before = ints[1, :n].repeat_interleave(ints[4, :n], output_size=rows)
-            self._track(ids, place, before, start, ints[4, :n], query, done[1], table, lens, offsets, scale, cap)
+            last = self._track(ids, place, before, start, ints[4, :n], query, done[1], table, lens, offsets, scale, cap)
+            self._note(seq_ids, counts, last, query, done[1], scale, cap)
         for s, t in zip(seq_ids, counts):  # behind the calls: a refused chunk leaves the sequences as they were
             self.lengths[s] += t
         return done
@@ -249,12 +284,29 @@ class PagedBatch:
             del self._pages_of[s][cols:]
             self._dropped[s] += self.lengths[s] - keep
             self.lengths[s] = self._settled[s] = keep
+            self._last.pop(s, None)
 
     def take_back(self, s: int, tokens: int) -> None:
         """Forget the last `tokens` own tokens of sequence `s` (drafted ones that were rejected); their pages stay
-        the sequence's and are written again. What evict() has moved cannot be taken back."""
-        if not 0 <= tokens <= self.lengths[s] - self._settled[s]:
-            raise ValueError(f"sequence {s} has {self.lengths[s] - self._settled[s]} tokens to take back, not {tokens}")
+        the sequence's and are written again. What evict() has moved cannot be taken back.
+
+        With track=True the weights that the forgotten tokens' queries gave to the others leave the sums: these are as if
+        only the tokens that stay had come. That holds for tokens of the sequence's last step or chunk, all of them or, of
+        a call of up to MOST_DRAFTED of its tokens, a part; others are refused."""
+        last = self._last.get(s)
+        most = self.lengths[s] - (self._settled[s] if self.sums is None else last.held if last is not None else self.lengths[s])
+        if not 0 <= tokens <= most:
+            raise ValueError(f"sequence {s} has {most} tokens to take back, not {tokens}")
+        if last is not None and tokens:
+            stay = most - tokens
+            if stay == 0:
+                self.sums[s].copy_(last.sums)
+            elif last.query is None:
+                raise ValueError(f"of a tracked chunk of more than {self.MOST_DRAFTED} tokens all are taken back or none, not {tokens} of {most}")
+            else:
+                ints = self._to_device(torch.tensor([0, stay, last.held + stay], dtype=torch.int32, pin_memory=True))
+                K.attention_sums(last.query[:stay], last.lse[:stay], self.pages, self.table[s : s + 1], ints[2:], ints[:2], last.scale, sums=last.sums[None], cap=last.cap,
+                                 scales=self.scales, out=self.sums[s : s + 1])
         self.lengths[s] -= tokens
 
     def read(self, s: int, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
