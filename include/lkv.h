@@ -675,7 +675,10 @@ int lkv_paged_write_rotated(const lkv_rotate_args* args, void* stream);
  * moves to the i-th such slot whose token is not kept, with its scales, sum and position. sums (float32) and
  * positions (int32) are [batch, h, cap], cap at least what lens says; out_sums and out_positions get their new
  * contents (0 and -1 in the slots behind) and may be sums and positions themselves; out_lens [batch] gets
- * min(lens[b], keep). Sequences of up to `keep` tokens keep them all. dtype is that of model-dtype pages.
+ * min(lens[b], keep). Sequences of up to `keep` tokens keep them all. dtype is that of model-dtype pages. Pages should
+ * reach to lens[b]: a token without a page is ranked like the others, and where either slot of a move has no page the sum and
+ * the position move without a row. A slot whose new token had no page then keeps the row of the dropped one, which is
+ * attended further under that position; a token that moves to a slot without a page is lost.
  * Workspace: lkv_paged_evict_workspace bytes, 8-byte aligned, any contents.
  */
 typedef struct {

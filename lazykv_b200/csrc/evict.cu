@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const EvictParams p) {
       const int2 m = moves[at + lane];
       out_sums[m.y] = sums[m.x], out_positions[m.y] = positions[m.x];
       from = row_of(p, b, j, m.x), to = row_of(p, b, j, m.y);
-      if (from < 0 || to < 0) from = to = -1;  // a token without a page has nothing to move
+      if (from < 0 || to < 0) from = to = -1;  // without either page there is no row to move (its sum and position have)
     }
     if (p.scales != nullptr && to >= 0) {
       const float ks = p.scales[from], vs = p.scales[from + bs];

@@ -646,7 +646,8 @@ def paged_evict(pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, su
     keep - 1 move into the slots of dropped ones, in place, with their scales, so slots are no longer in the order of
     the positions; attention does not need one, as long as new tokens follow in slots of their own. Returns (min(lens,
     keep), sums, positions): the last two new, or in `out`, which may be sums and positions themselves; 0 and -1 stand in
-    slots without a token. A token without a page is ranked like the others and not moved.
+    slots without a token. Pages should reach to lens[b]: a token without a page is ranked like the others, and where either
+    slot of a move has none, sum and position move without a row: the slot keeps the row it had, or the token is lost.
     """
     who = "paged_evict"
     index = pages.get_device()
