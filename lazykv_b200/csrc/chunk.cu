@@ -964,7 +964,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
           }
         };
         auto scales_of = [&](int t) {
-          scale = kv == 0 ? 1.0f : 0.0f;  // of a token that is not there
+          scale = 0.0f;  // of a token that is not there (its codes are what shared memory held: they choose no form of a capped score)
           there = id >= 0 && id < p.n_pages;
           if (there) {
             const int tile = un.t0 + t, pos = (tile < n_prefix ? tile : tile - n_prefix) * kTile + i;

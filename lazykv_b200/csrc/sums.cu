@@ -298,7 +298,8 @@ __global__ void __launch_bounds__(Geometry<D, INT8>::kThreads, 1) sums_kernel(co
       if (w.whole() && p.sums != nullptr && token < min(w.q.old, w.q.seen)) old = p.sums[at];
       ok = ok && wait_for(s, &s.info[info], (tile / kInfo) & 1);
       const bool there = token < w.q.seen && (s.have[info] >> (i / 16) & 1);
-      const float factor = INT8 && there ? p.scale * scale_ring[info * kTile + i] : p.scale;
+      // (The codes of a page that is not there are what shared memory held: next to a capped score they would choose its form.)
+      const float factor = !INT8 ? p.scale : there ? p.scale * scale_ring[info * kTile + i] : 0.0f;
       const uint64_t factor2 = pair(factor, factor);
       uint64_t sum[2] = {0, 0};
       bool wide_step = false;  // capped scores above their cap's size
