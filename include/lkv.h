@@ -758,10 +758,11 @@ int lkv_prefix_attention(const lkv_prefix_args* args, void* stream);
  * lists, and the first lens[b] - n + i + 1 own tokens, in any order of the slots before the chunk; a token without a page
  * is not attended. Scores are scale q k or, with cap > 0, cap tanh(scale q k / cap). out [rows, hq, d] bfloat16 and lse
  * [rows, hq] float32, both contiguous; a row that attends nothing gets out = 0, lse = -inf; rows of no sequence are
- * left alone. lens, offsets and the tables are read on the device. Two launches; the workspace
+ * left alone. log2(e) scale without a cap, or with one 2 log2(e) times cap and times scale / cap, have to be finite in float32,
+ * and scale / cap 0 or normal. lens, offsets and the tables are read on the device. Two launches; the workspace
  * (lkv_chunk_attention_workspace bytes with own_reach = table_cols * bs, 16-byte aligned, any contents) belongs to
  * one call at a time. batch <= 8192, rows * hq / h <= 2^30, n_pages * 2 * h * bs < 2^31.
- * Roundings: scores, references and sums are float32; a weight, times its value's scale of int8 pages, is rounded to
+ * Roundings: scores, references and sums are float32 (capped scores within 2^-20 of the cap); a weight, times its value's scale of int8 pages, is rounded to
  * bf16 (2^-8). Sums of weights times values are float32 before they are divided, with weights of up to 2^20: values above
  * 2^107 / keys may pass its end. An infinite value that is seen makes an infinite output (NaN where the weight is 0 in float32).
  * The kernels' waits are bounded (lkv_device_status 1): where one ran out, rows are right, hold NaN, or were not written.

@@ -1133,7 +1133,7 @@ int lkv_chunk_attention(const lkv_chunk_args* a, void* stream) {
   if ((int64_t)a->rows * group > (1 << 30)) return fail(LKV_ERR_ARG, "%s: %d rows of %d query heads per KV head in one call", who, a->rows, group);
   if (a->prefix_len < 0 || a->prefix_len > (1 << 30) || a->prefix_len > (int64_t)a->prefix_cols * a->bs)
     return fail(LKV_ERR_ARG, "%s: a prefix of %lld tokens in %d pages of %d", who, (long long)a->prefix_len, a->prefix_cols, a->bs);
-  if (!(a->cap >= 0.0f) || a->cap > FLT_MAX || !(fabsf(a->scale) <= FLT_MAX)) return fail(LKV_ERR_ARG, "%s: scale %g, cap %g", who, (double)a->scale, (double)a->cap);
+  if (!scores_fit(a->scale, a->cap)) return fail(LKV_ERR_ARG, "%s: scale %g with cap %g leaves float32", who, (double)a->scale, (double)a->cap);
   const int64_t page_rows = a->n_pages * 2 * a->h * a->bs;
   if (page_rows > INT32_MAX) return fail(LKV_ERR_ARG, "%s: %lld rows of pages", who, (long long)page_rows);
   if (a->rows == 0 || a->batch == 0) return LKV_OK;

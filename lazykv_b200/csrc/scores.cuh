@@ -1,10 +1,23 @@
 // What chunk.cu and sums.cu do with scores alike: their cap, and codes of int8 pages as bf16 operands.
 #pragma once
 
+#include <float.h>
+#include <math.h>
+
 #include "prefix.cuh"
 #include "tensor.cuh"
 
 namespace lkv {
+
+// Do a softmax scale and a cap (0: none) and what the kernels make of them stay within float32? Beyond it 0 times infinity
+// would be a score, and a quotient below the normal numbers would be short of bits.
+inline bool scores_fit(float scale, float cap) {
+  constexpr double kTwoLog2e = 2.0 * 1.4426950408889634;
+  if (!(fabsf(scale) <= FLT_MAX) || !(cap >= 0.0f)) return false;
+  if (cap == 0.0f) return fabs((double)scale) * kTwoLog2e <= 2.0 * (double)FLT_MAX;
+  const double by = fabs((double)scale) / (double)cap;
+  return (double)cap * kTwoLog2e <= (double)FLT_MAX && by * kTwoLog2e <= (double)FLT_MAX && (scale == 0.0f || by >= (double)FLT_MIN);
+}
 
 // c tanh(s / c) = c (1 - 2 / (1 + 2^(2 s log2(e) / c))): any size, two operations of the exponentials' unit.
 __device__ __forceinline__ float capped(float x, float c) {  // x: 2 s log2(e) / c

@@ -679,7 +679,7 @@ extern "C" int lkv_attention_sums(const lkv_sums_args* a, void* stream) {
   const int group = a->hq / a->h;
   if ((int64_t)a->rows * group > (1 << 30)) return fail(LKV_ERR_ARG, "%s: %d rows of %d query heads per KV head in one call", who, a->rows, group);
   if (a->last < 1) return fail(LKV_ERR_ARG, "%s: the last %d tokens of a chunk", who, a->last);
-  if (!(a->cap_scores >= 0.0f) || a->cap_scores > FLT_MAX || !(fabsf(a->scale) <= FLT_MAX)) return fail(LKV_ERR_ARG, "%s: scale %g, cap %g", who, (double)a->scale, (double)a->cap_scores);
+  if (!scores_fit(a->scale, a->cap_scores)) return fail(LKV_ERR_ARG, "%s: scale %g with cap %g leaves float32", who, (double)a->scale, (double)a->cap_scores);
   const int64_t page_rows = a->n_pages * 2 * a->h * a->bs;
   if (page_rows > INT32_MAX) return fail(LKV_ERR_ARG, "%s: %lld rows of pages", who, (long long)page_rows);
   if (a->batch == 0 || a->cap == 0) return LKV_OK;
