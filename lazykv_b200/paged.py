@@ -18,7 +18,7 @@ gets from its queries (kernels.attention_sums), and evict() keeps the tokens of 
 Layout (one layer): pages [n_pages, h, 2, page, d] in the model dtype, or int8 codes with scales
 [n_pages, h, 2, page] float32, one per token, head and key or value; page tables int32, -1 past a
 sequence's own pages. The prefix's tokens are positions 0 .. prefix_len - 1 of its own page list and a
-sequence's own tokens positions 0 .. of its; rotary positions are the caller's (prefix_len + position), or
+sequence's own tokens positions 0 .. of its; rotary positions are the caller's (from next_position() on), or
 chunk()'s own. After evict() a sequence's slots are in no order and differ by head; `positions` says which
 token is where.
 """
@@ -179,7 +179,7 @@ class PagedBatch:
         require_cuda(query, keys, values)
         self._reserve(seq_ids, [t] * n)
         lens = [self.lengths[s] for s in seq_ids]
-        first = [self._next(s) for s in seq_ids]
+        first = [self.next_position(s) for s in seq_ids]
         ints = self._to_device(torch.tensor([seq_ids, lens, [x + t for x in lens], first], dtype=torch.int32, pin_memory=True))
         table = self.table.index_select(0, ints[0])
         K.paged_write(keys, values, self.pages, table, ints[1], scales=self.scales)
@@ -196,8 +196,9 @@ class PagedBatch:
             self.lengths[s] += t
         return done
 
-    def _next(self, s: int) -> int:
-        """The rotary position of sequence `s`'s next token."""
+    def next_position(self, s: int) -> int:
+        """The position of sequence `s`'s next token, to which step()'s caller rotates it (chunk() does so itself): behind the
+        prefix and all tokens of its own, those that evict() dropped too."""
         return self.prefix_len + self._dropped[s] + self.lengths[s]
 
     def _track(self, ids: torch.Tensor, place: torch.Tensor, held: torch.Tensor, first: torch.Tensor, counts: int | torch.Tensor, query: torch.Tensor, lse: torch.Tensor,
@@ -239,7 +240,7 @@ class PagedBatch:
         require_cuda(query, keys, values)
         self._reserve(seq_ids, counts)
         held = [self.lengths[s] for s in seq_ids]
-        first = [self._next(s) for s in seq_ids]
+        first = [self.next_position(s) for s in seq_ids]
         ends = [sum(counts[:i]) for i in range(n + 1)]
         ints = self._to_device(torch.tensor([seq_ids + [0], held + [0], [x + t for x, t in zip(held, counts)] + [0], first + [0], counts + [0], ends], dtype=torch.int32, pin_memory=True))
         ids, lens, offsets = ints[0, :n], ints[2, :n], ints[5]
@@ -270,7 +271,7 @@ class PagedBatch:
         long = [s for s in seq_ids if self.lengths[s] > keep]
         if not long:
             return
-        ints = self._to_device(torch.tensor([long, [self.lengths[s] for s in long], [self._next(s) - recent for s in long]], dtype=torch.int32, pin_memory=True))
+        ints = self._to_device(torch.tensor([long, [self.lengths[s] for s in long], [self.next_position(s) - recent for s in long]], dtype=torch.int32, pin_memory=True))
         sums, positions = self.sums.index_select(0, ints[0]), self.positions.index_select(0, ints[0])
         K.paged_evict(self.pages, self.table.index_select(0, ints[0]), ints[1], sums, positions, keep, since=ints[2], sinks=self.prefix_len + sinks, scales=self.scales,
                       out=(sums, positions))

@@ -116,3 +116,22 @@ def test_an_untracked_batch_takes_back_any_tokens() -> None:
         batch.step([s], *(torch.randn(1, 2, n, D, generator=gen).bfloat16().cuda() for n in (H * G, H, H)), 0.125)
     batch.take_back(s, 5)
     assert batch.lengths[s] == 1
+
+
+def test_next_position_counts_what_was_evicted() -> None:
+    """What step()'s caller rotates to: the positions that the batch notes, through chunks, evictions and tokens taken back."""
+    gen = torch.Generator().manual_seed(4)
+    a, _, ids, rand = _filled("int8", gen)
+    assert [a.next_position(s) for s in ids] == [37 + 200, 37 + 40, 37 + 100]
+    a.evict(ids, 64, recent=8)
+    assert [a.lengths[s] for s in ids] == [64, 40, 64]
+    want = [37 + 200, 37 + 40, 37 + 100]
+    assert [a.next_position(s) for s in ids] == want
+    for t, behind in ((3, 0), (1, 3)):
+        a.step(ids, rand(3, t, H * G, D), rand(3, t, H, D), rand(3, t, H, D), 0.125)
+        for s, first in zip(ids, want):
+            n = a.lengths[s]
+            assert a.positions[s, :, n - t : n].tolist() == [list(range(first + behind, first + behind + t))] * H
+            assert a.next_position(s) == first + behind + t
+    a.take_back(ids[0], 1)
+    assert a.next_position(ids[0]) == want[0] + 3
