@@ -762,9 +762,10 @@ int lkv_prefix_attention(const lkv_prefix_args* args, void* stream);
  * and scale / cap 0 or normal. lens, offsets and the tables are read on the device. Two launches; the workspace
  * (lkv_chunk_attention_workspace bytes with own_reach = table_cols * bs, 16-byte aligned, any contents) belongs to
  * one call at a time. batch <= 8192, rows * hq / h <= 2^30, n_pages * 2 * h * bs < 2^31.
- * Roundings: scores, references and sums are float32 (capped scores within 2^-20 of the cap); a weight, times its value's scale of int8 pages, is rounded to
- * bf16 (2^-8). Sums of weights times values are float32 before they are divided, with weights of up to 2^20: values above
- * 2^107 / keys may pass its end. An infinite value that is seen makes an infinite output (NaN where the weight is 0 in float32).
+ * Roundings: scores, references and sums are float32 (capped scores within 2^-20 of the cap). bf16 pages: a weight is rounded
+ * to bf16 (2^-8). int8 pages: codes are exact, a weight times its value's scale is rounded to f16 (2^-11 of it, and 2^-31 of the
+ * row's largest such product times 127). Sums of weights times values are float32 before they are divided, with weights of up to
+ * 2^20: bf16 values above 2^107 / keys may pass its end; value scales of any size do not. An infinite value that is seen makes an infinite output (NaN where the weight is 0 in float32).
  * The kernels' waits are bounded (lkv_device_status 1): where one ran out, rows are right, hold NaN, or were not written.
  */
 typedef struct {

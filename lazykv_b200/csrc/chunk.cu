@@ -15,11 +15,13 @@
 // rows or fewer both tiles are the same queries and take the tiles of tokens by turns; they are joined at the end.
 // Warps 0-3 and 4-7 are the two tiles' rows, warp 8 issues the products, warp 9 the copies, warp 10 walks the
 // line, warp 11 cleans values (below); with int8 pages warps 12-15 turn codes of keys into bf16 operands, 16-19
-// those of values. mbarriers join them, every wait bounded.
+// those of values into f16. mbarriers join them, every wait bounded.
 //
-// Roundings: scores, references, sums are float32; a weight (times its value's scale, of int8 pages) is rounded to
-// bf16 once, 2^-9 of it on average half, and the output to bf16. Codes, and bf16 queries, keys and values, are
-// exact operands. Capped scores are c tanh(x / c), by a polynomial while a warp's scores of a tile stay within the cap,
+// Roundings: scores, references, sums are float32; a weight is rounded once, and the output to bf16. bf16 pages: the
+// weight to bf16, 2^-8 of it at most, since both operands of a product have one type and values need bf16's
+// range; a second term would cost a third of the time (prefix_tile.cu has it for float32 outputs). int8 pages: the weight
+// times its value's scale to f16, 2^-11 of it (and 2^-31 of the row's largest; prefix.cuh, kScaleShift), in which codes are
+// exact too. Codes, and bf16 queries, keys and values, are exact operands. Capped scores are c tanh(x / c), by a polynomial while a warp's scores of a tile stay within the cap,
 // and otherwise by exponentials (scores.cuh).
 //
 // Masks: a row sees a token if its page exists and the token is in front of the row's limit. Weights of others are
@@ -28,7 +30,7 @@
 // the rows that do see them at the end.
 //
 // Measured (8 KV heads, 4 query heads each, d 128): 4,096 tokens on 32,768 in 2,050 us in a short burst, 1.14 PFLOP/s (2,400 under
-// the power cap, 0.97); 2,048 on 16,384 int8 770 us. A row tile's period of 3,800 cycles a tile: its weights 1,830 (1,290 alone: the
+// the power cap, 0.97); 2,048 on 16,384 int8 777 us (770 with weights of int8 pages in bf16, 2^-8). A row tile's period of 3,800 cycles a tile: its weights 1,830 (1,290 alone: the
 // other row tile's exponentials share the unit), 320 until the products' warp has seen them, 960 for the two products, and the
 // waits between; products alone would take 1,760 us of the 2,050, weights alone 1,790.
 #include <cuda.h>
@@ -52,7 +54,14 @@ using namespace paged;
 using prefix::ex2;
 using prefix::kLn2;
 using prefix::kLog2e;
+using prefix::kMostF16;
+using prefix::kScaleDown;
+using prefix::kScaleShift;
 using prefix::pack_bf16;
+using prefix::pack_f16;
+using prefix::scaled_room;
+using prefix::scaled_top;
+using prefix::times_ex2;
 
 constexpr int kBlock = 2 * kTile;  // rows of a unit
 constexpr int kInfo = 8;           // tiles whose scales and page bits are kept (see the copies)
@@ -62,7 +71,7 @@ constexpr int kPad = 1;            // a unit's start and end count as this many 
 constexpr int kMinShare = 2;       // tiles of the line that a CTA takes at least
 constexpr int kMostBatch = 8192;
 constexpr int kLost = 4;           // of a part: its CTA gave up a wait, it may hold anything
-constexpr float kMostWeight = 1048576.0f;  // 2^20: what the sum of a thread's weights may grow to before its references are set again
+constexpr float kMostWeight = 1048576.0f;  // 2^20: what the sum of a thread's weights of bf16 pages may grow to before its references are set again
 
 struct ChunkParams {
   const __nv_bfloat16* q;
@@ -126,7 +135,7 @@ struct Tiles {
   // Registers per thread: the warpgroups that compute weights take what the others leave of the launch's.
   static constexpr int kMany = INT8 ? 160 : 208, kFew = INT8 ? 48 : 88;
   static_assert(256 * kMany + (kThreads - 256) * kFew <= kThreads * (INT8 ? 96 : 168), "the register split is the launch's own");
-  static constexpr int kScaleBytes = INT8 ? kInfo * 2 * kTile * 4 : 0;
+  static constexpr int kScaleBytes = INT8 ? kInfo * (2 * kTile + 4) * 4 : 0;
   static constexpr int kSmem = 2 * kBytes + kStages * kBytes + kRaw * kRawBytes + kScaleBytes + 1024;
   static constexpr int kReaders = INT8 ? 18 : 11;       // warps that read a unit: weights, products, copies, and cleaning or converters
   static_assert((2 + kStages) * kBytes >= kMostBatch * 12, "the plan fits the tiles");
@@ -145,6 +154,8 @@ struct Barriers {
   int n_long;
   int4 of[2];               // the parts that the walk handed out
 };
+
+static_assert(sizeof(Barriers) + std::max({Tiles<64, false>::kSmem, Tiles<128, false>::kSmem, Tiles<64, true>::kSmem, Tiles<128, true>::kSmem}) <= 227 * 1024, "a CTA's shared memory");
 
 // Tiles of row block i of a chunk of n tokens behind `base` others (a block that sees nothing has one all the same).
 __device__ __forceinline__ int own_seen(const ChunkParams& p, int64_t i, int n, int base, int reach) {
@@ -191,7 +202,8 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   char* q_tiles = smem;
   char* raws = q_tiles + (2 + T::kStages) * T::kBytes;
-  float* scale_ring = reinterpret_cast<float*>(raws + T::kRaw * T::kRawBytes);  // [kInfo][2][kTile]: keys', values'
+  float* scale_ring = reinterpret_cast<float*>(raws + T::kRaw * T::kRawBytes);  // [kInfo][2][kTile]: keys', values' x kScaleDown
+  [[maybe_unused]] int4* tops = reinterpret_cast<int4*>(scale_ring + kInfo * 2 * kTile);  // [kInfo]: 2^top is above every finite value scale x kScaleDown, per warp of converters
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int n_prefix = prefix_tiles(p), bs = 1 << p.page_shift;
   auto stalls = [&](int which) { return p.stall == which && (p.stall_cta < 0 || p.stall_cta == (int)blockIdx.x); };
@@ -350,6 +362,11 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
         const uint32_t have = (s.have[slot][0] | s.have[slot][1]) | (s.have[slot][2] | s.have[slot][3]);
         const int start = tile < n_prefix ? 0 : (tile - n_prefix) * kTile;
         const bool masked = have != 0xffu || (tile < n_prefix ? p.prefix_len - tile * kTile : lowest - start) < kTile;
+        float most_weight = kMostWeight;
+        if constexpr (INT8) {
+          const int4 top = tops[slot];
+          most_weight = __int_as_float((127 + kMostF16 - max(max(top.x, top.y), max(top.z, top.w))) << 23);
+        }
         // Pair 4 k: columns 8 k + c2, + 1.
         [[maybe_unused]] const uint64_t* ks = reinterpret_cast<const uint64_t*>(scale_ring + slot * 2 * kTile + c2);
         [[maybe_unused]] const uint64_t* vs = ks + kTile / 2;
@@ -406,12 +423,17 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
                   ld_wait(f);
 #pragma unroll
                   for (int k = 0; k < 2; ++k) {
-                    [[maybe_unused]] uint64_t kk = 0;
-                    if constexpr (INT8) kk = ks[4 * (2 * n + k)];
+                    [[maybe_unused]] uint64_t kk = 0, room = 0;
+                    if constexpr (INT8) {
+                      kk = ks[4 * (2 * n + k)];
+                      const uint64_t v = vs[4 * (2 * n + k)];
+                      room = pair(scaled_room(first_of(v)), scaled_room(second_of(v)));
+                    }
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                       uint64_t z = raw_score(f, k, r, kk);
                       if constexpr (CAP) z = wide(z);
+                      if constexpr (INT8) z = CAP ? add2(z, room) : fma2(z, pair(scale, scale), room);
                       z = seen(z, n, k, r);
                       top[r] = fmaxf(fmaxf(top[r], first_of(z)), second_of(z));
                     }
@@ -423,9 +445,9 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
                 for (int r = 0; r < 4; ++r) {
                   top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
                   top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                  const float want = CAP ? top[r] : top[r] * scale, to_ref = fmaxf(from[r], want);
+                  const float want = CAP || INT8 ? top[r] : top[r] * scale, to_ref = fmaxf(from[r], want);
                   by[r] = to_ref == -INFINITY ? 1.0f : ex2(from[r] - to_ref);
-                  l[r] *= by[r];
+                  l[r] = INT8 && to_ref > from[r] ? times_ex2(l[r], from[r] - to_ref) : l[r] * by[r];
                   from[r] = to_ref;
                   none = none || to_ref == -INFINITY;
                 }
@@ -485,7 +507,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
                         // A scale of a token that the row does not see may be anything.
                         z[r] = MASK ? pair(first_of(z[r]) == 0.0f ? 0.0f : first_of(x), second_of(z[r]) == 0.0f ? 0.0f : second_of(x)) : x;
                       }
-                      w[n][(r0 + r) / 2][2 * k + ((r0 + r) & 1)] = pack_bf16(first_of(z[r]), second_of(z[r]));
+                      w[n][(r0 + r) / 2][2 * k + ((r0 + r) & 1)] = INT8 ? pack_f16(first_of(z[r]), second_of(z[r])) : pack_bf16(first_of(z[r]), second_of(z[r]));
                     }
                   }
                 }
@@ -496,7 +518,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
               // No weight is above the sum that it is part of.
               bool over = false;
 #pragma unroll
-              for (int r = 0; r < 4; ++r) over = over || fmaxf(first_of(sum[r]), second_of(sum[r])) > kMostWeight;
+              for (int r = 0; r < 4; ++r) over = over || fmaxf(first_of(sum[r]), second_of(sum[r])) > most_weight;
               set = !again && __any_sync(0xffffffffu, over);
               if (set) continue;
 #pragma unroll
@@ -551,7 +573,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
             const float2 other = any_other ? s.other[base + 8 * i] : make_float2(-INFINITY, 0.0f);
             const float both = fmaxf(from[i], other.x), ref = both == -INFINITY ? 0.0f : both;
             f0[i] = ex2(from[i] - ref), f1[i] = ex2(other.x - ref);
-            l[i] = l[i] * f0[i] + other.y * f1[i];
+            l[i] = INT8 ? times_ex2(l[i], from[i] - ref) + times_ex2(other.y, other.x - ref) : l[i] * f0[i] + other.y * f1[i];
             from[i] = both;
           }
         }
@@ -566,6 +588,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
         for (int i = 0; i < 4; ++i) {
           const int row = base + 8 * i, x = un.row0 + row, t = x / p.group;
           to_row[i] = part ? (int64_t)un.slot * kBlock + row : (int64_t)(un.q0 + t) * (p.h * p.group) + un.j * p.group + (x - t * p.group);
+          if (INT8) from[i] += kScaleShift, l[i] *= kScaleDown;  // as the values' scales are
           by[i] = part ? 1.0f : l[i] == 0.0f ? 0.0f : 1.0f / l[i];
           if (!ok) by[i] = l[i] = __uint_as_float(0x7fc00000u);  // where a wait ran out the row is poisoned (its status word tells why)
           f0[i] *= by[i], f1[i] *= by[i];
@@ -627,7 +650,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
     tc_before();
   } else if (warp == 8) {
     // ---- matrix products: issued by one lane, in order -----------------------------------------------
-    constexpr uint32_t kQk = instruction<false>(kTile, false), kPv = instruction<false>(D, true);
+    constexpr uint32_t kQk = instruction<false>(kTile, false), kPv = instruction<INT8>(D, true);
     const uint32_t q_u = smem_u32(q_tiles), st_u = smem_u32(stages), mine = elect(), tm = __reduce_max_sync(0xffffffffu, tmem);
     int jobs[2] = {0, 0}, cleaned = 0;
     Cursor keys = {0, 0}, values = {1, 0};  // stages of the next tile's
@@ -932,7 +955,7 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
     }
   } else {
     if constexpr (INT8) {
-      // ---- codes to bf16 operands: warps 12-15 the keys', 16-19 the values'; thread i carries token i's scale --
+      // ---- codes to operands: warps 12-15 the keys' to bf16, 16-19 the values' to f16; thread i carries token i's scale --
       const int i = tid % kTile, kv = (tid - 12 * 32) / kTile;
       // A thread's pieces of 16 codes, one channel range of every kStep-th token. Eight lanes take 128 bytes
       // that lie in 32 different banks, and so do the chunks they write: two tokens of different parity, of
@@ -977,8 +1000,11 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
         for (int t = 0; t < un.n_tiles; ++t) {
           const int info = (tiles + t) % kInfo;
           // The ring entry's last reader is more than two tiles behind (see the copies): it is free.
-          scale_ring[(info * 2 + kv) * kTile + i] = scale;
-          if (kv == 0) {
+          scale_ring[(info * 2 + kv) * kTile + i] = kv == 0 ? scale : scale * kScaleDown;
+          if (kv == 1) {
+            const int top = __reduce_max_sync(0xffffffffu, scaled_top(scale * kScaleDown));
+            if (lane == 0) reinterpret_cast<int*>(tops + info)[warp - 16] = top;
+          } else {
             const uint32_t mask = __ballot_sync(0xffffffffu, there);
             if (lane == 0) s.have[info][warp - 12] = ((mask & 0xffffu) != 0 ? 1u : 0u) << (2 * (warp - 12)) | (mask >> 16 != 0 ? 2u : 0u) << (2 * (warp - 12));
           }
@@ -988,22 +1014,26 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) chunk_kernel(cons
           if (!ok) break;
           const char* src = raws + raw.slot * T::kRawBytes + from;
           char* dst = stages + to.slot * T::kBytes;
+          auto convert = [&](auto&& operand) {
 #pragma unroll
-          for (int x0 = 0; x0 < kPer; x0 += 4) {
-            uint4 w[4];
+            for (int x0 = 0; x0 < kPer; x0 += 4) {
+              uint4 w[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) w[x] = *reinterpret_cast<const uint4*>(src + (x0 + x) * (kStep * kPer * 16));
-            if (x0 + 4 >= kPer) {
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&s.raw_empty[raw.slot]);
+              for (int x = 0; x < 4; ++x) w[x] = *reinterpret_cast<const uint4*>(src + (x0 + x) * (kStep * kPer * 16));
+              if (x0 + 4 >= kPer) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s.raw_empty[raw.slot]);
+              }
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const uint2 a = operand(w[x].x), b = operand(w[x].y), d = operand(w[x].z), e = operand(w[x].w);
+                *reinterpret_cast<uint4*>(dst + to0 + kStep * (x0 + x) * 128) = make_uint4(a.x, a.y, b.x, b.y);
+                *reinterpret_cast<uint4*>(dst + to1 + kStep * (x0 + x) * 128) = make_uint4(d.x, d.y, e.x, e.y);
+              }
             }
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const uint2 a = codes_to_bf16(w[x].x), b = codes_to_bf16(w[x].y), d = codes_to_bf16(w[x].z), e = codes_to_bf16(w[x].w);
-              *reinterpret_cast<uint4*>(dst + to0 + kStep * (x0 + x) * 128) = make_uint4(a.x, a.y, b.x, b.y);
-              *reinterpret_cast<uint4*>(dst + to1 + kStep * (x0 + x) * 128) = make_uint4(d.x, d.y, e.x, e.y);
-            }
-          }
+          };
+          if (kv == 0) convert([](uint32_t x) { return codes_to_bf16(x); });
+          else convert([](uint32_t x) { return prefix::codes_to_f16(x); });
           fence_async();
           warp_arrive(&s.full[to.slot], lane);
           to.step(2, n_stages);
@@ -1051,7 +1081,7 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const ChunkParams p) {
       const int64_t at = (int64_t)(k == c ? 2 * c + 1 : 2 * k) * kBlock + row;
       const float2 ml = p.part_ml[at];
       const float f = ex2(ml.x - ref);
-      l += ml.y * f;
+      l += times_ex2(ml.y, ml.x - ref);  // (of int8 pages references are as far apart as value scales may be)
 #pragma unroll
       for (int x = 0; x < D / 32; x += 2) {
         const float2 v = *reinterpret_cast<const float2*>(p.part_o + at * D + (x / 2) * 64 + 2 * lane);

@@ -126,6 +126,17 @@ __device__ __forceinline__ float weight_room(float scale) {  // E - kScaleShift 
   return (float)(bits == 0xff ? -64 : max(bits - 126, -64)) - (kScaleShift + 7.0f);
 }
 
+// A value scale that kScaleDown has multiplied is below 2^scaled_top, one that is not finite claims nothing;
+// weight_room is 7 less.
+__device__ __forceinline__ int scaled_top(float scaled) {
+  const int bits = (__float_as_int(scaled) >> 23) & 0xff;
+  return bits == 0xff ? -80 : max(bits - 126, -80);
+}
+__device__ __forceinline__ float scaled_room(float scaled) { return (float)scaled_top(scaled) - 7.0f; }
+// int8: a weight times its value's scale has to stay below 2^kMostF16. That is asked of the sum and the tile's
+// largest scale: where a token of little weight has that scale, references are looked up for nothing.
+constexpr int kMostF16 = 15;
+
 // Stages of sequence b's own tokens (lens may lie outside [0, the table's reach]).
 __device__ __forceinline__ int own_len(const Params& p, int len) {
   return (int)min((int64_t)max(len, 0), (int64_t)p.table_cols << p.page_shift);

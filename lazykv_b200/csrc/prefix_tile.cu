@@ -55,9 +55,6 @@ constexpr int kInfo = 8;         // tiles whose scales and page bits are kept (s
 // What the sum of a thread's weights may grow to before its references are set again: a bf16 weight has
 // float32's range, of which the accumulated values need the rest.
 constexpr float kMostBf16 = 1048576.0f;  // 2^20
-// int8: a weight times its value's scale has to stay below 2^kMostF16. That is asked of the sum and the tile's
-// largest scale: where a token of little weight has that scale, references are looked up for nothing.
-constexpr int kMostF16 = 15;
 // int8: sums of codes times a query's f16 are below 2^15, and a key's scale may be 2^121: it is kept 2^9 smaller, and
 // the row's factor that much larger, so that no product passes float32's end. (A scale below 2^-117 loses bits: fourteen
 // are left at the least. The product of the two factors first would cost 3% of the time.)
@@ -95,14 +92,6 @@ struct Barriers {
   uint32_t tmem;
   int quit;
 };
-
-// A value scale that kScaleDown has multiplied is below 2^scaled_top, one that is not finite claims nothing;
-// weight_room is 7 less.
-__device__ __forceinline__ int scaled_top(float scaled) {
-  const int bits = (__float_as_int(scaled) >> 23) & 0xff;
-  return bits == 0xff ? -80 : max(bits - 126, -80);
-}
-__device__ __forceinline__ float scaled_room(float scaled) { return (float)scaled_top(scaled) - 7.0f; }
 
 // This thread's query row into its place of the operand tile; returns what its scores have to be
 // multiplied with for int8 pages (a power of two). `flip`: negated (a negative softmax scale).

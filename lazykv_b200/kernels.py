@@ -762,8 +762,8 @@ def chunk_attention(query: torch.Tensor, pages: torch.Tensor, table: torch.Tenso
     pages are bfloat16 or int8 with scales. Returns (out [rows, hq, d] bfloat16, lse [rows, hq] float32). A row that attends
     nothing gets out = 0 and lse = -inf; rows of no sequence are left alone (in new tensors: not set), so a batch may be
     padded, and sequences may have no new tokens. lens, offsets and the tables are read on the device, so a captured graph
-    follows them as they change; the shapes and prefix_len are fixed at capture. Scores and sums are float32, weights are
-    rounded to bfloat16 (2^-8) where they multiply the values. The workspace comes from torch's allocator call by call.
+    follows them as they change; the shapes and prefix_len are fixed at capture. Scores and sums are float32; weights are
+    rounded where they multiply the values, of bfloat16 pages to bfloat16 (2^-8), of int8 pages to 2^-11 as in prefix_attention. The workspace comes from torch's allocator call by call.
     """
     who = "chunk_attention"
     index = query.get_device()
