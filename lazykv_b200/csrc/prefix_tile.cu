@@ -618,6 +618,11 @@ __global__ void __launch_bounds__(Tiles<D, INT8>::kThreads, 1) prefix_tile_kerne
         warp_arrive(&s.info[info], lane);
         scales_of(t + 1);
         ok = ok && wait_for(s, &s.raw_full[raw], T::raw_round(t, kv) & 1);
+        // With an odd number of stages a stage holds keys and values by turns, and these warps wait for the product behind every
+        // second filling of it only. None of their waits meets a barrier two phases behind, which would let it pass at once: the
+        // filling before the last, of their own kind, was multiplied before what their wait for the tile before asked for. Three
+        // stages (two row tiles, products in the order K0 V0 K1 V1 ..): V(t - 3) before K(t - 2), K(t - 3) before V(t - 3); seven
+        // (one row tile, V(t) before K(t + 2)): V(t - 7) before K(t - 4), K(t - 7) before V(t - 5).
         if (ok && n >= n_stages) ok = wait_for(s, &s.empty[slot], (n / n_stages - 1) & 1);
         if (!ok) break;
         const char* src = raws + raw * T::kRawBytes + from;
