@@ -25,6 +25,7 @@ token is where.
 
 from __future__ import annotations
 
+import itertools
 from dataclasses import dataclass
 
 import torch
@@ -34,15 +35,24 @@ from lazykv_b200._lib import require_cuda
 
 
 @dataclass
-class _LastCall:
-    """What a sequence's last step or chunk added to its sums, as take_back() needs it."""
+class _Call:
+    """What a tracked step or chunk added to the sums, as take_back() needs it."""
 
-    held: int  # own tokens in front of the call's
-    sums: torch.Tensor  # [heads, slots] before it
-    query: torch.Tensor | None  # the call's rows and their lse, where some of them may stay
-    lse: torch.Tensor | None
+    sums: torch.Tensor  # [n, heads, slots] before it
+    query: torch.Tensor  # the packed rows, and their lse, of sequences with a few new tokens
+    lse: torch.Tensor
     scale: float
     cap: float
+
+
+@dataclass
+class _Part:
+    """A sequence's part of its last call."""
+
+    call: _Call
+    at: int  # its place in call.sums
+    row: int  # its first row of call.query, or -1: they are not kept
+    held: int  # own tokens in front of the call's
 
 
 class PagedBatch:
@@ -86,7 +96,7 @@ class PagedBatch:
         self._dropped: dict[int, int] = {}  # tokens that evict() has dropped of it
         self._settled: dict[int, int] = {}  # its tokens that evict() may have moved
         self._pages_of: dict[int, list[int]] = {}
-        self._last: dict[int, _LastCall] = {}  # of a tracked batch
+        self._last: dict[int, _Part] = {}  # of a tracked batch
 
     # -- the prefix and the sequences -------------------------------------------------------------------
 
@@ -189,8 +199,6 @@ class PagedBatch:
             place = torch.arange(t, dtype=torch.int32, device=self.dev).repeat(n)
             rows = query.reshape(n * t, -1, self.d)
             last = self._track(ints[0], place, ints[1].repeat_interleave(t), ints[3].repeat_interleave(t), t, rows, done[1].view(n * t, -1), table, ints[2], offsets, scale, 0.0)
-            if 1 < t <= self.MOST_DRAFTED:  # (the caller's tensor may change)
-                rows = rows.clone()
             self._note(seq_ids, [t] * n, last, rows, done[1].view(n * t, -1), scale, 0.0)
         for s in seq_ids:  # behind the calls: a refused step leaves the sequences as they were
             self.lengths[s] += t
@@ -213,15 +221,17 @@ class PagedBatch:
 
     def _note(self, seq_ids: list[int], counts: list[int], before: torch.Tensor, query: torch.Tensor, lse: torch.Tensor, scale: float, cap: float) -> None:
         """Keeps what take_back() needs of a call's packed rows (before the lengths grow)."""
-        if any(1 < t <= self.MOST_DRAFTED for t in counts):
-            lse = lse.clone()  # (the caller has it too)
-        at = 0
+        ends = [0, *itertools.accumulate(counts)]
+        few = [i for i, t in enumerate(counts) if 1 < t <= self.MOST_DRAFTED]  # (of one token all or none stays)
+        if len(few) == len(counts):  # (copies: the caller has both tensors too)
+            query, lse, first = query.clone(), lse.clone(), dict(enumerate(ends))
+        else:
+            query, lse = (torch.cat([x[:0], *(x[ends[i] : ends[i + 1]] for i in few)]) for x in (query, lse))
+            first = dict(zip(few, itertools.accumulate((counts[i] for i in few), initial=0)))
+        call = _Call(before, query, lse, scale, cap)
         for i, (s, t) in enumerate(zip(seq_ids, counts)):
             if t:
-                rows = slice(at, at + t)
-                part = 1 < t <= self.MOST_DRAFTED
-                self._last[s] = _LastCall(self.lengths[s], before[i], query[rows] if part else None, lse[rows] if part else None, scale, cap)
-            at += t
+                self._last[s] = _Part(call, i, first.get(i, -1), self.lengths[s])
 
     def chunk(self, seq_ids: list[int], counts: list[int], query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, scale: float,
               frequencies: torch.Tensor | None = None, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
@@ -287,28 +297,47 @@ class PagedBatch:
             self.lengths[s] = self._settled[s] = keep
             self._last.pop(s, None)
 
-    def take_back(self, s: int, tokens: int) -> None:
-        """Forget the last `tokens` own tokens of sequence `s` (drafted ones that were rejected); their pages stay
-        the sequence's and are written again. What evict() has moved cannot be taken back.
+    def take_back(self, s: int | list[int], tokens: int | list[int]) -> None:
+        """Forget the last `tokens` own tokens of sequence `s` (drafted ones that were rejected), or tokens[i] of each
+        sequence s[i] of a list; their pages stay the sequences' and are written again. What evict() has moved cannot be taken back.
 
         With track=True the weights that the forgotten tokens' queries gave to the others leave the sums: these are as if
         only the tokens that stay had come. That holds for tokens of the sequence's last step or chunk, all of them or, of
         a call of up to MOST_DRAFTED of its tokens, a part; others are refused."""
-        last = self._last.get(s)
-        most = self.lengths[s] - (self._settled[s] if self.sums is None else last.held if last is not None else self.lengths[s])
-        if not 0 <= tokens <= most:
-            raise ValueError(f"sequence {s} has {most} tokens to take back, not {tokens}")
-        if last is not None and tokens:
-            stay = most - tokens
-            if stay == 0:
-                self.sums[s].copy_(last.sums)
-            elif last.query is None:
-                raise ValueError(f"of a tracked chunk of more than {self.MOST_DRAFTED} tokens all are taken back or none, not {tokens} of {most}")
-            else:
-                ints = self._to_device(torch.tensor([0, stay, last.held + stay], dtype=torch.int32, pin_memory=True))
-                K.attention_sums(last.query[:stay], last.lse[:stay], self.pages, self.table[s : s + 1], ints[2:], ints[:2], last.scale, sums=last.sums[None], cap=last.cap,
-                                 scales=self.scales, out=self.sums[s : s + 1])
-        self.lengths[s] -= tokens
+        ids = list(s) if isinstance(s, (list, tuple)) else [s]
+        counts = list(tokens) if isinstance(tokens, (list, tuple)) else [tokens]
+        if len(set(ids)) != len(ids) or len(counts) != len(ids):
+            raise ValueError(f"expected a count of tokens for each of the sequences {ids}, each named once; got {counts}")
+        calls: dict[int, list[tuple[int, int, _Part]]] = {}  # by call: sequence, tokens of it that stay
+        for i, n in zip(ids, counts):
+            part = self._last.get(i)
+            most = self.lengths[i] - (self._settled[i] if self.sums is None else part.held if part is not None else self.lengths[i])
+            if not 0 <= n <= most:
+                raise ValueError(f"sequence {i} has {most} tokens to take back, not {n}")
+            if part is not None and n:
+                if n < most and part.row < 0:
+                    raise ValueError(f"of a tracked chunk of more than {self.MOST_DRAFTED} tokens all are taken back or none, not {n} of {most}")
+                calls.setdefault(id(part.call), []).append((i, most - n, part))
+        for parts in calls.values():
+            self._add_again(parts[0][2].call, parts)
+        for i, n in zip(ids, counts):
+            self.lengths[i] -= n
+
+    def _add_again(self, call: _Call, parts: list[tuple[int, int, _Part]]) -> None:
+        """Sums of sequences as if only the first so many tokens of their part of `call` had come."""
+        n = len(parts)
+        kept = [stay for _, stay, _ in parts]
+        ends = [0, *itertools.accumulate(kept)]
+        rows = [part.row + t for _, stay, part in parts for t in range(stay)]
+        flat = [i for i, _, _ in parts] + [part.at for _, _, part in parts] + [part.held + stay for _, stay, part in parts] + ends + rows
+        ints = self._to_device(torch.tensor(flat, dtype=torch.int32, pin_memory=True))
+        ids, at, lens, offsets, row = ints.split([n, n, n, n + 1, len(rows)])
+        sums = call.sums.index_select(0, at)
+        if rows:
+            K.attention_sums(call.query.index_select(0, row), call.lse.index_select(0, row), self.pages, self.table.index_select(0, ids), lens, offsets, call.scale, sums=sums,
+                             cap=call.cap, scales=self.scales, out=sums)
+        assert self.sums is not None
+        self.sums.index_copy_(0, ids.long(), sums)
 
     def read(self, s: int, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """The whole sequence, prefix and own tokens, as (keys, values) [h, L, d] in the model dtype (or `dtype`,

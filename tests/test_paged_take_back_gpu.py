@@ -54,11 +54,13 @@ def test_a_step_with_rejected_drafts(quant: str | None) -> None:
         a.step(ids, given, k, v, 0.125)
         given.fill_(9.0)  # the caller's own
         for s, kept in zip(ids, (2, 5, 0)):
-            if turn % 2:
+            if turn == 1:
                 for _ in range(5 - kept):
                     a.take_back(s, 1)
-            else:
+            elif turn == 0:
                 a.take_back(s, 5 - kept)
+        if turn == 2:
+            a.take_back(ids, [3, 0, 5])
         assert torch.equal(a.sums[ids[2]], before[ids[2]])  # nothing of the call stays
         b.step(ids[:1], q[:1, :2], k[:1, :2], v[:1, :2], 0.125)
         b.step(ids[1:2], q[1:2], k[1:2], v[1:2], 0.125)
@@ -93,6 +95,20 @@ def test_a_capped_chunk_and_eviction() -> None:
     assert torch.equal(a.sums[ids[2]], before[ids[2]])
     b.chunk(ids[:1], [2], q[:2], k[:2], v[:2], 0.125, **more)
     _near(a, b, ids)
+    # In one go, of two calls; a refused one of them leaves them all.
+    c = _batch("int8")
+    one, two = c.fork(), c.fork()
+    c.chunk([one, two], [5, 70], q[:75], k[:75], v[:75], 0.125, **more)
+    middle = c.sums.clone()
+    c.chunk([two], [3], q[75:78], k[75:78], v[75:78], 0.125, **more)
+    for sequences, counts in (([one, two], [1, 4]), ([one, one], [1, 1]), ([one, two], [1]), ([one], [1, 1]), (one, 6)):
+        with pytest.raises(ValueError):
+            c.take_back(sequences, counts)
+    assert c.lengths == {one: 5, two: 73}
+    c.take_back([two, one], [3, 2])
+    assert c.lengths == {one: 3, two: 70} and torch.equal(c.sums[two], middle[two])
+    c.take_back((one,), (3,))
+    assert c.lengths[one] == 0 and not bool(c.sums[one].any())
     # What the chunk before did to a sequence without new tokens is still its own to take back.
     a.take_back(ids[1], 5)
     assert a.lengths[ids[1]] == 35
