@@ -12,8 +12,8 @@
 // add up over distributed shared memory, then ranks of ties, of slots that lose and of tokens that move by
 // ballots in slot order, and the copies.
 //
-// Measured: 8 heads of 40,001 tokens down to 5,000, d 128, int8: 38 us, a third of it the copies (4,375 tokens a head); 64
-// sequences of 8 heads from up to 1,040 to 1,024, bf16: 12 us. The chain of barriers and dependent loads bounds both.
+// Measured: 8 heads of 40,001 tokens down to 5,000, d 128, int8: 37 us, a third of it the copies (4,375 tokens a head); 64
+// sequences of 8 heads from up to 1,040 to 1,024, bf16: 14 us. The chain of barriers and dependent loads bounds both.
 #include <cooperative_groups.h>
 
 #include <atomic>

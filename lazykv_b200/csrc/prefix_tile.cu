@@ -14,9 +14,9 @@
 // int8 pages warps 12-15 turn codes of keys into f16 operands and warps 16-19 those of values. All of it is
 // joined by mbarriers, every wait bounded.
 //
-// Measured at 512 rows of each of 8 KV heads on 32,768 tokens, d 128: int8 105 us, the tensor cores busy 32% of the
-// time and the exponentials' unit 38%; bf16 78 us, 43% and 51%. 128 sequences of 8 KV heads with 4 query heads each
-// on 131,072 int8 tokens: 332 us, 0.83 PFLOP/s, and 402 to 413 us with up to 2,000 own tokens each, which the stream
+// Measured at 512 rows of each of 8 KV heads on 32,768 tokens, d 128: int8 103 us, the tensor cores busy 36% of the
+// time and the exponentials' unit 39%; bf16 76 us, 49% and 51%. 128 sequences of 8 KV heads with 4 query heads each
+// on 131,072 int8 tokens: 332 to 342 us, 0.83 PFLOP/s, and 403 to 416 us with up to 2,000 own tokens each, which the stream
 // takes behind the tiles (no CTA of it fits beside one of these). What bounds it is the chain of one tile
 // of rows, scores -> weights -> products -> next scores: S and P share 128 columns of tensor memory (two tiles
 // of S and O of d 128 fill it), so a tile's next scores wait for its present product, and two tiles do not

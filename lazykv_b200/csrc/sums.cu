@@ -13,11 +13,11 @@
 // tile, its sums are parts that sums_merge_kernel adds, in order. Warps 0-3 and 4-7 sum, 8 issues the products, 9 copies
 // keys, 10 and 11 write what no tile covers, 12-15 bring the queries; with int8 pages 16-23 turn codes into bf16 operands.
 //
-// Measured (8 KV heads, 4 query heads each, d 128): one token of each of 48 sequences of up to 6,000 int8 tokens 79 us
-// (bf16 pages, twice the bytes: 58): the chain of a step of 256 tokens, copy, conversion, products, sums, takes 3,700 cycles, and
-// shared memory holds two steps' codes beside the operands. 32 tokens' queries over 40,032 bf16 tokens 29 us, half of it the
-// start, first copies and end. 499 and 999 tokens, 7 query heads a KV head, d 64, scores capped, over 9,001: 120 us (88 without
-// the cap): the float32 units, which make the polynomials.
+// Measured (8 KV heads, 4 query heads each, d 128): one token of each of 48 sequences of up to 6,000 int8 tokens 82 us
+// (bf16 pages, twice the bytes: 62): the chain of a step of 256 tokens, copy, conversion, products, sums, takes 3,700 cycles, and
+// shared memory holds two steps' codes beside the operands. 32 tokens' queries over 40,032 bf16 tokens 31 us, half of it the
+// start, first copies and end. 499 and 999 tokens, 7 query heads a KV head, d 64, scores capped, over 9,001: 121 us (85 without
+// the cap): two summing warps a scheduler, no unit busy to a half.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
