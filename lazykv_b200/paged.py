@@ -221,7 +221,7 @@ class PagedBatch:
 
     def _note(self, seq_ids: list[int], counts: list[int], before: torch.Tensor, query: torch.Tensor, lse: torch.Tensor, scale: float, cap: float) -> None:
         """Keeps what take_back() needs of a call's packed rows (before the lengths grow)."""
-        ends = [0, *itertools.accumulate(counts)]
+        query, lse, ends = query.detach(), lse.detach(), [0, *itertools.accumulate(counts)]
         few = [i for i, t in enumerate(counts) if 1 < t <= self.MOST_DRAFTED]  # (of one token all or none stays)
         if len(few) == len(counts):  # (copies: the caller has both tensors too)
             query, lse, first = query.clone(), lse.clone(), dict(enumerate(ends))

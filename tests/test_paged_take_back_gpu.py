@@ -134,6 +134,21 @@ def test_an_untracked_batch_takes_back_any_tokens() -> None:
     assert batch.lengths[s] == 1
 
 
+def test_what_is_kept_holds_no_graph() -> None:
+    gen = torch.Generator().manual_seed(5)
+    a, _, ids, rand = _filled(None, gen)
+    for counts in ([3, 3, 3], [3, 80, 0]):
+        q = rand(sum(counts), H * G, D).requires_grad_()
+        a.chunk(ids, counts, q, rand(sum(counts), H, D), rand(sum(counts), H, D), 0.125)
+        call = a._last[ids[0]].call
+        assert not (call.query.requires_grad or call.lse.requires_grad or call.sums.requires_grad)
+        assert call.query.shape[0] == (9 if counts[1] == 3 else 3)  # the long chunk's rows are not kept
+    q = rand(3, 2, H * G, D).requires_grad_()
+    a.step(ids, q, rand(3, 2, H, D), rand(3, 2, H, D), 0.125)
+    assert not a._last[ids[0]].call.query.requires_grad
+    a.take_back(ids, [1, 2, 0])
+
+
 def test_next_position_counts_what_was_evicted() -> None:
     """What step()'s caller rotates to: the positions that the batch notes, through chunks, evictions and tokens taken back."""
     gen = torch.Generator().manual_seed(4)
